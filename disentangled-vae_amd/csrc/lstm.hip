@@ -1560,6 +1560,7 @@ static void seq_residency(int kind, int64_t H, int* cus, int* per_cu) {
     }
     e[0] = n;
     e[1] = f < b ? f : b;
+    if (e[1] > 2) e[1] = 2;                 // what these kernels are laid out for, also where registers would allow more
   }
   *cus = e[0]; *per_cu = e[1];
 }
