@@ -1,0 +1,104 @@
+// What the sequence operators (selective scan, short convolution, residual norm) share: element types, wave-uniform
+// loads, and the walk over the borders of packed sequences.
+#pragma once
+#include "common.h"
+#include "../../include/dvae_hip.h"
+
+#define ST(s) ((hipStream_t)(s))
+
+struct bf16_t { uint16_t bits; };
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(bf16_t v) { return __uint_as_float((uint32_t)v.bits << 16); }
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ bf16_t from_f32<bf16_t>(float v) {      // round to nearest even
+  return bf16_t{__builtin_bit_cast(uint16_t, (__bf16)v)};
+}
+
+// V consecutive elements, moved as accesses of up to 16 bytes (V > 1 only where the host checked alignment)
+template <typename T, int V> struct alignas(sizeof(T) * V < 16 ? sizeof(T) * V : 16) Pack { T v[V]; };
+template <typename T, int V>
+__device__ __forceinline__ void load_pack(const T* p, float (&v)[V]) {
+  const Pack<T, V> r = *reinterpret_cast<const Pack<T, V>*>(p);
+#pragma unroll
+  for (int i = 0; i < V; ++i) v[i] = to_f32(r.v[i]);
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_pack(T* p, const float (&v)[V]) {
+  Pack<T, V> r;
+#pragma unroll
+  for (int i = 0; i < V; ++i) r.v[i] = from_f32<T>(v[i]);
+  *reinterpret_cast<Pack<T, V>*>(p) = r;
+}
+
+#define LOG2E_F 1.44269504088896341f
+#define LN2_F 0.693147180559945309f
+
+// exp(x) through the hardware's 2^x (1 ulp; results below 2^-126 become 0)
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float sigmoid_hw(float x) { return __builtin_amdgcn_rcpf(1.f + exp2_hw(-LOG2E_F * x)); }
+
+// softplus(x) = max(x, 0) + log(1 + e^-|x|).  The logarithm of 1 + e loses the low bits of a small e when the sum is
+// rounded; multiplying by e / ((1 + e) - 1), the ratio of what was meant to what was added, puts them back.
+__device__ __forceinline__ float softplus_hw(float x) {
+  const float e = exp2_hw(-LOG2E_F * fabsf(x));
+  const float w = 1.f + e;
+  const float r = w - 1.f;
+  const float l = LN2_F * __builtin_amdgcn_logf(w) * (e * __builtin_amdgcn_rcpf(r));
+  return fmaxf(x, 0.f) + (r == 0.f ? e : l);
+}
+
+// NaN has to come out as NaN: fmaxf(NaN, 0) is 0, but e and with it l are NaN.
+
+// Wave-uniform reads of data that no kernel in flight writes go through the constant address space: the compiler then
+// uses the scalar unit and its registers for them, whatever it knows about the kernel's other pointers.
+#define DVAE_UNIFORM __attribute__((address_space(4)))
+template <typename V> __device__ __forceinline__ V uniform_load(const V* p, int64_t i) {
+  return ((const DVAE_UNIFORM V*)p)[i];
+}
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// The sequence that a walk over tokens is in.  With `off`, sequence s is [off[s], off[s + 1]) of S ascending int32
+// positions; without, all S sequences have L tokens.  Positions are clamped to the tokens there are, so wrong offsets
+// give wrong results but never an access out of range, and every loop here ends: the index only moves one way.
+struct SeqWalk {
+  const int32_t* off;
+  int S, L;     // number of sequences; tokens of each (off == nullptr)
+  int tokens;   // all tokens
+  int s;        // current sequence; S (forward) or -1 (backward): none left
+  int b, e;     // its borders
+
+  __device__ __forceinline__ int at(int i) const {
+    return off ? min(max(uniform_load(off, i), 0), tokens) : i * L;
+  }
+  __device__ __forceinline__ void load() {
+    if (s >= 0 && s < S) { b = at(s); e = at(s + 1); } else { b = e = tokens; }
+  }
+  // the current sequence as an index that exists, also where wrong offsets have led the walk past the last one
+  __device__ __forceinline__ int64_t seq() const { return min(max(s, 0), S - 1); }
+  // first sequence that ends behind token t (empty ones are skipped by that)
+  __device__ __forceinline__ void seek(int t) {
+    if (!off) {
+      s = t / L;
+    } else {
+      int lo = 0, hi = S;
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (at(mid + 1) > t) hi = mid; else lo = mid + 1;
+      }
+      s = lo;
+    }
+    load();
+  }
+  // forward: the next sequence with tokens from t on
+  __device__ __forceinline__ void next(int t) {
+    do { ++s; } while (s < S && at(s + 1) <= t);
+    load();
+  }
+  // backward: the last sequence that starts at or before token t and has tokens
+  __device__ __forceinline__ void prev(int t) {
+    do { --s; } while (s >= 0 && (at(s) > t || at(s + 1) <= at(s)));
+    load();
+  }
+};

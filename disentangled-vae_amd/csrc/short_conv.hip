@@ -1,0 +1,383 @@
+// The short causal convolution over time, depthwise and channels-last: out[t] = act(bias + sum_k w[k] x[t - (W-1) + k]),
+// where tokens before a sequence's first are the carried state, or zero.  Bound by memory: every element of x is read
+// once (and a block's first W - 1 rows twice, out of the L2) and kept in registers for the W outputs that use it.
+//
+// A lane owns V neighbouring channels (16 bytes where the tensors' alignment allows it, else one element), a wave
+// CONV_TB consecutive tokens, loaded in groups of CONV_GROUP so that a group's loads are in flight together.  A batch is
+// walked as one line of tokens, sequence after sequence, so short clips fill the chip like long sequences do.
+#include "seq_common.h"
+
+#define CONV_TB 16
+#define CONV_GROUP 8
+
+struct ConvArgs {
+  const void *x, *dout, *state0, *dstate1;
+  int64_t x_sb, x_st, dout_sb, dout_st;
+  const float *w, *bias;
+  void *out, *state1, *dx, *dstate0;
+  float* part;                 // [workgroup row][W + 1][D]: partial sums of dw and dbias
+  const int32_t* offsets;
+  int D, S, L, tokens, silu, tiles;
+};
+
+// where token t of the walk's sequence lies
+template <typename T>
+__device__ __forceinline__ const T* token(const void* base, const SeqWalk& q, int64_t sb, int64_t st, int t) {
+  return (const T*)base + (q.off ? t * st : q.s * sb + (t - q.b) * st);
+}
+
+// the input at position t of the walk's sequence, t >= b - (W-1): a token, or what was carried in
+template <typename T, int V, int W>
+__device__ __forceinline__ void load_input(const ConvArgs& p, const SeqWalk& q, int t, int d, float (&v)[V]) {
+  if (t >= q.b) load_pack<T, V>(token<T>(p.x, q, p.x_sb, p.x_st, t) + d, v);
+  else if (p.state0) load_pack<T, V>((const T*)p.state0 + ((int64_t)q.s * (W - 1) + (t - q.b + W - 1)) * p.D + d, v);
+  else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = 0.f;
+  }
+}
+
+template <int V, int W>
+__device__ __forceinline__ void load_weights(const ConvArgs& p, int d, float (&w)[W][V], float (&bias)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    bias[i] = p.bias ? p.bias[d + i] : 0.f;
+#pragma unroll
+    for (int k = 0; k < W; ++k) w[k][i] = p.w[(int64_t)(d + i) * W + k];
+  }
+}
+
+template <typename T, int V, int W>
+__global__ void __launch_bounds__(256) conv_fwd_kernel(ConvArgs p) {
+  const int d = ((int)(blockIdx.x % p.tiles) * 64 + (threadIdx.x & 63)) * V;
+  const int t0 = ((int)(blockIdx.x / p.tiles) * 4 + uniform(threadIdx.x >> 6)) * CONV_TB;
+  if (t0 >= p.tokens || d >= p.D) return;
+  const int t1 = min(t0 + CONV_TB, p.tokens);
+  float w[W][V], bias[V], win[W][V];
+  load_weights<V, W>(p, d, w, bias);
+  SeqWalk q = {p.offsets, p.S, p.L, p.tokens, 0, 0, 0};
+  q.seek(t0);
+  if (q.s < q.S && q.b < t0) {
+#pragma unroll
+    for (int k = 1; k < W; ++k) load_input<T, V, W>(p, q, t0 - W + k, d, win[k]);
+  }
+  T* out = (T*)p.out + d;
+#pragma unroll 1
+  for (int t = t0; t < t1; ++t) {
+    if (q.s >= q.S || t < q.b) {
+      const float zero[V] = {};
+      store_pack<T, V>(out + (int64_t)t * p.D, zero);
+      continue;
+    }
+    if (t == q.b) {
+#pragma unroll
+      for (int k = 1; k < W; ++k) load_input<T, V, W>(p, q, t - W + k, d, win[k]);
+    }
+#pragma unroll
+    for (int k = 0; k + 1 < W; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i) win[k][i] = win[k + 1][i];
+    load_pack<T, V>(token<T>(p.x, q, p.x_sb, p.x_st, t) + d, win[W - 1]);
+    float y[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      y[i] = bias[i];
+#pragma unroll
+      for (int k = 0; k < W; ++k) y[i] = fmaf(w[k][i], win[k][i], y[i]);
+      if (p.silu) y[i] *= sigmoid_hw(y[i]);
+    }
+    store_pack<T, V>(out + (int64_t)t * p.D, y);
+    if (t + 1 == q.e) {
+      if (p.state1) {
+#pragma unroll
+        for (int k = 1; k < W; ++k)
+          store_pack<T, V>((T*)p.state1 + ((int64_t)q.s * (W - 1) + k - 1) * p.D + d, win[k]);
+      }
+      q.next(t + 1);
+    }
+  }
+}
+
+// gradient of the value before the activation at token t of the walk's sequence; the window ends up in win
+template <typename T, int V, int W>
+__device__ __forceinline__ void grad_pre(const ConvArgs& p, const float (&w)[W][V], const float (&bias)[V],
+                                         const float (&win)[W][V], const float (&g)[V], float (&dp)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    dp[i] = g[i];
+    if (p.silu) {
+      float y = bias[i];
+#pragma unroll
+      for (int k = 0; k < W; ++k) y = fmaf(w[k][i], win[k][i], y);
+      const float s = sigmoid_hw(y);
+      dp[i] *= s * fmaf(y, 1.f - s, 1.f);
+    }
+  }
+}
+
+// dx[t] = sum_k w[k] dpre[t + (W-1) - k] over the tokens of the same sequence; dw[k] = sum_t dpre[t] x[t - (W-1) + k].
+// A wave runs W - 1 tokens past its own, whose dpre its last tokens need.
+template <typename T, int V, int W>
+__global__ void __launch_bounds__(256) conv_bwd_kernel(ConvArgs p) {
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int d0 = ((int)(blockIdx.x % p.tiles) * 64 + lane) * V;
+  const bool on = d0 < p.D;
+  const int d = on ? d0 : 0;
+  const int t0 = ((int)(blockIdx.x / p.tiles) * 4 + wave) * CONV_TB;
+  const int t1 = min(t0 + CONV_TB, p.tokens);
+  float w[W][V], bias[V], win[W][V] = {}, acc[W][V] = {}, dw[W][V] = {}, db[V] = {};
+  if (t0 < p.tokens) {
+    load_weights<V, W>(p, d, w, bias);
+    SeqWalk q = {p.offsets, p.S, p.L, p.tokens, 0, 0, 0};
+    q.seek(t0);
+    if (q.s < q.S && q.b < t0) {
+#pragma unroll
+      for (int k = 1; k < W; ++k) load_input<T, V, W>(p, q, t0 - W + k, d, win[k]);
+    }
+#pragma unroll 1
+    for (int t = t0; t < t1 + W - 1; ++t) {
+      if (t < p.tokens && q.s < q.S && t >= q.b) {
+        if (t == q.b) {
+#pragma unroll
+          for (int k = 1; k < W; ++k) load_input<T, V, W>(p, q, t - W + k, d, win[k]);
+        }
+#pragma unroll
+        for (int k = 0; k + 1 < W; ++k)
+#pragma unroll
+          for (int i = 0; i < V; ++i) win[k][i] = win[k + 1][i];
+        load_pack<T, V>(token<T>(p.x, q, p.x_sb, p.x_st, t) + d, win[W - 1]);
+        float g[V], dp[V];
+        load_pack<T, V>(token<T>(p.dout, q, p.dout_sb, p.dout_st, t) + d, g);
+        grad_pre<T, V, W>(p, w, bias, win, g, dp);
+#pragma unroll
+        for (int k = 0; k < W; ++k)
+          if (t - (W - 1) + k >= q.b) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) acc[k][i] = fmaf(w[k][i], dp[i], acc[k][i]);
+          }
+        if (p.dstate1 && t >= q.e - (W - 1)) {
+          float c[V];
+          load_pack<T, V>((const T*)p.dstate1 + ((int64_t)q.s * (W - 1) + t - q.e + W - 1) * p.D + d, c);
+#pragma unroll
+          for (int i = 0; i < V; ++i) acc[W - 1][i] += c[i];
+        }
+        if (t < t1) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            db[i] += dp[i];
+#pragma unroll
+            for (int k = 0; k < W; ++k) dw[k][i] = fmaf(dp[i], win[k][i], dw[k][i]);
+          }
+        }
+        if (t + 1 == q.e) q.next(t + 1);
+      }
+      if (t - (W - 1) >= t0 && on) store_pack<T, V>((T*)p.dx + (int64_t)(t - (W - 1)) * p.D + d, acc[0]);
+#pragma unroll
+      for (int k = 0; k < W; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[k][i] = k + 1 < W ? acc[k + 1 < W ? k + 1 : k][i] : 0.f;
+    }
+  }
+  __shared__ float red[3][(W + 1) * V][64];
+  if (wave > 0) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+#pragma unroll
+      for (int k = 0; k < W; ++k) red[wave - 1][k * V + i][lane] = dw[k][i];
+      red[wave - 1][W * V + i][lane] = db[i];
+    }
+  }
+  __syncthreads();
+  if (wave == 0 && on) {
+    float* q = p.part + (int64_t)(blockIdx.x / p.tiles) * (W + 1) * p.D + d;
+#pragma unroll
+    for (int k = 0; k <= W; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        float s = k < W ? dw[k < W ? k : 0][i] : db[i];
+        for (int o = 0; o < 3; ++o) s += red[o][k * V + i][lane];
+        q[(int64_t)k * p.D + i] = s;
+      }
+  }
+}
+
+// dw [D][W] and dbias [D]: the sums of the partial rows, in their order
+__global__ void __launch_bounds__(256) conv_params_kernel(const float* part, float* dw, float* dbias, int parts, int W,
+                                                          int D) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= (W + 1) * D) return;
+  float s = 0.f;
+  for (int k = 0; k < parts; ++k) s += part[(int64_t)k * (W + 1) * D + i];
+  const int k = i / D, d = i % D;
+  if (k < W) { if (dw) dw[(int64_t)d * W + k] = s; }
+  else if (dbias) dbias[d] = s;
+}
+
+// the gradient of the carried inputs: row j of a sequence's state reaches the tokens p <= j with tap j - p, and the
+// final state where the sequence is shorter than the window
+template <typename T, int W>
+__global__ void __launch_bounds__(256) conv_dstate_kernel(ConvArgs p) {
+  const int d = (int)(blockIdx.x % p.tiles) * 256 + threadIdx.x;
+  SeqWalk q = {p.offsets, p.S, p.L, p.tokens, (int)(blockIdx.x / p.tiles), 0, 0};
+  q.load();
+  if (d >= p.D || q.e <= q.b) return;
+  float w[W][1], bias[1], ds[W] = {};
+  load_weights<1, W>(p, d, w, bias);
+#pragma unroll
+  for (int j = 0; j < W - 1; ++j) {
+    if (q.b + j >= q.e) continue;
+    float win[W][1], g[1], dp[1];
+#pragma unroll
+    for (int k = 0; k < W; ++k) load_input<T, 1, W>(p, q, q.b + j - (W - 1) + k, d, win[k]);
+    load_pack<T, 1>(token<T>(p.dout, q, p.dout_sb, p.dout_st, q.b + j) + d, g);
+    grad_pre<T, 1, W>(p, w, bias, win, g, dp);
+#pragma unroll
+    for (int r = j; r < W - 1; ++r) ds[r] = fmaf(w[r - j][0], dp[0], ds[r]);
+  }
+#pragma unroll
+  for (int r = 0; r < W - 1; ++r) {
+    const int from = r - (q.e - q.b);
+    if (p.dstate1 && from >= 0) ds[r] += to_f32(((const T*)p.dstate1)[((int64_t)q.s * (W - 1) + from) * p.D + d]);
+    ((T*)p.dstate0)[((int64_t)q.s * (W - 1) + r) * p.D + d] = from_f32<T>(ds[r]);
+  }
+}
+
+template <typename T, int V, int W>
+__global__ void __launch_bounds__(256) conv_step_kernel(ConvArgs p) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int per = p.D / V;
+  if (i >= (int64_t)p.tokens * per) return;
+  const int row = (int)(i / per), d = (int)(i % per) * V;
+  float w[W][V], bias[V], win[W][V], y[V];
+  load_weights<V, W>(p, d, w, bias);
+  T* st = (T*)p.state1 + (int64_t)row * (W - 1) * p.D + d;
+#pragma unroll
+  for (int k = 0; k + 1 < W; ++k) load_pack<T, V>(st + (int64_t)k * p.D, win[k]);
+  load_pack<T, V>((const T*)p.x + row * p.x_sb + d, win[W - 1]);
+#pragma unroll
+  for (int i2 = 0; i2 < V; ++i2) {
+    y[i2] = bias[i2];
+#pragma unroll
+    for (int k = 0; k < W; ++k) y[i2] = fmaf(w[k][i2], win[k][i2], y[i2]);
+    if (p.silu) y[i2] *= sigmoid_hw(y[i2]);
+  }
+  store_pack<T, V>((T*)p.out + (int64_t)row * p.D + d, y);
+#pragma unroll
+  for (int k = 0; k + 1 < W; ++k) store_pack<T, V>(st + (int64_t)k * p.D, win[k + 1]);
+}
+
+// ------------------------------------------------------------------------------------------------ host side
+static int conv_check(const char* what, int64_t rows, int64_t L, int64_t D, int64_t W, int64_t S,
+                      const int32_t* offsets, int dtype) {
+  DVAE_REQUIRE(dtype == DVAE_DT_F32 || dtype == DVAE_DT_BF16, "%s: dtype must be fp32 (0) or bf16 (1)", what);
+  DVAE_REQUIRE(W >= 2 && W <= 4, "%s: 2 to 4 taps, got %ld", what, (long)W);
+  DVAE_REQUIRE(rows >= 0 && L >= 0 && D > 0 && D < (1ll << 24), "%s: bad shape", what);
+  DVAE_REQUIRE(rows < (1ll << 31) && L < (1ll << 31) && rows * L < (1ll << 31) - 64, "%s: too many tokens", what);
+  DVAE_REQUIRE(!offsets || (rows == 1 && S >= 1 && S < (1ll << 30)), "%s: offsets go with one row and S >= 1", what);
+  return 0;
+}
+
+// 16 bytes per lane where every row of every tensor starts on 16 bytes, else one element
+static bool conv_wide(int64_t D, int dtype, const void* a, int64_t a_sb, int64_t a_st, const void* b, int64_t b_sb,
+                      int64_t b_st, const void* c, const void* d, const void* e) {
+  const int64_t V = dtype == DVAE_DT_F32 ? 4 : 8;
+  const uintptr_t ptrs = (uintptr_t)a | (uintptr_t)b | (uintptr_t)c | (uintptr_t)d | (uintptr_t)e;
+  return !(ptrs & 15) && !((D | a_sb | a_st | b_sb | b_st) & (V - 1));
+}
+
+#define CONV_W(K, T, V, W, grid, p, s)                                                     \
+  do {                                                                                     \
+    if (W == 2) DVAE_LAUNCH((K<T, V, 2>), grid, dim3(256), 0, s, p);                       \
+    else if (W == 3) DVAE_LAUNCH((K<T, V, 3>), grid, dim3(256), 0, s, p);                  \
+    else DVAE_LAUNCH((K<T, V, 4>), grid, dim3(256), 0, s, p);                              \
+  } while (0)
+#define CONV_DISPATCH(K, dtype, wide, W, grid, p, s)                                       \
+  do {                                                                                     \
+    if (dtype == DVAE_DT_F32) {                                                            \
+      if (wide) CONV_W(K, float, 4, W, grid, p, s); else CONV_W(K, float, 1, W, grid, p, s); \
+    } else {                                                                               \
+      if (wide) CONV_W(K, bf16_t, 8, W, grid, p, s); else CONV_W(K, bf16_t, 1, W, grid, p, s); \
+    }                                                                                      \
+  } while (0)
+
+static int conv_v(int dtype, bool wide) { return !wide ? 1 : dtype == DVAE_DT_F32 ? 4 : 8; }
+
+extern "C" int dvae_short_conv_fwd(const void* x, int64_t x_sb, int64_t x_st, const float* w, const float* bias, int silu,
+                                   const void* state0, void* state1, const int32_t* offsets, void* out, int64_t rows,
+                                   int64_t L, int64_t D, int64_t W, int64_t S, int dtype, dvae_stream_t stream) {
+  const int rc = conv_check("short_conv_fwd", rows, L, D, W, S, offsets, dtype);
+  if (rc) return rc;
+  if (rows * L == 0) return 0;
+  ConvArgs p = {};
+  p.x = x; p.x_sb = x_sb; p.x_st = x_st; p.w = w; p.bias = bias; p.silu = silu; p.state0 = state0; p.state1 = state1;
+  p.offsets = offsets; p.out = out; p.D = (int)D; p.S = (int)(offsets ? S : rows); p.L = (int)L;
+  p.tokens = (int)(rows * L);
+  const bool wide = conv_wide(D, dtype, x, x_sb, x_st, nullptr, 0, 0, state0, state1, out);
+  p.tiles = (int)ceil_div64(D, 64 * conv_v(dtype, wide));
+  const int64_t grid = p.tiles * ceil_div64(p.tokens, 4 * CONV_TB);
+  DVAE_REQUIRE(grid < (1ll << 31), "short_conv_fwd: too large");
+  const int e = dtype == DVAE_DT_F32 ? 4 : 2;
+  DVAE_WORK(2.0 * p.tokens * D * e, DVAE_UNIT_BYTE);
+  CONV_DISPATCH(conv_fwd_kernel, dtype, wide, W, dim3((unsigned)grid), p, ST(stream));
+  DVAE_LAUNCH_CHECK("short_conv_fwd");
+  return 0;
+}
+
+extern "C" int64_t dvae_short_conv_bwd_ws_floats(int64_t rows, int64_t L, int64_t D, int64_t W) {
+  return ceil_div64(rows * L, 4 * CONV_TB) * (W + 1) * D;
+}
+
+extern "C" int dvae_short_conv_bwd(const void* x, int64_t x_sb, int64_t x_st, const float* w, const float* bias, int silu,
+                                   const void* state0, const int32_t* offsets, const void* dout, int64_t dout_sb,
+                                   int64_t dout_st, const void* dstate1, void* dx, float* dw, float* dbias,
+                                   void* dstate0, int64_t rows, int64_t L, int64_t D, int64_t W, int64_t S, int dtype,
+                                   float* ws, dvae_stream_t stream) {
+  const int rc = conv_check("short_conv_bwd", rows, L, D, W, S, offsets, dtype);
+  if (rc) return rc;
+  DVAE_REQUIRE(rows * L > 0, "short_conv_bwd: no tokens");
+  ConvArgs p = {};
+  p.x = x; p.x_sb = x_sb; p.x_st = x_st; p.w = w; p.bias = bias; p.silu = silu; p.state0 = state0; p.offsets = offsets;
+  p.dout = dout; p.dout_sb = dout_sb; p.dout_st = dout_st; p.dstate1 = dstate1; p.dx = dx; p.dstate0 = dstate0;
+  p.D = (int)D; p.S = (int)(offsets ? S : rows); p.L = (int)L; p.tokens = (int)(rows * L); p.part = ws;
+  const bool wide = conv_wide(D, dtype, x, x_sb, x_st, dout, dout_sb, dout_st, state0, dstate1, dx);
+  p.tiles = (int)ceil_div64(D, 64 * conv_v(dtype, wide));
+  const int64_t parts = ceil_div64(p.tokens, 4 * CONV_TB);
+  DVAE_REQUIRE(p.tiles * parts < (1ll << 31), "short_conv_bwd: too large");
+  const int e = dtype == DVAE_DT_F32 ? 4 : 2;
+  DVAE_WORK(3.0 * p.tokens * D * e, DVAE_UNIT_BYTE);
+  CONV_DISPATCH(conv_bwd_kernel, dtype, wide, W, dim3((unsigned)(p.tiles * parts)), p, ST(stream));
+  DVAE_LAUNCH_CHECK("short_conv_bwd");
+  DVAE_LAUNCH(conv_params_kernel, dim3((unsigned)ceil_div64((W + 1) * D, 256)), dim3(256), 0, ST(stream), ws, dw, dbias,
+              (int)parts, (int)W, (int)D);
+  if (dstate0) {
+    p.tiles = (int)ceil_div64(D, 256);
+    DVAE_REQUIRE((int64_t)p.tiles * p.S < (1ll << 31), "short_conv_bwd: too many sequences");
+    const dim3 grid((unsigned)(p.tiles * p.S));
+#define CONV_DSTATE(T)                                                                     \
+  do {                                                                                     \
+    if (W == 2) DVAE_LAUNCH((conv_dstate_kernel<T, 2>), grid, dim3(256), 0, ST(stream), p); \
+    else if (W == 3) DVAE_LAUNCH((conv_dstate_kernel<T, 3>), grid, dim3(256), 0, ST(stream), p); \
+    else DVAE_LAUNCH((conv_dstate_kernel<T, 4>), grid, dim3(256), 0, ST(stream), p);       \
+  } while (0)
+    if (dtype == DVAE_DT_F32) CONV_DSTATE(float); else CONV_DSTATE(bf16_t);
+  }
+  DVAE_LAUNCH_CHECK("short_conv_bwd: sums");
+  return 0;
+}
+
+extern "C" int dvae_short_conv_step(void* state, const void* x, int64_t x_sb, const float* w, const float* bias, int silu,
+                                    void* out, int64_t rows, int64_t D, int64_t W, int dtype, dvae_stream_t stream) {
+  const int rc = conv_check("short_conv_step", rows, 1, D, W, rows, nullptr, dtype);
+  if (rc) return rc;
+  if (rows == 0) return 0;
+  ConvArgs p = {};
+  p.x = x; p.x_sb = x_sb; p.w = w; p.bias = bias; p.silu = silu; p.state1 = state; p.out = out; p.D = (int)D;
+  p.tokens = (int)rows;
+  const bool wide = conv_wide(D, dtype, x, x_sb, 0, nullptr, 0, 0, state, out, nullptr);
+  const int64_t grid = ceil_div64(rows * (D / conv_v(dtype, wide)), 256);
+  DVAE_REQUIRE(grid < (1ll << 31), "short_conv_step: too large");
+  DVAE_WORK((2.0 * W) * rows * D * (dtype == DVAE_DT_F32 ? 4 : 2), DVAE_UNIT_BYTE);
+  CONV_DISPATCH(conv_step_kernel, dtype, wide, W, dim3((unsigned)grid), p, ST(stream));
+  DVAE_LAUNCH_CHECK("short_conv_step");
+  return 0;
+}

@@ -122,6 +122,21 @@ SIGNATURES = {
     'dvae_copy_tensors_f32': (I, [L, POINTER(c_void_p), POINTER(c_void_p), POINTER(c_int64), P]),
     'dvae_adam_step_f32': (I, [L, POINTER(c_void_p), POINTER(c_void_p), POINTER(c_void_p), POINTER(c_void_p),
                                POINTER(c_int64), F, F, F, F, F, F, F, P, P, P]),
+    'dvae_selective_scan_ckpt_floats': (L, [L] * 4),
+    'dvae_selective_scan_fwd': (I, [P, L, L, P, L, L, P, P, L, L, L, P, L, L, L, P, P, L, L, P, I, P, P, P, P, P] + [L] * 6
+                                + [I, P]),
+    'dvae_selective_scan_bwd_ws_floats': (L, [L] * 5),
+    'dvae_selective_scan_bwd': (I, [P, L, L, P, L, L, P, P, L, L, L, P, L, L, L, P, P, L, L, P, I, P, P, P, L, L, P, P]
+                                + [P] * 9 + [L] * 6 + [I, P, P]),
+    'dvae_selective_scan_step': (I, [P, P, L, P, L, P, P, L, L, P, L, L, P, P, L, P, I, P] + [L] * 4 + [I, P]),
+    'dvae_short_conv_fwd': (I, [P, L, L, P, P, I, P, P, P, P] + [L] * 5 + [I, P]),
+    'dvae_short_conv_bwd_ws_floats': (L, [L] * 4),
+    'dvae_short_conv_bwd': (I, [P, L, L, P, P, I, P, P, P, L, L, P, P, P, P, P] + [L] * 5 + [I, P, P]),
+    'dvae_short_conv_step': (I, [P, P, L, P, P, I, P, L, L, L, I, P]),
+    'dvae_add_rms_norm_fwd': (I, [P, L, P, L, P, F, P, P, P, L, L, I, I, P]),
+    'dvae_add_rms_norm_q8': (I, [P, L, P, L, P, F, P, P, P, L, L, I, I, P]),
+    'dvae_add_rms_norm_bwd_ws_floats': (L, [L, L]),
+    'dvae_add_rms_norm_bwd': (I, [P, L, P, L, P, L, P, P, P, P, P, L, L, I, I, P, P]),
     'dvae_trace_begin': (I, [L]),
     'dvae_trace_end': (L, []),
     'dvae_trace_read': (I, [L, ctypes.c_char_p, L, POINTER(c_float), POINTER(c_double), POINTER(c_int)]),

@@ -9,6 +9,8 @@ libdvae_hip.so in both directions:
   LSTMEncoder  (bi)directional multi-layer LSTM over a sequence, returns the final hidden states
   LSTMDecoder  autoregressive multi-layer LSTM (x_t = top-layer h_{t-1})
   Reparam      z = mu + eps * exp(logvar / 2)
+  selective_scan, short_conv (+ their one-token steps), add_rms_norm (+ its 8-bit output): the operators of a selective
+               state-space layer, channels-last over [batch, length, channels] or packed [tokens, channels]
 
 Activations are NHWC with frames folded into the leading dimension; a layer's BatchNorm +
 LeakyReLU is never materialised between conv layers: the conv kernel writes the raw output plus
@@ -987,3 +989,163 @@ class LSTMDecoder(torch.autograd.Function):
             grads[4 * l + 2] = db
             grads[4 * l + 3] = db.clone()
         return (dh0, dc0, dinit, None, None, *grads)
+
+
+# ------------------------------------------------------------------------------------------------ sequence operators
+def _wants_grad(*ts: Optional[Tensor]) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
+class SelectiveScan(torch.autograd.Function):
+    """see selective_scan"""
+
+    @staticmethod
+    def forward(ctx, u, delta, A, B, C, D, z, delta_bias, delta_softplus, state, offsets, want_state):
+        a = ops.ScanArgs('selective_scan', u, delta, A, B, C, D, z, delta_bias, delta_softplus, state, offsets)
+        out, final, ckpt = ops.selective_scan_fwd(a, want_state, True)
+        ctx.save_for_backward(u, delta, A, B, C, D, z, delta_bias, state, offsets, ckpt)
+        ctx.delta_softplus = delta_softplus
+        ctx.set_materialize_grads(False)
+        return out, final
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout, dfinal):
+        u, delta, A, B, C, D, z, bias, state, offsets, ckpt = ctx.saved_tensors
+        a = ops.ScanArgs('selective_scan', u, delta, A, B, C, D, z, bias, ctx.delta_softplus, state, offsets)
+        if dout is None:
+            dout = torch.zeros(u.shape, dtype=u.dtype, device=u.device)
+        need = ctx.needs_input_grad
+        du, dd, dA, dB, dC, dD, dz, db, ds = ops.selective_scan_bwd(a, dout, dfinal, ckpt, need[9])
+        grads = [du, dd, dA, dB.view(B.shape), dC.view(C.shape), dD, dz, db, None, ds]
+        return tuple(g if n else None for g, n in zip(grads, need)) + (None, None)
+
+
+def selective_scan(u: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: Tensor, D: Optional[Tensor] = None,
+                   z: Optional[Tensor] = None, delta_bias: Optional[Tensor] = None, delta_softplus: bool = False,
+                   state: Optional[Tensor] = None, offsets: Optional[Tensor] = None, return_state: bool = False):
+    """The selective state-space recurrence over a sequence: with dt = softplus(delta + delta_bias) (without
+    delta_softplus: delta + delta_bias),
+
+        h = exp(dt A) h + dt u B        out = (sum over states of C h + D u) * silu(z)
+
+    u, delta, z [batch, length, channels] fp32 or bf16; A [channels, states], at most 16 states; B, C [batch, length,
+    groups, states] (or without the group dimension), groups dividing the channels; D, delta_bias [channels]; parameters
+    and states fp32.  Any strides: only the last dimension of an activation is copied if it is not contiguous.
+
+    `offsets` (int32, ascending, first 0): sequences of different lengths, some possibly empty, packed one after the
+    other into [tokens, channels]; sequence s is tokens offsets[s] to offsets[s + 1].  Tokens behind the last sequence
+    get 0, and gradients of 0.  The offsets are read on the device only and not checked.
+    `state` [sequences, channels, states]: what the sequences start from (default zeros); it is not modified.
+    `return_state`: also returns the final states.  Gradients flow to every tensor argument and through both states."""
+    if _wants_grad(u, delta, A, B, C, D, z, delta_bias, state):
+        out, final = SelectiveScan.apply(u, delta, A, B, C, D, z, delta_bias, delta_softplus, state, offsets, return_state)
+    else:
+        a = ops.ScanArgs('selective_scan', u, delta, A, B, C, D, z, delta_bias, delta_softplus, state, offsets)
+        out, final, _ = ops.selective_scan_fwd(a, return_state, False)
+    return (out, final) if return_state else out
+
+
+def selective_scan_step(state: Tensor, u: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: Tensor,
+                        D: Optional[Tensor] = None, z: Optional[Tensor] = None, delta_bias: Optional[Tensor] = None,
+                        delta_softplus: bool = False) -> Tensor:
+    """selective_scan for one token per sequence, u [rows, channels], B and C [rows, groups, states]: `state` [rows,
+    channels, states] is updated in place.  For inference: no gradients."""
+    _no_grad_form('selective_scan_step', state, u, delta, A, B, C, D, z, delta_bias)
+    return ops.selective_scan_step(state, u, delta, A, B, C, D, z, delta_bias, delta_softplus)
+
+
+def _no_grad_form(what: str, *ts):
+    if _wants_grad(*ts):
+        raise RuntimeError(f"{what} computes no gradients: call it under torch.no_grad()")
+
+
+class ShortConv(torch.autograd.Function):
+    """see short_conv"""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, silu, state, offsets, want_state):
+        out, final = ops.short_conv_fwd(ops.ConvArgs('short_conv', x, weight, bias, silu, state, offsets), want_state)
+        ctx.save_for_backward(x, weight, bias, state, offsets)
+        ctx.silu = silu
+        ctx.set_materialize_grads(False)
+        return out, final
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout, dfinal):
+        x, weight, bias, state, offsets = ctx.saved_tensors
+        a = ops.ConvArgs('short_conv', x, weight, bias, ctx.silu, state, offsets)
+        if dout is None:
+            dout = torch.zeros(x.shape, dtype=x.dtype, device=x.device)
+        need = ctx.needs_input_grad
+        dx, dw, db, ds = ops.short_conv_bwd(a, dout, dfinal, need[4])
+        return tuple(g if n else None for g, n in zip((dx, dw, db, None, ds), need)) + (None, None)
+
+
+def short_conv(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, silu: bool = False,
+               state: Optional[Tensor] = None, offsets: Optional[Tensor] = None, return_state: bool = False):
+    """Depthwise causal convolution over time: out[t] = bias + sum_k weight[:, k] x[t - (taps - 1) + k] within a
+    sequence, through silu if asked.  x [batch, length, channels] fp32 or bf16, weight [channels, taps] with 2 to 4 taps,
+    bias [channels], both fp32.  `state` [sequences, taps - 1, channels] of x's type holds the inputs before a sequence's
+    first token (default zeros); `return_state` also returns the last taps - 1 inputs of every sequence.  `offsets` as in
+    selective_scan.  Gradients flow to every tensor argument and through both states."""
+    if _wants_grad(x, weight, bias, state):
+        out, final = ShortConv.apply(x, weight, bias, silu, state, offsets, return_state)
+    else:
+        out, final = ops.short_conv_fwd(ops.ConvArgs('short_conv', x, weight, bias, silu, state, offsets), return_state)
+    return (out, final) if return_state else out
+
+
+def short_conv_step(state: Tensor, x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, silu: bool = False) -> Tensor:
+    """short_conv for one token per sequence, x [rows, channels]: `state` [rows, taps - 1, channels] is updated in place.
+    For inference: no gradients."""
+    _no_grad_form('short_conv_step', state, x, weight, bias)
+    return ops.short_conv_step(state, x, weight, bias, silu)
+
+
+class AddRMSNorm(torch.autograd.Function):
+    """see add_rms_norm"""
+
+    @staticmethod
+    def forward(ctx, x, residual, weight, eps):
+        a = ops.NormArgs('add_rms_norm', x, residual, weight)
+        y, total, rstd = ops.add_rms_norm_fwd(a, eps, True)
+        ctx.save_for_backward(total, a.weight, rstd)
+        ctx.x_dtype = x.dtype
+        ctx.set_materialize_grads(False)
+        if residual is None:
+            return y.view(x.shape)
+        return y.view(x.shape), total.view(x.shape)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dsum=None):
+        total, weight, rstd = ctx.saved_tensors
+        if dy is None:
+            if dsum is None:
+                return None, None, None, None
+            dy = torch.zeros(dsum.shape, dtype=ctx.x_dtype, device=dsum.device)
+        dx, dres, dw = ops.add_rms_norm_bwd(dy, dsum, total, weight, rstd, ctx.x_dtype)
+        need = ctx.needs_input_grad
+        return dx if need[0] else None, dres if need[1] else None, dw if need[2] else None, None
+
+
+def add_rms_norm(x: Tensor, residual: Optional[Tensor], weight: Tensor, eps: float = 1e-6):
+    """-> (y, sum): sum = x + residual, y = sum / sqrt(mean(sum^2) + eps) * weight over the last dimension.  x [...,
+    channels] fp32 or bf16, y of its type; residual of the same type or fp32 (a residual stream kept in fp32 beside bf16
+    activations), sum of the residual's; weight [channels] fp32.  The norm is that of the sum as stored.  Without a
+    residual the sum is x itself."""
+    if _wants_grad(x, residual, weight):
+        got = AddRMSNorm.apply(x, residual, weight, eps)
+        return (got, x) if residual is None else got
+    y, total, _ = ops.add_rms_norm_fwd(ops.NormArgs('add_rms_norm', x, residual, weight), eps, False)
+    return y.view(x.shape), x if residual is None else total.view(x.shape)
+
+
+def add_rms_norm_q8(x: Tensor, residual: Optional[Tensor], weight: Tensor, eps: float = 1e-6):
+    """add_rms_norm with y in 8 bits: -> (q, scale, sum), y = q * scale[..., None] with q of type float8_e4m3fn and
+    scale = max|y| / 448 of its row, so that the row's largest value is the type's largest (a row of zeros: 1).  For
+    inference: no gradients."""
+    _no_grad_form('add_rms_norm_q8', x, residual, weight)
+    return ops.add_rms_norm_q8(x, residual, weight, eps)

@@ -1053,6 +1053,373 @@ def adam_advance(dyn: Tensor, beta1: float, beta2: float):
     check(lib.dvae_adam_advance_f32(_p(dyn), float(beta1), float(beta2), _stream()), 'adam_advance')
 
 
+# ---------------------------------------------------------------------------- sequence operators
+# Activations are fp32 or bf16, channels contiguous, other strides free; parameters and states fp32.  Scratch comes
+# from torch's allocator per call, on the current stream: nothing is shared between streams or captured graphs.
+_ACT_DTYPES = {torch.float32: 0, torch.bfloat16: 1}
+
+
+class _On:
+    """Makes a tensor's device current for a call where it is not."""
+
+    def __init__(self, t: Tensor):
+        self.guard = torch.cuda.device(t.device) if t.device.index != torch.cuda.current_device() else None
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+        return False
+
+
+def _act_dtype(what: str, t: Tensor) -> int:
+    if not t.is_cuda:
+        raise RuntimeError(f"{what}: input is on {t.device}; hipvae ops need tensors on the GPU (no CPU path exists)")
+    code = _ACT_DTYPES.get(t.dtype)
+    if code is None:
+        raise RuntimeError(f"{what}: activations must be fp32 or bf16, got {t.dtype}")
+    return code
+
+
+def _act(what: str, name: str, t: Optional[Tensor], shape, like: Tensor) -> Optional[Tensor]:
+    """checks an activation; a copy where its last dimension is not contiguous"""
+    if t is None:
+        return None
+    if t.shape != shape:
+        raise RuntimeError(f"{what}: {name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if t.dtype != like.dtype or t.device != like.device:
+        raise RuntimeError(f"{what}: {name} is {t.dtype} on {t.device}, expected {like.dtype} on {like.device}")
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+
+
+def _param(what: str, name: str, t: Optional[Tensor], shape, like: Tensor, dtype=torch.float32) -> Optional[Tensor]:
+    """checks a parameter or state; contiguous"""
+    if t is None:
+        return None
+    if t.shape != shape:
+        raise RuntimeError(f"{what}: {name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if t.dtype != dtype or t.device != like.device:
+        raise RuntimeError(f"{what}: {name} is {t.dtype} on {t.device}, expected {dtype} on {like.device}")
+    return t.contiguous()
+
+
+def _in_place(what: str, t: Tensor, shape, like: Tensor, dtype=torch.float32) -> None:
+    if t.shape != shape or t.dtype != dtype or t.device != like.device or not t.is_contiguous():
+        raise RuntimeError(f"{what}: the state is updated in place: it must be a contiguous {dtype} tensor of shape "
+                           f"{tuple(shape)} on {like.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+def _sequence_form(what: str, x: Tensor, offsets: Optional[Tensor]):
+    """[B, L, D], or with offsets [T, D] -> (leading shape, rows, length, channels, sequences)"""
+    if offsets is None:
+        if x.dim() != 3:
+            raise RuntimeError(f"{what}: expected [batch, length, channels], got {tuple(x.shape)}")
+        B, L, D = x.shape
+        rows, S = B, B
+    else:
+        if x.dim() != 2:
+            raise RuntimeError(f"{what}: with offsets, expected [tokens, channels], got {tuple(x.shape)}")
+        if offsets.dim() != 1 or offsets.numel() < 2 or offsets.dtype != torch.int32 or offsets.device != x.device \
+                or not offsets.is_contiguous():
+            raise RuntimeError(f"{what}: offsets must be a contiguous int32 tensor of at least two positions on {x.device}")
+        L, D = x.shape
+        rows, S = 1, offsets.numel() - 1
+    if D < 1:
+        raise RuntimeError(f"{what}: no channels")
+    return x.shape[:-1], rows, L, D, S
+
+
+def _st2(t: Optional[Tensor]):
+    """(sequence, token) strides of an activation in either form"""
+    if t is None:
+        return 0, 0
+    return (t.stride(0), t.stride(1)) if t.dim() == 3 else (0, t.stride(0))
+
+
+def _bc_form(what: str, name: str, t: Tensor, lead, like: Tensor) -> Tensor:
+    """B or C as [..., groups, states] with contiguous states"""
+    if t.dim() == len(lead) + 1:
+        t = t.unsqueeze(-2)
+    if t.dim() != len(lead) + 2:
+        raise RuntimeError(f"{what}: {name} has shape {tuple(t.shape)}, expected {tuple(lead)} + (groups, states)")
+    return _act(what, name, t, tuple(lead) + tuple(t.shape[-2:]), like)
+
+
+def _st3(t: Tensor):
+    return (t.stride(0), t.stride(1), t.stride(2)) if t.dim() == 4 else (0, t.stride(0), t.stride(1))
+
+
+class ScanArgs:
+    """The checked arguments of a selective scan, as both directions hand them to the library."""
+
+    def __init__(self, what, u, delta, A, B, C, D, z, delta_bias, delta_softplus, state, offsets):
+        self.dtype = _act_dtype(what, u)
+        self.lead, self.rows, self.L, ch, self.S = _sequence_form(what, u, offsets)
+        self.D = ch
+        if A.dim() != 2:
+            raise RuntimeError(f"{what}: A must be [channels, states], got {tuple(A.shape)}")
+        N = self.N = A.shape[1]
+        self.u = _act(what, 'u', u, u.shape, u)
+        self.delta = _act(what, 'delta', delta, u.shape, u)
+        self.z = _act(what, 'z', z, u.shape, u)
+        self.B = _bc_form(what, 'B', B, self.lead, u)
+        G = self.G = self.B.shape[-2]
+        self.C = _bc_form(what, 'C', C, self.lead, u)
+        if self.C.shape != self.B.shape or self.B.shape[-1] != N:
+            raise RuntimeError(f"{what}: B {tuple(B.shape)} and C {tuple(C.shape)} must both be [..., groups, {N}]")
+        if G < 1 or ch % G:
+            raise RuntimeError(f"{what}: {ch} channels do not divide into {G} groups")
+        self.A = _param(what, 'A', A, (ch, N), u)
+        self.Dp = _param(what, 'D', D, (ch,), u)
+        self.bias = _param(what, 'delta_bias', delta_bias, (ch,), u)
+        self.state = _param(what, 'state', state, (self.S, ch, N), u)
+        self.softplus = int(bool(delta_softplus))
+        self.offsets = offsets
+
+    def head(self):
+        return (_p(self.u), *_st2(self.u), _p(self.delta), *_st2(self.delta), _p(self.A), _p(self.B), *_st3(self.B),
+                _p(self.C), *_st3(self.C), _p(self.Dp), _p(self.z), *_st2(self.z), _p(self.bias), self.softplus,
+                _p(self.state))
+
+    def shape(self):
+        return self.rows, self.L, self.D, self.G, self.N, self.S, self.dtype
+
+
+def _final_like(state: Optional[Tensor], shape, like: Tensor, dtype, offsets, tokens: int) -> Tensor:
+    """where final states go.  Sequences without tokens are not written: they keep what they entered with."""
+    if offsets is None and tokens > 0:
+        return torch.empty(shape, dtype=dtype, device=like.device)
+    return torch.zeros(shape, dtype=dtype, device=like.device) if state is None else state.clone()
+
+
+def selective_scan_fwd(a: ScanArgs, want_state: bool, keep: bool):
+    """-> (out, final state or None, what the backward pass starts from or None)"""
+    with _On(a.u):
+        out = torch.empty(a.u.shape, dtype=a.u.dtype, device=a.u.device)
+        final = _final_like(a.state, (a.S, a.D, a.N), a.u, torch.float32, a.offsets, a.rows * a.L) if want_state else None
+        ckpt = torch.empty(int(lib.dvae_selective_scan_ckpt_floats(a.rows, a.L, a.D, a.N)), dtype=torch.float32,
+                           device=a.u.device) if keep else None
+        check(lib.dvae_selective_scan_fwd(*a.head(), _p(final), _p(a.offsets), _p(out), _p(ckpt), *a.shape(), _stream()),
+              'selective_scan_fwd')
+    return out, final, ckpt
+
+
+def selective_scan_bwd(a: ScanArgs, dout: Tensor, dfinal: Optional[Tensor], ckpt: Tensor, want_dstate: bool):
+    """-> du, ddelta, dA, dB, dC, dD, dz, ddelta_bias, dstate (None where there is no such input)"""
+    what = 'selective_scan_bwd'
+    dout = _act(what, 'dout', dout, a.u.shape, a.u)
+    dfinal = _param(what, 'dstate', dfinal, (a.S, a.D, a.N), a.u)
+    dev = a.u.device
+    act = dict(dtype=a.u.dtype, device=dev)
+    par = dict(dtype=torch.float32, device=dev)
+    with _On(a.u):
+        du, dd = torch.empty(a.u.shape, **act), torch.empty(a.u.shape, **act)
+        dz = None if a.z is None else torch.empty(a.u.shape, **act)
+        dB, dC = torch.empty(a.B.shape, **act), torch.empty(a.B.shape, **act)
+        if a.rows * a.L == 0:
+            zero = lambda t: None if t is None else torch.zeros(t.shape, **par)                      # noqa: E731
+            return du, dd, zero(a.A), dB, dC, zero(a.Dp), dz, zero(a.bias), dfinal if want_dstate else None
+        dA = torch.empty(a.A.shape, **par)
+        dD = None if a.Dp is None else torch.empty(a.D, **par)
+        db = None if a.bias is None else torch.empty(a.D, **par)
+        ds = _final_like(dfinal, (a.S, a.D, a.N), a.u, torch.float32, a.offsets, a.rows * a.L) if want_dstate else None
+        ws = torch.empty(int(lib.dvae_selective_scan_bwd_ws_floats(a.rows, a.L, a.D, a.G, a.N)), **par)
+        check(lib.dvae_selective_scan_bwd(*a.head(), _p(a.offsets), _p(dout), *_st2(dout), _p(dfinal), _p(ckpt), _p(du),
+                                          _p(dd), _p(dA), _p(dB), _p(dC), _p(dD), _p(dz), _p(db), _p(ds), *a.shape(),
+                                          _p(ws), _stream()), what)
+    return du, dd, dA, dB, dC, dD, dz, db, ds
+
+
+def selective_scan_step(state, u, delta, A, B, C, D=None, z=None, delta_bias=None, delta_softplus=False) -> Tensor:
+    """one token per sequence: u, delta, z [rows, channels], B, C [rows, groups, states]; `state` [rows, channels,
+    states] is updated in place -> out [rows, channels]"""
+    what = 'selective_scan_step'
+    dtype = _act_dtype(what, u)
+    if u.dim() != 2 or A.dim() != 2:
+        raise RuntimeError(f"{what}: expected u [rows, channels] and A [channels, states], got {tuple(u.shape)} and "
+                           f"{tuple(A.shape)}")
+    rows, ch = u.shape
+    N = A.shape[1]
+    _in_place(what, state, (rows, ch, N), u)
+    u = _act(what, 'u', u, u.shape, u)
+    delta = _act(what, 'delta', delta, u.shape, u)
+    z = _act(what, 'z', z, u.shape, u)
+    B, C = _bc_form(what, 'B', B, (rows,), u), _bc_form(what, 'C', C, (rows,), u)
+    G = B.shape[1]
+    if C.shape != B.shape or B.shape[2] != N or G < 1 or ch % G:
+        raise RuntimeError(f"{what}: B {tuple(B.shape)} and C {tuple(C.shape)} must both be [{rows}, groups, {N}], groups "
+                           f"dividing {ch} channels")
+    A = _param(what, 'A', A, (ch, N), u)
+    D = _param(what, 'D', D, (ch,), u)
+    delta_bias = _param(what, 'delta_bias', delta_bias, (ch,), u)
+    with _On(u):
+        out = torch.empty(rows, ch, dtype=u.dtype, device=u.device)
+        check(lib.dvae_selective_scan_step(_p(state), _p(u), u.stride(0), _p(delta), delta.stride(0), _p(A), _p(B),
+                                           B.stride(0), B.stride(1), _p(C), C.stride(0), C.stride(1), _p(D), _p(z),
+                                           0 if z is None else z.stride(0), _p(delta_bias), int(bool(delta_softplus)),
+                                           _p(out), rows, ch, G, N, dtype, _stream()), what)
+    return out
+
+
+class ConvArgs:
+    """The checked arguments of a short convolution."""
+
+    def __init__(self, what, x, weight, bias, silu, state, offsets):
+        self.dtype = _act_dtype(what, x)
+        self.lead, self.rows, self.L, self.D, self.S = _sequence_form(what, x, offsets)
+        if weight.dim() != 2 or not 2 <= weight.shape[1] <= 4:
+            raise RuntimeError(f"{what}: weight must be [channels, 2 to 4 taps], got {tuple(weight.shape)}")
+        self.W = weight.shape[1]
+        self.x = _act(what, 'x', x, x.shape, x)
+        self.weight = _param(what, 'weight', weight, (self.D, self.W), x)
+        self.bias = _param(what, 'bias', bias, (self.D,), x)
+        self.state = _param(what, 'state', state, (self.S, self.W - 1, self.D), x, x.dtype)
+        self.silu = int(bool(silu))
+        self.offsets = offsets
+
+    def head(self):
+        return _p(self.x), *_st2(self.x), _p(self.weight), _p(self.bias), self.silu, _p(self.state)
+
+    def shape(self):
+        return self.rows, self.L, self.D, self.W, self.S, self.dtype
+
+
+def short_conv_fwd(a: ConvArgs, want_state: bool):
+    with _On(a.x):
+        out = torch.empty(a.x.shape, dtype=a.x.dtype, device=a.x.device)
+        final = _final_like(a.state, (a.S, a.W - 1, a.D), a.x, a.x.dtype, a.offsets, a.rows * a.L) if want_state else None
+        check(lib.dvae_short_conv_fwd(*a.head(), _p(final), _p(a.offsets), _p(out), *a.shape(), _stream()),
+              'short_conv_fwd')
+    return out, final
+
+
+def short_conv_bwd(a: ConvArgs, dout: Tensor, dfinal: Optional[Tensor], want_dstate: bool):
+    """-> dx, dweight, dbias, dstate"""
+    what = 'short_conv_bwd'
+    dout = _act(what, 'dout', dout, a.x.shape, a.x)
+    shape = (a.S, a.W - 1, a.D)
+    dfinal = _param(what, 'dstate', dfinal, shape, a.x, a.x.dtype)
+    dev = a.x.device
+    with _On(a.x):
+        dx = torch.empty(a.x.shape, dtype=a.x.dtype, device=dev)
+        if a.rows * a.L == 0:
+            return (dx, torch.zeros(a.D, a.W, device=dev), None if a.bias is None else torch.zeros(a.D, device=dev),
+                    dfinal if want_dstate else None)
+        dw = torch.empty(a.D, a.W, dtype=torch.float32, device=dev)
+        db = None if a.bias is None else torch.empty(a.D, dtype=torch.float32, device=dev)
+        ds = _final_like(dfinal, shape, a.x, a.x.dtype, a.offsets, a.rows * a.L) if want_dstate else None
+        ws = torch.empty(int(lib.dvae_short_conv_bwd_ws_floats(a.rows, a.L, a.D, a.W)), dtype=torch.float32, device=dev)
+        check(lib.dvae_short_conv_bwd(*a.head(), _p(a.offsets), _p(dout), *_st2(dout), _p(dfinal), _p(dx), _p(dw), _p(db),
+                                      _p(ds), *a.shape(), _p(ws), _stream()), what)
+    return dx, dw, db, ds
+
+
+def short_conv_step(state, x, weight, bias=None, silu=False) -> Tensor:
+    """one token per sequence: x [rows, channels]; `state` [rows, taps - 1, channels], the inputs before it in x's type,
+    is updated in place -> out [rows, channels]"""
+    what = 'short_conv_step'
+    dtype = _act_dtype(what, x)
+    if x.dim() != 2 or weight.dim() != 2 or not 2 <= weight.shape[1] <= 4:
+        raise RuntimeError(f"{what}: expected x [rows, channels] and weight [channels, 2 to 4 taps], got "
+                           f"{tuple(x.shape)} and {tuple(weight.shape)}")
+    rows, ch = x.shape
+    W = weight.shape[1]
+    _in_place(what, state, (rows, W - 1, ch), x, x.dtype)
+    x = _act(what, 'x', x, x.shape, x)
+    weight = _param(what, 'weight', weight, (ch, W), x)
+    bias = _param(what, 'bias', bias, (ch,), x)
+    with _On(x):
+        out = torch.empty(rows, ch, dtype=x.dtype, device=x.device)
+        check(lib.dvae_short_conv_step(_p(state), _p(x), x.stride(0), _p(weight), _p(bias), int(bool(silu)), _p(out), rows,
+                                       ch, W, dtype, _stream()), what)
+    return out
+
+
+def _norm_rows(what: str, name: str, t: Optional[Tensor], shape, like: Tensor, dtypes) -> Optional[Tensor]:
+    """an activation [..., channels] as rows of equal stride"""
+    if t is None:
+        return None
+    if t.shape != shape:
+        raise RuntimeError(f"{what}: {name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if t.dtype not in dtypes or t.device != like.device:
+        raise RuntimeError(f"{what}: {name} is {t.dtype} on {t.device}, expected {' or '.join(map(str, dtypes))} on "
+                           f"{like.device}")
+    t = t.reshape(-1, shape[-1])
+    return t if t.stride(1) == 1 or shape[-1] == 1 else t.contiguous()
+
+
+class NormArgs:
+    def __init__(self, what, x, residual, weight):
+        self.dtype = _act_dtype(what, x)
+        if x.dim() < 1 or x.shape[-1] < 1:
+            raise RuntimeError(f"{what}: expected [..., channels], got {tuple(x.shape)}")
+        self.shape, self.D = x.shape, x.shape[-1]
+        self.rows = x.numel() // self.D
+        self.x = _norm_rows(what, 'x', x, x.shape, x, (x.dtype,))
+        self.residual = _norm_rows(what, 'residual', residual, x.shape, x, (x.dtype, torch.float32))
+        self.weight = _param(what, 'weight', weight, (self.D,), x)
+        self.sum_dtype = x.dtype if residual is None else residual.dtype
+        self.rdtype = _ACT_DTYPES[self.sum_dtype]
+
+    def head(self, eps):
+        return (_p(self.x), self.x.stride(0), _p(self.residual), 0 if self.residual is None else self.residual.stride(0),
+                _p(self.weight), float(eps))
+
+
+def add_rms_norm_fwd(a: NormArgs, eps: float, keep: bool):
+    """-> y, sum [rows, channels] (x itself without a residual), rstd [rows] or None"""
+    dev = a.x.device
+    with _On(a.x):
+        y = torch.empty(a.rows, a.D, dtype=a.x.dtype, device=dev)
+        total = a.x if a.residual is None else torch.empty(a.rows, a.D, dtype=a.sum_dtype, device=dev)
+        rstd = torch.empty(a.rows, dtype=torch.float32, device=dev) if keep else None
+        check(lib.dvae_add_rms_norm_fwd(*a.head(eps), _p(y), None if a.residual is None else _p(total), _p(rstd), a.rows,
+                                        a.D, a.dtype, a.rdtype, _stream()), 'add_rms_norm_fwd')
+    return y, total, rstd
+
+
+def add_rms_norm_q8(x: Tensor, residual: Optional[Tensor], weight: Tensor, eps: float = 1e-6):
+    """add_rms_norm with the output in 8 bits -> (q of type float8_e4m3fn, scale [...] fp32, sum): the normalised row
+    is q * scale, scale = max|y| / 448 of the row (1 for a row of zeros)"""
+    a = NormArgs('add_rms_norm_q8', x, residual, weight)
+    dev = a.x.device
+    with _On(a.x):
+        q = torch.empty(a.rows, a.D, dtype=torch.float8_e4m3fn, device=dev)
+        scale = torch.empty(a.rows, dtype=torch.float32, device=dev)
+        total = None if a.residual is None else torch.empty(a.rows, a.D, dtype=a.sum_dtype, device=dev)
+        check(lib.dvae_add_rms_norm_q8(*a.head(eps), _p(q), _p(scale), _p(total), a.rows, a.D, a.dtype, a.rdtype,
+                                       _stream()), 'add_rms_norm_q8')
+    return q.view(a.shape), scale.view(a.shape[:-1]), x if total is None else total.view(a.shape)
+
+
+def add_rms_norm_bwd(dy: Tensor, dsum: Optional[Tensor], total: Tensor, weight: Tensor, rstd: Tensor, dx_dtype):
+    """dy [..., channels] of x's type, dsum and total of the sum's -> dx, dresidual (the same tensor where the types are
+    the same: autograd then copies before it keeps either), dweight"""
+    what = 'add_rms_norm_bwd'
+    shape = dy.shape
+    D = shape[-1]
+    dy2 = _norm_rows(what, 'dy', dy, shape, dy, (dx_dtype,))
+    ds2 = _norm_rows(what, 'dsum', dsum, shape, dy, (total.dtype,))
+    rows, dev = dy2.shape[0], dy.device
+    if rows == 0:
+        none = torch.empty(shape, dtype=dx_dtype, device=dev)
+        return none, none.to(total.dtype), torch.zeros(D, device=dev)
+    with _On(dy):
+        dres = torch.empty(rows, D, dtype=total.dtype, device=dev)
+        dx = dres if total.dtype == dx_dtype else torch.empty(rows, D, dtype=dx_dtype, device=dev)
+        dw = torch.empty(D, dtype=torch.float32, device=dev)
+        ws = torch.empty(int(lib.dvae_add_rms_norm_bwd_ws_floats(rows, D)), dtype=torch.float32, device=dev)
+        check(lib.dvae_add_rms_norm_bwd(_p(dy2), dy2.stride(0), _p(ds2), 0 if ds2 is None else ds2.stride(0), _p(total),
+                                        total.stride(0), _p(weight), _p(rstd), _p(dres), _p(dx), _p(dw), rows, D,
+                                        _ACT_DTYPES[dx_dtype], _ACT_DTYPES[total.dtype], _p(ws), _stream()), what)
+    same = dx is dres
+    dres = dres.view(shape)
+    return dres if same else dx.view(shape), dres, dw
+
+
 # ---------------------------------------------------------------------------- launch trace (benchmarks)
 def trace_begin(max_launches: int = 1 << 16):
     """From here to trace_collect() every kernel launch of the library is timed with two events on its

@@ -569,6 +569,83 @@ int dvae_adam_step_f32(int64_t n, float* const* params, const float* const* grad
                        const float* grad_coef, const float* dyn, dvae_stream_t stream);
 int dvae_adam_advance_f32(float* dyn, double beta1, double beta2, dvae_stream_t stream);
 
+/* ---- sequence operators: a selective state-space layer's scan, its short causal convolution, and the residual
+ *      root-mean-square norm.  No counterpart in the reference, whose time axis is handled by nn.LSTM
+ *      (models/encoders.py:128-173).
+ *      Activations (u, delta, z, B, C, x, out and their gradients) are all fp32 or all bfloat16 (`dtype`), the last
+ *      dimension contiguous; `*_sb` / `*_st` / `*_sg` are the element strides of their rows (sequences of a batch),
+ *      tokens and groups.  Outputs and gradients are contiguous.  Parameters, states and their gradients are fp32.
+ *      A batch is `rows` sequences of L tokens.  With `offsets` (S + 1 ascending int32 positions on the device, the
+ *      first 0) there is one row of L tokens that holds S sequences one after the other, some possibly empty; tokens
+ *      behind the last one belong to none: outputs and gradients are 0 there.  Offsets are not checked: wrong ones give
+ *      wrong results, never an access outside the tensors.  S is the number of sequences in either form. */
+#define DVAE_DT_F32 0
+#define DVAE_DT_BF16 1
+
+/* dt = softplus(delta + bias) (softplus != 0; else delta + bias), h[n] = exp(dt A[d,n]) h[n] + dt u B[n],
+ * out = (sum_n C[n] h[n] + Dp u) silu(z).  u, delta, z, out [rows,L,D]; A [D,N], N <= 16; B, C [rows,L,G,N], G divides D;
+ * Dp, bias [D]; state0 (entering) and state1 (final) [S,D,N].  NULL: Dp, z, bias, state0, state1, offsets, ckpt.
+ * Final states of sequences without tokens are not written.  ckpt (dvae_selective_scan_ckpt_floats): the states that
+ * the backward pass starts from, kept if not NULL. */
+int64_t dvae_selective_scan_ckpt_floats(int64_t rows, int64_t L, int64_t D, int64_t N);
+int dvae_selective_scan_fwd(const void* u, int64_t u_sb, int64_t u_st, const void* delta, int64_t delta_sb,
+                            int64_t delta_st, const float* A, const void* B, int64_t B_sb, int64_t B_st, int64_t B_sg,
+                            const void* C, int64_t C_sb, int64_t C_st, int64_t C_sg, const float* Dp, const void* z,
+                            int64_t z_sb, int64_t z_st, const float* bias, int softplus, const float* state0,
+                            float* state1, const int32_t* offsets, void* out, float* ckpt, int64_t rows, int64_t L,
+                            int64_t D, int64_t G, int64_t N, int64_t S, int dtype, dvae_stream_t stream);
+/* Gradients from dout and (NULL: zero) dstate1, the gradient of the final states.  dA, dD, dbias, dstate0 may be NULL;
+ * dstate0 of sequences without tokens is not written.  ckpt as the forward pass filled it. */
+int64_t dvae_selective_scan_bwd_ws_floats(int64_t rows, int64_t L, int64_t D, int64_t G, int64_t N);
+int dvae_selective_scan_bwd(const void* u, int64_t u_sb, int64_t u_st, const void* delta, int64_t delta_sb,
+                            int64_t delta_st, const float* A, const void* B, int64_t B_sb, int64_t B_st, int64_t B_sg,
+                            const void* C, int64_t C_sb, int64_t C_st, int64_t C_sg, const float* Dp, const void* z,
+                            int64_t z_sb, int64_t z_st, const float* bias, int softplus, const float* state0,
+                            const int32_t* offsets, const void* dout, int64_t dout_sb, int64_t dout_st,
+                            const float* dstate1, const float* ckpt, void* du, void* ddelta, float* dA, void* dB,
+                            void* dC, float* dD, void* dz, float* dbias, float* dstate0, int64_t rows, int64_t L,
+                            int64_t D, int64_t G, int64_t N, int64_t S, int dtype, float* ws, dvae_stream_t stream);
+/* One token per row: state [rows,D,N] is updated in place; u, delta, z, out [rows,D]; B, C [rows,G,N]. */
+int dvae_selective_scan_step(float* state, const void* u, int64_t u_sb, const void* delta, int64_t delta_sb,
+                             const float* A, const void* B, int64_t B_sb, int64_t B_sg, const void* C, int64_t C_sb,
+                             int64_t C_sg, const float* Dp, const void* z, int64_t z_sb, const float* bias, int softplus,
+                             void* out, int64_t rows, int64_t D, int64_t G, int64_t N, int dtype, dvae_stream_t stream);
+
+/* Depthwise convolution over the last W tokens (2 <= W <= 4) of the same sequence:
+ * out[t] = act(bias + sum_k w[d,k] x[t - (W-1) + k]), act = silu if `silu` != 0.  x, out [rows,L,D]; w [D,W]; bias [D] or
+ * NULL.  What lies before a sequence's first token is state0 [S,W-1,D] (type `dtype`; NULL: zeros); state1, if not NULL,
+ * receives the last W - 1 inputs of every sequence that has tokens. */
+int dvae_short_conv_fwd(const void* x, int64_t x_sb, int64_t x_st, const float* w, const float* bias, int silu,
+                        const void* state0, void* state1, const int32_t* offsets, void* out, int64_t rows, int64_t L,
+                        int64_t D, int64_t W, int64_t S, int dtype, dvae_stream_t stream);
+/* dx, dw [D,W], dbias [D] (NULL: not wanted) and dstate0 (NULL likewise) from dout and dstate1 (NULL: zero). */
+int64_t dvae_short_conv_bwd_ws_floats(int64_t rows, int64_t L, int64_t D, int64_t W);
+int dvae_short_conv_bwd(const void* x, int64_t x_sb, int64_t x_st, const float* w, const float* bias, int silu,
+                        const void* state0, const int32_t* offsets, const void* dout, int64_t dout_sb, int64_t dout_st,
+                        const void* dstate1, void* dx, float* dw, float* dbias, void* dstate0, int64_t rows, int64_t L,
+                        int64_t D, int64_t W, int64_t S, int dtype, float* ws, dvae_stream_t stream);
+/* One token per row: state [rows,W-1,D] is updated in place; x, out [rows,D]. */
+int dvae_short_conv_step(void* state, const void* x, int64_t x_sb, const float* w, const float* bias, int silu, void* out,
+                         int64_t rows, int64_t D, int64_t W, int dtype, dvae_stream_t stream);
+
+/* sum = x + residual, rounded to its stored type; y = sum / sqrt(mean(sum^2) + eps) * w, of x's type `dtype`.
+ * x, residual, sum, y [rows,D] with row strides x_st, r_st (sum and y contiguous).  residual and sum are of type
+ * `rdtype`: that of x, or fp32.  residual NULL: sum is x itself, and is not written.  rstd [rows]: 1 / sqrt(...), kept
+ * for the backward pass if not NULL. */
+int dvae_add_rms_norm_fwd(const void* x, int64_t x_st, const void* residual, int64_t r_st, const float* w, float eps,
+                          void* y, void* sum, float* rstd, int64_t rows, int64_t D, int dtype, int rdtype,
+                          dvae_stream_t stream);
+/* The same with y in 8 bits (e4m3, no infinities): scale[row] = max|y| / 448, or 1 for a row of zeros, q = y / scale. */
+int dvae_add_rms_norm_q8(const void* x, int64_t x_st, const void* residual, int64_t r_st, const float* w, float eps,
+                         void* q, float* scale, void* sum, int64_t rows, int64_t D, int dtype, int rdtype,
+                         dvae_stream_t stream);
+/* dsum_out = rstd (w dy - hat mean(w dy hat)) + dsum, the gradient of the sum, written as dres (type `rdtype`) and, if
+ * the types differ and dx is not NULL, as dx (type `dtype`); dw [D].  `sum` (strides s_st) as stored; dsum NULL: zero. */
+int64_t dvae_add_rms_norm_bwd_ws_floats(int64_t rows, int64_t D);
+int dvae_add_rms_norm_bwd(const void* dy, int64_t dy_st, const void* dsum, int64_t ds_st, const void* sum, int64_t s_st,
+                          const float* w, const float* rstd, void* dres, void* dx, float* dw, int64_t rows, int64_t D,
+                          int dtype, int rdtype, float* ws, dvae_stream_t stream);
+
 /* ---- launch tracing for benchmarks.  No counterpart in the reference (it times whole calls with a host
  *      clock, evaluation/metrics.py:143-177).  Between dvae_trace_begin and dvae_trace_end every kernel
  *      launch of the library is bracketed by two events on the stream it is launched on and recorded with
