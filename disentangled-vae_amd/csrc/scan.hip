@@ -7,10 +7,18 @@
 // A lane owns one channel and keeps its N states in registers, so the sum over n is a chain of fused multiply-adds and
 // neighbouring lanes read neighbouring channels.  B and C of a token are the same for all lanes: they come through the
 // scalar unit and enter the vector instructions as scalar operands.
+//
+// One wave per 64 channels of a sequence would leave most of the chip idle where there are few sequences, so the time
+// axis is split into chunks that run side by side.  A chunk needs the state that enters it: a first pass computes each
+// chunk's state as if it started from zero (and the sum of its step sizes, whose exponential is the chunk's decay), a
+// second joins those along the axis, the third computes the outputs.  The way back does the same from the right.  Both
+// extra passes are left out where there is one chunk.
 #include "seq_common.h"
 
 #define SCAN_Q 8       // tokens per block: what is loaded ahead, and how far apart training keeps states
 #define SCAN_MAX_N 16
+#define SCAN_WAVES 2048    // waves that a launch aims at: two per SIMD
+#define SCAN_MIN_CHUNK 32  // tokens: below this a chunk's fixed costs (its state in and out) weigh as much as its tokens
 
 struct ScanArgs {
   const void *u, *delta, *z, *B, *C, *dout;
@@ -21,8 +29,11 @@ struct ScanArgs {
   void *out, *du, *ddelta, *dz;
   float *ckpt;                 // [row][block of SCAN_Q tokens][n][D]: the state that enters the block
   float *part_bc, *part_a;     // partial sums of the gradients of B and C, and of A, D and bias
+  float *enter, *leave;        // the states that enter the chunks, and the adjoints that enter them from the right
+  float *sumdt, *keep;         // [row][chunk][D]: sum of step sizes; [row][chunk]: 1 where no sequence starts
   const int32_t* offsets;
-  int rows, L, D, G, N, S, Dg, tpg, ntiles, softplus, blocks;
+  int rows, L, D, G, N, S, Dg, tpg, ntiles, wpg, softplus, blocks;
+  int nch, CL, enter_row, enter_step;   // chunks, their tokens; slots of `enter` per row and from chunk to chunk
 };
 
 // what happens inside a block of n tokens from t0 on: bit j of `start` / `end` / `valid`: token t0 + j is its
@@ -77,17 +88,27 @@ template <typename T, int NP> struct BCLoad<T, NP, false> {
   }
 };
 
-// One wave: 64 channels of one group of one row.
+// One wave: 64 channels of one group, one chunk of one row.  A workgroup's four waves are neighbours in a group.
 struct Tile {
-  int g, d, lane, dl;
+  int g, d, lane, wave, part, chunk, row, t0, t1;
   bool on;
-  __device__ __forceinline__ Tile(const ScanArgs& p, int tile) {
+  __device__ __forceinline__ explicit Tile(const ScanArgs& p) {
     lane = threadIdx.x & 63;
-    g = tile / p.tpg;
-    const int c = (tile % p.tpg) * 64 + lane;
+    wave = uniform(threadIdx.x >> 6);
+    const int wg = blockIdx.x % p.wpg;
+    const int rc = blockIdx.x / p.wpg;
+    const int per = (p.tpg + 3) / 4;
+    g = wg / per;
+    part = wg % per;
+    chunk = rc % p.nch;
+    row = rc / p.nch;
+    t0 = chunk * p.CL;
+    t1 = min(t0 + p.CL, p.L);
+    const int c = (part * 4 + wave) * 64 + lane;
     on = c < p.Dg;
     d = g * p.Dg + (on ? c : p.Dg - 1);          // lanes past the group's last channel read it too, and write nothing
   }
+  __device__ __forceinline__ bool idle(const ScanArgs& p) const { return part * 4 + wave >= p.tpg; }
 };
 
 template <int NP>
@@ -113,20 +134,37 @@ __device__ __forceinline__ void entering_state(const ScanArgs& p, int64_t seq, i
   }
 }
 
-template <typename T, int NP, bool PACKED, bool FAST>
+template <int NP>
+__device__ __forceinline__ void load_slot(const float* slot, const ScanArgs& p, int d, float (&h)[NP]) {
+#pragma unroll
+  for (int n = 0; n < NP; ++n) h[n] = n < p.N ? slot[(int64_t)n * p.D + d] : 0.f;
+}
+template <int NP>
+__device__ __forceinline__ void store_slot(float* slot, const ScanArgs& p, int d, const float (&h)[NP]) {
+#pragma unroll
+  for (int n = 0; n < NP; ++n)
+    if (n < p.N) slot[(int64_t)n * p.D + d] = h[n];
+}
+__device__ __forceinline__ float* enter_slot(const ScanArgs& p, int row, int chunk) {
+  return p.enter + ((int64_t)row * p.enter_row + (int64_t)chunk * p.enter_step) * p.N * p.D;
+}
+__device__ __forceinline__ float* leave_slot(const ScanArgs& p, int row, int chunk) {
+  return p.leave + ((int64_t)row * p.nch + chunk) * p.N * p.D;
+}
+
+// STATE_ONLY: the chunk's last state from a zero start, into the next chunk's slot; else the outputs
+template <typename T, int NP, bool PACKED, bool FAST, bool STATE_ONLY>
 __global__ void __launch_bounds__(256) scan_fwd_kernel(ScanArgs p) {
-  const int wave = uniform(threadIdx.x >> 6);
-  const int tgroups = (p.ntiles + 3) / 4;
-  const int tile = (int)(blockIdx.x % tgroups) * 4 + wave;
-  const int row = blockIdx.x / tgroups;
-  if (tile >= p.ntiles) return;
-  const Tile w(p, tile);
+  const Tile w(p);
+  if (w.idle(p) || (STATE_ONLY && w.chunk + 1 == p.nch)) return;
+  const int row = w.row;
   float A2[NP], h[NP];
 #pragma unroll
   for (int n = 0; n < NP; ++n) {
     A2[n] = n < p.N ? p.A[(int64_t)w.d * p.N + n] * LOG2E_F : 0.f;
     h[n] = 0.f;
   }
+  if (!STATE_ONLY && w.chunk > 0) load_slot<NP>(enter_slot(p, row, w.chunk), p, w.d, h);
   const float Dp = p.Dp ? p.Dp[w.d] : 0.f, bias = p.bias ? p.bias[w.d] : 0.f;
   const T* u = (const T*)p.u + row * p.u_sb;
   const T* dl = (const T*)p.delta + row * p.delta_sb;
@@ -135,47 +173,95 @@ __global__ void __launch_bounds__(256) scan_fwd_kernel(ScanArgs p) {
   const T* C = (const T*)p.C + row * p.C_sb + w.g * p.C_sg;
   T* out = (T*)p.out + (int64_t)row * p.L * p.D;
   SeqWalk q = {p.offsets, p.S, p.L, p.L, row, 0, p.L};
-  if (PACKED) q.seek(0);
+  if (PACKED) q.seek(w.t0);
+  float total = 0.f;
+  bool cut = false;
 
-  for (int t0 = 0; t0 < p.L; t0 += SCAN_Q) {
-    const int n = min(SCAN_Q, p.L - t0);
+  for (int t0 = w.t0; t0 < w.t1; t0 += SCAN_Q) {
+    const int n = min(SCAN_Q, w.t1 - t0);
     const Marks m = block_marks<PACKED>(q, t0, n, p.L);
-    if (p.ckpt && w.on) {
-      float* ck = p.ckpt + ((int64_t)row * p.blocks + t0 / SCAN_Q) * p.N * p.D + w.d;
-#pragma unroll
-      for (int i = 0; i < NP; ++i)
-        if (i < p.N) ck[(int64_t)i * p.D] = h[i];
-    }
+    if (!STATE_ONLY && p.ckpt && w.on)
+      store_slot<NP>(p.ckpt + ((int64_t)row * p.blocks + t0 / SCAN_Q) * p.N * p.D, p, w.d, h);
 #pragma unroll 1
     for (int j = 0; j < n; ++j) {
       const int64_t t = t0 + j;
       if (!(m.valid >> j & 1)) {
-        if (w.on) out[t * p.D + w.d] = from_f32<T>(0.f);
+        if (!STATE_ONLY && w.on) out[t * p.D + w.d] = from_f32<T>(0.f);
         continue;
       }
-      if (m.start >> j & 1) entering_state<NP>(p, q.seq(), w.d, h);
+      if (m.start >> j & 1) {
+        entering_state<NP>(p, q.seq(), w.d, h);
+        cut = true;
+      }
       const float uu = to_f32(u[t * p.u_st + w.d]);
       const float pre = to_f32(dl[t * p.delta_st + w.d]) + bias;
       const float dt = p.softplus ? softplus_hw(pre) : pre;
-      float Bv[NP], Cv[NP];
+      float Bv[NP];
       BCLoad<T, NP, FAST>::get(B, t * p.B_st, p.N, Bv);
-      BCLoad<T, NP, FAST>::get(C, t * p.C_st, p.N, Cv);
       const float x = dt * uu;
-      float y = Dp * uu;
+      if (STATE_ONLY) {
+        total += dt;
 #pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        h[i] = fmaf(exp2_hw(dt * A2[i]), h[i], x * Bv[i]);
-        y = fmaf(Cv[i], h[i], y);
+        for (int i = 0; i < NP; ++i) h[i] = fmaf(exp2_hw(dt * A2[i]), h[i], x * Bv[i]);
+      } else {
+        float Cv[NP];
+        BCLoad<T, NP, FAST>::get(C, t * p.C_st, p.N, Cv);
+        float y = Dp * uu;
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          h[i] = fmaf(exp2_hw(dt * A2[i]), h[i], x * Bv[i]);
+          y = fmaf(Cv[i], h[i], y);
+        }
+        if (z) {
+          const float zz = to_f32(z[t * p.z_st + w.d]);
+          y *= zz * sigmoid_hw(zz);
+        }
+        if (w.on) out[t * p.D + w.d] = from_f32<T>(y);
       }
-      if (z) {
-        const float zz = to_f32(z[t * p.z_st + w.d]);
-        y *= zz * sigmoid_hw(zz);
-      }
-      if (w.on) out[t * p.D + w.d] = from_f32<T>(y);
       if (m.end >> j & 1) {
-        if (p.state1 && w.on) store_state<NP>(p.state1, q.seq(), p, w.d, h);
+        if (!STATE_ONLY && p.state1 && w.on) store_state<NP>(p.state1, q.seq(), p, w.d, h);
         if (PACKED) q.next((int)t + 1);
       }
+    }
+  }
+  if (STATE_ONLY) {
+    if (w.on) {
+      store_slot<NP>(enter_slot(p, row, w.chunk + 1), p, w.d, h);
+      p.sumdt[((int64_t)row * p.nch + w.chunk) * p.D + w.d] = total;
+    }
+    if (w.g == 0 && w.part == 0 && threadIdx.x == 0) p.keep[row * p.nch + w.chunk] = cut ? 0.f : 1.f;
+  }
+}
+
+// The states (or, BACK, the adjoints) that enter the chunks: x = decay * x + own, along the axis.  Where a sequence
+// starts inside a chunk nothing of what enters it gets through.  A thread owns one state of one channel.
+#define JOIN_AHEAD 8
+template <bool BACK>
+__global__ void __launch_bounds__(256) scan_join_kernel(ScanArgs p) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t ND = (int64_t)p.N * p.D;
+  if (i >= ND) return;
+  const int row = blockIdx.y, d = (int)(i % p.D), n = (int)(i / p.D);
+  const float A2 = p.A[(int64_t)d * p.N + n] * LOG2E_F;
+  const float* sumdt = p.sumdt + (int64_t)row * p.nch * p.D + d;
+  float x = 0.f;
+  for (int k0 = 0; k0 + 1 < p.nch; k0 += JOIN_AHEAD) {
+    float own[JOIN_AHEAD], dec[JOIN_AHEAD], keep[JOIN_AHEAD];
+#pragma unroll
+    for (int j = 0; j < JOIN_AHEAD; ++j) {
+      const int k = min(k0 + j, p.nch - 2);
+      const int c = BACK ? p.nch - 1 - k : k;              // the chunk that x passes through
+      own[j] = (BACK ? leave_slot(p, row, c - 1) : enter_slot(p, row, c + 1))[i];
+      dec[j] = sumdt[(int64_t)c * p.D];
+      keep[j] = uniform_load(p.keep, (int64_t)row * p.nch + c);
+    }
+#pragma unroll
+    for (int j = 0; j < JOIN_AHEAD; ++j) {
+      const int k = k0 + j;
+      if (k + 1 >= p.nch) break;
+      const int c = BACK ? p.nch - 1 - k : k;
+      x = keep[j] != 0.f ? fmaf(exp2_hw(dec[j] * A2), x, own[j]) : own[j];
+      (BACK ? leave_slot(p, row, c - 1) : enter_slot(p, row, c + 1))[i] = x;
     }
   }
 }
@@ -186,21 +272,126 @@ __global__ void __launch_bounds__(256) scan_fwd_kernel(ScanArgs p) {
 //   w      = a[n] dh[n] (what goes on to the token before);  k = w h_before[n]
 //   dA[n] += k dt          ddt += k A[n] + dh[n] B[n] u  du += dh[n] B[n] dt
 // The states are computed again, SCAN_Q tokens at a time, from those that the forward pass kept.
+template <int CTRL> __device__ __forceinline__ float dpp(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false));
+}
+#define DPP_HALF_MIRROR 0x141
+#define DPP_ROR8 0x128
+#define DPP_XOR2 0x4e     // quad_perm [2,3,0,1]
+#define DPP_XOR1 0xb1     // quad_perm [1,0,3,2]
+
+// Sums of 2 * NP values over the 64 lanes, all at once: a step adds the two halves of the wave (then of a half, ...) and
+// lets one half go on with one value, the other with another, so the number of values halves with the number of lanes
+// that still hold parts of one.  The sum of value sum_index(lane) ends up in `lane`.
+template <int M> struct WaveSums {
+  static __device__ __forceinline__ float run(float (&v)[M], int lane) {
+    // 32 lanes apart, then 16: the swaps exchange the upper half of one register with the lower half of the other
+#pragma unroll
+    for (int i = 0; i < M / 2; ++i) {
+      const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[i]), __float_as_uint(v[i + M / 2]), false, false);
+      v[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+#pragma unroll
+    for (int i = 0; i < M / 4; ++i) {
+      const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[i]), __float_as_uint(v[i + M / 4]), false, false);
+      v[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+#pragma unroll
+    for (int i = 0; i < M / 8; ++i) {
+      const float a = lane & 8 ? v[i + M / 8] : v[i], b = lane & 8 ? v[i] : v[i + M / 8];
+      v[i] = a + dpp<DPP_ROR8>(b);
+    }
+#pragma unroll
+    for (int i = 0; i < M / 16; ++i) {
+      const float a = lane & 4 ? v[i + M / 16] : v[i], b = lane & 4 ? v[i] : v[i + M / 16];
+      v[i] = a + dpp<DPP_HALF_MIRROR>(b);
+    }
+    if (M == 32) {
+      const float a = lane & 2 ? v[1] : v[0], b = lane & 2 ? v[0] : v[1];
+      v[0] = a + dpp<DPP_XOR2>(b);
+    } else {
+      v[0] += dpp<DPP_XOR2>(v[0]);
+    }
+    return v[0] + dpp<DPP_XOR1>(v[0]);
+  }
+  static __device__ __forceinline__ int index(int lane) {
+    return (lane & 32 ? M / 2 : 0) + (lane & 16 ? M / 4 : 0) + (lane & 8 ? M / 8 : 0) + (lane & 4 ? M / 16 : 0) +
+           (M == 32 && lane & 2 ? 1 : 0);
+  }
+};
+
+// The adjoint that leaves a chunk to the left if nothing enters it from the right: the sum of C[n] g of its tokens up to
+// the first start of a sequence, each through the decays from the chunk's first token to its own.
+template <typename T, int NP, bool PACKED, bool FAST>
+__global__ void __launch_bounds__(256) scan_bwd_state_kernel(ScanArgs p) {
+  const Tile w(p);
+  if (w.idle(p) || w.chunk == 0) return;
+  const int row = w.row;
+  float A2[NP], x[NP];
+#pragma unroll
+  for (int n = 0; n < NP; ++n) {
+    A2[n] = n < p.N ? p.A[(int64_t)w.d * p.N + n] * LOG2E_F : 0.f;
+    x[n] = 0.f;
+  }
+  const float bias = p.bias ? p.bias[w.d] : 0.f;
+  const T* dl = (const T*)p.delta + row * p.delta_sb;
+  const T* z = p.z ? (const T*)p.z + row * p.z_sb : nullptr;
+  const T* go = (const T*)p.dout + row * p.dout_sb;
+  const T* C = (const T*)p.C + row * p.C_sb + w.g * p.C_sg;
+  SeqWalk q = {p.offsets, p.S, p.L, p.L, row, 0, p.L};
+  if (PACKED) q.seek(w.t0);
+  float total = 0.f;
+  bool cut = false;
+  for (int t0 = w.t0; t0 < w.t1 && !cut; t0 += SCAN_Q) {
+    const int n = min(SCAN_Q, w.t1 - t0);
+    const Marks m = block_marks<PACKED>(q, t0, n, p.L);
+#pragma unroll 1
+    for (int j = 0; j < n; ++j) {
+      const int64_t t = t0 + j;
+      if (!(m.valid >> j & 1)) continue;
+      if (m.start >> j & 1) { cut = true; break; }
+      const float pre = to_f32(dl[t * p.delta_st + w.d]) + bias;
+      total += p.softplus ? softplus_hw(pre) : pre;
+      float g = to_f32(go[t * p.dout_st + w.d]);
+      if (z) {
+        const float zz = to_f32(z[t * p.z_st + w.d]);
+        g *= zz * sigmoid_hw(zz);
+      }
+      float Cv[NP];
+      BCLoad<T, NP, FAST>::get(C, t * p.C_st, p.N, Cv);
+#pragma unroll
+      for (int i = 0; i < NP; ++i) x[i] = fmaf(exp2_hw(total * A2[i]), Cv[i] * g, x[i]);
+      if (m.end >> j & 1) {
+        if (p.dstate1) {
+          float e[NP];
+          load_state<NP>(p.dstate1, q.seq(), p, w.d, e);
+#pragma unroll
+          for (int i = 0; i < NP; ++i) x[i] = fmaf(exp2_hw(total * A2[i]), e[i], x[i]);
+        }
+        if (PACKED) q.next((int)t + 1);
+      }
+    }
+  }
+  if (w.on) {
+    store_slot<NP>(leave_slot(p, row, w.chunk - 1), p, w.d, x);
+    p.sumdt[((int64_t)row * p.nch + w.chunk) * p.D + w.d] = total;
+  }
+  if (w.g == 0 && w.part == 0 && threadIdx.x == 0) p.keep[row * p.nch + w.chunk] = cut ? 0.f : 1.f;
+}
+
 template <typename T, int NP, bool PACKED, bool FAST>
 __global__ void __launch_bounds__(256) scan_bwd_kernel(ScanArgs p) {
-  const int wave = uniform(threadIdx.x >> 6);
-  const int tgroups = (p.ntiles + 3) / 4;
-  const int tile = (int)(blockIdx.x % tgroups) * 4 + wave;
-  const int row = blockIdx.x / tgroups;
-  if (tile >= p.ntiles) return;
-  const Tile w(p, tile);
-  const int tig = tile % p.tpg;
-  float A2[NP], dh[NP], dA[NP], hs[SCAN_Q + 1][NP];
+  __shared__ float red[2][SCAN_Q][4][2 * NP];      // [block parity][token][wave][dB, dC]
+  const Tile w(p);
+  const int row = w.row;
+  const bool idle = w.idle(p);                     // such a wave only takes part in the sums
+  float A2[NP], dh[NP], dA[NP];
 #pragma unroll
   for (int n = 0; n < NP; ++n) {
     A2[n] = n < p.N ? p.A[(int64_t)w.d * p.N + n] * LOG2E_F : 0.f;
     dh[n] = dA[n] = 0.f;
   }
+  if (w.chunk + 1 < p.nch && !idle) load_slot<NP>(leave_slot(p, row, w.chunk), p, w.d, dh);
   float dD = 0.f, dbias = 0.f;
   const float Dp = p.Dp ? p.Dp[w.d] : 0.f, bias = p.bias ? p.bias[w.d] : 0.f;
   const T* u = (const T*)p.u + row * p.u_sb;
@@ -211,107 +402,115 @@ __global__ void __launch_bounds__(256) scan_bwd_kernel(ScanArgs p) {
   const T* C = (const T*)p.C + row * p.C_sb + w.g * p.C_sg;
   const int64_t flat = (int64_t)row * p.L;
   SeqWalk q = {p.offsets, p.S, p.L, p.L, row, 0, p.L};      // the sequence that the way back is in
-  if (PACKED) { q.s = p.S; q.prev(p.L - 1); }
+  if (PACKED) {                                             // the last one that has a token before the chunk's end
+    q.seek(w.t1 - 1);
+    if (q.s >= q.S || q.b >= w.t1) q.prev(w.t1 - 1);
+  }
+  int turn = 0;
 
-  for (int t0 = (p.L - 1) / SCAN_Q * SCAN_Q; t0 >= 0; t0 -= SCAN_Q) {
-    const int n = min(SCAN_Q, p.L - t0);
+  for (int t0 = w.t0 + (w.t1 - w.t0 - 1) / SCAN_Q * SCAN_Q; t0 >= w.t0; t0 -= SCAN_Q, turn ^= 1) {
+    const int n = min(SCAN_Q, w.t1 - t0);
     SeqWalk f = q;                                     // and the one that the states' second computation is in
     if (PACKED) f.seek(t0);
     const Marks m = block_marks<PACKED>(f, t0, n, p.L);
-    const float* ck = p.ckpt + ((int64_t)row * p.blocks + t0 / SCAN_Q) * p.N * p.D + w.d;
+    if (idle) {
+      for (int i = w.lane; i < SCAN_Q * 2 * NP; i += 64) red[turn][i / (2 * NP)][w.wave][i % (2 * NP)] = 0.f;
+    } else {
+      float hs[SCAN_Q + 1][NP];
+      load_slot<NP>(p.ckpt + ((int64_t)row * p.blocks + t0 / SCAN_Q) * p.N * p.D, p, w.d, hs[0]);
+      float ub[SCAN_Q], pb[SCAN_Q], db[SCAN_Q];
 #pragma unroll
-    for (int i = 0; i < NP; ++i) hs[0][i] = i < p.N ? ck[(int64_t)i * p.D] : 0.f;
-    float ub[SCAN_Q], pb[SCAN_Q], db[SCAN_Q];
+      for (int j = 0; j < SCAN_Q; ++j) {
 #pragma unroll
-    for (int j = 0; j < SCAN_Q; ++j) {
+        for (int i = 0; i < NP; ++i) hs[j + 1][i] = hs[j][i];
+        if (!(m.valid >> j & 1)) continue;
+        const int64_t t = t0 + j;
+        ub[j] = to_f32(u[t * p.u_st + w.d]);
+        pb[j] = to_f32(dl[t * p.delta_st + w.d]) + bias;
+        db[j] = p.softplus ? softplus_hw(pb[j]) : pb[j];
+        if (m.start >> j & 1) entering_state<NP>(p, f.seq(), w.d, hs[j + 1]);
+        float Bv[NP];
+        BCLoad<T, NP, FAST>::get(B, t * p.B_st, p.N, Bv);
+        const float x = db[j] * ub[j];
 #pragma unroll
-      for (int i = 0; i < NP; ++i) hs[j + 1][i] = hs[j][i];
-      if (!(m.valid >> j & 1)) continue;
-      const int64_t t = t0 + j;
-      ub[j] = to_f32(u[t * p.u_st + w.d]);
-      pb[j] = to_f32(dl[t * p.delta_st + w.d]) + bias;
-      db[j] = p.softplus ? softplus_hw(pb[j]) : pb[j];
-      if (m.start >> j & 1) entering_state<NP>(p, f.seq(), w.d, hs[j + 1]);
-      float Bv[NP];
-      BCLoad<T, NP, FAST>::get(B, t * p.B_st, p.N, Bv);
-      const float x = db[j] * ub[j];
+        for (int i = 0; i < NP; ++i) hs[j + 1][i] = fmaf(exp2_hw(db[j] * A2[i]), hs[j + 1][i], x * Bv[i]);
+        if (PACKED && (m.end >> j & 1)) f.next((int)t + 1);
+      }
 #pragma unroll
-      for (int i = 0; i < NP; ++i) hs[j + 1][i] = fmaf(exp2_hw(db[j] * A2[i]), hs[j + 1][i], x * Bv[i]);
-      if (PACKED && (m.end >> j & 1)) f.next((int)t + 1);
-    }
+      for (int j = SCAN_Q - 1; j >= 0; --j) {
+        if (j >= n) continue;
+        const int64_t t = t0 + j, o = (flat + t) * p.D + w.d;
+        if (!(m.valid >> j & 1)) {
+          if (w.on) {
+            ((T*)p.du)[o] = from_f32<T>(0.f);
+            ((T*)p.ddelta)[o] = from_f32<T>(0.f);
+            if (z) ((T*)p.dz)[o] = from_f32<T>(0.f);
+          }
+          if (w.lane < 2 * NP) red[turn][j][w.wave][w.lane] = 0.f;
+          continue;
+        }
+        if (m.end >> j & 1) {
+          if (p.dstate1) load_state<NP>(p.dstate1, q.seq(), p, w.d, dh);
+          else {
 #pragma unroll
-    for (int j = SCAN_Q - 1; j >= 0; --j) {
-      if (j >= n) continue;
-      const int64_t t = t0 + j, o = (flat + t) * p.D + w.d;
-      if (!(m.valid >> j & 1)) {
+            for (int i = 0; i < NP; ++i) dh[i] = 0.f;
+          }
+        }
+        float Bv[NP], Cv[NP];
+        BCLoad<T, NP, FAST>::get(B, t * p.B_st, p.N, Bv);
+        BCLoad<T, NP, FAST>::get(C, t * p.C_st, p.N, Cv);
+        float g = w.on ? to_f32(go[t * p.dout_st + w.d]) : 0.f;
+        if (z) {
+          const float zz = to_f32(z[t * p.z_st + w.d]);
+          const float sg = sigmoid_hw(zz);
+          float y = Dp * ub[j];
+#pragma unroll
+          for (int i = 0; i < NP; ++i) y = fmaf(Cv[i], hs[j + 1][i], y);
+          if (w.on) ((T*)p.dz)[o] = from_f32<T>(g * y * sg * fmaf(zz, 1.f - sg, 1.f));
+          g *= zz * sg;
+        }
+        const float x = w.on ? db[j] * ub[j] : 0.f;
+        float through = 0.f, ka = 0.f, pv[2 * NP], hb[NP];
+#pragma unroll
+        for (int i = 0; i < NP; ++i) hb[i] = hs[j][i];
+        if (m.start >> j & 1) entering_state<NP>(p, q.seq(), w.d, hb);
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          const float a = exp2_hw(db[j] * A2[i]);
+          const float d = fmaf(Cv[i], g, dh[i]);
+          pv[i] = d * x;
+          pv[NP + i] = g * hs[j + 1][i];
+          through = fmaf(d, Bv[i], through);
+          dh[i] = d * a;
+          const float k = dh[i] * hb[i];
+          dA[i] = fmaf(k, db[j], dA[i]);
+          ka = fmaf(k, A2[i], ka);
+        }
+        const float sum = WaveSums<2 * NP>::run(pv, w.lane);
+        if (!(w.lane & (NP == 16 ? 1 : 3))) red[turn][j][w.wave][WaveSums<2 * NP>::index(w.lane)] = sum;
+        dD = fmaf(g, ub[j], dD);
+        float dd = fmaf(ka, LN2_F, through * ub[j]);
+        if (p.softplus) dd *= sigmoid_hw(pb[j]);
+        dbias += dd;
         if (w.on) {
-          ((T*)p.du)[o] = from_f32<T>(0.f);
-          ((T*)p.ddelta)[o] = from_f32<T>(0.f);
-          if (z) ((T*)p.dz)[o] = from_f32<T>(0.f);
+          ((T*)p.du)[o] = from_f32<T>(fmaf(through, db[j], Dp * g));
+          ((T*)p.ddelta)[o] = from_f32<T>(dd);
         }
-        for (int i = w.lane; i < 2 * p.N; i += 64)
-          p.part_bc[(((int64_t)tig * p.rows * p.L + flat + t) * p.G + w.g) * 2 * p.N + i] = 0.f;
-        continue;
-      }
-      if (m.end >> j & 1) {
-        if (p.dstate1) load_state<NP>(p.dstate1, q.seq(), p, w.d, dh);
-        else {
-#pragma unroll
-          for (int i = 0; i < NP; ++i) dh[i] = 0.f;
+        if (m.start >> j & 1) {
+          if (p.dstate0 && w.on) store_state<NP>(p.dstate0, q.seq(), p, w.d, dh);
+          if (PACKED) q.prev((int)t - 1);
         }
       }
-      float Bv[NP], Cv[NP];
-      BCLoad<T, NP, FAST>::get(B, t * p.B_st, p.N, Bv);
-      BCLoad<T, NP, FAST>::get(C, t * p.C_st, p.N, Cv);
-      float g = w.on ? to_f32(go[t * p.dout_st + w.d]) : 0.f;
-      if (z) {
-        const float zz = to_f32(z[t * p.z_st + w.d]);
-        const float sg = sigmoid_hw(zz);
-        float y = Dp * ub[j];
-#pragma unroll
-        for (int i = 0; i < NP; ++i) y = fmaf(Cv[i], hs[j + 1][i], y);
-        if (w.on) ((T*)p.dz)[o] = from_f32<T>(g * y * sg * fmaf(zz, 1.f - sg, 1.f));
-        g *= zz * sg;
-      }
-      const float x = w.on ? db[j] * ub[j] : 0.f;
-      float through = 0.f, ka = 0.f, pc[NP], pd[NP], hb[NP];
-#pragma unroll
-      for (int i = 0; i < NP; ++i) hb[i] = hs[j][i];
-      if (m.start >> j & 1) entering_state<NP>(p, q.seq(), w.d, hb);
-#pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        const float a = exp2_hw(db[j] * A2[i]);
-        const float d = fmaf(Cv[i], g, dh[i]);
-        pc[i] = g * hs[j + 1][i];
-        pd[i] = d * x;
-        through = fmaf(d, Bv[i], through);
-        dh[i] = d * a;
-        const float k = dh[i] * hb[i];
-        dA[i] = fmaf(k, db[j], dA[i]);
-        ka = fmaf(k, A2[i], ka);
-      }
-      float* pb_ = p.part_bc + (((int64_t)tig * p.rows * p.L + flat + t) * p.G + w.g) * 2 * p.N;
-#pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        const float sb = wave_sum(pd[i]), sc = wave_sum(pc[i]);
-        if (w.lane == 0 && i < p.N) { pb_[i] = sb; pb_[p.N + i] = sc; }
-      }
-      dD = fmaf(g, ub[j], dD);
-      float dd = fmaf(ka, LN2_F, through * ub[j]);
-      if (p.softplus) dd *= sigmoid_hw(pb[j]);
-      dbias += dd;
-      if (w.on) {
-        ((T*)p.du)[o] = from_f32<T>(fmaf(through, db[j], Dp * g));
-        ((T*)p.ddelta)[o] = from_f32<T>(dd);
-      }
-      if (m.start >> j & 1) {
-        if (p.dstate0 && w.on) store_state<NP>(p.dstate0, q.seq(), p, w.d, dh);
-        if (PACKED) q.prev((int)t - 1);
-      }
+    }
+    __syncthreads();           // the other parity's buffer was read before the last of these, so one barrier is enough
+    for (int i = threadIdx.x; i < n * 2 * p.N; i += 256) {
+      const int j = i / (2 * p.N), c = i % (2 * p.N), k = c < p.N ? c : c - p.N + NP;
+      const float s = (red[turn][j][0][k] + red[turn][j][1][k]) + (red[turn][j][2][k] + red[turn][j][3][k]);
+      p.part_bc[(((int64_t)w.part * p.rows * p.L + flat + t0 + j) * p.G + w.g) * 2 * p.N + c] = s;
     }
   }
-  if (w.on) {
-    float* pa = p.part_a + (int64_t)row * (p.N + 2) * p.D + w.d;
+  if (w.on && !idle) {
+    float* pa = p.part_a + ((int64_t)row * p.nch + w.chunk) * (p.N + 2) * p.D + w.d;
 #pragma unroll
     for (int i = 0; i < NP; ++i)
       if (i < p.N) pa[(int64_t)i * p.D] = dA[i];
@@ -391,8 +590,24 @@ static void scan_shape(ScanArgs& p, int64_t rows, int64_t L, int64_t D, int64_t 
   p.rows = (int)rows; p.L = (int)L; p.D = (int)D; p.G = (int)G; p.N = (int)N; p.S = (int)S;
   p.Dg = (int)(D / G);
   p.tpg = (p.Dg + 63) / 64;
-  p.ntiles = p.tpg * p.G;
+  p.wpg = p.G * ((p.tpg + 3) / 4);
   p.blocks = (int)ceil_div64(L, SCAN_Q);
+  // as many chunks as it takes to reach SCAN_WAVES waves, none shorter than SCAN_MIN_CHUNK tokens
+  const int64_t waves = rows * p.tpg * G;
+  int64_t n = waves > 0 ? ceil_div64(SCAN_WAVES, waves) : 1;
+  const int64_t most = L / SCAN_MIN_CHUNK;
+  n = n < most ? n : most;
+  p.CL = (int)(n > 1 ? ceil_div64(ceil_div64(L, n), SCAN_Q) * SCAN_Q : p.blocks * SCAN_Q);
+  p.nch = (int)(L > 0 ? ceil_div64(L, p.CL) : 1);
+}
+
+// where the states that enter the chunks lie: among those that training keeps, else in scratch of their own
+static float* scan_scratch(ScanArgs& p, float* ws) {
+  if (p.ckpt) { p.enter = p.ckpt; p.enter_row = p.blocks; p.enter_step = p.CL / SCAN_Q; }
+  else { p.enter = ws; p.enter_row = p.nch; p.enter_step = 1; ws += (int64_t)p.rows * p.nch * p.N * p.D; }
+  p.sumdt = ws; ws += (int64_t)p.rows * p.nch * p.D;
+  p.keep = ws;
+  return ws + (((int64_t)p.rows * p.nch + 3) & ~3ll);
 }
 
 // whether B and C of every token and group can be read as whole aligned words
@@ -403,23 +618,38 @@ static bool scan_words(const ScanArgs& p, int dtype, int NP) {
   return !(odd & 1) && !(((uintptr_t)p.B | (uintptr_t)p.C) & 3);
 }
 
-#define SCAN_LAUNCH(K, T, NP, grid, p, s)                                                             \
+template <typename T, int NP, bool PACKED, bool FAST> static void scan_fwd_launch(const ScanArgs& p, hipStream_t s) {
+  const dim3 grid((unsigned)((int64_t)p.rows * p.nch * p.wpg)), block(256);
+  if (p.nch > 1) {
+    DVAE_LAUNCH((scan_fwd_kernel<T, NP, PACKED, FAST, true>), grid, block, 0, s, p);
+    DVAE_LAUNCH((scan_join_kernel<false>), dim3((unsigned)ceil_div64((int64_t)p.N * p.D, 256), p.rows), block, 0, s, p);
+  }
+  DVAE_LAUNCH((scan_fwd_kernel<T, NP, PACKED, FAST, false>), grid, block, 0, s, p);
+}
+template <typename T, int NP, bool PACKED, bool FAST> static void scan_bwd_launch(const ScanArgs& p, hipStream_t s) {
+  const dim3 grid((unsigned)((int64_t)p.rows * p.nch * p.wpg)), block(256);
+  if (p.nch > 1) {
+    DVAE_LAUNCH((scan_bwd_state_kernel<T, NP, PACKED, FAST>), grid, block, 0, s, p);
+    DVAE_LAUNCH((scan_join_kernel<true>), dim3((unsigned)ceil_div64((int64_t)p.N * p.D, 256), p.rows), block, 0, s, p);
+  }
+  DVAE_LAUNCH((scan_bwd_kernel<T, NP, PACKED, FAST>), grid, block, 0, s, p);
+}
+
+#define SCAN_LAUNCH(K, T, NP, p, s)                                                                   \
   do {                                                                                                \
     const bool fast__ = scan_words(p, sizeof(T) == 4 ? DVAE_DT_F32 : DVAE_DT_BF16, NP);               \
     if (p.offsets) {                                                                                  \
-      if (fast__) DVAE_LAUNCH((K<T, NP, true, true>), dim3(grid), dim3(256), 0, s, p);                \
-      else DVAE_LAUNCH((K<T, NP, true, false>), dim3(grid), dim3(256), 0, s, p);                      \
+      if (fast__) K<T, NP, true, true>(p, s); else K<T, NP, true, false>(p, s);                       \
     } else {                                                                                          \
-      if (fast__) DVAE_LAUNCH((K<T, NP, false, true>), dim3(grid), dim3(256), 0, s, p);               \
-      else DVAE_LAUNCH((K<T, NP, false, false>), dim3(grid), dim3(256), 0, s, p);                     \
+      if (fast__) K<T, NP, false, true>(p, s); else K<T, NP, false, false>(p, s);                     \
     }                                                                                                 \
   } while (0)
-#define SCAN_DISPATCH(K, dtype, grid, p, s)                                                           \
+#define SCAN_DISPATCH(K, dtype, p, s)                                                                 \
   do {                                                                                                \
     if (dtype == DVAE_DT_F32) {                                                                       \
-      if (p.N <= 8) SCAN_LAUNCH(K, float, 8, grid, p, s); else SCAN_LAUNCH(K, float, 16, grid, p, s); \
+      if (p.N <= 8) SCAN_LAUNCH(K, float, 8, p, s); else SCAN_LAUNCH(K, float, 16, p, s);             \
     } else {                                                                                          \
-      if (p.N <= 8) SCAN_LAUNCH(K, bf16_t, 8, grid, p, s); else SCAN_LAUNCH(K, bf16_t, 16, grid, p, s); \
+      if (p.N <= 8) SCAN_LAUNCH(K, bf16_t, 8, p, s); else SCAN_LAUNCH(K, bf16_t, 16, p, s);           \
     }                                                                                                 \
   } while (0)
 
@@ -427,9 +657,19 @@ extern "C" int64_t dvae_selective_scan_ckpt_floats(int64_t rows, int64_t L, int6
   return rows * ceil_div64(L, SCAN_Q) * N * D;
 }
 
+extern "C" int64_t dvae_selective_scan_fwd_ws_floats(int64_t rows, int64_t L, int64_t D, int64_t G, int64_t N, int keep) {
+  ScanArgs p = {};
+  if (rows * L <= 0 || D <= 0 || G <= 0) return 0;
+  scan_shape(p, rows, L, D, G, N, 1);
+  return p.nch == 1 ? 0 : rows * p.nch * ((keep ? 1 : N + 1) * D + 1) + 4;
+}
+
 extern "C" int64_t dvae_selective_scan_bwd_ws_floats(int64_t rows, int64_t L, int64_t D, int64_t G, int64_t N) {
-  const int64_t tpg = ceil_div64(D / G, 64);
-  return tpg * rows * L * G * 2 * N + rows * (N + 2) * D;
+  ScanArgs p = {};
+  if (rows * L <= 0 || D <= 0 || G <= 0) return 0;
+  scan_shape(p, rows, L, D, G, N, 1);
+  const int64_t parts = (p.tpg + 3) / 4, chunks = rows * p.nch;
+  return parts * rows * L * G * 2 * N + chunks * (N + 2) * D + (p.nch == 1 ? 0 : chunks * ((N + 1) * D + 1) + 4);
 }
 
 extern "C" int dvae_selective_scan_fwd(const void* u, int64_t u_sb, int64_t u_st, const void* delta, int64_t delta_sb,
@@ -438,7 +678,7 @@ extern "C" int dvae_selective_scan_fwd(const void* u, int64_t u_sb, int64_t u_st
                                        const float* Dp, const void* z, int64_t z_sb, int64_t z_st, const float* bias,
                                        int softplus, const float* state0, float* state1, const int32_t* offsets,
                                        void* out, float* ckpt, int64_t rows, int64_t L, int64_t D, int64_t G, int64_t N,
-                                       int64_t S, int dtype, dvae_stream_t stream) {
+                                       int64_t S, int dtype, float* ws, dvae_stream_t stream) {
   const int rc = scan_check("selective_scan_fwd", rows, L, D, G, N, S, offsets, dtype);
   if (rc) return rc;
   if (rows * L == 0) return 0;
@@ -448,11 +688,11 @@ extern "C" int dvae_selective_scan_fwd(const void* u, int64_t u_sb, int64_t u_st
   p.Dp = Dp; p.z = z; p.z_sb = z_sb; p.z_st = z_st; p.bias = bias; p.softplus = softplus;
   p.state0 = state0; p.state1 = state1; p.offsets = offsets; p.out = out; p.ckpt = ckpt;
   scan_shape(p, rows, L, D, G, N, S);
-  const int64_t grid = rows * ceil_div64(p.ntiles, 4);
-  DVAE_REQUIRE(grid < (1ll << 31), "selective_scan_fwd: too many rows");
+  scan_scratch(p, ws);
+  DVAE_REQUIRE(rows * p.nch * p.wpg < (1ll << 31), "selective_scan_fwd: too many rows");
   const int e = dtype == DVAE_DT_F32 ? 4 : 2;
   DVAE_WORK(rows * L * (double)e * ((z ? 4 : 3) * D + 2 * G * N), DVAE_UNIT_BYTE);
-  SCAN_DISPATCH(scan_fwd_kernel, dtype, grid, p, ST(stream));
+  SCAN_DISPATCH(scan_fwd_launch, dtype, p, ST(stream));
   DVAE_LAUNCH_CHECK("selective_scan_fwd");
   return 0;
 }
@@ -478,22 +718,25 @@ extern "C" int dvae_selective_scan_bwd(const void* u, int64_t u_sb, int64_t u_st
   p.dstate1 = dstate1; p.dstate0 = dstate0; p.ckpt = const_cast<float*>(ckpt);
   p.du = du; p.ddelta = ddelta; p.dz = dz;
   scan_shape(p, rows, L, D, G, N, S);
-  p.part_bc = ws;
-  p.part_a = ws + (int64_t)p.tpg * rows * L * G * 2 * N;
-  const int64_t grid = rows * ceil_div64(p.ntiles, 4);
-  DVAE_REQUIRE(grid < (1ll << 31), "selective_scan_bwd: too many rows");
+  const int parts = (p.tpg + 3) / 4;
+  float* after = scan_scratch(p, ws);
+  if (p.nch == 1) after = ws;
+  else { p.leave = after; after += (int64_t)rows * p.nch * N * D; }
+  p.part_bc = after;
+  p.part_a = after + (int64_t)parts * rows * L * G * 2 * N;
+  DVAE_REQUIRE(rows * p.nch * p.wpg < (1ll << 31), "selective_scan_bwd: too many rows");
   const int e = dtype == DVAE_DT_F32 ? 4 : 2;
   DVAE_WORK(rows * L * (double)e * ((z ? 7 : 5) * D + 4 * G * N), DVAE_UNIT_BYTE);
-  SCAN_DISPATCH(scan_bwd_kernel, dtype, grid, p, ST(stream));
+  SCAN_DISPATCH(scan_bwd_launch, dtype, p, ST(stream));
   DVAE_LAUNCH_CHECK("selective_scan_bwd");
   const int64_t bc = rows * L * G;
   const dim3 gbc((unsigned)ceil_div64(bc * 2 * N, 256));
   if (dtype == DVAE_DT_F32)
-    DVAE_LAUNCH((scan_bc_kernel<float>), gbc, dim3(256), 0, ST(stream), p.part_bc, (float*)dB, (float*)dC, bc, p.N, p.tpg);
+    DVAE_LAUNCH((scan_bc_kernel<float>), gbc, dim3(256), 0, ST(stream), p.part_bc, (float*)dB, (float*)dC, bc, p.N, parts);
   else
-    DVAE_LAUNCH((scan_bc_kernel<bf16_t>), gbc, dim3(256), 0, ST(stream), p.part_bc, (bf16_t*)dB, (bf16_t*)dC, bc, p.N, p.tpg);
+    DVAE_LAUNCH((scan_bc_kernel<bf16_t>), gbc, dim3(256), 0, ST(stream), p.part_bc, (bf16_t*)dB, (bf16_t*)dC, bc, p.N, parts);
   DVAE_LAUNCH(scan_params_kernel, dim3((unsigned)ceil_div64((int64_t)(p.N + 2) * D, 256)), dim3(256), 0, ST(stream),
-              p.part_a, dA, dD, dbias, p.rows, p.N, p.D);
+              p.part_a, dA, dD, dbias, p.rows * p.nch, p.N, p.D);
   DVAE_LAUNCH_CHECK("selective_scan_bwd: sums");
   return 0;
 }

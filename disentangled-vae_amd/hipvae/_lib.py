@@ -124,7 +124,8 @@ SIGNATURES = {
                                POINTER(c_int64), F, F, F, F, F, F, F, P, P, P]),
     'dvae_selective_scan_ckpt_floats': (L, [L] * 4),
     'dvae_selective_scan_fwd': (I, [P, L, L, P, L, L, P, P, L, L, L, P, L, L, L, P, P, L, L, P, I, P, P, P, P, P] + [L] * 6
-                                + [I, P]),
+                                + [I, P, P]),
+    'dvae_selective_scan_fwd_ws_floats': (L, [L] * 5 + [I]),
     'dvae_selective_scan_bwd_ws_floats': (L, [L] * 5),
     'dvae_selective_scan_bwd': (I, [P, L, L, P, L, L, P, P, L, L, L, P, L, L, L, P, P, L, L, P, I, P, P, P, L, L, P, P]
                                 + [P] * 9 + [L] * 6 + [I, P, P]),

@@ -1202,8 +1202,10 @@ def selective_scan_fwd(a: ScanArgs, want_state: bool, keep: bool):
         final = _final_like(a.state, (a.S, a.D, a.N), a.u, torch.float32, a.offsets, a.rows * a.L) if want_state else None
         ckpt = torch.empty(int(lib.dvae_selective_scan_ckpt_floats(a.rows, a.L, a.D, a.N)), dtype=torch.float32,
                            device=a.u.device) if keep else None
-        check(lib.dvae_selective_scan_fwd(*a.head(), _p(final), _p(a.offsets), _p(out), _p(ckpt), *a.shape(), _stream()),
-              'selective_scan_fwd')
+        n = int(lib.dvae_selective_scan_fwd_ws_floats(a.rows, a.L, a.D, a.G, a.N, int(keep)))
+        ws = torch.empty(n, dtype=torch.float32, device=a.u.device) if n else None
+        check(lib.dvae_selective_scan_fwd(*a.head(), _p(final), _p(a.offsets), _p(out), _p(ckpt), *a.shape(), _p(ws),
+                                          _stream()), 'selective_scan_fwd')
     return out, final, ckpt
 
 

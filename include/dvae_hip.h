@@ -588,12 +588,13 @@ int dvae_adam_advance_f32(float* dyn, double beta1, double beta2, dvae_stream_t 
  * Final states of sequences without tokens are not written.  ckpt (dvae_selective_scan_ckpt_floats): the states that
  * the backward pass starts from, kept if not NULL. */
 int64_t dvae_selective_scan_ckpt_floats(int64_t rows, int64_t L, int64_t D, int64_t N);
+int64_t dvae_selective_scan_fwd_ws_floats(int64_t rows, int64_t L, int64_t D, int64_t G, int64_t N, int keep /* ckpt given */);
 int dvae_selective_scan_fwd(const void* u, int64_t u_sb, int64_t u_st, const void* delta, int64_t delta_sb,
                             int64_t delta_st, const float* A, const void* B, int64_t B_sb, int64_t B_st, int64_t B_sg,
                             const void* C, int64_t C_sb, int64_t C_st, int64_t C_sg, const float* Dp, const void* z,
                             int64_t z_sb, int64_t z_st, const float* bias, int softplus, const float* state0,
                             float* state1, const int32_t* offsets, void* out, float* ckpt, int64_t rows, int64_t L,
-                            int64_t D, int64_t G, int64_t N, int64_t S, int dtype, dvae_stream_t stream);
+                            int64_t D, int64_t G, int64_t N, int64_t S, int dtype, float* ws, dvae_stream_t stream);
 /* Gradients from dout and (NULL: zero) dstate1, the gradient of the final states.  dA, dD, dbias, dstate0 may be NULL;
  * dstate0 of sequences without tokens is not written.  ckpt as the forward pass filled it. */
 int64_t dvae_selective_scan_bwd_ws_floats(int64_t rows, int64_t L, int64_t D, int64_t G, int64_t N);

@@ -78,7 +78,7 @@ def _scan_fwd(rows=2, L=8, D=16, G=1, N=16, S=2, dtype=0, offsets=None):
     lib = _lib()
     n = None
     return lib.dvae_selective_scan_fwd(n, 0, 0, n, 0, 0, n, n, 0, 0, 0, n, 0, 0, 0, n, n, 0, 0, n, 1, n, n, offsets, n, n,
-                                       rows, L, D, G, N, S, dtype, n)
+                                       rows, L, D, G, N, S, dtype, n, n)
 
 
 @pytest.mark.parametrize('bad,text', [
