@@ -88,6 +88,50 @@ template <typename T, int NP> struct BCLoad<T, NP, false> {
   }
 };
 
+// The same, requested ahead.  Scalar loads return in any order, so waiting for one means waiting for all: `arrived`
+// makes the words of this token a dependence of the address of the next one's, which puts the wait before the next
+// request and a token's arithmetic between a request and its wait.
+template <int K> struct Words { typedef uint32_t vec __attribute__((ext_vector_type(K), aligned(4))); };
+template <typename T, int NP, bool FAST> struct BCAhead {
+  typename Words<NP * sizeof(T) / 4>::vec b, c;
+  typedef typename Words<NP * sizeof(T) / 4>::vec vec;
+  __device__ __forceinline__ void request(const T* B, const T* C, int) {
+    b = *(const DVAE_UNIFORM vec*)(uint64_t)B;
+    c = *(const DVAE_UNIFORM vec*)(uint64_t)C;
+  }
+  __device__ __forceinline__ void request_b(const T* B, int) { b = *(const DVAE_UNIFORM vec*)(uint64_t)B; }
+  __device__ __forceinline__ void arrived(const T*& B, const T*& C) {
+    asm volatile("" : "+s"(b), "+s"(c), "+s"(B), "+s"(C));
+  }
+  __device__ __forceinline__ void arrived_b(const T*& B) { asm volatile("" : "+s"(b), "+s"(B)); }
+  static __device__ __forceinline__ void unpack(const vec w, float (&v)[NP]) {
+#pragma unroll
+    for (int n = 0; n < NP; ++n)
+      v[n] = sizeof(T) == 4 ? __uint_as_float(w[n * sizeof(T) / 4])
+                            : __uint_as_float(n & 1 ? w[n / 2] & 0xffff0000u : w[n / 2] << 16);
+  }
+  __device__ __forceinline__ void get(float (&bv)[NP], float (&cv)[NP]) const { unpack(b, bv); unpack(c, cv); }
+  __device__ __forceinline__ void get_b(float (&bv)[NP]) const { unpack(b, bv); }
+};
+template <typename T, int NP> struct BCAhead<T, NP, false> {
+  float b[NP], c[NP];
+  __device__ __forceinline__ void request(const T* B, const T* C, int N) {
+    BCLoad<T, NP, false>::get(B, 0, N, b);
+    BCLoad<T, NP, false>::get(C, 0, N, c);
+  }
+  __device__ __forceinline__ void request_b(const T* B, int N) { BCLoad<T, NP, false>::get(B, 0, N, b); }
+  __device__ __forceinline__ void arrived(const T*&, const T*&) {}
+  __device__ __forceinline__ void arrived_b(const T*&) {}
+  __device__ __forceinline__ void get(float (&bv)[NP], float (&cv)[NP]) const {
+#pragma unroll
+    for (int n = 0; n < NP; ++n) { bv[n] = b[n]; cv[n] = c[n]; }
+  }
+  __device__ __forceinline__ void get_b(float (&bv)[NP]) const {
+#pragma unroll
+    for (int n = 0; n < NP; ++n) bv[n] = b[n];
+  }
+};
+
 // One wave: 64 channels of one group, one chunk of one row.  A workgroup's four waves are neighbours in a group.
 struct Tile {
   int g, d, lane, wave, part, chunk, row, t0, t1;
@@ -134,16 +178,31 @@ __device__ __forceinline__ void entering_state(const ScanArgs& p, int64_t seq, i
   }
 }
 
-template <int NP>
+// An element of a row: wave-uniform address of the row, the lane's place in it in bytes.  The address is kept in scalar
+// registers (else the compiler adds the lane's place first, once, and the row's in 64-bit vector arithmetic per access).
+#define DVAE_GLOBAL __attribute__((address_space(1)))
+template <typename T> __device__ __forceinline__ T lane_load(const T* row, uint32_t at) {
+  uint64_t r = (uint64_t)row;
+  asm("" : "+s"(r));
+  return *(const DVAE_GLOBAL T*)((const DVAE_GLOBAL char*)r + at);
+}
+template <typename T> __device__ __forceinline__ void lane_store(T* row, uint32_t at, T v) {
+  uint64_t r = (uint64_t)row;
+  asm("" : "+s"(r));
+  *(DVAE_GLOBAL T*)((DVAE_GLOBAL char*)r + at) = v;
+}
+
+// FULL: all NP states exist
+template <int NP, bool FULL>
 __device__ __forceinline__ void load_slot(const float* slot, const ScanArgs& p, int d, float (&h)[NP]) {
 #pragma unroll
-  for (int n = 0; n < NP; ++n) h[n] = n < p.N ? slot[(int64_t)n * p.D + d] : 0.f;
+  for (int n = 0; n < NP; ++n) h[n] = FULL || n < p.N ? lane_load(slot + (int64_t)n * p.D, d * 4u) : 0.f;
 }
-template <int NP>
+template <int NP, bool FULL>
 __device__ __forceinline__ void store_slot(float* slot, const ScanArgs& p, int d, const float (&h)[NP]) {
 #pragma unroll
   for (int n = 0; n < NP; ++n)
-    if (n < p.N) slot[(int64_t)n * p.D + d] = h[n];
+    if (FULL || n < p.N) lane_store(slot + (int64_t)n * p.D, d * 4u, h[n]);
 }
 __device__ __forceinline__ float* enter_slot(const ScanArgs& p, int row, int chunk) {
   return p.enter + ((int64_t)row * p.enter_row + (int64_t)chunk * p.enter_step) * p.N * p.D;
@@ -152,7 +211,33 @@ __device__ __forceinline__ float* leave_slot(const ScanArgs& p, int row, int chu
   return p.leave + ((int64_t)row * p.nch + chunk) * p.N * p.D;
 }
 
-// STATE_ONLY: the chunk's last state from a zero start, into the next chunk's slot; else the outputs
+// What a block of tokens reads per channel, as stored.  Tokens past the chunk's last are the last one again.
+template <typename T> struct FwdRaw {
+  T u[SCAN_Q], dl[SCAN_Q], z[SCAN_Q];
+  // from the rows that the pointers are at; they end up at the block's last row
+  template <bool Z>
+  __device__ __forceinline__ void load(const T*& up, int64_t u_st, const T*& dp, int64_t d_st, const T*& zp, int64_t z_st,
+                                       int n, uint32_t at) {
+#pragma unroll
+    for (int j = 0; j < SCAN_Q; ++j) {
+      u[j] = lane_load(up, at);
+      dl[j] = lane_load(dp, at);
+      if (Z) z[j] = lane_load(zp, at);
+      const bool more = j + 1 < SCAN_Q && j + 1 < n;
+      up += more ? u_st : 0;
+      dp += more ? d_st : 0;
+      if (Z) zp += more ? z_st : 0;
+    }
+  }
+};
+
+// STATE_ONLY: the chunk's last state from a zero start, into the next chunk's slot; else the outputs.
+//
+// A block of SCAN_Q tokens in which no sequence starts or ends is straight-line code: its inputs were requested a block
+// ahead, and the compiler can request B and C tokens ahead.  Nothing in it is conditional.  Lanes past the group's last
+// channel compute that channel too and store the same values to the same places; tokens past the chunk's last repeat the
+// last one with a step size of 0, which leaves the state as it is and gives the same output again.
+// Other blocks (packed sequences' borders) go token by token.
 template <typename T, int NP, bool PACKED, bool FAST, bool STATE_ONLY>
 __global__ void __launch_bounds__(256) scan_fwd_kernel(ScanArgs p) {
   const Tile w(p);
@@ -164,38 +249,97 @@ __global__ void __launch_bounds__(256) scan_fwd_kernel(ScanArgs p) {
     A2[n] = n < p.N ? p.A[(int64_t)w.d * p.N + n] * LOG2E_F : 0.f;
     h[n] = 0.f;
   }
-  if (!STATE_ONLY && w.chunk > 0) load_slot<NP>(enter_slot(p, row, w.chunk), p, w.d, h);
+  if (!STATE_ONLY && w.chunk > 0) load_slot<NP, FAST>(enter_slot(p, row, w.chunk), p, w.d, h);
+  if (!PACKED && w.chunk == 0) entering_state<NP>(p, row, w.d, h);
   const float Dp = p.Dp ? p.Dp[w.d] : 0.f, bias = p.bias ? p.bias[w.d] : 0.f;
+  const bool gated = p.z != nullptr, plus = p.softplus;
   const T* u = (const T*)p.u + row * p.u_sb;
   const T* dl = (const T*)p.delta + row * p.delta_sb;
-  const T* z = p.z ? (const T*)p.z + row * p.z_sb : nullptr;
+  const T* z = gated ? (const T*)p.z + row * p.z_sb : u;        // (read and not used without z)
+  const int64_t z_st = gated ? p.z_st : p.u_st;
   const T* B = (const T*)p.B + row * p.B_sb + w.g * p.B_sg;
   const T* C = (const T*)p.C + row * p.C_sb + w.g * p.C_sg;
   T* out = (T*)p.out + (int64_t)row * p.L * p.D;
+  const uint32_t at = w.d * (uint32_t)sizeof(T);
   SeqWalk q = {p.offsets, p.S, p.L, p.L, row, 0, p.L};
   if (PACKED) q.seek(w.t0);
   float total = 0.f;
   bool cut = false;
+  FwdRaw<T> next;
+  BCAhead<T, NP, FAST> ahead;
+  const T *un = u + w.t0 * p.u_st, *dn = dl + w.t0 * p.delta_st, *zn = z + w.t0 * z_st;    // rows of the block ahead
+  next.template load<!STATE_ONLY>(un, p.u_st, dn, p.delta_st, zn, z_st, w.t1 - w.t0, at);
 
   for (int t0 = w.t0; t0 < w.t1; t0 += SCAN_Q) {
     const int n = min(SCAN_Q, w.t1 - t0);
-    const Marks m = block_marks<PACKED>(q, t0, n, p.L);
-    if (!STATE_ONLY && p.ckpt && w.on)
-      store_slot<NP>(p.ckpt + ((int64_t)row * p.blocks + t0 / SCAN_Q) * p.N * p.D, p, w.d, h);
+    const FwdRaw<T> raw = next;
+    const int left = w.t1 - t0 - SCAN_Q;
+    un += left > 0 ? p.u_st : 0;
+    dn += left > 0 ? p.delta_st : 0;
+    zn += left > 0 ? z_st : 0;
+    next.template load<!STATE_ONLY>(un, p.u_st, dn, p.delta_st, zn, z_st, left, at);
+    if (!STATE_ONLY && p.ckpt)
+      store_slot<NP, FAST>(p.ckpt + ((int64_t)row * p.blocks + t0 / SCAN_Q) * p.N * p.D, p, w.d, h);
+    Marks m = {0u, 0u, 0u};
+    if (PACKED) m = block_marks<PACKED>(q, t0, n, p.L);
+    if (!PACKED || !(m.start | m.end | (m.valid ^ ((1u << n) - 1u)))) {
+      const T *Bt = B + t0 * p.B_st, *Ct = C + t0 * p.C_st;
+      T* ot = out + (int64_t)t0 * p.D;
+      if (STATE_ONLY) ahead.request_b(Bt, p.N);
+      else ahead.request(Bt, Ct, p.N);
+#pragma unroll
+      for (int j = 0; j < SCAN_Q; ++j) {
+        BCAhead<T, NP, FAST> now = ahead;
+        float Bv[NP], Cv[NP];
+        Bt += j + 1 < n ? p.B_st : 0;
+        Ct += j + 1 < n ? p.C_st : 0;
+        if (STATE_ONLY) {
+          now.arrived_b(Bt);
+          if (j + 1 < SCAN_Q) ahead.request_b(Bt, p.N);
+          now.get_b(Bv);
+        } else {
+          now.arrived(Bt, Ct);
+          if (j + 1 < SCAN_Q) ahead.request(Bt, Ct, p.N);
+          now.get(Bv, Cv);
+        }
+        const float uu = to_f32(raw.u[j]);
+        const float pre = to_f32(raw.dl[j]) + bias;
+        const float sp = softplus_hw(pre);
+        const float dt = j < n ? (plus ? sp : pre) : 0.f;
+        const float x = dt * uu;
+        if (STATE_ONLY) {
+          total += dt;
+#pragma unroll
+          for (int i = 0; i < NP; ++i) h[i] = fmaf(exp2_hw(dt * A2[i]), h[i], x * Bv[i]);
+        } else {
+          float y = Dp * uu;
+#pragma unroll
+          for (int i = 0; i < NP; ++i) {
+            h[i] = fmaf(exp2_hw(dt * A2[i]), h[i], x * Bv[i]);
+            y = fmaf(Cv[i], h[i], y);
+          }
+          const float zz = to_f32(raw.z[j]);
+          const float gate = zz * sigmoid_hw(zz);
+          lane_store(ot, at, from_f32<T>(gated ? y * gate : y));
+          ot += j + 1 < n ? p.D : 0;
+        }
+      }
+      continue;
+    }
 #pragma unroll 1
     for (int j = 0; j < n; ++j) {
       const int64_t t = t0 + j;
       if (!(m.valid >> j & 1)) {
-        if (!STATE_ONLY && w.on) out[t * p.D + w.d] = from_f32<T>(0.f);
+        if (!STATE_ONLY) lane_store(out + t * p.D, at, from_f32<T>(0.f));
         continue;
       }
       if (m.start >> j & 1) {
         entering_state<NP>(p, q.seq(), w.d, h);
         cut = true;
       }
-      const float uu = to_f32(u[t * p.u_st + w.d]);
-      const float pre = to_f32(dl[t * p.delta_st + w.d]) + bias;
-      const float dt = p.softplus ? softplus_hw(pre) : pre;
+      const float uu = to_f32(lane_load(u + t * p.u_st, at));
+      const float pre = to_f32(lane_load(dl + t * p.delta_st, at)) + bias;
+      const float dt = plus ? softplus_hw(pre) : pre;
       float Bv[NP];
       BCLoad<T, NP, FAST>::get(B, t * p.B_st, p.N, Bv);
       const float x = dt * uu;
@@ -212,24 +356,26 @@ __global__ void __launch_bounds__(256) scan_fwd_kernel(ScanArgs p) {
           h[i] = fmaf(exp2_hw(dt * A2[i]), h[i], x * Bv[i]);
           y = fmaf(Cv[i], h[i], y);
         }
-        if (z) {
-          const float zz = to_f32(z[t * p.z_st + w.d]);
+        if (gated) {
+          const float zz = to_f32(lane_load(z + t * z_st, at));
           y *= zz * sigmoid_hw(zz);
         }
-        if (w.on) out[t * p.D + w.d] = from_f32<T>(y);
+        lane_store(out + t * p.D, at, from_f32<T>(y));
       }
       if (m.end >> j & 1) {
         if (!STATE_ONLY && p.state1 && w.on) store_state<NP>(p.state1, q.seq(), p, w.d, h);
-        if (PACKED) q.next((int)t + 1);
+        q.next((int)t + 1);
       }
     }
   }
   if (STATE_ONLY) {
     if (w.on) {
-      store_slot<NP>(enter_slot(p, row, w.chunk + 1), p, w.d, h);
+      store_slot<NP, FAST>(enter_slot(p, row, w.chunk + 1), p, w.d, h);
       p.sumdt[((int64_t)row * p.nch + w.chunk) * p.D + w.d] = total;
     }
     if (w.g == 0 && w.part == 0 && threadIdx.x == 0) p.keep[row * p.nch + w.chunk] = cut ? 0.f : 1.f;
+  } else if (!PACKED && p.state1 && w.on && w.chunk + 1 == p.nch) {
+    store_state<NP>(p.state1, row, p, w.d, h);
   }
 }
 
@@ -373,7 +519,7 @@ __global__ void __launch_bounds__(256) scan_bwd_state_kernel(ScanArgs p) {
     }
   }
   if (w.on) {
-    store_slot<NP>(leave_slot(p, row, w.chunk - 1), p, w.d, x);
+    store_slot<NP, FAST>(leave_slot(p, row, w.chunk - 1), p, w.d, x);
     p.sumdt[((int64_t)row * p.nch + w.chunk) * p.D + w.d] = total;
   }
   if (w.g == 0 && w.part == 0 && threadIdx.x == 0) p.keep[row * p.nch + w.chunk] = cut ? 0.f : 1.f;
@@ -391,7 +537,7 @@ __global__ void __launch_bounds__(256) scan_bwd_kernel(ScanArgs p) {
     A2[n] = n < p.N ? p.A[(int64_t)w.d * p.N + n] * LOG2E_F : 0.f;
     dh[n] = dA[n] = 0.f;
   }
-  if (w.chunk + 1 < p.nch && !idle) load_slot<NP>(leave_slot(p, row, w.chunk), p, w.d, dh);
+  if (w.chunk + 1 < p.nch && !idle) load_slot<NP, FAST>(leave_slot(p, row, w.chunk), p, w.d, dh);
   float dD = 0.f, dbias = 0.f;
   const float Dp = p.Dp ? p.Dp[w.d] : 0.f, bias = p.bias ? p.bias[w.d] : 0.f;
   const T* u = (const T*)p.u + row * p.u_sb;
@@ -417,7 +563,7 @@ __global__ void __launch_bounds__(256) scan_bwd_kernel(ScanArgs p) {
       for (int i = w.lane; i < SCAN_Q * 2 * NP; i += 64) red[turn][i / (2 * NP)][w.wave][i % (2 * NP)] = 0.f;
     } else {
       float hs[SCAN_Q + 1][NP];
-      load_slot<NP>(p.ckpt + ((int64_t)row * p.blocks + t0 / SCAN_Q) * p.N * p.D, p, w.d, hs[0]);
+      load_slot<NP, FAST>(p.ckpt + ((int64_t)row * p.blocks + t0 / SCAN_Q) * p.N * p.D, p, w.d, hs[0]);
       float ub[SCAN_Q], pb[SCAN_Q], db[SCAN_Q];
 #pragma unroll
       for (int j = 0; j < SCAN_Q; ++j) {

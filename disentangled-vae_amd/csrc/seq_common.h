@@ -6,14 +6,14 @@
 
 #define ST(s) ((hipStream_t)(s))
 
-struct bf16_t { uint16_t bits; };
+enum bf16_t : uint16_t {};
 
 __device__ __forceinline__ float to_f32(float v) { return v; }
-__device__ __forceinline__ float to_f32(bf16_t v) { return __uint_as_float((uint32_t)v.bits << 16); }
+__device__ __forceinline__ float to_f32(bf16_t v) { return __uint_as_float((uint32_t)v << 16); }
 template <typename T> __device__ __forceinline__ T from_f32(float v);
 template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
 template <> __device__ __forceinline__ bf16_t from_f32<bf16_t>(float v) {      // round to nearest even
-  return bf16_t{__builtin_bit_cast(uint16_t, (__bf16)v)};
+  return (bf16_t)__builtin_bit_cast(uint16_t, (__bf16)v);
 }
 
 // V consecutive elements, moved as accesses of up to 16 bytes (V > 1 only where the host checked alignment)
