@@ -104,6 +104,7 @@ template <typename T, int NP, bool FAST> struct BCAhead {
     asm volatile("" : "+s"(b), "+s"(c), "+s"(B), "+s"(C));
   }
   __device__ __forceinline__ void arrived_b(const T*& B) { asm volatile("" : "+s"(b), "+s"(B)); }
+  // (alone, C travels in b's place: request_b, arrived_b and get_b serve either)
   static __device__ __forceinline__ void unpack(const vec w, float (&v)[NP]) {
 #pragma unroll
     for (int n = 0; n < NP; ++n)
@@ -466,6 +467,27 @@ template <int M> struct WaveSums {
   }
 };
 
+// What a block of tokens reads per channel on the way back, as stored; tokens past the chunk's last are the last one again.
+template <typename T> struct BwdRaw {
+  T u[SCAN_Q], dl[SCAN_Q], z[SCAN_Q], g[SCAN_Q];
+  template <bool U>
+  __device__ __forceinline__ void load(const T* up, int64_t u_st, const T* dp, int64_t d_st, const T* zp, int64_t z_st,
+                                       const T* gp, int64_t g_st, int n, uint32_t at) {
+#pragma unroll
+    for (int j = 0; j < SCAN_Q; ++j) {
+      if (U) u[j] = lane_load(up, at);
+      dl[j] = lane_load(dp, at);
+      z[j] = lane_load(zp, at);
+      g[j] = lane_load(gp, at);
+      const bool more = j + 1 < SCAN_Q && j + 1 < n;
+      if (U) up += more ? u_st : 0;
+      dp += more ? d_st : 0;
+      zp += more ? z_st : 0;
+      gp += more ? g_st : 0;
+    }
+  }
+};
+
 // The adjoint that leaves a chunk to the left if nothing enters it from the right: the sum of C[n] g of its tokens up to
 // the first start of a sequence, each through the decays from the chunk's first token to its own.
 template <typename T, int NP, bool PACKED, bool FAST>
@@ -480,27 +502,61 @@ __global__ void __launch_bounds__(256) scan_bwd_state_kernel(ScanArgs p) {
     x[n] = 0.f;
   }
   const float bias = p.bias ? p.bias[w.d] : 0.f;
+  const bool gated = p.z != nullptr, plus = p.softplus;
   const T* dl = (const T*)p.delta + row * p.delta_sb;
-  const T* z = p.z ? (const T*)p.z + row * p.z_sb : nullptr;
   const T* go = (const T*)p.dout + row * p.dout_sb;
+  const T* z = gated ? (const T*)p.z + row * p.z_sb : go;
+  const int64_t z_st = gated ? p.z_st : p.dout_st;
   const T* C = (const T*)p.C + row * p.C_sb + w.g * p.C_sg;
+  const uint32_t at = w.d * (uint32_t)sizeof(T);
   SeqWalk q = {p.offsets, p.S, p.L, p.L, row, 0, p.L};
   if (PACKED) q.seek(w.t0);
   float total = 0.f;
   bool cut = false;
+  BwdRaw<T> next;
+  next.template load<false>(nullptr, 0, dl + w.t0 * p.delta_st, p.delta_st, z + w.t0 * z_st, z_st,
+                            go + w.t0 * p.dout_st, p.dout_st, w.t1 - w.t0, at);
   for (int t0 = w.t0; t0 < w.t1 && !cut; t0 += SCAN_Q) {
     const int n = min(SCAN_Q, w.t1 - t0);
-    const Marks m = block_marks<PACKED>(q, t0, n, p.L);
+    const BwdRaw<T> raw = next;
+    const int64_t tn = min(t0 + SCAN_Q, w.t1 - 1);
+    next.template load<false>(nullptr, 0, dl + tn * p.delta_st, p.delta_st, z + tn * z_st, z_st, go + tn * p.dout_st,
+                              p.dout_st, w.t1 - t0 - SCAN_Q, at);
+    Marks m = {0u, 0u, 0u};
+    if (PACKED) m = block_marks<PACKED>(q, t0, n, p.L);
+    if (!PACKED || !(m.start | m.end | (m.valid ^ ((1u << n) - 1u)))) {
+      BCAhead<T, NP, FAST> ahead;
+      const T* Ct = C + t0 * p.C_st;
+      ahead.request_b(Ct, p.N);
+#pragma unroll
+      for (int j = 0; j < SCAN_Q; ++j) {
+        BCAhead<T, NP, FAST> now = ahead;
+        float Cv[NP];
+        Ct += j + 1 < n ? p.C_st : 0;
+        now.arrived_b(Ct);
+        if (j + 1 < SCAN_Q) ahead.request_b(Ct, p.N);
+        now.get_b(Cv);
+        const float pre = to_f32(raw.dl[j]) + bias;
+        const float sp = softplus_hw(pre);
+        total += j < n ? (plus ? sp : pre) : 0.f;
+        const float zz = to_f32(raw.z[j]), gate = zz * sigmoid_hw(zz);
+        float g = to_f32(raw.g[j]);
+        g = j < n ? (gated ? g * gate : g) : 0.f;
+#pragma unroll
+        for (int i = 0; i < NP; ++i) x[i] = fmaf(exp2_hw(total * A2[i]), Cv[i] * g, x[i]);
+      }
+      continue;
+    }
 #pragma unroll 1
     for (int j = 0; j < n; ++j) {
       const int64_t t = t0 + j;
       if (!(m.valid >> j & 1)) continue;
       if (m.start >> j & 1) { cut = true; break; }
-      const float pre = to_f32(dl[t * p.delta_st + w.d]) + bias;
-      total += p.softplus ? softplus_hw(pre) : pre;
-      float g = to_f32(go[t * p.dout_st + w.d]);
-      if (z) {
-        const float zz = to_f32(z[t * p.z_st + w.d]);
+      const float pre = to_f32(lane_load(dl + t * p.delta_st, at)) + bias;
+      total += plus ? softplus_hw(pre) : pre;
+      float g = to_f32(lane_load(go + t * p.dout_st, at));
+      if (gated) {
+        const float zz = to_f32(lane_load(z + t * z_st, at));
         g *= zz * sigmoid_hw(zz);
       }
       float Cv[NP];
@@ -514,9 +570,15 @@ __global__ void __launch_bounds__(256) scan_bwd_state_kernel(ScanArgs p) {
 #pragma unroll
           for (int i = 0; i < NP; ++i) x[i] = fmaf(exp2_hw(total * A2[i]), e[i], x[i]);
         }
-        if (PACKED) q.next((int)t + 1);
+        q.next((int)t + 1);
       }
     }
+  }
+  if (!PACKED && p.dstate1 && w.chunk + 1 == p.nch) {
+    float e[NP];
+    load_state<NP>(p.dstate1, row, p, w.d, e);
+#pragma unroll
+    for (int i = 0; i < NP; ++i) x[i] = fmaf(exp2_hw(total * A2[i]), e[i], x[i]);
   }
   if (w.on) {
     store_slot<NP, FAST>(leave_slot(p, row, w.chunk - 1), p, w.d, x);
@@ -526,7 +588,7 @@ __global__ void __launch_bounds__(256) scan_bwd_state_kernel(ScanArgs p) {
 }
 
 template <typename T, int NP, bool PACKED, bool FAST>
-__global__ void __launch_bounds__(256) scan_bwd_kernel(ScanArgs p) {
+__global__ void __launch_bounds__(256, 1) scan_bwd_kernel(ScanArgs p) {
   __shared__ float red[2][SCAN_Q][4][2 * NP];      // [block parity][token][wave][dB, dC]
   const Tile w(p);
   const int row = w.row;
@@ -537,33 +599,126 @@ __global__ void __launch_bounds__(256) scan_bwd_kernel(ScanArgs p) {
     A2[n] = n < p.N ? p.A[(int64_t)w.d * p.N + n] * LOG2E_F : 0.f;
     dh[n] = dA[n] = 0.f;
   }
-  if (w.chunk + 1 < p.nch && !idle) load_slot<NP, FAST>(leave_slot(p, row, w.chunk), p, w.d, dh);
+  if (w.chunk + 1 < p.nch) load_slot<NP, FAST>(leave_slot(p, row, w.chunk), p, w.d, dh);
+  else if (!PACKED && p.dstate1) load_state<NP>(p.dstate1, row, p, w.d, dh);
   float dD = 0.f, dbias = 0.f;
   const float Dp = p.Dp ? p.Dp[w.d] : 0.f, bias = p.bias ? p.bias[w.d] : 0.f;
   const T* u = (const T*)p.u + row * p.u_sb;
   const T* dl = (const T*)p.delta + row * p.delta_sb;
-  const T* z = p.z ? (const T*)p.z + row * p.z_sb : nullptr;
+  const bool gated = p.z != nullptr, plus = p.softplus;
   const T* go = (const T*)p.dout + row * p.dout_sb;
+  const T* z = gated ? (const T*)p.z + row * p.z_sb : go;             // (read and not used without z)
+  const int64_t z_st = gated ? p.z_st : p.dout_st;
+  T* dzp = gated ? (T*)p.dz : (T*)p.du;                                // (written and written over by du without z)
   const T* B = (const T*)p.B + row * p.B_sb + w.g * p.B_sg;
   const T* C = (const T*)p.C + row * p.C_sb + w.g * p.C_sg;
   const int64_t flat = (int64_t)row * p.L;
+  const uint32_t at = w.d * (uint32_t)sizeof(T);
   SeqWalk q = {p.offsets, p.S, p.L, p.L, row, 0, p.L};      // the sequence that the way back is in
   if (PACKED) {                                             // the last one that has a token before the chunk's end
     q.seek(w.t1 - 1);
     if (q.s >= q.S || q.b >= w.t1) q.prev(w.t1 - 1);
   }
   int turn = 0;
+  const int first = w.t0 + (w.t1 - w.t0 - 1) / SCAN_Q * SCAN_Q;
+  const float* ck = p.ckpt + ((int64_t)row * p.blocks + first / SCAN_Q) * p.N * p.D;
+  BwdRaw<T> next;
+  float hn[NP];                                    // the state that enters the block ahead
+  next.template load<true>(u + first * p.u_st, p.u_st, dl + first * p.delta_st, p.delta_st, z + first * z_st, z_st,
+                           go + first * p.dout_st, p.dout_st, w.t1 - first, at);
+  load_slot<NP, FAST>(ck, p, w.d, hn);
 
-  for (int t0 = w.t0 + (w.t1 - w.t0 - 1) / SCAN_Q * SCAN_Q; t0 >= w.t0; t0 -= SCAN_Q, turn ^= 1) {
+  for (int t0 = first; t0 >= w.t0; t0 -= SCAN_Q, turn ^= 1) {
     const int n = min(SCAN_Q, w.t1 - t0);
-    SeqWalk f = q;                                     // and the one that the states' second computation is in
-    if (PACKED) f.seek(t0);
-    const Marks m = block_marks<PACKED>(f, t0, n, p.L);
+    const BwdRaw<T> raw = next;
+    float hs[SCAN_Q + 1][NP];
+#pragma unroll
+    for (int i = 0; i < NP; ++i) hs[0][i] = hn[i];
+    {
+      const int64_t tn = max(t0 - SCAN_Q, w.t0);
+      ck -= t0 > w.t0 ? (int64_t)p.N * p.D : 0;
+      next.template load<true>(u + tn * p.u_st, p.u_st, dl + tn * p.delta_st, p.delta_st, z + tn * z_st, z_st,
+                               go + tn * p.dout_st, p.dout_st, w.t1 - tn, at);
+      load_slot<NP, FAST>(ck, p, w.d, hn);
+    }
+    SeqWalk f = q;                                 // the sequence that the states' second computation is in
+    Marks m = {0u, 0u, 0u};
+    if (PACKED) {
+      f.seek(t0);
+      m = block_marks<PACKED>(f, t0, n, p.L);
+    }
     if (idle) {
       for (int i = w.lane; i < SCAN_Q * 2 * NP; i += 64) red[turn][i / (2 * NP)][w.wave][i % (2 * NP)] = 0.f;
+    } else if (!PACKED || !(m.start | m.end | (m.valid ^ ((1u << n) - 1u)))) {
+      // no sequence starts or ends here: straight-line code, as in the forward pass.  Tokens past the chunk's last have
+      // a step size and a gradient of 0, which changes nothing, and what they store is stored over by the last token.
+      float a[SCAN_Q][NP], db[SCAN_Q], slope[SCAN_Q];
+      BCAhead<T, NP, FAST> ahead;
+      const T *Bt = B + t0 * p.B_st, *Ct = C + t0 * p.C_st;
+      ahead.request_b(Bt, p.N);
+#pragma unroll
+      for (int j = 0; j < SCAN_Q; ++j) {
+        BCAhead<T, NP, FAST> now = ahead;
+        float Bv[NP];
+        Bt += j + 1 < n ? p.B_st : 0;
+        Ct += j + 1 < n ? p.C_st : 0;
+        now.arrived_b(Bt);
+        if (j + 1 < SCAN_Q) ahead.request_b(Bt, p.N);
+        else ahead.request(Bt, Ct, p.N);           // the last token's, where the way back begins
+        now.get_b(Bv);
+        const float pre = to_f32(raw.dl[j]) + bias;
+        const float sp = softplus_hw(pre, slope[j]);
+        db[j] = j < n ? (plus ? sp : pre) : 0.f;
+        slope[j] = plus ? slope[j] : 1.f;
+        const float x = db[j] * to_f32(raw.u[j]);
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          a[j][i] = exp2_hw(db[j] * A2[i]);
+          hs[j + 1][i] = fmaf(a[j][i], hs[j][i], x * Bv[i]);
+        }
+      }
+      int64_t o = (flat + t0 + n - 1) * p.D;
+#pragma unroll
+      for (int j = SCAN_Q - 1; j >= 0; --j) {
+        BCAhead<T, NP, FAST> now = ahead;
+        float Bv[NP], Cv[NP];
+        Bt -= j > 0 && j < n ? p.B_st : 0;
+        Ct -= j > 0 && j < n ? p.C_st : 0;
+        now.arrived(Bt, Ct);
+        if (j > 0) ahead.request(Bt, Ct, p.N);
+        now.get(Bv, Cv);
+        const float uu = to_f32(raw.u[j]), zz = to_f32(raw.z[j]), sg = sigmoid_hw(zz);
+        float g = j < n ? to_f32(raw.g[j]) : 0.f;
+        float y = Dp * uu;
+#pragma unroll
+        for (int i = 0; i < NP; ++i) y = fmaf(Cv[i], hs[j + 1][i], y);
+        lane_store(dzp + o, at, from_f32<T>(g * y * sg * fmaf(zz, 1.f - sg, 1.f)));
+        g = gated ? g * (zz * sg) : g;
+        // lanes past the last channel add nothing to the sums over the channels
+        const float x = w.on ? db[j] * uu : 0.f, gs = w.on ? g : 0.f;
+        float through = 0.f, ka = 0.f, pv[2 * NP];
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          const float d = fmaf(Cv[i], g, dh[i]);
+          pv[i] = d * x;
+          pv[NP + i] = gs * hs[j + 1][i];
+          through = fmaf(d, Bv[i], through);
+          dh[i] = d * a[j][i];
+          const float k = dh[i] * hs[j][i];
+          dA[i] = fmaf(k, db[j], dA[i]);
+          ka = fmaf(k, A2[i], ka);
+        }
+        const float sum = WaveSums<2 * NP>::run(pv, w.lane);
+        if (!(w.lane & (NP == 16 ? 1 : 3))) red[turn][j][w.wave][WaveSums<2 * NP>::index(w.lane)] = sum;
+        dD = fmaf(g, uu, dD);
+        float dd = fmaf(ka, LN2_F, through * uu) * slope[j];
+        dd = j < n ? dd : 0.f;
+        dbias += dd;
+        lane_store((T*)p.du + o, at, from_f32<T>(fmaf(through, db[j], Dp * g)));
+        lane_store((T*)p.ddelta + o, at, from_f32<T>(dd));
+        o -= j < n ? p.D : 0;
+      }
     } else {
-      float hs[SCAN_Q + 1][NP];
-      load_slot<NP, FAST>(p.ckpt + ((int64_t)row * p.blocks + t0 / SCAN_Q) * p.N * p.D, p, w.d, hs[0]);
       float ub[SCAN_Q], pb[SCAN_Q], db[SCAN_Q];
 #pragma unroll
       for (int j = 0; j < SCAN_Q; ++j) {
@@ -571,9 +726,9 @@ __global__ void __launch_bounds__(256) scan_bwd_kernel(ScanArgs p) {
         for (int i = 0; i < NP; ++i) hs[j + 1][i] = hs[j][i];
         if (!(m.valid >> j & 1)) continue;
         const int64_t t = t0 + j;
-        ub[j] = to_f32(u[t * p.u_st + w.d]);
-        pb[j] = to_f32(dl[t * p.delta_st + w.d]) + bias;
-        db[j] = p.softplus ? softplus_hw(pb[j]) : pb[j];
+        ub[j] = to_f32(raw.u[j]);
+        pb[j] = to_f32(raw.dl[j]) + bias;
+        db[j] = plus ? softplus_hw(pb[j]) : pb[j];
         if (m.start >> j & 1) entering_state<NP>(p, f.seq(), w.d, hs[j + 1]);
         float Bv[NP];
         BCLoad<T, NP, FAST>::get(B, t * p.B_st, p.N, Bv);
@@ -590,7 +745,7 @@ __global__ void __launch_bounds__(256) scan_bwd_kernel(ScanArgs p) {
           if (w.on) {
             ((T*)p.du)[o] = from_f32<T>(0.f);
             ((T*)p.ddelta)[o] = from_f32<T>(0.f);
-            if (z) ((T*)p.dz)[o] = from_f32<T>(0.f);
+            if (gated) ((T*)p.dz)[o] = from_f32<T>(0.f);
           }
           if (w.lane < 2 * NP) red[turn][j][w.wave][w.lane] = 0.f;
           continue;
@@ -605,9 +760,9 @@ __global__ void __launch_bounds__(256) scan_bwd_kernel(ScanArgs p) {
         float Bv[NP], Cv[NP];
         BCLoad<T, NP, FAST>::get(B, t * p.B_st, p.N, Bv);
         BCLoad<T, NP, FAST>::get(C, t * p.C_st, p.N, Cv);
-        float g = w.on ? to_f32(go[t * p.dout_st + w.d]) : 0.f;
-        if (z) {
-          const float zz = to_f32(z[t * p.z_st + w.d]);
+        float g = to_f32(raw.g[j]);
+        if (gated) {
+          const float zz = to_f32(raw.z[j]);
           const float sg = sigmoid_hw(zz);
           float y = Dp * ub[j];
 #pragma unroll
@@ -615,7 +770,7 @@ __global__ void __launch_bounds__(256) scan_bwd_kernel(ScanArgs p) {
           if (w.on) ((T*)p.dz)[o] = from_f32<T>(g * y * sg * fmaf(zz, 1.f - sg, 1.f));
           g *= zz * sg;
         }
-        const float x = w.on ? db[j] * ub[j] : 0.f;
+        const float x = w.on ? db[j] * ub[j] : 0.f, gs = w.on ? g : 0.f;
         float through = 0.f, ka = 0.f, pv[2 * NP], hb[NP];
 #pragma unroll
         for (int i = 0; i < NP; ++i) hb[i] = hs[j][i];
@@ -625,7 +780,7 @@ __global__ void __launch_bounds__(256) scan_bwd_kernel(ScanArgs p) {
           const float a = exp2_hw(db[j] * A2[i]);
           const float d = fmaf(Cv[i], g, dh[i]);
           pv[i] = d * x;
-          pv[NP + i] = g * hs[j + 1][i];
+          pv[NP + i] = gs * hs[j + 1][i];
           through = fmaf(d, Bv[i], through);
           dh[i] = d * a;
           const float k = dh[i] * hb[i];
@@ -636,7 +791,7 @@ __global__ void __launch_bounds__(256) scan_bwd_kernel(ScanArgs p) {
         if (!(w.lane & (NP == 16 ? 1 : 3))) red[turn][j][w.wave][WaveSums<2 * NP>::index(w.lane)] = sum;
         dD = fmaf(g, ub[j], dD);
         float dd = fmaf(ka, LN2_F, through * ub[j]);
-        if (p.softplus) dd *= sigmoid_hw(pb[j]);
+        if (plus) dd *= sigmoid_hw(pb[j]);
         dbias += dd;
         if (w.on) {
           ((T*)p.du)[o] = from_f32<T>(fmaf(through, db[j], Dp * g));
@@ -655,6 +810,7 @@ __global__ void __launch_bounds__(256) scan_bwd_kernel(ScanArgs p) {
       p.part_bc[(((int64_t)w.part * p.rows * p.L + flat + t0 + j) * p.G + w.g) * 2 * p.N + c] = s;
     }
   }
+  if (!PACKED && w.chunk == 0 && p.dstate0 && w.on && !idle) store_state<NP>(p.dstate0, row, p, w.d, dh);
   if (w.on && !idle) {
     float* pa = p.part_a + ((int64_t)row * p.nch + w.chunk) * (p.N + 2) * p.D + w.d;
 #pragma unroll

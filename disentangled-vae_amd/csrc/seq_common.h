@@ -49,6 +49,16 @@ __device__ __forceinline__ float softplus_hw(float x) {
   return fmaxf(x, 0.f) + (r == 0.f ? e : l);
 }
 
+// softplus and its derivative, the sigmoid: 1 / (1 + e^-x), with e as above and x < 0 turned round
+__device__ __forceinline__ float softplus_hw(float x, float& slope) {
+  const float e = exp2_hw(-LOG2E_F * fabsf(x));
+  const float w = 1.f + e;
+  const float r = w - 1.f;
+  const float l = LN2_F * __builtin_amdgcn_logf(w) * (e * __builtin_amdgcn_rcpf(r));
+  slope = (x < 0.f ? e : 1.f) * __builtin_amdgcn_rcpf(w);
+  return fmaxf(x, 0.f) + (r == 0.f ? e : l);
+}
+
 // NaN has to come out as NaN: fmaxf(NaN, 0) is 0, but e and with it l are NaN.
 
 // Wave-uniform reads of data that no kernel in flight writes go through the constant address space: the compiler then
