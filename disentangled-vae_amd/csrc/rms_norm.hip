@@ -255,12 +255,10 @@ __global__ void __launch_bounds__(256) norm_dw_any_kernel(NormArgs p, int tiles)
   p.part[part * p.D + d] = a;
 }
 
-__global__ void __launch_bounds__(256) norm_dw_sum_kernel(const float* part, float* dw, int64_t parts, int D) {
-  const int d = blockIdx.x * 256 + threadIdx.x;
-  if (d >= D) return;
-  float s = 0.f;
-  for (int64_t k = 0; k < parts; ++k) s += part[k * D + d];
-  dw[d] = s;
+__global__ void __launch_bounds__(64 * SUM_WAVES) norm_dw_sum_kernel(const float* part, float* dw, int64_t parts, int D) {
+  const int d = blockIdx.x * 64 + (threadIdx.x & 63);
+  const float s = column_sum(part, parts, D, d, d < D);
+  if (threadIdx.x < 64 && d < D) dw[d] = s;
 }
 
 // ------------------------------------------------------------------------------------------------ host side
@@ -375,7 +373,7 @@ extern "C" int dvae_add_rms_norm_bwd(const void* dy, int64_t dy_st, const void* 
   } while (0)
     NORM_TYPES(NORM_BWD_ANY);
   }
-  DVAE_LAUNCH(norm_dw_sum_kernel, dim3((unsigned)ceil_div64(D, 256)), dim3(256), 0, s, ws, dw, parts, (int)D);
+  DVAE_LAUNCH(norm_dw_sum_kernel, dim3((unsigned)ceil_div64(D, 64)), dim3(64 * SUM_WAVES), 0, s, ws, dw, parts, (int)D);
   DVAE_LAUNCH_CHECK("add_rms_norm_bwd");
   return 0;
 }

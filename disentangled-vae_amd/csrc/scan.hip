@@ -835,14 +835,13 @@ __global__ void __launch_bounds__(256) scan_bc_kernel(const float* part, T* dB, 
   else dC[r * N + c - N] = from_f32<T>(s);
 }
 
-// dA [D][N], dD [D], dbias [D] from the partial rows [parts][N + 2][D], in the parts' order
-__global__ void __launch_bounds__(256) scan_params_kernel(const float* part, float* dA, float* dD, float* dbias,
-                                                          int parts, int N, int D) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+// dA [D][N], dD [D], dbias [D] from the partial rows [parts][N + 2][D]
+__global__ void __launch_bounds__(64 * SUM_WAVES) scan_params_kernel(const float* part, float* dA, float* dD, float* dbias,
+                                                                     int parts, int N, int D) {
   const int64_t total = (int64_t)(N + 2) * D;
-  if (i >= total) return;
-  float s = 0.f;
-  for (int k = 0; k < parts; ++k) s += part[k * total + i];
+  const int64_t i = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
+  const float s = column_sum(part, parts, total, i, i < total);
+  if (threadIdx.x >= 64 || i >= total) return;
   const int n = (int)(i / D), d = (int)(i % D);
   if (n < N) { if (dA) dA[(int64_t)d * N + n] = s; }
   else if (n == N) { if (dD) dD[d] = s; }
@@ -1037,7 +1036,7 @@ extern "C" int dvae_selective_scan_bwd(const void* u, int64_t u_sb, int64_t u_st
     DVAE_LAUNCH((scan_bc_kernel<float>), gbc, dim3(256), 0, ST(stream), p.part_bc, (float*)dB, (float*)dC, bc, p.N, parts);
   else
     DVAE_LAUNCH((scan_bc_kernel<bf16_t>), gbc, dim3(256), 0, ST(stream), p.part_bc, (bf16_t*)dB, (bf16_t*)dC, bc, p.N, parts);
-  DVAE_LAUNCH(scan_params_kernel, dim3((unsigned)ceil_div64((int64_t)(p.N + 2) * D, 256)), dim3(256), 0, ST(stream),
+  DVAE_LAUNCH(scan_params_kernel, dim3((unsigned)ceil_div64((int64_t)(p.N + 2) * D, 64)), dim3(64 * SUM_WAVES), 0, ST(stream),
               p.part_a, dA, dD, dbias, p.rows * p.nch, p.N, p.D);
   DVAE_LAUNCH_CHECK("selective_scan_bwd: sums");
   return 0;

@@ -61,6 +61,33 @@ __device__ __forceinline__ float softplus_hw(float x, float& slope) {
 
 // NaN has to come out as NaN: fmaxf(NaN, 0) is 0, but e and with it l are NaN.
 
+// Sum over `parts` rows of column `col` of part[parts][stride], for the 64 columns of a workgroup of SUM_WAVES waves: a
+// wave adds every SUM_WAVES-th row, eight loads in flight, and the waves' sums are added in their order, so the result
+// does not depend on timing.  Valid in wave 0; every thread takes part.
+#define SUM_WAVES 16
+__device__ __forceinline__ float column_sum(const float* part, int64_t parts, int64_t stride, int64_t col, bool ok) {
+  __shared__ float red[SUM_WAVES][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  float s = 0.f;
+  if (ok) {
+    int64_t k = wave;
+    for (; k + 7 * SUM_WAVES < parts; k += 8 * SUM_WAVES) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = part[(k + i * SUM_WAVES) * stride + col];
+      s += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+    }
+    for (; k < parts; k += SUM_WAVES) s += part[k * stride + col];
+  }
+  red[wave][lane] = s;
+  __syncthreads();
+  if (wave > 0) return 0.f;
+  s = red[0][lane];
+#pragma unroll
+  for (int i = 1; i < SUM_WAVES; ++i) s += red[i][lane];
+  return s;
+}
+
 // Wave-uniform reads of data that no kernel in flight writes go through the constant address space: the compiler then
 // uses the scalar unit and its registers for them, whatever it knows about the kernel's other pointers.
 #define DVAE_UNIFORM __attribute__((address_space(4)))

@@ -201,14 +201,14 @@ __global__ void __launch_bounds__(256) conv_bwd_kernel(ConvArgs p) {
   }
 }
 
-// dw [D][W] and dbias [D]: the sums of the partial rows, in their order
-__global__ void __launch_bounds__(256) conv_params_kernel(const float* part, float* dw, float* dbias, int parts, int W,
-                                                          int D) {
-  const int i = blockIdx.x * 256 + threadIdx.x;
-  if (i >= (W + 1) * D) return;
-  float s = 0.f;
-  for (int k = 0; k < parts; ++k) s += part[(int64_t)k * (W + 1) * D + i];
-  const int k = i / D, d = i % D;
+// dw [D][W] and dbias [D] from the partial rows [parts][W + 1][D]
+__global__ void __launch_bounds__(64 * SUM_WAVES) conv_params_kernel(const float* part, float* dw, float* dbias, int parts,
+                                                                     int W, int D) {
+  const int64_t total = (int64_t)(W + 1) * D;
+  const int64_t i = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
+  const float s = column_sum(part, parts, total, i, i < total);
+  if (threadIdx.x >= 64 || i >= total) return;
+  const int k = (int)(i / D), d = (int)(i % D);
   if (k < W) { if (dw) dw[(int64_t)d * W + k] = s; }
   else if (dbias) dbias[d] = s;
 }
@@ -347,8 +347,8 @@ extern "C" int dvae_short_conv_bwd(const void* x, int64_t x_sb, int64_t x_st, co
   DVAE_WORK(3.0 * p.tokens * D * e, DVAE_UNIT_BYTE);
   CONV_DISPATCH(conv_bwd_kernel, dtype, wide, W, dim3((unsigned)(p.tiles * parts)), p, ST(stream));
   DVAE_LAUNCH_CHECK("short_conv_bwd");
-  DVAE_LAUNCH(conv_params_kernel, dim3((unsigned)ceil_div64((W + 1) * D, 256)), dim3(256), 0, ST(stream), ws, dw, dbias,
-              (int)parts, (int)W, (int)D);
+  DVAE_LAUNCH(conv_params_kernel, dim3((unsigned)ceil_div64((W + 1) * D, 64)), dim3(64 * SUM_WAVES), 0, ST(stream), ws, dw,
+              dbias, (int)parts, (int)W, (int)D);
   if (dstate0) {
     p.tiles = (int)ceil_div64(D, 256);
     DVAE_REQUIRE((int64_t)p.tiles * p.S < (1ll << 31), "short_conv_bwd: too many sequences");
