@@ -17,8 +17,10 @@
 
 #define SCAN_Q 8       // tokens per block: what is loaded ahead, and how far apart training keeps states
 #define SCAN_MAX_N 16
-#define SCAN_WAVES 2048    // waves that a launch aims at: two per SIMD
-#define SCAN_MIN_CHUNK 32  // tokens: below this a chunk's fixed costs (its state in and out) weigh as much as its tokens
+#ifndef SCAN_WPE
+#define SCAN_WPE
+#endif
+#define SCAN_WAVES 2048    // two waves for each of the chip's SIMDs
 
 struct ScanArgs {
   const void *u, *delta, *z, *B, *C, *dout;
@@ -133,13 +135,14 @@ template <typename T, int NP> struct BCAhead<T, NP, false> {
   }
 };
 
-// One wave: 64 channels of one group, one chunk of one row.  A workgroup's four waves are neighbours in a group.
+// 64 channels of one group, one chunk of one row.  A workgroup's four tiles are neighbours in a group; a tile is the work
+// of one wave, or of `share` waves that have a part of the states each.
 struct Tile {
   int g, d, lane, wave, part, chunk, row, t0, t1;
   bool on;
-  __device__ __forceinline__ explicit Tile(const ScanArgs& p) {
+  __device__ __forceinline__ explicit Tile(const ScanArgs& p, int share = 1) {
     lane = threadIdx.x & 63;
-    wave = uniform(threadIdx.x >> 6);
+    wave = uniform(threadIdx.x >> 6) / share;
     const int wg = blockIdx.x % p.wpg;
     const int rc = blockIdx.x / p.wpg;
     const int per = (p.tpg + 3) / 4;
@@ -156,23 +159,25 @@ struct Tile {
   __device__ __forceinline__ bool idle(const ScanArgs& p) const { return part * 4 + wave >= p.tpg; }
 };
 
+// NP states of a channel from the n0-th on, of a state tensor [S][D][N]
 template <int NP>
-__device__ __forceinline__ void load_state(const float* s, int64_t seq, const ScanArgs& p, int d, float (&h)[NP]) {
-  const float* q = s + (seq * p.D + d) * p.N;
+__device__ __forceinline__ void load_state(const float* s, int64_t seq, const ScanArgs& p, int d, float (&h)[NP], int n0 = 0) {
+  const float* q = s + (seq * p.D + d) * p.N + n0;
 #pragma unroll
-  for (int n = 0; n < NP; ++n) h[n] = n < p.N ? q[n] : 0.f;
+  for (int n = 0; n < NP; ++n) h[n] = n0 + n < p.N ? q[n] : 0.f;
 }
 template <int NP>
-__device__ __forceinline__ void store_state(float* s, int64_t seq, const ScanArgs& p, int d, const float (&h)[NP]) {
-  float* q = s + (seq * p.D + d) * p.N;
+__device__ __forceinline__ void store_state(float* s, int64_t seq, const ScanArgs& p, int d, const float (&h)[NP], int n0 = 0) {
+  float* q = s + (seq * p.D + d) * p.N + n0;
 #pragma unroll
   for (int n = 0; n < NP; ++n)
-    if (n < p.N) q[n] = h[n];
+    if (n0 + n < p.N) q[n] = h[n];
 }
+
 // the state that a sequence starts with
 template <int NP>
-__device__ __forceinline__ void entering_state(const ScanArgs& p, int64_t seq, int d, float (&h)[NP]) {
-  if (p.state0) load_state<NP>(p.state0, seq, p, d, h);
+__device__ __forceinline__ void entering_state(const ScanArgs& p, int64_t seq, int d, float (&h)[NP], int n0 = 0) {
+  if (p.state0) load_state<NP>(p.state0, seq, p, d, h, n0);
   else {
 #pragma unroll
     for (int n = 0; n < NP; ++n) h[n] = 0.f;
@@ -193,17 +198,17 @@ template <typename T> __device__ __forceinline__ void lane_store(T* row, uint32_
   *(DVAE_GLOBAL T*)((DVAE_GLOBAL char*)r + at) = v;
 }
 
-// FULL: all NP states exist
+// FULL: all NP states exist, else the first N
 template <int NP, bool FULL>
-__device__ __forceinline__ void load_slot(const float* slot, const ScanArgs& p, int d, float (&h)[NP]) {
+__device__ __forceinline__ void load_slot(const float* slot, const ScanArgs& p, int d, float (&h)[NP], int N) {
 #pragma unroll
-  for (int n = 0; n < NP; ++n) h[n] = FULL || n < p.N ? lane_load(slot + (int64_t)n * p.D, d * 4u) : 0.f;
+  for (int n = 0; n < NP; ++n) h[n] = FULL || n < N ? lane_load(slot + (int64_t)n * p.D, d * 4u) : 0.f;
 }
 template <int NP, bool FULL>
-__device__ __forceinline__ void store_slot(float* slot, const ScanArgs& p, int d, const float (&h)[NP]) {
+__device__ __forceinline__ void store_slot(float* slot, const ScanArgs& p, int d, const float (&h)[NP], int N) {
 #pragma unroll
   for (int n = 0; n < NP; ++n)
-    if (FULL || n < p.N) lane_store(slot + (int64_t)n * p.D, d * 4u, h[n]);
+    if (FULL || n < N) lane_store(slot + (int64_t)n * p.D, d * 4u, h[n]);
 }
 __device__ __forceinline__ float* enter_slot(const ScanArgs& p, int row, int chunk) {
   return p.enter + ((int64_t)row * p.enter_row + (int64_t)chunk * p.enter_step) * p.N * p.D;
@@ -212,22 +217,23 @@ __device__ __forceinline__ float* leave_slot(const ScanArgs& p, int row, int chu
   return p.leave + ((int64_t)row * p.nch + chunk) * p.N * p.D;
 }
 
-// What a block of tokens reads per channel, as stored.  Tokens past the chunk's last are the last one again.
-template <typename T> struct FwdRaw {
-  T u[SCAN_Q], dl[SCAN_Q], z[SCAN_Q];
-  // from the rows that the pointers are at; they end up at the block's last row
-  template <bool Z>
-  __device__ __forceinline__ void load(const T*& up, int64_t u_st, const T*& dp, int64_t d_st, const T*& zp, int64_t z_st,
-                                       int n, uint32_t at) {
+// One tensor's element of a channel, token by token within a block: the block's row as a scalar address, the lane's place
+// in it and the tokens passed as a 32-bit offset, so that eight loads take one scalar address between them (a scalar
+// address each, requested together, spilled a hundred scalar registers).
+template <typename T> struct Rows {
+  const T* base;       // row of the block's first token
+  int64_t block;       // elements from block to block
+  uint32_t step;       // bytes from token to token (the host checked that a block's rows span less than 2 GiB)
+  __device__ __forceinline__ Rows(const void* p, int64_t sb, int64_t st, int row, int t0)
+      : base((const T*)p + row * sb + t0 * st), block(st * SCAN_Q), step((uint32_t)st * (uint32_t)sizeof(T)) {}
+  // token 0 .. SCAN_Q - 1 of the block; those past the n-th are the n-th again
+  __device__ __forceinline__ void load(T (&v)[SCAN_Q], int n, uint32_t at) const {
+    uint64_t r = (uint64_t)base;
+    asm("" : "+s"(r));           // (keeps the compiler from adding the lane's place to it)
 #pragma unroll
     for (int j = 0; j < SCAN_Q; ++j) {
-      u[j] = lane_load(up, at);
-      dl[j] = lane_load(dp, at);
-      if (Z) z[j] = lane_load(zp, at);
-      const bool more = j + 1 < SCAN_Q && j + 1 < n;
-      up += more ? u_st : 0;
-      dp += more ? d_st : 0;
-      if (Z) zp += more ? z_st : 0;
+      v[j] = *(const DVAE_GLOBAL T*)((const DVAE_GLOBAL char*)r + at);
+      at += j + 1 < n ? step : 0u;
     }
   }
 };
@@ -240,7 +246,7 @@ template <typename T> struct FwdRaw {
 // last one with a step size of 0, which leaves the state as it is and gives the same output again.
 // Other blocks (packed sequences' borders) go token by token.
 template <typename T, int NP, bool PACKED, bool FAST, bool STATE_ONLY>
-__global__ void __launch_bounds__(256) scan_fwd_kernel(ScanArgs p) {
+__global__ void __launch_bounds__(256) SCAN_WPE scan_fwd_kernel(ScanArgs p) {
   const Tile w(p);
   if (w.idle(p) || (STATE_ONLY && w.chunk + 1 == p.nch)) return;
   const int row = w.row;
@@ -250,7 +256,7 @@ __global__ void __launch_bounds__(256) scan_fwd_kernel(ScanArgs p) {
     A2[n] = n < p.N ? p.A[(int64_t)w.d * p.N + n] * LOG2E_F : 0.f;
     h[n] = 0.f;
   }
-  if (!STATE_ONLY && w.chunk > 0) load_slot<NP, FAST>(enter_slot(p, row, w.chunk), p, w.d, h);
+  if (!STATE_ONLY && w.chunk > 0) load_slot<NP, FAST>(enter_slot(p, row, w.chunk), p, w.d, h, p.N);
   if (!PACKED && w.chunk == 0) entering_state<NP>(p, row, w.d, h);
   const float Dp = p.Dp ? p.Dp[w.d] : 0.f, bias = p.bias ? p.bias[w.d] : 0.f;
   const bool gated = p.z != nullptr, plus = p.softplus;
@@ -266,21 +272,26 @@ __global__ void __launch_bounds__(256) scan_fwd_kernel(ScanArgs p) {
   if (PACKED) q.seek(w.t0);
   float total = 0.f;
   bool cut = false;
-  FwdRaw<T> next;
+  Rows<T> ur(p.u, p.u_sb, p.u_st, row, w.t0), dr(p.delta, p.delta_sb, p.delta_st, row, w.t0);
+  Rows<T> zr(gated ? p.z : p.u, gated ? p.z_sb : p.u_sb, z_st, row, w.t0);
+  T un[SCAN_Q], dn[SCAN_Q], zn[SCAN_Q];            // the block ahead
   BCAhead<T, NP, FAST> ahead;
-  const T *un = u + w.t0 * p.u_st, *dn = dl + w.t0 * p.delta_st, *zn = z + w.t0 * z_st;    // rows of the block ahead
-  next.template load<!STATE_ONLY>(un, p.u_st, dn, p.delta_st, zn, z_st, w.t1 - w.t0, at);
+  ur.load(un, w.t1 - w.t0, at);
+  dr.load(dn, w.t1 - w.t0, at);
+  if (!STATE_ONLY) zr.load(zn, w.t1 - w.t0, at);
 
   for (int t0 = w.t0; t0 < w.t1; t0 += SCAN_Q) {
     const int n = min(SCAN_Q, w.t1 - t0);
-    const FwdRaw<T> raw = next;
+    T ub[SCAN_Q], pb[SCAN_Q], zb[SCAN_Q];
+#pragma unroll
+    for (int j = 0; j < SCAN_Q; ++j) { ub[j] = un[j]; pb[j] = dn[j]; if (!STATE_ONLY) zb[j] = zn[j]; }
     const int left = w.t1 - t0 - SCAN_Q;
-    un += left > 0 ? p.u_st : 0;
-    dn += left > 0 ? p.delta_st : 0;
-    zn += left > 0 ? z_st : 0;
-    next.template load<!STATE_ONLY>(un, p.u_st, dn, p.delta_st, zn, z_st, left, at);
+    if (left > 0) { ur.base += ur.block; dr.base += dr.block; zr.base += zr.block; }
+    ur.load(un, left, at);                         // (the same block again where it was the last)
+    dr.load(dn, left, at);
+    if (!STATE_ONLY) zr.load(zn, left, at);
     if (!STATE_ONLY && p.ckpt)
-      store_slot<NP, FAST>(p.ckpt + ((int64_t)row * p.blocks + t0 / SCAN_Q) * p.N * p.D, p, w.d, h);
+      store_slot<NP, FAST>(p.ckpt + ((int64_t)row * p.blocks + t0 / SCAN_Q) * p.N * p.D, p, w.d, h, p.N);
     Marks m = {0u, 0u, 0u};
     if (PACKED) m = block_marks<PACKED>(q, t0, n, p.L);
     if (!PACKED || !(m.start | m.end | (m.valid ^ ((1u << n) - 1u)))) {
@@ -303,8 +314,8 @@ __global__ void __launch_bounds__(256) scan_fwd_kernel(ScanArgs p) {
           if (j + 1 < SCAN_Q) ahead.request(Bt, Ct, p.N);
           now.get(Bv, Cv);
         }
-        const float uu = to_f32(raw.u[j]);
-        const float pre = to_f32(raw.dl[j]) + bias;
+        const float uu = to_f32(ub[j]);
+        const float pre = to_f32(pb[j]) + bias;
         const float sp = softplus_hw(pre);
         const float dt = j < n ? (plus ? sp : pre) : 0.f;
         const float x = dt * uu;
@@ -319,7 +330,7 @@ __global__ void __launch_bounds__(256) scan_fwd_kernel(ScanArgs p) {
             h[i] = fmaf(exp2_hw(dt * A2[i]), h[i], x * Bv[i]);
             y = fmaf(Cv[i], h[i], y);
           }
-          const float zz = to_f32(raw.z[j]);
+          const float zz = to_f32(zb[j]);
           const float gate = zz * sigmoid_hw(zz);
           lane_store(ot, at, from_f32<T>(gated ? y * gate : y));
           ot += j + 1 < n ? p.D : 0;
@@ -371,7 +382,7 @@ __global__ void __launch_bounds__(256) scan_fwd_kernel(ScanArgs p) {
   }
   if (STATE_ONLY) {
     if (w.on) {
-      store_slot<NP, FAST>(enter_slot(p, row, w.chunk + 1), p, w.d, h);
+      store_slot<NP, FAST>(enter_slot(p, row, w.chunk + 1), p, w.d, h, p.N);
       p.sumdt[((int64_t)row * p.nch + w.chunk) * p.D + w.d] = total;
     }
     if (w.g == 0 && w.part == 0 && threadIdx.x == 0) p.keep[row * p.nch + w.chunk] = cut ? 0.f : 1.f;
@@ -382,7 +393,7 @@ __global__ void __launch_bounds__(256) scan_fwd_kernel(ScanArgs p) {
 
 // The states (or, BACK, the adjoints) that enter the chunks: x = decay * x + own, along the axis.  Where a sequence
 // starts inside a chunk nothing of what enters it gets through.  A thread owns one state of one channel.
-#define JOIN_AHEAD 8
+#define JOIN_AHEAD 16
 template <bool BACK>
 __global__ void __launch_bounds__(256) scan_join_kernel(ScanArgs p) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -405,10 +416,11 @@ __global__ void __launch_bounds__(256) scan_join_kernel(ScanArgs p) {
 #pragma unroll
     for (int j = 0; j < JOIN_AHEAD; ++j) {
       const int k = k0 + j;
-      if (k + 1 >= p.nch) break;
-      const int c = BACK ? p.nch - 1 - k : k;
-      x = keep[j] != 0.f ? fmaf(exp2_hw(dec[j] * A2), x, own[j]) : own[j];
-      (BACK ? leave_slot(p, row, c - 1) : enter_slot(p, row, c + 1))[i] = x;
+      if (k + 1 < p.nch) {
+        const int c = BACK ? p.nch - 1 - k : k;
+        x = keep[j] != 0.f ? fmaf(exp2_hw(dec[j] * A2), x, own[j]) : own[j];
+        (BACK ? leave_slot(p, row, c - 1) : enter_slot(p, row, c + 1))[i] = x;
+      }
     }
   }
 }
@@ -427,71 +439,37 @@ template <int CTRL> __device__ __forceinline__ float dpp(float v) {
 #define DPP_XOR2 0x4e     // quad_perm [2,3,0,1]
 #define DPP_XOR1 0xb1     // quad_perm [1,0,3,2]
 
-// Sums of 2 * NP values over the 64 lanes, all at once: a step adds the two halves of the wave (then of a half, ...) and
-// lets one half go on with one value, the other with another, so the number of values halves with the number of lanes
-// that still hold parts of one.  The sum of value sum_index(lane) ends up in `lane`.
-template <int M> struct WaveSums {
-  static __device__ __forceinline__ float run(float (&v)[M], int lane) {
-    // 32 lanes apart, then 16: the swaps exchange the upper half of one register with the lower half of the other
+// Sums of 16 values over the 64 lanes, all at once: a step adds the two halves of the wave (then of a half, ...) and lets
+// one half go on with one value, the other with another, so the number of values halves with the number of lanes that
+// still hold parts of one.  The sum of value sum_index(lane) ends up in `lane`, in four lanes alike.
+__device__ __forceinline__ int sum_index(int lane) { return lane >> 2; }
+__device__ __forceinline__ float wave_sums16(float (&v)[16], int lane) {
+  // 32 lanes apart, then 16: the swaps exchange the upper half of one register with the lower half of the other
 #pragma unroll
-    for (int i = 0; i < M / 2; ++i) {
-      const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[i]), __float_as_uint(v[i + M / 2]), false, false);
-      v[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-    }
-#pragma unroll
-    for (int i = 0; i < M / 4; ++i) {
-      const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[i]), __float_as_uint(v[i + M / 4]), false, false);
-      v[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-    }
-#pragma unroll
-    for (int i = 0; i < M / 8; ++i) {
-      const float a = lane & 8 ? v[i + M / 8] : v[i], b = lane & 8 ? v[i] : v[i + M / 8];
-      v[i] = a + dpp<DPP_ROR8>(b);
-    }
-#pragma unroll
-    for (int i = 0; i < M / 16; ++i) {
-      const float a = lane & 4 ? v[i + M / 16] : v[i], b = lane & 4 ? v[i] : v[i + M / 16];
-      v[i] = a + dpp<DPP_HALF_MIRROR>(b);
-    }
-    if (M == 32) {
-      const float a = lane & 2 ? v[1] : v[0], b = lane & 2 ? v[0] : v[1];
-      v[0] = a + dpp<DPP_XOR2>(b);
-    } else {
-      v[0] += dpp<DPP_XOR2>(v[0]);
-    }
-    return v[0] + dpp<DPP_XOR1>(v[0]);
+  for (int i = 0; i < 8; ++i) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[i]), __float_as_uint(v[i + 8]), false, false);
+    v[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
   }
-  static __device__ __forceinline__ int index(int lane) {
-    return (lane & 32 ? M / 2 : 0) + (lane & 16 ? M / 4 : 0) + (lane & 8 ? M / 8 : 0) + (lane & 4 ? M / 16 : 0) +
-           (M == 32 && lane & 2 ? 1 : 0);
-  }
-};
-
-// What a block of tokens reads per channel on the way back, as stored; tokens past the chunk's last are the last one again.
-template <typename T> struct BwdRaw {
-  T u[SCAN_Q], dl[SCAN_Q], z[SCAN_Q], g[SCAN_Q];
-  template <bool U>
-  __device__ __forceinline__ void load(const T* up, int64_t u_st, const T* dp, int64_t d_st, const T* zp, int64_t z_st,
-                                       const T* gp, int64_t g_st, int n, uint32_t at) {
 #pragma unroll
-    for (int j = 0; j < SCAN_Q; ++j) {
-      if (U) u[j] = lane_load(up, at);
-      dl[j] = lane_load(dp, at);
-      z[j] = lane_load(zp, at);
-      g[j] = lane_load(gp, at);
-      const bool more = j + 1 < SCAN_Q && j + 1 < n;
-      if (U) up += more ? u_st : 0;
-      dp += more ? d_st : 0;
-      zp += more ? z_st : 0;
-      gp += more ? g_st : 0;
-    }
+  for (int i = 0; i < 4; ++i) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[i]), __float_as_uint(v[i + 4]), false, false);
+    v[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
   }
-};
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float a = lane & 8 ? v[i + 2] : v[i], b = lane & 8 ? v[i] : v[i + 2];
+    v[i] = a + dpp<DPP_ROR8>(b);
+  }
+  const float a = lane & 4 ? v[1] : v[0], b = lane & 4 ? v[0] : v[1];
+  float s = a + dpp<DPP_HALF_MIRROR>(b);
+  s += dpp<DPP_XOR2>(s);
+  return s + dpp<DPP_XOR1>(s);
+}
 
 // The adjoint that leaves a chunk to the left if nothing enters it from the right: the sum of C[n] g of its tokens up to
 // the first start of a sequence, each through the decays from the chunk's first token to its own.
 template <typename T, int NP, bool PACKED, bool FAST>
-__global__ void __launch_bounds__(256) scan_bwd_state_kernel(ScanArgs p) {
+__global__ void __launch_bounds__(256) SCAN_WPE scan_bwd_state_kernel(ScanArgs p) {
   const Tile w(p);
   if (w.idle(p) || w.chunk == 0) return;
   const int row = w.row;
@@ -513,15 +491,22 @@ __global__ void __launch_bounds__(256) scan_bwd_state_kernel(ScanArgs p) {
   if (PACKED) q.seek(w.t0);
   float total = 0.f;
   bool cut = false;
-  BwdRaw<T> next;
-  next.template load<false>(nullptr, 0, dl + w.t0 * p.delta_st, p.delta_st, z + w.t0 * z_st, z_st,
-                            go + w.t0 * p.dout_st, p.dout_st, w.t1 - w.t0, at);
+  Rows<T> dr(p.delta, p.delta_sb, p.delta_st, row, w.t0), gr(p.dout, p.dout_sb, p.dout_st, row, w.t0);
+  Rows<T> zr(gated ? p.z : p.dout, gated ? p.z_sb : p.dout_sb, z_st, row, w.t0);
+  T dn[SCAN_Q], zn[SCAN_Q], gn[SCAN_Q];            // the block ahead
+  dr.load(dn, w.t1 - w.t0, at);
+  zr.load(zn, w.t1 - w.t0, at);
+  gr.load(gn, w.t1 - w.t0, at);
   for (int t0 = w.t0; t0 < w.t1 && !cut; t0 += SCAN_Q) {
     const int n = min(SCAN_Q, w.t1 - t0);
-    const BwdRaw<T> raw = next;
-    const int64_t tn = min(t0 + SCAN_Q, w.t1 - 1);
-    next.template load<false>(nullptr, 0, dl + tn * p.delta_st, p.delta_st, z + tn * z_st, z_st, go + tn * p.dout_st,
-                              p.dout_st, w.t1 - t0 - SCAN_Q, at);
+    T pb[SCAN_Q], zb[SCAN_Q], gb[SCAN_Q];
+#pragma unroll
+    for (int j = 0; j < SCAN_Q; ++j) { pb[j] = dn[j]; zb[j] = zn[j]; gb[j] = gn[j]; }
+    const int left = w.t1 - t0 - SCAN_Q;
+    if (left > 0) { dr.base += dr.block; zr.base += zr.block; gr.base += gr.block; }
+    dr.load(dn, left, at);
+    zr.load(zn, left, at);
+    gr.load(gn, left, at);
     Marks m = {0u, 0u, 0u};
     if (PACKED) m = block_marks<PACKED>(q, t0, n, p.L);
     if (!PACKED || !(m.start | m.end | (m.valid ^ ((1u << n) - 1u)))) {
@@ -536,11 +521,11 @@ __global__ void __launch_bounds__(256) scan_bwd_state_kernel(ScanArgs p) {
         now.arrived_b(Ct);
         if (j + 1 < SCAN_Q) ahead.request_b(Ct, p.N);
         now.get_b(Cv);
-        const float pre = to_f32(raw.dl[j]) + bias;
+        const float pre = to_f32(pb[j]) + bias;
         const float sp = softplus_hw(pre);
         total += j < n ? (plus ? sp : pre) : 0.f;
-        const float zz = to_f32(raw.z[j]), gate = zz * sigmoid_hw(zz);
-        float g = to_f32(raw.g[j]);
+        const float zz = to_f32(zb[j]), gate = zz * sigmoid_hw(zz);
+        float g = to_f32(gb[j]);
         g = j < n ? (gated ? g * gate : g) : 0.f;
 #pragma unroll
         for (int i = 0; i < NP; ++i) x[i] = fmaf(exp2_hw(total * A2[i]), Cv[i] * g, x[i]);
@@ -581,37 +566,41 @@ __global__ void __launch_bounds__(256) scan_bwd_state_kernel(ScanArgs p) {
     for (int i = 0; i < NP; ++i) x[i] = fmaf(exp2_hw(total * A2[i]), e[i], x[i]);
   }
   if (w.on) {
-    store_slot<NP, FAST>(leave_slot(p, row, w.chunk - 1), p, w.d, x);
+    store_slot<NP, FAST>(leave_slot(p, row, w.chunk - 1), p, w.d, x, p.N);
     p.sumdt[((int64_t)row * p.nch + w.chunk) * p.D + w.d] = total;
   }
   if (w.g == 0 && w.part == 0 && threadIdx.x == 0) p.keep[row * p.nch + w.chunk] = cut ? 0.f : 1.f;
 }
 
+// The states of a tile are shared out over SHARE = NP / 8 waves, eight states each: what one wave keeps of a block (the
+// states before its tokens and the decays, computed once for both directions) then fits 256 registers, so that two waves
+// run per SIMD and fill each other's waits; with sixteen states in a wave it took 480 and ran alone (8 x 2048 x 2048 bf16:
+// SHARE1 against SHARE2 us).  The waves add up their parts of y, of the sum of dh B and of that of k A through LDS, once
+// per block, and each finishes the gradients of its share of the block's tokens.
+#define SCAN_NW 8
 template <typename T, int NP, bool PACKED, bool FAST>
-__global__ void __launch_bounds__(256, 1) scan_bwd_kernel(ScanArgs p) {
-  __shared__ float red[2][SCAN_Q][4][2 * NP];      // [block parity][token][wave][dB, dC]
-  const Tile w(p);
-  const int row = w.row;
+__global__ void __launch_bounds__(256 * (NP / SCAN_NW), 2) scan_bwd_kernel(ScanArgs p) {
+  constexpr int SHARE = NP / SCAN_NW, OWN = SCAN_Q / SHARE;      // waves per tile; tokens of a block that a wave finishes
+  __shared__ float red[SCAN_Q][4][2 * NP];                       // [token][tile][dB, dC]
+  __shared__ float part[SCAN_Q][3][4 * SHARE][64];               // [token][y, dh B, k A][wave][lane]
+  const Tile w(p, SHARE);
+  const int row = w.row, wv = uniform(threadIdx.x >> 6), half = wv % SHARE, n0 = half * SCAN_NW;
   const bool idle = w.idle(p);                     // such a wave only takes part in the sums
-  float A2[NP], dh[NP], dA[NP];
+  const int Nw = min(max(p.N - n0, 0), SCAN_NW);   // states that this wave has
+  float A2[SCAN_NW], dh[SCAN_NW], dA[SCAN_NW];
 #pragma unroll
-  for (int n = 0; n < NP; ++n) {
-    A2[n] = n < p.N ? p.A[(int64_t)w.d * p.N + n] * LOG2E_F : 0.f;
-    dh[n] = dA[n] = 0.f;
+  for (int i = 0; i < SCAN_NW; ++i) {
+    A2[i] = i < Nw ? p.A[(int64_t)w.d * p.N + n0 + i] * LOG2E_F : 0.f;
+    dh[i] = dA[i] = 0.f;
   }
-  if (w.chunk + 1 < p.nch) load_slot<NP, FAST>(leave_slot(p, row, w.chunk), p, w.d, dh);
-  else if (!PACKED && p.dstate1) load_state<NP>(p.dstate1, row, p, w.d, dh);
+  const int64_t skip = (int64_t)n0 * p.D;          // this wave's rows of a slot
+  if (w.chunk + 1 < p.nch) load_slot<SCAN_NW, FAST>(leave_slot(p, row, w.chunk) + skip, p, w.d, dh, Nw);
+  else if (!PACKED && p.dstate1) load_state<SCAN_NW>(p.dstate1, row, p, w.d, dh, n0);
   float dD = 0.f, dbias = 0.f;
   const float Dp = p.Dp ? p.Dp[w.d] : 0.f, bias = p.bias ? p.bias[w.d] : 0.f;
-  const T* u = (const T*)p.u + row * p.u_sb;
-  const T* dl = (const T*)p.delta + row * p.delta_sb;
   const bool gated = p.z != nullptr, plus = p.softplus;
-  const T* go = (const T*)p.dout + row * p.dout_sb;
-  const T* z = gated ? (const T*)p.z + row * p.z_sb : go;             // (read and not used without z)
-  const int64_t z_st = gated ? p.z_st : p.dout_st;
-  T* dzp = gated ? (T*)p.dz : (T*)p.du;                                // (written and written over by du without z)
-  const T* B = (const T*)p.B + row * p.B_sb + w.g * p.B_sg;
-  const T* C = (const T*)p.C + row * p.C_sb + w.g * p.C_sg;
+  const T* B = (const T*)p.B + row * p.B_sb + w.g * p.B_sg + n0;
+  const T* C = (const T*)p.C + row * p.C_sb + w.g * p.C_sg + n0;
   const int64_t flat = (int64_t)row * p.L;
   const uint32_t at = w.d * (uint32_t)sizeof(T);
   SeqWalk q = {p.offsets, p.S, p.L, p.L, row, 0, p.L};      // the sequence that the way back is in
@@ -619,205 +608,249 @@ __global__ void __launch_bounds__(256, 1) scan_bwd_kernel(ScanArgs p) {
     q.seek(w.t1 - 1);
     if (q.s >= q.S || q.b >= w.t1) q.prev(w.t1 - 1);
   }
-  int turn = 0;
   const int first = w.t0 + (w.t1 - w.t0 - 1) / SCAN_Q * SCAN_Q;
-  const float* ck = p.ckpt + ((int64_t)row * p.blocks + first / SCAN_Q) * p.N * p.D;
-  BwdRaw<T> next;
-  float hn[NP];                                    // the state that enters the block ahead
-  next.template load<true>(u + first * p.u_st, p.u_st, dl + first * p.delta_st, p.delta_st, z + first * z_st, z_st,
-                           go + first * p.dout_st, p.dout_st, w.t1 - first, at);
-  load_slot<NP, FAST>(ck, p, w.d, hn);
+  const float* ck = p.ckpt + ((int64_t)row * p.blocks + first / SCAN_Q) * p.N * p.D + skip;
+  Rows<T> ur(p.u, p.u_sb, p.u_st, row, first), dr(p.delta, p.delta_sb, p.delta_st, row, first);
+  Rows<T> gr(p.dout, p.dout_sb, p.dout_st, row, first);
+  Rows<T> zr(gated ? p.z : p.dout, gated ? p.z_sb : p.dout_sb, gated ? p.z_st : p.dout_st, row, first);  // (not used without z)
+  T un[SCAN_Q], dn[SCAN_Q], zn[SCAN_Q], gn[SCAN_Q];   // the block ahead,
+  float hn[SCAN_NW];                                  // and the state that enters it
+  ur.load(un, w.t1 - first, at);
+  dr.load(dn, w.t1 - first, at);
+  zr.load(zn, w.t1 - first, at);
+  gr.load(gn, w.t1 - first, at);
+  load_slot<SCAN_NW, FAST>(ck, p, w.d, hn, Nw);
 
-  for (int t0 = first; t0 >= w.t0; t0 -= SCAN_Q, turn ^= 1) {
+  for (int t0 = first; t0 >= w.t0; t0 -= SCAN_Q) {
     const int n = min(SCAN_Q, w.t1 - t0);
-    const BwdRaw<T> raw = next;
-    float hs[SCAN_Q + 1][NP];
+    T ub[SCAN_Q], zb[SCAN_Q], gb[SCAN_Q];
+    float hs[SCAN_Q + 1][SCAN_NW], db[SCAN_Q], slope[SCAN_Q];
 #pragma unroll
-    for (int i = 0; i < NP; ++i) hs[0][i] = hn[i];
-    {
-      const int64_t tn = max(t0 - SCAN_Q, w.t0);
-      ck -= t0 > w.t0 ? (int64_t)p.N * p.D : 0;
-      next.template load<true>(u + tn * p.u_st, p.u_st, dl + tn * p.delta_st, p.delta_st, z + tn * z_st, z_st,
-                               go + tn * p.dout_st, p.dout_st, w.t1 - tn, at);
-      load_slot<NP, FAST>(ck, p, w.d, hn);
-    }
+    for (int i = 0; i < SCAN_NW; ++i) hs[0][i] = hn[i];
     SeqWalk f = q;                                 // the sequence that the states' second computation is in
     Marks m = {0u, 0u, 0u};
     if (PACKED) {
       f.seek(t0);
       m = block_marks<PACKED>(f, t0, n, p.L);
     }
-    if (idle) {
-      for (int i = w.lane; i < SCAN_Q * 2 * NP; i += 64) red[turn][i / (2 * NP)][w.wave][i % (2 * NP)] = 0.f;
-    } else if (!PACKED || !(m.start | m.end | (m.valid ^ ((1u << n) - 1u)))) {
+    const bool plain = !PACKED || !(m.start | m.end | (m.valid ^ ((1u << n) - 1u)));
+    // Requests the block before this one.  Called when half of this one's tokens are done, whose registers it takes.
+    auto request = [&]() {
+      if (t0 > w.t0) {
+        ck -= (int64_t)p.N * p.D;
+        ur.base -= ur.block; dr.base -= dr.block; zr.base -= zr.block; gr.base -= gr.block;
+      }
+      const int left = t0 > w.t0 ? SCAN_Q : n;
+      ur.load(un, left, at);
+      dr.load(dn, left, at);
+      zr.load(zn, left, at);
+      gr.load(gn, left, at);
+      load_slot<SCAN_NW, FAST>(ck, p, w.d, hn, Nw);
+    };
+#pragma unroll
+    for (int j = 0; j < SCAN_Q; ++j) {             // tokens past the chunk's last: a step size of 0
+      ub[j] = un[j]; zb[j] = zn[j]; gb[j] = gn[j];
+      const float pre = to_f32(dn[j]) + bias;
+      const float sp = softplus_hw(pre, slope[j]);
+      db[j] = j < n ? (plus ? sp : pre) : 0.f;
+      slope[j] = plus ? slope[j] : 1.f;
+    }
+    if (plain) {
       // no sequence starts or ends here: straight-line code, as in the forward pass.  Tokens past the chunk's last have
-      // a step size and a gradient of 0, which changes nothing, and what they store is stored over by the last token.
-      float a[SCAN_Q][NP], db[SCAN_Q], slope[SCAN_Q];
-      BCAhead<T, NP, FAST> ahead;
+      // a step size and a gradient of 0, which changes nothing.
+      float a[SCAN_Q][SCAN_NW];
+      BCAhead<T, SCAN_NW, FAST> ahead;
       const T *Bt = B + t0 * p.B_st, *Ct = C + t0 * p.C_st;
-      ahead.request_b(Bt, p.N);
+      ahead.request_b(Bt, Nw);
 #pragma unroll
       for (int j = 0; j < SCAN_Q; ++j) {
-        BCAhead<T, NP, FAST> now = ahead;
-        float Bv[NP];
+        BCAhead<T, SCAN_NW, FAST> now = ahead;
+        float Bv[SCAN_NW];
         Bt += j + 1 < n ? p.B_st : 0;
         Ct += j + 1 < n ? p.C_st : 0;
         now.arrived_b(Bt);
-        if (j + 1 < SCAN_Q) ahead.request_b(Bt, p.N);
-        else ahead.request(Bt, Ct, p.N);           // the last token's, where the way back begins
+        if (j + 1 < SCAN_Q) ahead.request_b(Bt, Nw);
+        else ahead.request(Bt, Ct, Nw);            // the last token's, where the way back begins
         now.get_b(Bv);
-        const float pre = to_f32(raw.dl[j]) + bias;
-        const float sp = softplus_hw(pre, slope[j]);
-        db[j] = j < n ? (plus ? sp : pre) : 0.f;
-        slope[j] = plus ? slope[j] : 1.f;
-        const float x = db[j] * to_f32(raw.u[j]);
+        const float x = db[j] * to_f32(ub[j]);
 #pragma unroll
-        for (int i = 0; i < NP; ++i) {
+        for (int i = 0; i < SCAN_NW; ++i) {
           a[j][i] = exp2_hw(db[j] * A2[i]);
           hs[j + 1][i] = fmaf(a[j][i], hs[j][i], x * Bv[i]);
         }
+        __builtin_amdgcn_sched_barrier(0);         // (mixing tokens spills registers: SB0 against SB2 us)
       }
-      int64_t o = (flat + t0 + n - 1) * p.D;
+      __syncthreads();                             // everyone has read the sums of the block behind
 #pragma unroll
       for (int j = SCAN_Q - 1; j >= 0; --j) {
-        BCAhead<T, NP, FAST> now = ahead;
-        float Bv[NP], Cv[NP];
+        if (j == SCAN_Q / 2 - 1) request();
+        BCAhead<T, SCAN_NW, FAST> now = ahead;
+        float Bv[SCAN_NW], Cv[SCAN_NW];
         Bt -= j > 0 && j < n ? p.B_st : 0;
         Ct -= j > 0 && j < n ? p.C_st : 0;
         now.arrived(Bt, Ct);
-        if (j > 0) ahead.request(Bt, Ct, p.N);
+        if (j > 0) ahead.request(Bt, Ct, Nw);
         now.get(Bv, Cv);
-        const float uu = to_f32(raw.u[j]), zz = to_f32(raw.z[j]), sg = sigmoid_hw(zz);
-        float g = j < n ? to_f32(raw.g[j]) : 0.f;
-        float y = Dp * uu;
-#pragma unroll
-        for (int i = 0; i < NP; ++i) y = fmaf(Cv[i], hs[j + 1][i], y);
-        lane_store(dzp + o, at, from_f32<T>(g * y * sg * fmaf(zz, 1.f - sg, 1.f)));
-        g = gated ? g * (zz * sg) : g;
+        const float zz = to_f32(zb[j]);
+        float g = j < n ? to_f32(gb[j]) : 0.f;
+        g = gated ? g * (zz * sigmoid_hw(zz)) : g;
         // lanes past the last channel add nothing to the sums over the channels
-        const float x = w.on ? db[j] * uu : 0.f, gs = w.on ? g : 0.f;
-        float through = 0.f, ka = 0.f, pv[2 * NP];
+        const float x = w.on ? db[j] * to_f32(ub[j]) : 0.f, gs = w.on ? g : 0.f;
+        float y = 0.f, through = 0.f, ka = 0.f, pv[2 * SCAN_NW];
 #pragma unroll
-        for (int i = 0; i < NP; ++i) {
+        for (int i = 0; i < SCAN_NW; ++i) {
+          y = fmaf(Cv[i], hs[j + 1][i], y);
           const float d = fmaf(Cv[i], g, dh[i]);
           pv[i] = d * x;
-          pv[NP + i] = gs * hs[j + 1][i];
+          pv[SCAN_NW + i] = gs * hs[j + 1][i];
           through = fmaf(d, Bv[i], through);
           dh[i] = d * a[j][i];
           const float k = dh[i] * hs[j][i];
           dA[i] = fmaf(k, db[j], dA[i]);
           ka = fmaf(k, A2[i], ka);
         }
-        const float sum = WaveSums<2 * NP>::run(pv, w.lane);
-        if (!(w.lane & (NP == 16 ? 1 : 3))) red[turn][j][w.wave][WaveSums<2 * NP>::index(w.lane)] = sum;
-        dD = fmaf(g, uu, dD);
-        float dd = fmaf(ka, LN2_F, through * uu) * slope[j];
-        dd = j < n ? dd : 0.f;
-        dbias += dd;
-        lane_store((T*)p.du + o, at, from_f32<T>(fmaf(through, db[j], Dp * g)));
-        lane_store((T*)p.ddelta + o, at, from_f32<T>(dd));
-        o -= j < n ? p.D : 0;
+        part[j][0][wv][w.lane] = y;
+        part[j][1][wv][w.lane] = through;
+        part[j][2][wv][w.lane] = ka;
+        const float sum = wave_sums16(pv, w.lane);
+        const int c = sum_index(w.lane);
+        red[j][w.wave][c < SCAN_NW ? n0 + c : NP + n0 + c - SCAN_NW] = idle ? 0.f : sum;    // (four lanes alike)
+        __builtin_amdgcn_sched_barrier(0);
       }
     } else {
-      float ub[SCAN_Q], pb[SCAN_Q], db[SCAN_Q];
 #pragma unroll
       for (int j = 0; j < SCAN_Q; ++j) {
 #pragma unroll
-        for (int i = 0; i < NP; ++i) hs[j + 1][i] = hs[j][i];
+        for (int i = 0; i < SCAN_NW; ++i) hs[j + 1][i] = hs[j][i];
         if (!(m.valid >> j & 1)) continue;
         const int64_t t = t0 + j;
-        ub[j] = to_f32(raw.u[j]);
-        pb[j] = to_f32(raw.dl[j]) + bias;
-        db[j] = plus ? softplus_hw(pb[j]) : pb[j];
-        if (m.start >> j & 1) entering_state<NP>(p, f.seq(), w.d, hs[j + 1]);
-        float Bv[NP];
-        BCLoad<T, NP, FAST>::get(B, t * p.B_st, p.N, Bv);
-        const float x = db[j] * ub[j];
+        if (m.start >> j & 1) entering_state<SCAN_NW>(p, f.seq(), w.d, hs[j + 1], n0);
+        float Bv[SCAN_NW];
+        BCLoad<T, SCAN_NW, FAST>::get(B, t * p.B_st, Nw, Bv);
+        const float x = db[j] * to_f32(ub[j]);
 #pragma unroll
-        for (int i = 0; i < NP; ++i) hs[j + 1][i] = fmaf(exp2_hw(db[j] * A2[i]), hs[j + 1][i], x * Bv[i]);
-        if (PACKED && (m.end >> j & 1)) f.next((int)t + 1);
+        for (int i = 0; i < SCAN_NW; ++i) hs[j + 1][i] = fmaf(exp2_hw(db[j] * A2[i]), hs[j + 1][i], x * Bv[i]);
+        if (m.end >> j & 1) f.next((int)t + 1);
       }
+      __syncthreads();
+      request();
 #pragma unroll
       for (int j = SCAN_Q - 1; j >= 0; --j) {
         if (j >= n) continue;
-        const int64_t t = t0 + j, o = (flat + t) * p.D + w.d;
+        const int64_t t = t0 + j;
         if (!(m.valid >> j & 1)) {
-          if (w.on) {
-            ((T*)p.du)[o] = from_f32<T>(0.f);
-            ((T*)p.ddelta)[o] = from_f32<T>(0.f);
-            if (gated) ((T*)p.dz)[o] = from_f32<T>(0.f);
-          }
-          if (w.lane < 2 * NP) red[turn][j][w.wave][w.lane] = 0.f;
+          if (w.lane < 2 * SCAN_NW) red[j][w.wave][w.lane < SCAN_NW ? n0 + w.lane : NP + n0 + w.lane - SCAN_NW] = 0.f;
           continue;
         }
         if (m.end >> j & 1) {
-          if (p.dstate1) load_state<NP>(p.dstate1, q.seq(), p, w.d, dh);
+          if (p.dstate1) load_state<SCAN_NW>(p.dstate1, q.seq(), p, w.d, dh, n0);
           else {
 #pragma unroll
-            for (int i = 0; i < NP; ++i) dh[i] = 0.f;
+            for (int i = 0; i < SCAN_NW; ++i) dh[i] = 0.f;
           }
         }
-        float Bv[NP], Cv[NP];
-        BCLoad<T, NP, FAST>::get(B, t * p.B_st, p.N, Bv);
-        BCLoad<T, NP, FAST>::get(C, t * p.C_st, p.N, Cv);
-        float g = to_f32(raw.g[j]);
-        if (gated) {
-          const float zz = to_f32(raw.z[j]);
-          const float sg = sigmoid_hw(zz);
-          float y = Dp * ub[j];
+        float Bv[SCAN_NW], Cv[SCAN_NW];
+        BCLoad<T, SCAN_NW, FAST>::get(B, t * p.B_st, Nw, Bv);
+        BCLoad<T, SCAN_NW, FAST>::get(C, t * p.C_st, Nw, Cv);
+        float g = to_f32(gb[j]);
+        const float zz = to_f32(zb[j]);
+        g = gated ? g * (zz * sigmoid_hw(zz)) : g;
+        const float x = w.on ? db[j] * to_f32(ub[j]) : 0.f, gs = w.on ? g : 0.f;
+        float y = 0.f, through = 0.f, ka = 0.f, pv[2 * SCAN_NW], hb[SCAN_NW];
 #pragma unroll
-          for (int i = 0; i < NP; ++i) y = fmaf(Cv[i], hs[j + 1][i], y);
-          if (w.on) ((T*)p.dz)[o] = from_f32<T>(g * y * sg * fmaf(zz, 1.f - sg, 1.f));
-          g *= zz * sg;
-        }
-        const float x = w.on ? db[j] * ub[j] : 0.f, gs = w.on ? g : 0.f;
-        float through = 0.f, ka = 0.f, pv[2 * NP], hb[NP];
+        for (int i = 0; i < SCAN_NW; ++i) hb[i] = hs[j][i];
+        if (m.start >> j & 1) entering_state<SCAN_NW>(p, q.seq(), w.d, hb, n0);
 #pragma unroll
-        for (int i = 0; i < NP; ++i) hb[i] = hs[j][i];
-        if (m.start >> j & 1) entering_state<NP>(p, q.seq(), w.d, hb);
-#pragma unroll
-        for (int i = 0; i < NP; ++i) {
-          const float a = exp2_hw(db[j] * A2[i]);
+        for (int i = 0; i < SCAN_NW; ++i) {
+          y = fmaf(Cv[i], hs[j + 1][i], y);
           const float d = fmaf(Cv[i], g, dh[i]);
           pv[i] = d * x;
-          pv[NP + i] = gs * hs[j + 1][i];
+          pv[SCAN_NW + i] = gs * hs[j + 1][i];
           through = fmaf(d, Bv[i], through);
-          dh[i] = d * a;
+          dh[i] = d * exp2_hw(db[j] * A2[i]);
           const float k = dh[i] * hb[i];
           dA[i] = fmaf(k, db[j], dA[i]);
           ka = fmaf(k, A2[i], ka);
         }
-        const float sum = WaveSums<2 * NP>::run(pv, w.lane);
-        if (!(w.lane & (NP == 16 ? 1 : 3))) red[turn][j][w.wave][WaveSums<2 * NP>::index(w.lane)] = sum;
-        dD = fmaf(g, ub[j], dD);
-        float dd = fmaf(ka, LN2_F, through * ub[j]);
-        if (plus) dd *= sigmoid_hw(pb[j]);
-        dbias += dd;
-        if (w.on) {
-          ((T*)p.du)[o] = from_f32<T>(fmaf(through, db[j], Dp * g));
-          ((T*)p.ddelta)[o] = from_f32<T>(dd);
-        }
+        part[j][0][wv][w.lane] = y;
+        part[j][1][wv][w.lane] = through;
+        part[j][2][wv][w.lane] = ka;
+        const float sum = wave_sums16(pv, w.lane);
+        const int c = sum_index(w.lane);
+        red[j][w.wave][c < SCAN_NW ? n0 + c : NP + n0 + c - SCAN_NW] = idle ? 0.f : sum;    // (four lanes alike)
         if (m.start >> j & 1) {
-          if (p.dstate0 && w.on) store_state<NP>(p.dstate0, q.seq(), p, w.d, dh);
-          if (PACKED) q.prev((int)t - 1);
+          if (p.dstate0 && w.on && !idle) store_state<SCAN_NW>(p.dstate0, q.seq(), p, w.d, dh, n0);
+          q.prev((int)t - 1);
         }
       }
     }
-    __syncthreads();           // the other parity's buffer was read before the last of these, so one barrier is enough
-    for (int i = threadIdx.x; i < n * 2 * p.N; i += 256) {
+    __syncthreads();
+    // this wave's tokens: j = half * OWN + jj
+    int64_t o = (flat + t0 + half * OWN) * p.D;
+#pragma unroll
+    for (int jj = 0; jj < OWN; ++jj) {
+      const int j = half * OWN + jj;
+      float uu = to_f32(ub[jj]), zz = to_f32(zb[jj]), g0 = to_f32(gb[jj]), dt = db[jj], sl = slope[jj];
+#pragma unroll
+      for (int k = 1; k < SHARE; ++k) {            // (the registers of token j, chosen by the wave)
+        const bool mine = half == k;
+        uu = mine ? to_f32(ub[k * OWN + jj]) : uu;
+        zz = mine ? to_f32(zb[k * OWN + jj]) : zz;
+        g0 = mine ? to_f32(gb[k * OWN + jj]) : g0;
+        dt = mine ? db[k * OWN + jj] : dt;
+        sl = mine ? slope[k * OWN + jj] : sl;
+      }
+      if (j < n) {
+        float du = 0.f, dd = 0.f, dz = 0.f;
+        if (!PACKED || (m.valid >> j & 1)) {
+          float y = Dp * uu, through = 0.f, ka = 0.f;
+#pragma unroll
+          for (int k = 0; k < SHARE; ++k) {
+            y += part[j][0][w.wave * SHARE + k][w.lane];
+            through += part[j][1][w.wave * SHARE + k][w.lane];
+            ka += part[j][2][w.wave * SHARE + k][w.lane];
+          }
+          const float sg = sigmoid_hw(zz);
+          const float g = gated ? g0 * (zz * sg) : g0;
+          dz = g0 * y * sg * fmaf(zz, 1.f - sg, 1.f);
+          du = fmaf(through, dt, Dp * g);
+          dd = fmaf(ka, LN2_F, through * uu) * sl;
+          dD = fmaf(g, uu, dD);
+          dbias += dd;
+        }
+        if (!idle) {
+          if (gated) lane_store((T*)p.dz + o, at, from_f32<T>(dz));
+          lane_store((T*)p.du + o, at, from_f32<T>(du));
+          lane_store((T*)p.ddelta + o, at, from_f32<T>(dd));
+        }
+      }
+      o += p.D;
+    }
+    for (int i = threadIdx.x; i < n * 2 * p.N; i += 256 * SHARE) {
       const int j = i / (2 * p.N), c = i % (2 * p.N), k = c < p.N ? c : c - p.N + NP;
-      const float s = (red[turn][j][0][k] + red[turn][j][1][k]) + (red[turn][j][2][k] + red[turn][j][3][k]);
+      const float s = (red[j][0][k] + red[j][1][k]) + (red[j][2][k] + red[j][3][k]);
       p.part_bc[(((int64_t)w.part * p.rows * p.L + flat + t0 + j) * p.G + w.g) * 2 * p.N + c] = s;
     }
   }
-  if (!PACKED && w.chunk == 0 && p.dstate0 && w.on && !idle) store_state<NP>(p.dstate0, row, p, w.d, dh);
+  if (!PACKED && w.chunk == 0 && p.dstate0 && w.on && !idle) store_state<SCAN_NW>(p.dstate0, row, p, w.d, dh, n0);
+  __syncthreads();
+  part[0][0][wv][w.lane] = dD;
+  part[0][1][wv][w.lane] = dbias;
+  __syncthreads();
   if (w.on && !idle) {
     float* pa = p.part_a + ((int64_t)row * p.nch + w.chunk) * (p.N + 2) * p.D + w.d;
 #pragma unroll
-    for (int i = 0; i < NP; ++i)
-      if (i < p.N) pa[(int64_t)i * p.D] = dA[i];
-    pa[(int64_t)p.N * p.D] = dD;
-    pa[(int64_t)(p.N + 1) * p.D] = dbias;
+    for (int i = 0; i < SCAN_NW; ++i)
+      if (i < Nw) pa[(int64_t)(n0 + i) * p.D] = dA[i];
+    if (half == 0) {
+#pragma unroll
+      for (int k = 1; k < SHARE; ++k) {
+        dD += part[0][0][w.wave * SHARE + k][w.lane];
+        dbias += part[0][1][w.wave * SHARE + k][w.lane];
+      }
+      pa[(int64_t)p.N * p.D] = dD;
+      pa[(int64_t)(p.N + 1) * p.D] = dbias;
+    }
   }
 }
 
@@ -848,32 +881,65 @@ __global__ void __launch_bounds__(64 * SUM_WAVES) scan_params_kernel(const float
   else if (dbias) dbias[d] = s;
 }
 
-// One token per row: a lane owns one state of one channel at a time, a channel's states in neighbouring lanes, so that
-// the state, nearly all of the traffic, is read and written in whole lines.
-template <typename T>
+// One token per row.  Nearly all of the traffic is the state, read and written once: a lane owns four states of a channel
+// (one 16-byte access each way where N is a multiple of 4), a channel's LPC lanes are neighbours, and the sum over them
+// takes two lane exchanges.  What a channel reads besides (inputs, step size) its lanes read and compute alike.  A lane
+// goes through R rows whose loads are in flight together and share its A.
+template <typename T, int LPC, int R, bool VEC>
 __global__ void __launch_bounds__(256) scan_step_kernel(ScanArgs p) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t total = (int64_t)p.rows * p.D;
-  if (i >= total) return;
-  const int row = (int)(i / p.D), d = (int)(i % p.D), g = d / p.Dg;
-  const float uu = to_f32(((const T*)p.u)[row * p.u_sb + d]);
-  const float pre = to_f32(((const T*)p.delta)[row * p.delta_sb + d]) + (p.bias ? p.bias[d] : 0.f);
-  const float dt = p.softplus ? softplus_hw(pre) : pre;
-  const T* B = (const T*)p.B + row * p.B_sb + g * p.B_sg;
-  const T* C = (const T*)p.C + row * p.C_sb + g * p.C_sg;
-  float* h = p.state1 + i * p.N;
-  float y = p.Dp ? p.Dp[d] * uu : 0.f;
-  const float x = dt * uu;
-  for (int n = 0; n < p.N; ++n) {
-    const float v = fmaf(exp2_hw(dt * (p.A[(int64_t)d * p.N + n] * LOG2E_F)), h[n], x * to_f32(B[n]));
-    h[n] = v;
-    y = fmaf(to_f32(C[n]), v, y);
+  const int q = (int)(i % LPC), d = (int)(i / LPC % p.D), n0 = q * 4;
+  const int row0 = (int)(i / LPC / p.D) * R;
+  if (row0 >= p.rows) return;
+  const int g = d / p.Dg;
+  float A2[4], h[R][4], Bv[R][4], Cv[R][4], uu[R], pre[R], zz[R];
+  const float* A = p.A + (int64_t)d * p.N + n0;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int row = min(row0 + r, p.rows - 1);            // a row past the last is the last again, and not written
+    const float* s = p.state1 + ((int64_t)row * p.D + d) * p.N + n0;
+    const T* B = (const T*)p.B + row * p.B_sb + g * p.B_sg + n0;
+    const T* C = (const T*)p.C + row * p.C_sb + g * p.C_sg + n0;
+    if (VEC && n0 < p.N) load_pack<float, 4>(s, h[r]);
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const bool there = n0 + n < p.N;
+      if (!VEC || n0 >= p.N) h[r][n] = there ? s[n] : 0.f;
+      Bv[r][n] = there ? to_f32(B[n]) : 0.f;
+      Cv[r][n] = there ? to_f32(C[n]) : 0.f;
+    }
+    uu[r] = to_f32(((const T*)p.u)[row * p.u_sb + d]);
+    pre[r] = to_f32(((const T*)p.delta)[row * p.delta_sb + d]);
+    zz[r] = p.z ? to_f32(((const T*)p.z)[row * p.z_sb + d]) : 0.f;
   }
-  if (p.z) {
-    const float zz = to_f32(((const T*)p.z)[row * p.z_sb + d]);
-    y *= zz * sigmoid_hw(zz);
+#pragma unroll
+  for (int n = 0; n < 4; ++n) A2[n] = n0 + n < p.N ? A[n] * LOG2E_F : 0.f;
+  const float bias = p.bias ? p.bias[d] : 0.f, Dp = p.Dp ? p.Dp[d] : 0.f;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int row = row0 + r;
+    const float v = pre[r] + bias, dt = p.softplus ? softplus_hw(v) : v, x = dt * uu[r];
+    float y = 0.f;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      h[r][n] = fmaf(exp2_hw(dt * A2[n]), h[r][n], x * Bv[r][n]);
+      y = fmaf(Cv[r][n], h[r][n], y);
+    }
+    if (LPC >= 2) y += dpp<DPP_XOR1>(y);
+    if (LPC >= 4) y += dpp<DPP_XOR2>(y);
+    y = fmaf(Dp, uu[r], y);
+    if (p.z) y *= zz[r] * sigmoid_hw(zz[r]);
+    if (row >= p.rows) continue;
+    float* s = p.state1 + ((int64_t)row * p.D + d) * p.N + n0;
+    if (VEC) {
+      if (n0 < p.N) store_pack<float, 4>(s, h[r]);
+    } else {
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+        if (n0 + n < p.N) s[n] = h[r][n];
+    }
+    if (q == 0) ((T*)p.out)[(int64_t)row * p.D + d] = from_f32<T>(y);
   }
-  ((T*)p.out)[i] = from_f32<T>(y);
 }
 
 // ------------------------------------------------------------------------------------------------ host side
@@ -887,17 +953,21 @@ static int scan_check(const char* what, int64_t rows, int64_t L, int64_t D, int6
   return 0;
 }
 
+// the kernels step through a block's rows by 32-bit byte offsets
+static bool scan_stride_ok(int64_t st) { return st >= 0 && st < (1ll << 31) / (SCAN_Q * 4); }
+
 static void scan_shape(ScanArgs& p, int64_t rows, int64_t L, int64_t D, int64_t G, int64_t N, int64_t S) {
   p.rows = (int)rows; p.L = (int)L; p.D = (int)D; p.G = (int)G; p.N = (int)N; p.S = (int)S;
   p.Dg = (int)(D / G);
   p.tpg = (p.Dg + 63) / 64;
   p.wpg = p.G * ((p.tpg + 3) / 4);
   p.blocks = (int)ceil_div64(L, SCAN_Q);
-  // as many chunks as it takes to reach SCAN_WAVES waves, none shorter than SCAN_MIN_CHUNK tokens
+  // chunks: as many as it takes to reach two waves per SIMD, none shorter than 32 tokens; from there on to four per SIMD,
+  // none shorter than 128.  NOTE_CHUNKS
   const int64_t waves = rows * p.tpg * G;
-  int64_t n = waves > 0 ? ceil_div64(SCAN_WAVES, waves) : 1;
-  const int64_t most = L / SCAN_MIN_CHUNK;
-  n = n < most ? n : most;
+  const int64_t two = waves > 0 ? ceil_div64(SCAN_WAVES, waves) : 1, four = 2 * two;
+  const int64_t n2 = two < L / 32 ? two : L / 32, n4 = four < L / 128 ? four : L / 128;
+  const int64_t n = n2 > n4 ? n2 : n4;
   p.CL = (int)(n > 1 ? ceil_div64(ceil_div64(L, n), SCAN_Q) * SCAN_Q : p.blocks * SCAN_Q);
   p.nch = (int)(L > 0 ? ceil_div64(L, p.CL) : 1);
 }
@@ -933,7 +1003,7 @@ template <typename T, int NP, bool PACKED, bool FAST> static void scan_bwd_launc
     DVAE_LAUNCH((scan_bwd_state_kernel<T, NP, PACKED, FAST>), grid, block, 0, s, p);
     DVAE_LAUNCH((scan_join_kernel<true>), dim3((unsigned)ceil_div64((int64_t)p.N * p.D, 256), p.rows), block, 0, s, p);
   }
-  DVAE_LAUNCH((scan_bwd_kernel<T, NP, PACKED, FAST>), grid, block, 0, s, p);
+  DVAE_LAUNCH((scan_bwd_kernel<T, NP, PACKED, FAST>), grid, dim3(256 * (NP / SCAN_NW)), 0, s, p);
 }
 
 #define SCAN_LAUNCH(K, T, NP, p, s)                                                                   \
@@ -983,6 +1053,8 @@ extern "C" int dvae_selective_scan_fwd(const void* u, int64_t u_sb, int64_t u_st
   const int rc = scan_check("selective_scan_fwd", rows, L, D, G, N, S, offsets, dtype);
   if (rc) return rc;
   if (rows * L == 0) return 0;
+  DVAE_REQUIRE(scan_stride_ok(u_st) && scan_stride_ok(delta_st) && scan_stride_ok(z_st),
+               "selective_scan_fwd: token strides must be below 2^26 elements");
   ScanArgs p = {};
   p.u = u; p.u_sb = u_sb; p.u_st = u_st; p.delta = delta; p.delta_sb = delta_sb; p.delta_st = delta_st; p.A = A;
   p.B = B; p.B_sb = B_sb; p.B_st = B_st; p.B_sg = B_sg; p.C = C; p.C_sb = C_sb; p.C_st = C_st; p.C_sg = C_sg;
@@ -1011,6 +1083,8 @@ extern "C" int dvae_selective_scan_bwd(const void* u, int64_t u_sb, int64_t u_st
   if (rc) return rc;
   DVAE_REQUIRE(rows * L > 0, "selective_scan_bwd: no tokens");
   DVAE_REQUIRE(!z || dz, "selective_scan_bwd: dz is needed with z");
+  DVAE_REQUIRE(scan_stride_ok(u_st) && scan_stride_ok(delta_st) && scan_stride_ok(z_st) && scan_stride_ok(dout_st),
+               "selective_scan_bwd: token strides must be below 2^26 elements");
   ScanArgs p = {};
   p.u = u; p.u_sb = u_sb; p.u_st = u_st; p.delta = delta; p.delta_sb = delta_sb; p.delta_st = delta_st; p.A = A;
   p.B = B; p.B_sb = B_sb; p.B_st = B_st; p.B_sg = B_sg; p.C = C; p.C_sb = C_sb; p.C_st = C_st; p.C_sg = C_sg;
@@ -1055,11 +1129,24 @@ extern "C" int dvae_selective_scan_step(float* state, const void* u, int64_t u_s
   p.C = C; p.C_sb = C_sb; p.C_sg = C_sg; p.Dp = Dp; p.z = z; p.z_sb = z_sb; p.bias = bias; p.softplus = softplus;
   p.state1 = state; p.out = out;
   scan_shape(p, rows, 1, D, G, N, rows);
-  const int64_t grid = ceil_div64(rows * D, 256);
+  // four rows per lane where that leaves two workgroups per compute unit: 256 x 2048 x 16, STEP4 against STEP1 us
+  const int lpc = N > 8 ? 4 : N > 4 ? 2 : 1;
+  const bool many = ceil_div64(rows, 4) * D * lpc >= 512 * 256;
+  const bool vec = N % 4 == 0 && !((uintptr_t)state & 15);
+  const int64_t grid = ceil_div64(ceil_div64(rows, many ? 4 : 1) * D * lpc, 256);
   DVAE_REQUIRE(grid < (1ll << 31), "selective_scan_step: too many rows");
   DVAE_WORK(rows * (double)D * N * 8, DVAE_UNIT_BYTE);
-  if (dtype == DVAE_DT_F32) DVAE_LAUNCH((scan_step_kernel<float>), dim3(grid), dim3(256), 0, ST(stream), p);
-  else DVAE_LAUNCH((scan_step_kernel<bf16_t>), dim3(grid), dim3(256), 0, ST(stream), p);
+#define SCAN_STEP(T, LPC, R)                                                                               \
+  do {                                                                                                     \
+    if (vec) DVAE_LAUNCH((scan_step_kernel<T, LPC, R, true>), dim3((unsigned)grid), dim3(256), 0, ST(stream), p); \
+    else DVAE_LAUNCH((scan_step_kernel<T, LPC, R, false>), dim3((unsigned)grid), dim3(256), 0, ST(stream), p);    \
+  } while (0)
+#define SCAN_STEP_N(T, R)                                                                                  \
+  do {                                                                                                     \
+    if (lpc == 4) SCAN_STEP(T, 4, R); else if (lpc == 2) SCAN_STEP(T, 2, R); else SCAN_STEP(T, 1, R);      \
+  } while (0)
+  if (dtype == DVAE_DT_F32) { if (many) SCAN_STEP_N(float, 4); else SCAN_STEP_N(float, 1); }
+  else { if (many) SCAN_STEP_N(bf16_t, 4); else SCAN_STEP_N(bf16_t, 1); }
   DVAE_LAUNCH_CHECK("selective_scan_step");
   return 0;
 }
