@@ -392,45 +392,69 @@ __global__ void __launch_bounds__(256) SCAN_WPE scan_fwd_kernel(ScanArgs p) {
 }
 
 // The states (or, BACK, the adjoints) that enter the chunks: x = decay * x + own, along the axis.  Where a sequence
-// starts inside a chunk nothing of what enters it gets through.  A thread owns one state of one channel.
+// starts inside a chunk nothing of what enters it gets through.  Bound by the wait for memory, so a workgroup takes 64
+// elements and WAVES * JOIN_AHEAD chunks at a time, all requested at once: a wave runs through its JOIN_AHEAD chunks
+// from zero, the waves' ends are joined through LDS, and each runs through its chunks again from what really enters them.
 #define JOIN_AHEAD 16
-template <bool BACK>
-__global__ void __launch_bounds__(256) scan_join_kernel(ScanArgs p) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+template <bool BACK, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES) scan_join_kernel(ScanArgs p) {
+  __shared__ float end[WAVES][3][64];         // [wave][own, decay, 1 if nothing gets through][lane]
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int64_t ND = (int64_t)p.N * p.D;
-  if (i >= ND) return;
+  const int64_t i = min((int64_t)blockIdx.x * 64 + lane, ND - 1);      // (lanes past the last do as it does)
   const int row = blockIdx.y, d = (int)(i % p.D), n = (int)(i / p.D);
   const float A2 = p.A[(int64_t)d * p.N + n] * LOG2E_F;
   const float* sumdt = p.sumdt + (int64_t)row * p.nch * p.D + d;
-  float x = 0.f;
-  for (int k0 = 0; k0 + 1 < p.nch; k0 += JOIN_AHEAD) {
+  float x = 0.f;                                   // what enters the chunks of this round
+  for (int k0 = 0; k0 + 1 < p.nch; k0 += WAVES * JOIN_AHEAD) {
+    const int kw = k0 + wave * JOIN_AHEAD;
     float own[JOIN_AHEAD], dec[JOIN_AHEAD], keep[JOIN_AHEAD];
+    float X = 0.f, P = 1.f, cut = 0.f;
+    if (kw + 1 < p.nch) {
 #pragma unroll
-    for (int j = 0; j < JOIN_AHEAD; ++j) {
-      const int k = min(k0 + j, p.nch - 2);
-      const int c = BACK ? p.nch - 1 - k : k;              // the chunk that x passes through
-      own[j] = (BACK ? leave_slot(p, row, c - 1) : enter_slot(p, row, c + 1))[i];
-      dec[j] = sumdt[(int64_t)c * p.D];
-      keep[j] = uniform_load(p.keep, (int64_t)row * p.nch + c);
+      for (int j = 0; j < JOIN_AHEAD; ++j) {
+        const int k = min(kw + j, p.nch - 2);
+        const int c = BACK ? p.nch - 1 - k : k;              // the chunk that x passes through
+        own[j] = (BACK ? leave_slot(p, row, c - 1) : enter_slot(p, row, c + 1))[i];
+        dec[j] = sumdt[(int64_t)c * p.D];
+        keep[j] = uniform_load(p.keep, (int64_t)row * p.nch + c);
+      }
+#pragma unroll
+      for (int j = 0; j < JOIN_AHEAD; ++j) {
+        if (kw + j + 1 < p.nch) {
+          const bool through = keep[j] != 0.f;
+          dec[j] = exp2_hw(dec[j] * A2);
+          X = through ? fmaf(dec[j], X, own[j]) : own[j];
+          P = through ? P * dec[j] : 0.f;
+          cut = through ? cut : 1.f;
+        }
+      }
     }
+    end[wave][0][lane] = X;
+    end[wave][1][lane] = P;
+    end[wave][2][lane] = cut;
+    __syncthreads();
+    float mine = x;
 #pragma unroll
-    for (int j = 0; j < JOIN_AHEAD; ++j) {
-      const int k = k0 + j;
-      if (k + 1 < p.nch) {
-        const int c = BACK ? p.nch - 1 - k : k;
-        x = keep[j] != 0.f ? fmaf(exp2_hw(dec[j] * A2), x, own[j]) : own[j];
-        (BACK ? leave_slot(p, row, c - 1) : enter_slot(p, row, c + 1))[i] = x;
+    for (int v = 0; v < WAVES; ++v) {
+      if (v == wave) mine = x;
+      x = end[v][2][lane] != 0.f ? end[v][0][lane] : fmaf(end[v][1][lane], x, end[v][0][lane]);
+    }
+    __syncthreads();
+    if (kw + 1 < p.nch) {
+#pragma unroll
+      for (int j = 0; j < JOIN_AHEAD; ++j) {
+        const int k = kw + j;
+        if (k + 1 < p.nch) {
+          const int c = BACK ? p.nch - 1 - k : k;
+          mine = keep[j] != 0.f ? fmaf(dec[j], mine, own[j]) : own[j];
+          (BACK ? leave_slot(p, row, c - 1) : enter_slot(p, row, c + 1))[i] = mine;
+        }
       }
     }
   }
 }
 
-// The way back.  With g = dout silu(z), for a sequence's tokens from the last to the first:
-//   dh[n]  = C[n] g + (a[n] dh[n] of the token behind)
-//   dC[n] += g h[n]        dB[n] += dh[n] dt u          (sums over the group's channels)
-//   w      = a[n] dh[n] (what goes on to the token before);  k = w h_before[n]
-//   dA[n] += k dt          ddt += k A[n] + dh[n] B[n] u  du += dh[n] B[n] dt
-// The states are computed again, SCAN_Q tokens at a time, from those that the forward pass kept.
 template <int CTRL> __device__ __forceinline__ float dpp(float v) {
   return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false));
 }
@@ -989,11 +1013,18 @@ static bool scan_words(const ScanArgs& p, int dtype, int NP) {
   return !(odd & 1) && !(((uintptr_t)p.B | (uintptr_t)p.C) & 3);
 }
 
+// eight waves per workgroup where one would go round more than twice: 126 chunks of 1002 channels 18 -> 9 us, but 16
+// chunks of 8 x 2048 channels 10 -> 27 us
+template <bool BACK> static void scan_join(const ScanArgs& p, hipStream_t s) {
+  const dim3 grid((unsigned)ceil_div64((int64_t)p.N * p.D, 64), p.rows);
+  if (p.nch > 2 * JOIN_AHEAD + 1) DVAE_LAUNCH((scan_join_kernel<BACK, 8>), grid, dim3(64 * 8), 0, s, p);
+  else DVAE_LAUNCH((scan_join_kernel<BACK, 1>), grid, dim3(64), 0, s, p);
+}
 template <typename T, int NP, bool PACKED, bool FAST> static void scan_fwd_launch(const ScanArgs& p, hipStream_t s) {
   const dim3 grid((unsigned)((int64_t)p.rows * p.nch * p.wpg)), block(256);
   if (p.nch > 1) {
     DVAE_LAUNCH((scan_fwd_kernel<T, NP, PACKED, FAST, true>), grid, block, 0, s, p);
-    DVAE_LAUNCH((scan_join_kernel<false>), dim3((unsigned)ceil_div64((int64_t)p.N * p.D, 256), p.rows), block, 0, s, p);
+    scan_join<false>(p, s);
   }
   DVAE_LAUNCH((scan_fwd_kernel<T, NP, PACKED, FAST, false>), grid, block, 0, s, p);
 }
@@ -1001,7 +1032,7 @@ template <typename T, int NP, bool PACKED, bool FAST> static void scan_bwd_launc
   const dim3 grid((unsigned)((int64_t)p.rows * p.nch * p.wpg)), block(256);
   if (p.nch > 1) {
     DVAE_LAUNCH((scan_bwd_state_kernel<T, NP, PACKED, FAST>), grid, block, 0, s, p);
-    DVAE_LAUNCH((scan_join_kernel<true>), dim3((unsigned)ceil_div64((int64_t)p.N * p.D, 256), p.rows), block, 0, s, p);
+    scan_join<true>(p, s);
   }
   DVAE_LAUNCH((scan_bwd_kernel<T, NP, PACKED, FAST>), grid, dim3(256 * (NP / SCAN_NW)), 0, s, p);
 }

@@ -18,6 +18,26 @@ template <> __device__ __forceinline__ bf16_t from_f32<bf16_t>(float v) {      /
 
 // V consecutive elements, moved as accesses of up to 16 bytes (V > 1 only where the host checked alignment)
 template <typename T, int V> struct alignas(sizeof(T) * V < 16 ? sizeof(T) * V : 16) Pack { T v[V]; };
+// The same as it lies in memory, in whole registers (an array of 16-bit values would take one each)
+template <typename T, int V> struct Packed {
+  static constexpr int K = sizeof(T) * V < 4 ? 1 : sizeof(T) * V / 4;
+  uint32_t w[K];
+  __device__ __forceinline__ void load(const T* p) {
+    if (sizeof(T) * V < 4) {
+      w[0] = (uint32_t)*(const uint16_t*)p;
+    } else {
+      const Pack<uint32_t, K> r = *reinterpret_cast<const Pack<uint32_t, K>*>(p);
+#pragma unroll
+      for (int i = 0; i < K; ++i) w[i] = r.v[i];
+    }
+  }
+  __device__ __forceinline__ void get(float (&v)[V]) const {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      v[i] = sizeof(T) == 4 ? __uint_as_float(w[i < K ? i : 0])
+                            : __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+  }
+};
 template <typename T, int V>
 __device__ __forceinline__ void load_pack(const T* p, float (&v)[V]) {
   const Pack<T, V> r = *reinterpret_cast<const Pack<T, V>*>(p);

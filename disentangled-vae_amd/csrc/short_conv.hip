@@ -2,13 +2,14 @@
 // where tokens before a sequence's first are the carried state, or zero.  Bound by memory: every element of x is read
 // once (and a block's first W - 1 rows twice, out of the L2) and kept in registers for the W outputs that use it.
 //
-// A lane owns V neighbouring channels (16 bytes where the tensors' alignment allows it, else one element), a wave
-// CONV_TB consecutive tokens, loaded in groups of CONV_GROUP so that a group's loads are in flight together.  A batch is
-// walked as one line of tokens, sequence after sequence, so short clips fill the chip like long sequences do.
+// A lane owns one 32-bit word of a row (V = 2 bf16 channels where the tensors' alignment allows it, else one): with 16 bytes
+// per lane the window, the taps and what is in flight take so many registers that too few waves run (backward, 8 x 2048 x
+// 2048 bf16, four taps: 125 us with 16 bytes, 72 with 8, 57 with 4).  A wave takes p.tb consecutive tokens.  CONV_AHEAD tokens are in flight at any time: a token's registers receive the one CONV_AHEAD further
+// on as soon as it has been used.  A batch is walked as one line of tokens, sequence after sequence, so short clips fill the
+// chip like long sequences do.
 #include "seq_common.h"
 
-#define CONV_TB 16
-#define CONV_GROUP 8
+#define CONV_AHEAD 8
 
 struct ConvArgs {
   const void *x, *dout, *state0, *dstate1;
@@ -18,6 +19,7 @@ struct ConvArgs {
   float* part;                 // [workgroup row][W + 1][D]: partial sums of dw and dbias
   const int32_t* offsets;
   int D, S, L, tokens, silu, tiles;
+  int tb;                      // tokens whose inputs a wave reads
 };
 
 // where token t of the walk's sequence lies
@@ -25,6 +27,41 @@ template <typename T>
 __device__ __forceinline__ const T* token(const void* base, const SeqWalk& q, int64_t sb, int64_t st, int t) {
   return (const T*)base + (q.off ? t * st : q.s * sb + (t - q.b) * st);
 }
+
+// The rows of a tensor token by token, in the order of the walk, CONV_AHEAD of them requested; the last one again when
+// there are no more.
+template <typename T, int V> struct Feed {
+  const T* p;                  // row of the next token to be requested
+  int64_t st, turn;            // to the next token's row, within a sequence of the batch and into the next one
+  int left, L, more;           // tokens left in the sequence (batch) and of those to be requested
+  Packed<T, V> raw[CONV_AHEAD];
+  __device__ __forceinline__ Feed(const void* base, const SeqWalk& q, int64_t sb, int64_t st_, int t0, int n, int d)
+      : st(st_), turn(st_), left(q.tokens), L(q.tokens), more(n - 1) {
+    p = (const T*)base + t0 * st;
+    if (!q.off) {
+      L = q.L;
+      p = (const T*)base + q.s * sb + (t0 - q.b) * st;
+      turn = sb - (int64_t)(L - 1) * st;
+      left = q.e - t0;
+    }
+#pragma unroll
+    for (int j = 0; j < CONV_AHEAD; ++j) request(j, d);
+  }
+  __device__ __forceinline__ void request(int j, int d) {
+    raw[j].load(p + d);
+    if (more > 0) {
+      --more;
+      --left;
+      p += left ? st : turn;
+      left = left ? left : L;
+    }
+  }
+  // token j of the group; its place is taken by the one CONV_AHEAD further on
+  __device__ __forceinline__ void take(int j, int d, float (&v)[V]) {
+    raw[j].get(v);
+    request(j, d);
+  }
+};
 
 // the input at position t of the walk's sequence, t >= b - (W-1): a token, or what was carried in
 template <typename T, int V, int W>
@@ -50,9 +87,9 @@ __device__ __forceinline__ void load_weights(const ConvArgs& p, int d, float (&w
 template <typename T, int V, int W>
 __global__ void __launch_bounds__(256) conv_fwd_kernel(ConvArgs p) {
   const int d = ((int)(blockIdx.x % p.tiles) * 64 + (threadIdx.x & 63)) * V;
-  const int t0 = ((int)(blockIdx.x / p.tiles) * 4 + uniform(threadIdx.x >> 6)) * CONV_TB;
+  const int t0 = ((int)(blockIdx.x / p.tiles) * 4 + uniform(threadIdx.x >> 6)) * p.tb;
   if (t0 >= p.tokens || d >= p.D) return;
-  const int t1 = min(t0 + CONV_TB, p.tokens);
+  const int t1 = min(t0 + p.tb, p.tokens);
   float w[W][V], bias[V], win[W][V];
   load_weights<V, W>(p, d, w, bias);
   SeqWalk q = {p.offsets, p.S, p.L, p.tokens, 0, 0, 0};
@@ -62,38 +99,42 @@ __global__ void __launch_bounds__(256) conv_fwd_kernel(ConvArgs p) {
     for (int k = 1; k < W; ++k) load_input<T, V, W>(p, q, t0 - W + k, d, win[k]);
   }
   T* out = (T*)p.out + d;
-#pragma unroll 1
-  for (int t = t0; t < t1; ++t) {
-    if (q.s >= q.S || t < q.b) {
-      const float zero[V] = {};
-      store_pack<T, V>(out + (int64_t)t * p.D, zero);
-      continue;
-    }
-    if (t == q.b) {
+  Feed<T, V> x(p.x, q, p.x_sb, p.x_st, t0, t1 - t0, d);
+  for (int g = t0; g < t1; g += CONV_AHEAD) {
 #pragma unroll
-      for (int k = 1; k < W; ++k) load_input<T, V, W>(p, q, t - W + k, d, win[k]);
-    }
-#pragma unroll
-    for (int k = 0; k + 1 < W; ++k)
-#pragma unroll
-      for (int i = 0; i < V; ++i) win[k][i] = win[k + 1][i];
-    load_pack<T, V>(token<T>(p.x, q, p.x_sb, p.x_st, t) + d, win[W - 1]);
-    float y[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      y[i] = bias[i];
-#pragma unroll
-      for (int k = 0; k < W; ++k) y[i] = fmaf(w[k][i], win[k][i], y[i]);
-      if (p.silu) y[i] *= sigmoid_hw(y[i]);
-    }
-    store_pack<T, V>(out + (int64_t)t * p.D, y);
-    if (t + 1 == q.e) {
-      if (p.state1) {
-#pragma unroll
-        for (int k = 1; k < W; ++k)
-          store_pack<T, V>((T*)p.state1 + ((int64_t)q.s * (W - 1) + k - 1) * p.D + d, win[k]);
+    for (int j = 0; j < CONV_AHEAD; ++j) {
+      const int t = g + j;
+      if (t >= t1) continue;
+      float y[V], now[V];
+      x.take(j, d, now);
+      if (q.s >= q.S || t < q.b) {
+        const float zero[V] = {};
+        store_pack<T, V>(out + (int64_t)t * p.D, zero);
+        continue;
       }
-      q.next(t + 1);
+      if (t == q.b) {
+#pragma unroll
+        for (int k = 1; k < W; ++k) load_input<T, V, W>(p, q, t - W + k, d, win[k]);
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+#pragma unroll
+        for (int k = 0; k + 1 < W; ++k) win[k][i] = win[k + 1][i];
+        win[W - 1][i] = now[i];
+        y[i] = bias[i];
+#pragma unroll
+        for (int k = 0; k < W; ++k) y[i] = fmaf(w[k][i], win[k][i], y[i]);
+        if (p.silu) y[i] *= sigmoid_hw(y[i]);
+      }
+      store_pack<T, V>(out + (int64_t)t * p.D, y);
+      if (t + 1 == q.e) {
+        if (p.state1) {
+#pragma unroll
+          for (int k = 1; k < W; ++k)
+            store_pack<T, V>((T*)p.state1 + ((int64_t)q.s * (W - 1) + k - 1) * p.D + d, win[k]);
+        }
+        q.next(t + 1);
+      }
     }
   }
 }
@@ -116,15 +157,15 @@ __device__ __forceinline__ void grad_pre(const ConvArgs& p, const float (&w)[W][
 }
 
 // dx[t] = sum_k w[k] dpre[t + (W-1) - k] over the tokens of the same sequence; dw[k] = sum_t dpre[t] x[t - (W-1) + k].
-// A wave runs W - 1 tokens past its own, whose dpre its last tokens need.
+// A wave's own tokens are p.tb - (W-1); it runs W - 1 past them, whose dpre its last ones need.
 template <typename T, int V, int W>
 __global__ void __launch_bounds__(256) conv_bwd_kernel(ConvArgs p) {
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int d0 = ((int)(blockIdx.x % p.tiles) * 64 + lane) * V;
   const bool on = d0 < p.D;
   const int d = on ? d0 : 0;
-  const int t0 = ((int)(blockIdx.x / p.tiles) * 4 + wave) * CONV_TB;
-  const int t1 = min(t0 + CONV_TB, p.tokens);
+  const int t0 = ((int)(blockIdx.x / p.tiles) * 4 + wave) * (p.tb - (W - 1));
+  const int t1 = min(t0 + p.tb - (W - 1), p.tokens);
   float w[W][V], bias[V], win[W][V] = {}, acc[W][V] = {}, dw[W][V] = {}, db[V] = {};
   if (t0 < p.tokens) {
     load_weights<V, W>(p, d, w, bias);
@@ -134,48 +175,56 @@ __global__ void __launch_bounds__(256) conv_bwd_kernel(ConvArgs p) {
 #pragma unroll
       for (int k = 1; k < W; ++k) load_input<T, V, W>(p, q, t0 - W + k, d, win[k]);
     }
-#pragma unroll 1
-    for (int t = t0; t < t1 + W - 1; ++t) {
-      if (t < p.tokens && q.s < q.S && t >= q.b) {
-        if (t == q.b) {
+    const int n = min(t1 + W - 1, p.tokens) - t0;
+    Feed<T, V> x(p.x, q, p.x_sb, p.x_st, t0, n, d), go(p.dout, q, p.dout_sb, p.dout_st, t0, n, d);
+    for (int g0 = t0; g0 < t1 + W - 1; g0 += CONV_AHEAD) {
 #pragma unroll
-          for (int k = 1; k < W; ++k) load_input<T, V, W>(p, q, t - W + k, d, win[k]);
-        }
+      for (int j = 0; j < CONV_AHEAD; ++j) {
+        const int t = g0 + j;
+        if (t >= t1 + W - 1) continue;
+        float now[V], g[V], dp[V];
+        x.take(j, d, now);
+        go.take(j, d, g);
+        if (t < p.tokens && q.s < q.S && t >= q.b) {
+          if (t == q.b) {
 #pragma unroll
-        for (int k = 0; k + 1 < W; ++k)
-#pragma unroll
-          for (int i = 0; i < V; ++i) win[k][i] = win[k + 1][i];
-        load_pack<T, V>(token<T>(p.x, q, p.x_sb, p.x_st, t) + d, win[W - 1]);
-        float g[V], dp[V];
-        load_pack<T, V>(token<T>(p.dout, q, p.dout_sb, p.dout_st, t) + d, g);
-        grad_pre<T, V, W>(p, w, bias, win, g, dp);
-#pragma unroll
-        for (int k = 0; k < W; ++k)
-          if (t - (W - 1) + k >= q.b) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) acc[k][i] = fmaf(w[k][i], dp[i], acc[k][i]);
+            for (int k = 1; k < W; ++k) load_input<T, V, W>(p, q, t - W + k, d, win[k]);
           }
-        if (p.dstate1 && t >= q.e - (W - 1)) {
-          float c[V];
-          load_pack<T, V>((const T*)p.dstate1 + ((int64_t)q.s * (W - 1) + t - q.e + W - 1) * p.D + d, c);
-#pragma unroll
-          for (int i = 0; i < V; ++i) acc[W - 1][i] += c[i];
-        }
-        if (t < t1) {
 #pragma unroll
           for (int i = 0; i < V; ++i) {
-            db[i] += dp[i];
 #pragma unroll
-            for (int k = 0; k < W; ++k) dw[k][i] = fmaf(dp[i], win[k][i], dw[k][i]);
+            for (int k = 0; k + 1 < W; ++k) win[k][i] = win[k + 1][i];
+            win[W - 1][i] = now[i];
           }
+          grad_pre<T, V, W>(p, w, bias, win, g, dp);
+#pragma unroll
+          for (int k = 0; k < W; ++k)
+            if (t - (W - 1) + k >= q.b) {
+#pragma unroll
+              for (int i = 0; i < V; ++i) acc[k][i] = fmaf(w[k][i], dp[i], acc[k][i]);
+            }
+          if (p.dstate1 && t >= q.e - (W - 1)) {
+            float c[V];
+            load_pack<T, V>((const T*)p.dstate1 + ((int64_t)q.s * (W - 1) + t - q.e + W - 1) * p.D + d, c);
+#pragma unroll
+            for (int i = 0; i < V; ++i) acc[W - 1][i] += c[i];
+          }
+          if (t < t1) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              db[i] += dp[i];
+#pragma unroll
+              for (int k = 0; k < W; ++k) dw[k][i] = fmaf(dp[i], win[k][i], dw[k][i]);
+            }
+          }
+          if (t + 1 == q.e) q.next(t + 1);
         }
-        if (t + 1 == q.e) q.next(t + 1);
+        if (t - (W - 1) >= t0 && on) store_pack<T, V>((T*)p.dx + (int64_t)(t - (W - 1)) * p.D + d, acc[0]);
+#pragma unroll
+        for (int k = 0; k < W; ++k)
+#pragma unroll
+          for (int i = 0; i < V; ++i) acc[k][i] = k + 1 < W ? acc[k + 1 < W ? k + 1 : k][i] : 0.f;
       }
-      if (t - (W - 1) >= t0 && on) store_pack<T, V>((T*)p.dx + (int64_t)(t - (W - 1)) * p.D + d, acc[0]);
-#pragma unroll
-      for (int k = 0; k < W; ++k)
-#pragma unroll
-        for (int i = 0; i < V; ++i) acc[k][i] = k + 1 < W ? acc[k + 1 < W ? k + 1 : k][i] : 0.f;
     }
   }
   __shared__ float red[3][(W + 1) * V][64];
@@ -277,12 +326,23 @@ static int conv_check(const char* what, int64_t rows, int64_t L, int64_t D, int6
   return 0;
 }
 
-// 16 bytes per lane where every row of every tensor starts on 16 bytes, else one element
-static bool conv_wide(int64_t D, int dtype, const void* a, int64_t a_sb, int64_t a_st, const void* b, int64_t b_sb,
-                      int64_t b_st, const void* c, const void* d, const void* e) {
-  const int64_t V = dtype == DVAE_DT_F32 ? 4 : 8;
+// two bf16 channels per lane where every row of every tensor starts on 4 bytes
+static bool conv_pairs(int64_t D, int dtype, const void* a, int64_t a_sb, int64_t a_st, const void* b, int64_t b_sb,
+                       int64_t b_st, const void* c, const void* d, const void* e) {
   const uintptr_t ptrs = (uintptr_t)a | (uintptr_t)b | (uintptr_t)c | (uintptr_t)d | (uintptr_t)e;
-  return !(ptrs & 15) && !((D | a_sb | a_st | b_sb | b_st) & (V - 1));
+  return dtype == DVAE_DT_BF16 && !(ptrs & 3) && !((D | a_sb | a_st | b_sb | b_st) & 1);
+}
+
+// Tokens per wave: 32, or fewer (at least `least`) where that would leave less than four waves per SIMD: 5003 x 1001 fp32
+// forward, three taps: 18.4 us with 32, 14.6 with 16; 8 x 2048 x 2048 bf16: 32 with 32, 35 with 16, 39 with 64.
+// `past`: tokens that a wave reads beyond its own.
+static int conv_tb(int64_t tokens, int64_t tiles, int past, int least) {
+  int tb = 32;
+  while (tb > least && tiles * ceil_div64(tokens, tb - past) < 4096) tb /= 2;
+  return tb;
+}
+static int64_t conv_parts(int64_t tokens, int64_t D, int v, int W) {
+  return ceil_div64(tokens, 4 * (conv_tb(tokens, ceil_div64(D, 64 * v), W - 1, 16) - (W - 1)));
 }
 
 #define CONV_W(K, T, V, W, grid, p, s)                                                     \
@@ -291,16 +351,15 @@ static bool conv_wide(int64_t D, int dtype, const void* a, int64_t a_sb, int64_t
     else if (W == 3) DVAE_LAUNCH((K<T, V, 3>), grid, dim3(256), 0, s, p);                  \
     else DVAE_LAUNCH((K<T, V, 4>), grid, dim3(256), 0, s, p);                              \
   } while (0)
-#define CONV_DISPATCH(K, dtype, wide, W, grid, p, s)                                       \
+#define CONV_DISPATCH(K, dtype, pairs, W, grid, p, s)                                      \
   do {                                                                                     \
     if (dtype == DVAE_DT_F32) {                                                            \
-      if (wide) CONV_W(K, float, 4, W, grid, p, s); else CONV_W(K, float, 1, W, grid, p, s); \
+      CONV_W(K, float, 1, W, grid, p, s);                                                  \
     } else {                                                                               \
-      if (wide) CONV_W(K, bf16_t, 8, W, grid, p, s); else CONV_W(K, bf16_t, 1, W, grid, p, s); \
+      if (pairs) CONV_W(K, bf16_t, 2, W, grid, p, s); else CONV_W(K, bf16_t, 1, W, grid, p, s); \
     }                                                                                      \
   } while (0)
 
-static int conv_v(int dtype, bool wide) { return !wide ? 1 : dtype == DVAE_DT_F32 ? 4 : 8; }
 
 extern "C" int dvae_short_conv_fwd(const void* x, int64_t x_sb, int64_t x_st, const float* w, const float* bias, int silu,
                                    const void* state0, void* state1, const int32_t* offsets, void* out, int64_t rows,
@@ -312,19 +371,22 @@ extern "C" int dvae_short_conv_fwd(const void* x, int64_t x_sb, int64_t x_st, co
   p.x = x; p.x_sb = x_sb; p.x_st = x_st; p.w = w; p.bias = bias; p.silu = silu; p.state0 = state0; p.state1 = state1;
   p.offsets = offsets; p.out = out; p.D = (int)D; p.S = (int)(offsets ? S : rows); p.L = (int)L;
   p.tokens = (int)(rows * L);
-  const bool wide = conv_wide(D, dtype, x, x_sb, x_st, nullptr, 0, 0, state0, state1, out);
-  p.tiles = (int)ceil_div64(D, 64 * conv_v(dtype, wide));
-  const int64_t grid = p.tiles * ceil_div64(p.tokens, 4 * CONV_TB);
+  const bool pairs = conv_pairs(D, dtype, x, x_sb, x_st, nullptr, 0, 0, state0, state1, out);
+  p.tiles = (int)ceil_div64(D, 64 * (pairs ? 2 : 1));
+  p.tb = conv_tb(p.tokens, p.tiles, 0, 8);
+  const int64_t grid = p.tiles * ceil_div64(p.tokens, 4 * p.tb);
   DVAE_REQUIRE(grid < (1ll << 31), "short_conv_fwd: too large");
   const int e = dtype == DVAE_DT_F32 ? 4 : 2;
   DVAE_WORK(2.0 * p.tokens * D * e, DVAE_UNIT_BYTE);
-  CONV_DISPATCH(conv_fwd_kernel, dtype, wide, W, dim3((unsigned)grid), p, ST(stream));
+  CONV_DISPATCH(conv_fwd_kernel, dtype, pairs, W, dim3((unsigned)grid), p, ST(stream));
   DVAE_LAUNCH_CHECK("short_conv_fwd");
   return 0;
 }
 
 extern "C" int64_t dvae_short_conv_bwd_ws_floats(int64_t rows, int64_t L, int64_t D, int64_t W) {
-  return ceil_div64(rows * L, 4 * CONV_TB) * (W + 1) * D;
+  if (rows * L <= 0 || W < 2 || W > 4) return 0;
+  const int64_t a = conv_parts(rows * L, D, 1, (int)W), b = conv_parts(rows * L, D, 2, (int)W);
+  return (a > b ? a : b) * (W + 1) * D;
 }
 
 extern "C" int dvae_short_conv_bwd(const void* x, int64_t x_sb, int64_t x_st, const float* w, const float* bias, int silu,
@@ -339,13 +401,14 @@ extern "C" int dvae_short_conv_bwd(const void* x, int64_t x_sb, int64_t x_st, co
   p.x = x; p.x_sb = x_sb; p.x_st = x_st; p.w = w; p.bias = bias; p.silu = silu; p.state0 = state0; p.offsets = offsets;
   p.dout = dout; p.dout_sb = dout_sb; p.dout_st = dout_st; p.dstate1 = dstate1; p.dx = dx; p.dstate0 = dstate0;
   p.D = (int)D; p.S = (int)(offsets ? S : rows); p.L = (int)L; p.tokens = (int)(rows * L); p.part = ws;
-  const bool wide = conv_wide(D, dtype, x, x_sb, x_st, dout, dout_sb, dout_st, state0, dstate1, dx);
-  p.tiles = (int)ceil_div64(D, 64 * conv_v(dtype, wide));
-  const int64_t parts = ceil_div64(p.tokens, 4 * CONV_TB);
+  const bool pairs = conv_pairs(D, dtype, x, x_sb, x_st, dout, dout_sb, dout_st, state0, dstate1, dx);
+  p.tiles = (int)ceil_div64(D, 64 * (pairs ? 2 : 1));
+  p.tb = conv_tb(p.tokens, p.tiles, (int)W - 1, 16);
+  const int64_t parts = conv_parts(p.tokens, D, pairs ? 2 : 1, (int)W);
   DVAE_REQUIRE(p.tiles * parts < (1ll << 31), "short_conv_bwd: too large");
   const int e = dtype == DVAE_DT_F32 ? 4 : 2;
   DVAE_WORK(3.0 * p.tokens * D * e, DVAE_UNIT_BYTE);
-  CONV_DISPATCH(conv_bwd_kernel, dtype, wide, W, dim3((unsigned)(p.tiles * parts)), p, ST(stream));
+  CONV_DISPATCH(conv_bwd_kernel, dtype, pairs, W, dim3((unsigned)(p.tiles * parts)), p, ST(stream));
   DVAE_LAUNCH_CHECK("short_conv_bwd");
   DVAE_LAUNCH(conv_params_kernel, dim3((unsigned)ceil_div64((W + 1) * D, 64)), dim3(64 * SUM_WAVES), 0, ST(stream), ws, dw,
               dbias, (int)parts, (int)W, (int)D);
@@ -373,11 +436,11 @@ extern "C" int dvae_short_conv_step(void* state, const void* x, int64_t x_sb, co
   ConvArgs p = {};
   p.x = x; p.x_sb = x_sb; p.w = w; p.bias = bias; p.silu = silu; p.state1 = state; p.out = out; p.D = (int)D;
   p.tokens = (int)rows;
-  const bool wide = conv_wide(D, dtype, x, x_sb, 0, nullptr, 0, 0, state, out, nullptr);
-  const int64_t grid = ceil_div64(rows * (D / conv_v(dtype, wide)), 256);
+  const bool pairs = conv_pairs(D, dtype, x, x_sb, 0, nullptr, 0, 0, state, out, nullptr);
+  const int64_t grid = ceil_div64(rows * (D / (pairs ? 2 : 1)), 256);
   DVAE_REQUIRE(grid < (1ll << 31), "short_conv_step: too large");
   DVAE_WORK((2.0 * W) * rows * D * (dtype == DVAE_DT_F32 ? 4 : 2), DVAE_UNIT_BYTE);
-  CONV_DISPATCH(conv_step_kernel, dtype, wide, W, dim3((unsigned)grid), p, ST(stream));
+  CONV_DISPATCH(conv_step_kernel, dtype, pairs, W, dim3((unsigned)grid), p, ST(stream));
   DVAE_LAUNCH_CHECK("short_conv_step");
   return 0;
 }
