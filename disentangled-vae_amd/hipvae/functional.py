@@ -993,7 +993,11 @@ class LSTMDecoder(torch.autograd.Function):
 
 # ------------------------------------------------------------------------------------------------ sequence operators
 def _wants_grad(*ts: Optional[Tensor]) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 class SelectiveScan(torch.autograd.Function):
@@ -1111,12 +1115,10 @@ class AddRMSNorm(torch.autograd.Function):
     def forward(ctx, x, residual, weight, eps):
         a = ops.NormArgs('add_rms_norm', x, residual, weight)
         y, total, rstd = ops.add_rms_norm_fwd(a, eps, True)
-        ctx.save_for_backward(total, a.weight, rstd)
+        ctx.save_for_backward(x if residual is None else total, a.weight, rstd)
         ctx.x_dtype = x.dtype
         ctx.set_materialize_grads(False)
-        if residual is None:
-            return y.view(x.shape)
-        return y.view(x.shape), total.view(x.shape)
+        return y if residual is None else (y, total)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -1140,7 +1142,7 @@ def add_rms_norm(x: Tensor, residual: Optional[Tensor], weight: Tensor, eps: flo
         got = AddRMSNorm.apply(x, residual, weight, eps)
         return (got, x) if residual is None else got
     y, total, _ = ops.add_rms_norm_fwd(ops.NormArgs('add_rms_norm', x, residual, weight), eps, False)
-    return y.view(x.shape), x if residual is None else total.view(x.shape)
+    return y, x if residual is None else total
 
 
 def add_rms_norm_q8(x: Tensor, residual: Optional[Tensor], weight: Tensor, eps: float = 1e-6):

@@ -1059,20 +1059,8 @@ def adam_advance(dyn: Tensor, beta1: float, beta2: float):
 _ACT_DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 
 
-class _On:
-    """Makes a tensor's device current for a call where it is not."""
-
-    def __init__(self, t: Tensor):
-        self.guard = torch.cuda.device(t.device) if t.device.index != torch.cuda.current_device() else None
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-        return False
+_device_now = torch._C._cuda_getDevice
+_stream_of = torch._C._cuda_getCurrentRawStream      # raw handle of a device's current stream
 
 
 def _act_dtype(what: str, t: Tensor) -> int:
@@ -1197,41 +1185,46 @@ def _final_like(state: Optional[Tensor], shape, like: Tensor, dtype, offsets, to
 
 def selective_scan_fwd(a: ScanArgs, want_state: bool, keep: bool):
     """-> (out, final state or None, what the backward pass starts from or None)"""
-    with _On(a.u):
-        out = torch.empty(a.u.shape, dtype=a.u.dtype, device=a.u.device)
-        final = _final_like(a.state, (a.S, a.D, a.N), a.u, torch.float32, a.offsets, a.rows * a.L) if want_state else None
-        ckpt = torch.empty(int(lib.dvae_selective_scan_ckpt_floats(a.rows, a.L, a.D, a.N)), dtype=torch.float32,
-                           device=a.u.device) if keep else None
-        n = int(lib.dvae_selective_scan_fwd_ws_floats(a.rows, a.L, a.D, a.G, a.N, int(keep)))
-        ws = torch.empty(n, dtype=torch.float32, device=a.u.device) if n else None
-        check(lib.dvae_selective_scan_fwd(*a.head(), _p(final), _p(a.offsets), _p(out), _p(ckpt), *a.shape(), _p(ws),
-                                          _stream()), 'selective_scan_fwd')
+    dev = a.u.device
+    if dev.index != _device_now():
+        with torch.cuda.device(dev):
+            return selective_scan_fwd(a, want_state, keep)
+    out = torch.empty(a.u.shape, dtype=a.u.dtype, device=dev)
+    final = _final_like(a.state, (a.S, a.D, a.N), a.u, torch.float32, a.offsets, a.rows * a.L) if want_state else None
+    ckpt = torch.empty(lib.dvae_selective_scan_ckpt_floats(a.rows, a.L, a.D, a.N), dtype=torch.float32,
+                       device=dev) if keep else None
+    n = lib.dvae_selective_scan_fwd_ws_floats(a.rows, a.L, a.D, a.G, a.N, int(keep))
+    ws = torch.empty(n, dtype=torch.float32, device=dev) if n else None
+    check(lib.dvae_selective_scan_fwd(*a.head(), _p(final), _p(a.offsets), _p(out), _p(ckpt), *a.shape(), _p(ws),
+                                      _stream_of(dev.index)), 'selective_scan_fwd')
     return out, final, ckpt
 
 
 def selective_scan_bwd(a: ScanArgs, dout: Tensor, dfinal: Optional[Tensor], ckpt: Tensor, want_dstate: bool):
     """-> du, ddelta, dA, dB, dC, dD, dz, ddelta_bias, dstate (None where there is no such input)"""
     what = 'selective_scan_bwd'
+    dev = a.u.device
+    if dev.index != _device_now():
+        with torch.cuda.device(dev):
+            return selective_scan_bwd(a, dout, dfinal, ckpt, want_dstate)
     dout = _act(what, 'dout', dout, a.u.shape, a.u)
     dfinal = _param(what, 'dstate', dfinal, (a.S, a.D, a.N), a.u)
-    dev = a.u.device
     act = dict(dtype=a.u.dtype, device=dev)
     par = dict(dtype=torch.float32, device=dev)
-    with _On(a.u):
-        du, dd = torch.empty(a.u.shape, **act), torch.empty(a.u.shape, **act)
-        dz = None if a.z is None else torch.empty(a.u.shape, **act)
-        dB, dC = torch.empty(a.B.shape, **act), torch.empty(a.B.shape, **act)
-        if a.rows * a.L == 0:
-            zero = lambda t: None if t is None else torch.zeros(t.shape, **par)                      # noqa: E731
-            return du, dd, zero(a.A), dB, dC, zero(a.Dp), dz, zero(a.bias), dfinal if want_dstate else None
-        dA = torch.empty(a.A.shape, **par)
-        dD = None if a.Dp is None else torch.empty(a.D, **par)
-        db = None if a.bias is None else torch.empty(a.D, **par)
-        ds = _final_like(dfinal, (a.S, a.D, a.N), a.u, torch.float32, a.offsets, a.rows * a.L) if want_dstate else None
-        ws = torch.empty(int(lib.dvae_selective_scan_bwd_ws_floats(a.rows, a.L, a.D, a.G, a.N)), **par)
-        check(lib.dvae_selective_scan_bwd(*a.head(), _p(a.offsets), _p(dout), *_st2(dout), _p(dfinal), _p(ckpt), _p(du),
-                                          _p(dd), _p(dA), _p(dB), _p(dC), _p(dD), _p(dz), _p(db), _p(ds), *a.shape(),
-                                          _p(ws), _stream()), what)
+    du, dd = torch.empty(a.u.shape, **act), torch.empty(a.u.shape, **act)
+    dz = None if a.z is None else torch.empty(a.u.shape, **act)
+    dB, dC = torch.empty(a.B.shape, **act), torch.empty(a.B.shape, **act)
+    if a.rows * a.L == 0:
+        zero = lambda t: None if t is None else torch.zeros(t.shape, **par)                          # noqa: E731
+        return du, dd, zero(a.A), dB, dC, zero(a.Dp), dz, zero(a.bias), dfinal if want_dstate else None
+    dA = torch.empty(a.A.shape, **par)
+    dD = None if a.Dp is None else torch.empty(a.D, **par)
+    db = None if a.bias is None else torch.empty(a.D, **par)
+    ds = _final_like(dfinal, (a.S, a.D, a.N), a.u, torch.float32, a.offsets, a.rows * a.L) if want_dstate else None
+    ws = torch.empty(lib.dvae_selective_scan_bwd_ws_floats(a.rows, a.L, a.D, a.G, a.N), **par)
+    check(lib.dvae_selective_scan_bwd(*a.head(), _p(a.offsets), _p(dout), *_st2(dout), _p(dfinal), _p(ckpt), _p(du), _p(dd),
+                                      _p(dA), _p(dB), _p(dC), _p(dD), _p(dz), _p(db), _p(ds), *a.shape(), _p(ws),
+                                      _stream_of(dev.index)), what)
     return du, dd, dA, dB, dC, dD, dz, db, ds
 
 
@@ -1240,6 +1233,9 @@ def selective_scan_step(state, u, delta, A, B, C, D=None, z=None, delta_bias=Non
     states] is updated in place -> out [rows, channels]"""
     what = 'selective_scan_step'
     dtype = _act_dtype(what, u)
+    if u.device.index != _device_now():
+        with torch.cuda.device(u.device):
+            return selective_scan_step(state, u, delta, A, B, C, D, z, delta_bias, delta_softplus)
     if u.dim() != 2 or A.dim() != 2:
         raise RuntimeError(f"{what}: expected u [rows, channels] and A [channels, states], got {tuple(u.shape)} and "
                            f"{tuple(A.shape)}")
@@ -1257,12 +1253,12 @@ def selective_scan_step(state, u, delta, A, B, C, D=None, z=None, delta_bias=Non
     A = _param(what, 'A', A, (ch, N), u)
     D = _param(what, 'D', D, (ch,), u)
     delta_bias = _param(what, 'delta_bias', delta_bias, (ch,), u)
-    with _On(u):
-        out = torch.empty(rows, ch, dtype=u.dtype, device=u.device)
-        check(lib.dvae_selective_scan_step(_p(state), _p(u), u.stride(0), _p(delta), delta.stride(0), _p(A), _p(B),
-                                           B.stride(0), B.stride(1), _p(C), C.stride(0), C.stride(1), _p(D), _p(z),
-                                           0 if z is None else z.stride(0), _p(delta_bias), int(bool(delta_softplus)),
-                                           _p(out), rows, ch, G, N, dtype, _stream()), what)
+    out = torch.empty((rows, ch), dtype=u.dtype, device=u.device)
+    check(lib.dvae_selective_scan_step(state.data_ptr(), u.data_ptr(), u.stride(0), delta.data_ptr(), delta.stride(0),
+                                       A.data_ptr(), B.data_ptr(), B.stride(0), B.stride(1), C.data_ptr(), C.stride(0),
+                                       C.stride(1), _p(D), _p(z), 0 if z is None else z.stride(0), _p(delta_bias),
+                                       int(bool(delta_softplus)), out.data_ptr(), rows, ch, G, N, dtype,
+                                       _stream_of(u.device.index)), what)
     return out
 
 
@@ -1290,32 +1286,38 @@ class ConvArgs:
 
 
 def short_conv_fwd(a: ConvArgs, want_state: bool):
-    with _On(a.x):
-        out = torch.empty(a.x.shape, dtype=a.x.dtype, device=a.x.device)
-        final = _final_like(a.state, (a.S, a.W - 1, a.D), a.x, a.x.dtype, a.offsets, a.rows * a.L) if want_state else None
-        check(lib.dvae_short_conv_fwd(*a.head(), _p(final), _p(a.offsets), _p(out), *a.shape(), _stream()),
-              'short_conv_fwd')
+    """-> out, final state or None"""
+    dev = a.x.device
+    if dev.index != _device_now():
+        with torch.cuda.device(dev):
+            return short_conv_fwd(a, want_state)
+    out = torch.empty(a.x.shape, dtype=a.x.dtype, device=dev)
+    final = _final_like(a.state, (a.S, a.W - 1, a.D), a.x, a.x.dtype, a.offsets, a.rows * a.L) if want_state else None
+    check(lib.dvae_short_conv_fwd(*a.head(), _p(final), _p(a.offsets), _p(out), *a.shape(), _stream_of(dev.index)),
+          'short_conv_fwd')
     return out, final
 
 
 def short_conv_bwd(a: ConvArgs, dout: Tensor, dfinal: Optional[Tensor], want_dstate: bool):
     """-> dx, dweight, dbias, dstate"""
     what = 'short_conv_bwd'
+    dev = a.x.device
+    if dev.index != _device_now():
+        with torch.cuda.device(dev):
+            return short_conv_bwd(a, dout, dfinal, want_dstate)
     dout = _act(what, 'dout', dout, a.x.shape, a.x)
     shape = (a.S, a.W - 1, a.D)
     dfinal = _param(what, 'dstate', dfinal, shape, a.x, a.x.dtype)
-    dev = a.x.device
-    with _On(a.x):
-        dx = torch.empty(a.x.shape, dtype=a.x.dtype, device=dev)
-        if a.rows * a.L == 0:
-            return (dx, torch.zeros(a.D, a.W, device=dev), None if a.bias is None else torch.zeros(a.D, device=dev),
-                    dfinal if want_dstate else None)
-        dw = torch.empty(a.D, a.W, dtype=torch.float32, device=dev)
-        db = None if a.bias is None else torch.empty(a.D, dtype=torch.float32, device=dev)
-        ds = _final_like(dfinal, shape, a.x, a.x.dtype, a.offsets, a.rows * a.L) if want_dstate else None
-        ws = torch.empty(int(lib.dvae_short_conv_bwd_ws_floats(a.rows, a.L, a.D, a.W)), dtype=torch.float32, device=dev)
-        check(lib.dvae_short_conv_bwd(*a.head(), _p(a.offsets), _p(dout), *_st2(dout), _p(dfinal), _p(dx), _p(dw), _p(db),
-                                      _p(ds), *a.shape(), _p(ws), _stream()), what)
+    dx = torch.empty(a.x.shape, dtype=a.x.dtype, device=dev)
+    if a.rows * a.L == 0:
+        return (dx, torch.zeros(a.D, a.W, device=dev), None if a.bias is None else torch.zeros(a.D, device=dev),
+                dfinal if want_dstate else None)
+    dw = torch.empty(a.D, a.W, dtype=torch.float32, device=dev)
+    db = None if a.bias is None else torch.empty(a.D, dtype=torch.float32, device=dev)
+    ds = _final_like(dfinal, shape, a.x, a.x.dtype, a.offsets, a.rows * a.L) if want_dstate else None
+    ws = torch.empty(lib.dvae_short_conv_bwd_ws_floats(a.rows, a.L, a.D, a.W), dtype=torch.float32, device=dev)
+    check(lib.dvae_short_conv_bwd(*a.head(), _p(a.offsets), _p(dout), *_st2(dout), _p(dfinal), _p(dx), _p(dw), _p(db),
+                                  _p(ds), *a.shape(), _p(ws), _stream_of(dev.index)), what)
     return dx, dw, db, ds
 
 
@@ -1324,6 +1326,9 @@ def short_conv_step(state, x, weight, bias=None, silu=False) -> Tensor:
     is updated in place -> out [rows, channels]"""
     what = 'short_conv_step'
     dtype = _act_dtype(what, x)
+    if x.device.index != _device_now():
+        with torch.cuda.device(x.device):
+            return short_conv_step(state, x, weight, bias, silu)
     if x.dim() != 2 or weight.dim() != 2 or not 2 <= weight.shape[1] <= 4:
         raise RuntimeError(f"{what}: expected x [rows, channels] and weight [channels, 2 to 4 taps], got "
                            f"{tuple(x.shape)} and {tuple(weight.shape)}")
@@ -1333,14 +1338,13 @@ def short_conv_step(state, x, weight, bias=None, silu=False) -> Tensor:
     x = _act(what, 'x', x, x.shape, x)
     weight = _param(what, 'weight', weight, (ch, W), x)
     bias = _param(what, 'bias', bias, (ch,), x)
-    with _On(x):
-        out = torch.empty(rows, ch, dtype=x.dtype, device=x.device)
-        check(lib.dvae_short_conv_step(_p(state), _p(x), x.stride(0), _p(weight), _p(bias), int(bool(silu)), _p(out), rows,
-                                       ch, W, dtype, _stream()), what)
+    out = torch.empty((rows, ch), dtype=x.dtype, device=x.device)
+    check(lib.dvae_short_conv_step(state.data_ptr(), x.data_ptr(), x.stride(0), weight.data_ptr(), _p(bias),
+                                   int(bool(silu)), out.data_ptr(), rows, ch, W, dtype, _stream_of(x.device.index)), what)
     return out
 
 
-def _norm_rows(what: str, name: str, t: Optional[Tensor], shape, like: Tensor, dtypes) -> Optional[Tensor]:
+def _norm_rows(what: str, name: str, t: Optional[Tensor], shape, like: Tensor, *dtypes) -> Optional[Tensor]:
     """an activation [..., channels] as rows of equal stride"""
     if t is None:
         return None
@@ -1349,37 +1353,44 @@ def _norm_rows(what: str, name: str, t: Optional[Tensor], shape, like: Tensor, d
     if t.dtype not in dtypes or t.device != like.device:
         raise RuntimeError(f"{what}: {name} is {t.dtype} on {t.device}, expected {' or '.join(map(str, dtypes))} on "
                            f"{like.device}")
-    t = t.reshape(-1, shape[-1])
+    if len(shape) != 2:
+        t = t.reshape(-1, shape[-1])
     return t if t.stride(1) == 1 or shape[-1] == 1 else t.contiguous()
 
 
 class NormArgs:
+    """The checked arguments of a norm."""
+
     def __init__(self, what, x, residual, weight):
         self.dtype = _act_dtype(what, x)
-        if x.dim() < 1 or x.shape[-1] < 1:
-            raise RuntimeError(f"{what}: expected [..., channels], got {tuple(x.shape)}")
-        self.shape, self.D = x.shape, x.shape[-1]
-        self.rows = x.numel() // self.D
-        self.x = _norm_rows(what, 'x', x, x.shape, x, (x.dtype,))
-        self.residual = _norm_rows(what, 'residual', residual, x.shape, x, (x.dtype, torch.float32))
+        shape = self.shape = x.shape
+        if len(shape) < 1 or shape[-1] < 1:
+            raise RuntimeError(f"{what}: expected [..., channels], got {tuple(shape)}")
+        self.D = shape[-1]
+        self.x = _norm_rows(what, 'x', x, shape, x, x.dtype)
+        self.rows = self.x.shape[0]
+        self.residual = _norm_rows(what, 'residual', residual, shape, x, x.dtype, torch.float32)
         self.weight = _param(what, 'weight', weight, (self.D,), x)
         self.sum_dtype = x.dtype if residual is None else residual.dtype
         self.rdtype = _ACT_DTYPES[self.sum_dtype]
 
     def head(self, eps):
-        return (_p(self.x), self.x.stride(0), _p(self.residual), 0 if self.residual is None else self.residual.stride(0),
-                _p(self.weight), float(eps))
+        r = self.residual
+        return (self.x.data_ptr(), self.x.stride(0), None if r is None else r.data_ptr(), 0 if r is None else r.stride(0),
+                self.weight.data_ptr(), eps)
 
 
 def add_rms_norm_fwd(a: NormArgs, eps: float, keep: bool):
-    """-> y, sum [rows, channels] (x itself without a residual), rstd [rows] or None"""
+    """-> y, sum [..., channels] (None without a residual: it is x), rstd [rows] or None"""
     dev = a.x.device
-    with _On(a.x):
-        y = torch.empty(a.rows, a.D, dtype=a.x.dtype, device=dev)
-        total = a.x if a.residual is None else torch.empty(a.rows, a.D, dtype=a.sum_dtype, device=dev)
-        rstd = torch.empty(a.rows, dtype=torch.float32, device=dev) if keep else None
-        check(lib.dvae_add_rms_norm_fwd(*a.head(eps), _p(y), None if a.residual is None else _p(total), _p(rstd), a.rows,
-                                        a.D, a.dtype, a.rdtype, _stream()), 'add_rms_norm_fwd')
+    if dev.index != _device_now():
+        with torch.cuda.device(dev):
+            return add_rms_norm_fwd(a, eps, keep)
+    y = torch.empty(a.shape, dtype=a.x.dtype, device=dev)
+    total = None if a.residual is None else torch.empty(a.shape, dtype=a.sum_dtype, device=dev)
+    rstd = torch.empty(a.rows, dtype=torch.float32, device=dev) if keep else None
+    check(lib.dvae_add_rms_norm_fwd(*a.head(eps), y.data_ptr(), _p(total), _p(rstd), a.rows, a.D, a.dtype, a.rdtype,
+                                    _stream_of(dev.index)), 'add_rms_norm_fwd')
     return y, total, rstd
 
 
@@ -1388,38 +1399,41 @@ def add_rms_norm_q8(x: Tensor, residual: Optional[Tensor], weight: Tensor, eps: 
     is q * scale, scale = max|y| / 448 of the row (1 for a row of zeros)"""
     a = NormArgs('add_rms_norm_q8', x, residual, weight)
     dev = a.x.device
-    with _On(a.x):
-        q = torch.empty(a.rows, a.D, dtype=torch.float8_e4m3fn, device=dev)
-        scale = torch.empty(a.rows, dtype=torch.float32, device=dev)
-        total = None if a.residual is None else torch.empty(a.rows, a.D, dtype=a.sum_dtype, device=dev)
-        check(lib.dvae_add_rms_norm_q8(*a.head(eps), _p(q), _p(scale), _p(total), a.rows, a.D, a.dtype, a.rdtype,
-                                       _stream()), 'add_rms_norm_q8')
-    return q.view(a.shape), scale.view(a.shape[:-1]), x if total is None else total.view(a.shape)
+    if dev.index != _device_now():
+        with torch.cuda.device(dev):
+            return add_rms_norm_q8(x, residual, weight, eps)
+    q = torch.empty(a.shape, dtype=torch.float8_e4m3fn, device=dev)
+    scale = torch.empty(a.shape[:-1], dtype=torch.float32, device=dev)
+    total = None if a.residual is None else torch.empty(a.shape, dtype=a.sum_dtype, device=dev)
+    check(lib.dvae_add_rms_norm_q8(*a.head(eps), q.data_ptr(), scale.data_ptr(), _p(total), a.rows, a.D, a.dtype, a.rdtype,
+                                   _stream_of(dev.index)), 'add_rms_norm_q8')
+    return q, scale, x if total is None else total
 
 
 def add_rms_norm_bwd(dy: Tensor, dsum: Optional[Tensor], total: Tensor, weight: Tensor, rstd: Tensor, dx_dtype):
     """dy [..., channels] of x's type, dsum and total of the sum's -> dx, dresidual (the same tensor where the types are
     the same: autograd then copies before it keeps either), dweight"""
     what = 'add_rms_norm_bwd'
+    dev = dy.device
+    if dev.index != _device_now():
+        with torch.cuda.device(dev):
+            return add_rms_norm_bwd(dy, dsum, total, weight, rstd, dx_dtype)
     shape = dy.shape
     D = shape[-1]
-    dy2 = _norm_rows(what, 'dy', dy, shape, dy, (dx_dtype,))
-    ds2 = _norm_rows(what, 'dsum', dsum, shape, dy, (total.dtype,))
-    rows, dev = dy2.shape[0], dy.device
+    dy2 = _norm_rows(what, 'dy', dy, shape, dy, dx_dtype)
+    ds2 = _norm_rows(what, 'dsum', dsum, shape, dy, total.dtype)
+    s2 = _norm_rows(what, 'sum', total, shape, dy, total.dtype)
+    rows = dy2.shape[0]
+    dres = torch.empty(shape, dtype=total.dtype, device=dev)
+    dx = dres if total.dtype == dx_dtype else torch.empty(shape, dtype=dx_dtype, device=dev)
     if rows == 0:
-        none = torch.empty(shape, dtype=dx_dtype, device=dev)
-        return none, none.to(total.dtype), torch.zeros(D, device=dev)
-    with _On(dy):
-        dres = torch.empty(rows, D, dtype=total.dtype, device=dev)
-        dx = dres if total.dtype == dx_dtype else torch.empty(rows, D, dtype=dx_dtype, device=dev)
-        dw = torch.empty(D, dtype=torch.float32, device=dev)
-        ws = torch.empty(int(lib.dvae_add_rms_norm_bwd_ws_floats(rows, D)), dtype=torch.float32, device=dev)
-        check(lib.dvae_add_rms_norm_bwd(_p(dy2), dy2.stride(0), _p(ds2), 0 if ds2 is None else ds2.stride(0), _p(total),
-                                        total.stride(0), _p(weight), _p(rstd), _p(dres), _p(dx), _p(dw), rows, D,
-                                        _ACT_DTYPES[dx_dtype], _ACT_DTYPES[total.dtype], _p(ws), _stream()), what)
-    same = dx is dres
-    dres = dres.view(shape)
-    return dres if same else dx.view(shape), dres, dw
+        return dx, dres, torch.zeros(D, dtype=torch.float32, device=dev)
+    dw = torch.empty(D, dtype=torch.float32, device=dev)
+    ws = torch.empty(lib.dvae_add_rms_norm_bwd_ws_floats(rows, D), dtype=torch.float32, device=dev)
+    check(lib.dvae_add_rms_norm_bwd(_p(dy2), dy2.stride(0), _p(ds2), 0 if ds2 is None else ds2.stride(0), _p(s2),
+                                    s2.stride(0), _p(weight), _p(rstd), _p(dres), _p(dx), _p(dw), rows, D,
+                                    _ACT_DTYPES[dx_dtype], _ACT_DTYPES[total.dtype], _p(ws), _stream_of(dev.index)), what)
+    return dx, dres, dw
 
 
 # ---------------------------------------------------------------------------- launch trace (benchmarks)
