@@ -135,28 +135,29 @@ template <typename T, int NP> struct BCAhead<T, NP, false> {
   }
 };
 
-// 64 channels of one group, one chunk of one row.  A workgroup's four tiles are neighbours in a group; a tile is the work
-// of one wave, or of `share` waves that have a part of the states each.
+// 64 channels of one group, one chunk of one row.  A workgroup's tiles are neighbours in a group; a tile is the work of
+// one wave, or of `share` waves that have a part of the states each.
 struct Tile {
   int g, d, lane, wave, part, chunk, row, t0, t1;
-  bool on;
-  __device__ __forceinline__ explicit Tile(const ScanArgs& p, int share = 1) {
+  bool on, idle;
+  __device__ __forceinline__ explicit Tile(const ScanArgs& p, int tiles = 4, int share = 1) {
     lane = threadIdx.x & 63;
     wave = uniform(threadIdx.x >> 6) / share;
-    const int wg = blockIdx.x % p.wpg;
-    const int rc = blockIdx.x / p.wpg;
-    const int per = (p.tpg + 3) / 4;
+    const int per = (p.tpg + tiles - 1) / tiles;
+    const int wg = blockIdx.x % (p.G * per);
+    const int rc = blockIdx.x / (p.G * per);
     g = wg / per;
     part = wg % per;
     chunk = rc % p.nch;
     row = rc / p.nch;
     t0 = chunk * p.CL;
     t1 = min(t0 + p.CL, p.L);
-    const int c = (part * 4 + wave) * 64 + lane;
+    const int tile = part * tiles + wave;
+    const int c = tile * 64 + lane;
+    idle = tile >= p.tpg;
     on = c < p.Dg;
     d = g * p.Dg + (on ? c : p.Dg - 1);          // lanes past the group's last channel read it too, and write nothing
   }
-  __device__ __forceinline__ bool idle(const ScanArgs& p) const { return part * 4 + wave >= p.tpg; }
 };
 
 // NP states of a channel from the n0-th on, of a state tensor [S][D][N]
@@ -226,14 +227,15 @@ template <typename T> struct Rows {
   uint32_t step;       // bytes from token to token (the host checked that a block's rows span less than 2 GiB)
   __device__ __forceinline__ Rows(const void* p, int64_t sb, int64_t st, int row, int t0)
       : base((const T*)p + row * sb + t0 * st), block(st * SCAN_Q), step((uint32_t)st * (uint32_t)sizeof(T)) {}
-  // token 0 .. SCAN_Q - 1 of the block; those past the n-th are the n-th again
-  __device__ __forceinline__ void load(T (&v)[SCAN_Q], int n, uint32_t at) const {
+  // K tokens of the block from the j0-th on; those past the n-th are the n-th again
+  template <int K> __device__ __forceinline__ void load(T (&v)[K], int n, uint32_t at, int j0 = 0) const {
     uint64_t r = (uint64_t)base;
     asm("" : "+s"(r));           // (keeps the compiler from adding the lane's place to it)
+    at += (uint32_t)max(min(j0, n - 1), 0) * step;
 #pragma unroll
-    for (int j = 0; j < SCAN_Q; ++j) {
+    for (int j = 0; j < K; ++j) {
       v[j] = *(const DVAE_GLOBAL T*)((const DVAE_GLOBAL char*)r + at);
-      at += j + 1 < n ? step : 0u;
+      at += j0 + j + 1 < n ? step : 0u;
     }
   }
 };
@@ -248,7 +250,7 @@ template <typename T> struct Rows {
 template <typename T, int NP, bool PACKED, bool FAST, bool STATE_ONLY>
 __global__ void __launch_bounds__(256) SCAN_WPE scan_fwd_kernel(ScanArgs p) {
   const Tile w(p);
-  if (w.idle(p) || (STATE_ONLY && w.chunk + 1 == p.nch)) return;
+  if (w.idle || (STATE_ONLY && w.chunk + 1 == p.nch)) return;
   const int row = w.row;
   float A2[NP], h[NP];
 #pragma unroll
@@ -495,7 +497,7 @@ __device__ __forceinline__ float wave_sums16(float (&v)[16], int lane) {
 template <typename T, int NP, bool PACKED, bool FAST>
 __global__ void __launch_bounds__(256) SCAN_WPE scan_bwd_state_kernel(ScanArgs p) {
   const Tile w(p);
-  if (w.idle(p) || w.chunk == 0) return;
+  if (w.idle || w.chunk == 0) return;
   const int row = w.row;
   float A2[NP], x[NP];
 #pragma unroll
@@ -599,17 +601,22 @@ __global__ void __launch_bounds__(256) SCAN_WPE scan_bwd_state_kernel(ScanArgs p
 // The states of a tile are shared out over SHARE = NP / 8 waves, eight states each: what one wave keeps of a block (the
 // states before its tokens and the decays, computed once for both directions) then fits 256 registers, so that two waves
 // run per SIMD and fill each other's waits; with sixteen states in a wave it took 480 and ran alone (8 x 2048 x 2048 bf16:
-// SHARE1 against SHARE2 us).  The waves add up their parts of y, of the sum of dh B and of that of k A through LDS, once
-// per block, and each finishes the gradients of its share of the block's tokens.
+// 790 against 651 us).  What a channel's token needs besides its states, each wave of a tile does for its share of the
+// block's tokens: it loads their inputs, computes their step sizes and gates for the others, and finishes their gradients
+// from the waves' parts of y, of the sum of dh B and of that of k A, all by way of LDS.
 #define SCAN_NW 8
+#ifndef SCAN_BT
+#define SCAN_BT 2
+#endif
 template <typename T, int NP, bool PACKED, bool FAST>
-__global__ void __launch_bounds__(256 * (NP / SCAN_NW), 2) scan_bwd_kernel(ScanArgs p) {
+__global__ void __launch_bounds__(64 * SCAN_BT * (NP / SCAN_NW), 2) scan_bwd_kernel(ScanArgs p) {
   constexpr int SHARE = NP / SCAN_NW, OWN = SCAN_Q / SHARE;      // waves per tile; tokens of a block that a wave finishes
-  __shared__ float red[SCAN_Q][4][2 * NP];                       // [token][tile][dB, dC]
-  __shared__ float part[SCAN_Q][3][4 * SHARE][64];               // [token][y, dh B, k A][wave][lane]
-  const Tile w(p, SHARE);
-  const int row = w.row, wv = uniform(threadIdx.x >> 6), half = wv % SHARE, n0 = half * SCAN_NW;
-  const bool idle = w.idle(p);                     // such a wave only takes part in the sums
+  __shared__ float red[SCAN_Q][SCAN_BT][2 * NP];                       // [token][tile][dB, dC]
+  __shared__ float part[SCAN_Q][3][SCAN_BT * SHARE][64];               // [token][y, dh B, k A][wave][lane]
+  __shared__ float in[SCAN_Q][3][SCAN_BT][64];                         // [token][dt, dt u, g][tile][lane]
+  const Tile w(p, SCAN_BT, SHARE);
+  const int row = w.row, wv = uniform(threadIdx.x >> 6), half = wv % SHARE, n0 = half * SCAN_NW, j0 = half * OWN;
+  const bool idle = w.idle;                     // such a wave only takes part in the sums
   const int Nw = min(max(p.N - n0, 0), SCAN_NW);   // states that this wave has
   float A2[SCAN_NW], dh[SCAN_NW], dA[SCAN_NW];
 #pragma unroll
@@ -637,18 +644,18 @@ __global__ void __launch_bounds__(256 * (NP / SCAN_NW), 2) scan_bwd_kernel(ScanA
   Rows<T> ur(p.u, p.u_sb, p.u_st, row, first), dr(p.delta, p.delta_sb, p.delta_st, row, first);
   Rows<T> gr(p.dout, p.dout_sb, p.dout_st, row, first);
   Rows<T> zr(gated ? p.z : p.dout, gated ? p.z_sb : p.dout_sb, gated ? p.z_st : p.dout_st, row, first);  // (not used without z)
-  T un[SCAN_Q], dn[SCAN_Q], zn[SCAN_Q], gn[SCAN_Q];   // the block ahead,
+  T un[OWN], dn[OWN], zn[OWN], gn[OWN];               // this wave's tokens of the block ahead,
   float hn[SCAN_NW];                                  // and the state that enters it
-  ur.load(un, w.t1 - first, at);
-  dr.load(dn, w.t1 - first, at);
-  zr.load(zn, w.t1 - first, at);
-  gr.load(gn, w.t1 - first, at);
+  ur.load(un, w.t1 - first, at, j0);
+  dr.load(dn, w.t1 - first, at, j0);
+  zr.load(zn, w.t1 - first, at, j0);
+  gr.load(gn, w.t1 - first, at, j0);
   load_slot<SCAN_NW, FAST>(ck, p, w.d, hn, Nw);
 
   for (int t0 = first; t0 >= w.t0; t0 -= SCAN_Q) {
     const int n = min(SCAN_Q, w.t1 - t0);
-    T ub[SCAN_Q], zb[SCAN_Q], gb[SCAN_Q];
-    float hs[SCAN_Q + 1][SCAN_NW], db[SCAN_Q], slope[SCAN_Q];
+    float hs[SCAN_Q + 1][SCAN_NW];
+    float dt_[OWN], slope[OWN], u_[OWN], z_[OWN], g_[OWN];      // of this wave's tokens
 #pragma unroll
     for (int i = 0; i < SCAN_NW; ++i) hs[0][i] = hn[i];
     SeqWalk f = q;                                 // the sequence that the states' second computation is in
@@ -665,26 +672,37 @@ __global__ void __launch_bounds__(256 * (NP / SCAN_NW), 2) scan_bwd_kernel(ScanA
         ur.base -= ur.block; dr.base -= dr.block; zr.base -= zr.block; gr.base -= gr.block;
       }
       const int left = t0 > w.t0 ? SCAN_Q : n;
-      ur.load(un, left, at);
-      dr.load(dn, left, at);
-      zr.load(zn, left, at);
-      gr.load(gn, left, at);
+      ur.load(un, left, at, j0);
+      dr.load(dn, left, at, j0);
+      zr.load(zn, left, at, j0);
+      gr.load(gn, left, at, j0);
       load_slot<SCAN_NW, FAST>(ck, p, w.d, hn, Nw);
     };
 #pragma unroll
-    for (int j = 0; j < SCAN_Q; ++j) {             // tokens past the chunk's last: a step size of 0
-      ub[j] = un[j]; zb[j] = zn[j]; gb[j] = gn[j];
-      const float pre = to_f32(dn[j]) + bias;
-      const float sp = softplus_hw(pre, slope[j]);
-      db[j] = j < n ? (plus ? sp : pre) : 0.f;
-      slope[j] = plus ? slope[j] : 1.f;
+    for (int jj = 0; jj < OWN; ++jj) {
+      // tokens past the chunk's last have a step size and a gradient of 0, which changes nothing, and so have lanes past
+      // the group's last channel, which keeps them out of the sums over the channels
+      const bool there = j0 + jj < n && w.on;
+      const float pre = to_f32(dn[jj]) + bias;
+      const float sp = softplus_hw(pre, slope[jj]);
+      dt_[jj] = there ? (plus ? sp : pre) : 0.f;
+      slope[jj] = plus ? slope[jj] : 1.f;
+      u_[jj] = to_f32(un[jj]);
+      z_[jj] = to_f32(zn[jj]);
+      g_[jj] = there ? to_f32(gn[jj]) : 0.f;
+      in[j0 + jj][0][w.wave][w.lane] = dt_[jj];
+      in[j0 + jj][1][w.wave][w.lane] = dt_[jj] * u_[jj];
+      in[j0 + jj][2][w.wave][w.lane] = gated ? g_[jj] * (z_[jj] * sigmoid_hw(z_[jj])) : g_[jj];
     }
+    __syncthreads();                               // and everyone has read the sums of the block behind
     if (plain) {
-      // no sequence starts or ends here: straight-line code, as in the forward pass.  Tokens past the chunk's last have
-      // a step size and a gradient of 0, which changes nothing.
+      // no sequence starts or ends here: straight-line code, as in the forward pass
       float a[SCAN_Q][SCAN_NW];
       BCAhead<T, SCAN_NW, FAST> ahead;
       const T *Bt = B + t0 * p.B_st, *Ct = C + t0 * p.C_st;
+      // What is read from LDS is read a token ahead too, beside the request for B and C: waiting for LDS alone is not
+      // possible while scalar loads are on the way.
+      float dtn = in[0][0][w.wave][w.lane], xn = in[0][1][w.wave][w.lane], gn_;
       ahead.request_b(Bt, Nw);
 #pragma unroll
       for (int j = 0; j < SCAN_Q; ++j) {
@@ -696,15 +714,20 @@ __global__ void __launch_bounds__(256 * (NP / SCAN_NW), 2) scan_bwd_kernel(ScanA
         if (j + 1 < SCAN_Q) ahead.request_b(Bt, Nw);
         else ahead.request(Bt, Ct, Nw);            // the last token's, where the way back begins
         now.get_b(Bv);
-        const float x = db[j] * to_f32(ub[j]);
+        const float dt = dtn, x = xn;
+        if (j + 1 < SCAN_Q) {
+          dtn = in[j + 1][0][w.wave][w.lane];
+          xn = in[j + 1][1][w.wave][w.lane];
+        } else {
+          gn_ = in[j][2][w.wave][w.lane];
+        }
 #pragma unroll
         for (int i = 0; i < SCAN_NW; ++i) {
-          a[j][i] = exp2_hw(db[j] * A2[i]);
+          a[j][i] = exp2_hw(dt * A2[i]);
           hs[j + 1][i] = fmaf(a[j][i], hs[j][i], x * Bv[i]);
         }
         __builtin_amdgcn_sched_barrier(0);         // (mixing tokens spills registers: SB0 against SB2 us)
       }
-      __syncthreads();                             // everyone has read the sums of the block behind
 #pragma unroll
       for (int j = SCAN_Q - 1; j >= 0; --j) {
         if (j == SCAN_Q / 2 - 1) request();
@@ -715,22 +738,23 @@ __global__ void __launch_bounds__(256 * (NP / SCAN_NW), 2) scan_bwd_kernel(ScanA
         now.arrived(Bt, Ct);
         if (j > 0) ahead.request(Bt, Ct, Nw);
         now.get(Bv, Cv);
-        const float zz = to_f32(zb[j]);
-        float g = j < n ? to_f32(gb[j]) : 0.f;
-        g = gated ? g * (zz * sigmoid_hw(zz)) : g;
-        // lanes past the last channel add nothing to the sums over the channels
-        const float x = w.on ? db[j] * to_f32(ub[j]) : 0.f, gs = w.on ? g : 0.f;
+        const float dt = dtn, x = xn, g = gn_;
+        if (j > 0) {
+          dtn = in[j - 1][0][w.wave][w.lane];
+          xn = in[j - 1][1][w.wave][w.lane];
+          gn_ = in[j - 1][2][w.wave][w.lane];
+        }
         float y = 0.f, through = 0.f, ka = 0.f, pv[2 * SCAN_NW];
 #pragma unroll
         for (int i = 0; i < SCAN_NW; ++i) {
           y = fmaf(Cv[i], hs[j + 1][i], y);
           const float d = fmaf(Cv[i], g, dh[i]);
           pv[i] = d * x;
-          pv[SCAN_NW + i] = gs * hs[j + 1][i];
+          pv[SCAN_NW + i] = g * hs[j + 1][i];
           through = fmaf(d, Bv[i], through);
           dh[i] = d * a[j][i];
           const float k = dh[i] * hs[j][i];
-          dA[i] = fmaf(k, db[j], dA[i]);
+          dA[i] = fmaf(k, dt, dA[i]);
           ka = fmaf(k, A2[i], ka);
         }
         part[j][0][wv][w.lane] = y;
@@ -738,7 +762,7 @@ __global__ void __launch_bounds__(256 * (NP / SCAN_NW), 2) scan_bwd_kernel(ScanA
         part[j][2][wv][w.lane] = ka;
         const float sum = wave_sums16(pv, w.lane);
         const int c = sum_index(w.lane);
-        red[j][w.wave][c < SCAN_NW ? n0 + c : NP + n0 + c - SCAN_NW] = idle ? 0.f : sum;    // (four lanes alike)
+        red[j][w.wave][c < SCAN_NW ? n0 + c : NP + n0 + c - SCAN_NW] = sum;    // (four lanes alike)
         __builtin_amdgcn_sched_barrier(0);
       }
     } else {
@@ -751,12 +775,11 @@ __global__ void __launch_bounds__(256 * (NP / SCAN_NW), 2) scan_bwd_kernel(ScanA
         if (m.start >> j & 1) entering_state<SCAN_NW>(p, f.seq(), w.d, hs[j + 1], n0);
         float Bv[SCAN_NW];
         BCLoad<T, SCAN_NW, FAST>::get(B, t * p.B_st, Nw, Bv);
-        const float x = db[j] * to_f32(ub[j]);
+        const float dt = in[j][0][w.wave][w.lane], x = in[j][1][w.wave][w.lane];
 #pragma unroll
-        for (int i = 0; i < SCAN_NW; ++i) hs[j + 1][i] = fmaf(exp2_hw(db[j] * A2[i]), hs[j + 1][i], x * Bv[i]);
+        for (int i = 0; i < SCAN_NW; ++i) hs[j + 1][i] = fmaf(exp2_hw(dt * A2[i]), hs[j + 1][i], x * Bv[i]);
         if (m.end >> j & 1) f.next((int)t + 1);
       }
-      __syncthreads();
       request();
 #pragma unroll
       for (int j = SCAN_Q - 1; j >= 0; --j) {
@@ -776,10 +799,7 @@ __global__ void __launch_bounds__(256 * (NP / SCAN_NW), 2) scan_bwd_kernel(ScanA
         float Bv[SCAN_NW], Cv[SCAN_NW];
         BCLoad<T, SCAN_NW, FAST>::get(B, t * p.B_st, Nw, Bv);
         BCLoad<T, SCAN_NW, FAST>::get(C, t * p.C_st, Nw, Cv);
-        float g = to_f32(gb[j]);
-        const float zz = to_f32(zb[j]);
-        g = gated ? g * (zz * sigmoid_hw(zz)) : g;
-        const float x = w.on ? db[j] * to_f32(ub[j]) : 0.f, gs = w.on ? g : 0.f;
+        const float dt = in[j][0][w.wave][w.lane], x = in[j][1][w.wave][w.lane], g = in[j][2][w.wave][w.lane];
         float y = 0.f, through = 0.f, ka = 0.f, pv[2 * SCAN_NW], hb[SCAN_NW];
 #pragma unroll
         for (int i = 0; i < SCAN_NW; ++i) hb[i] = hs[j][i];
@@ -789,11 +809,11 @@ __global__ void __launch_bounds__(256 * (NP / SCAN_NW), 2) scan_bwd_kernel(ScanA
           y = fmaf(Cv[i], hs[j + 1][i], y);
           const float d = fmaf(Cv[i], g, dh[i]);
           pv[i] = d * x;
-          pv[SCAN_NW + i] = gs * hs[j + 1][i];
+          pv[SCAN_NW + i] = g * hs[j + 1][i];
           through = fmaf(d, Bv[i], through);
-          dh[i] = d * exp2_hw(db[j] * A2[i]);
+          dh[i] = d * exp2_hw(dt * A2[i]);
           const float k = dh[i] * hb[i];
-          dA[i] = fmaf(k, db[j], dA[i]);
+          dA[i] = fmaf(k, dt, dA[i]);
           ka = fmaf(k, A2[i], ka);
         }
         part[j][0][wv][w.lane] = y;
@@ -801,7 +821,7 @@ __global__ void __launch_bounds__(256 * (NP / SCAN_NW), 2) scan_bwd_kernel(ScanA
         part[j][2][wv][w.lane] = ka;
         const float sum = wave_sums16(pv, w.lane);
         const int c = sum_index(w.lane);
-        red[j][w.wave][c < SCAN_NW ? n0 + c : NP + n0 + c - SCAN_NW] = idle ? 0.f : sum;    // (four lanes alike)
+        red[j][w.wave][c < SCAN_NW ? n0 + c : NP + n0 + c - SCAN_NW] = sum;    // (four lanes alike)
         if (m.start >> j & 1) {
           if (p.dstate0 && w.on && !idle) store_state<SCAN_NW>(p.dstate0, q.seq(), p, w.d, dh, n0);
           q.prev((int)t - 1);
@@ -809,40 +829,29 @@ __global__ void __launch_bounds__(256 * (NP / SCAN_NW), 2) scan_bwd_kernel(ScanA
       }
     }
     __syncthreads();
-    // this wave's tokens: j = half * OWN + jj
-    int64_t o = (flat + t0 + half * OWN) * p.D;
+    int64_t o = (flat + t0 + j0) * p.D;
 #pragma unroll
     for (int jj = 0; jj < OWN; ++jj) {
-      const int j = half * OWN + jj;
-      float uu = to_f32(ub[jj]), zz = to_f32(zb[jj]), g0 = to_f32(gb[jj]), dt = db[jj], sl = slope[jj];
-#pragma unroll
-      for (int k = 1; k < SHARE; ++k) {            // (the registers of token j, chosen by the wave)
-        const bool mine = half == k;
-        uu = mine ? to_f32(ub[k * OWN + jj]) : uu;
-        zz = mine ? to_f32(zb[k * OWN + jj]) : zz;
-        g0 = mine ? to_f32(gb[k * OWN + jj]) : g0;
-        dt = mine ? db[k * OWN + jj] : dt;
-        sl = mine ? slope[k * OWN + jj] : sl;
-      }
+      const int j = j0 + jj;
       if (j < n) {
         float du = 0.f, dd = 0.f, dz = 0.f;
         if (!PACKED || (m.valid >> j & 1)) {
-          float y = Dp * uu, through = 0.f, ka = 0.f;
+          float y = Dp * u_[jj], through = 0.f, ka = 0.f;
 #pragma unroll
           for (int k = 0; k < SHARE; ++k) {
             y += part[j][0][w.wave * SHARE + k][w.lane];
             through += part[j][1][w.wave * SHARE + k][w.lane];
             ka += part[j][2][w.wave * SHARE + k][w.lane];
           }
-          const float sg = sigmoid_hw(zz);
-          const float g = gated ? g0 * (zz * sg) : g0;
-          dz = g0 * y * sg * fmaf(zz, 1.f - sg, 1.f);
-          du = fmaf(through, dt, Dp * g);
-          dd = fmaf(ka, LN2_F, through * uu) * sl;
-          dD = fmaf(g, uu, dD);
+          const float sg = sigmoid_hw(z_[jj]);
+          const float g = gated ? g_[jj] * (z_[jj] * sg) : g_[jj];
+          dz = g_[jj] * y * sg * fmaf(z_[jj], 1.f - sg, 1.f);
+          du = fmaf(through, dt_[jj], Dp * g);
+          dd = fmaf(ka, LN2_F, through * u_[jj]) * slope[jj];
+          dD = fmaf(g, u_[jj], dD);
           dbias += dd;
         }
-        if (!idle) {
+        if (w.on && !idle) {
           if (gated) lane_store((T*)p.dz + o, at, from_f32<T>(dz));
           lane_store((T*)p.du + o, at, from_f32<T>(du));
           lane_store((T*)p.ddelta + o, at, from_f32<T>(dd));
@@ -850,9 +859,11 @@ __global__ void __launch_bounds__(256 * (NP / SCAN_NW), 2) scan_bwd_kernel(ScanA
       }
       o += p.D;
     }
-    for (int i = threadIdx.x; i < n * 2 * p.N; i += 256 * SHARE) {
+    for (int i = threadIdx.x; i < n * 2 * p.N; i += 64 * SCAN_BT * SHARE) {
       const int j = i / (2 * p.N), c = i % (2 * p.N), k = c < p.N ? c : c - p.N + NP;
-      const float s = (red[j][0][k] + red[j][1][k]) + (red[j][2][k] + red[j][3][k]);
+      float s = red[j][0][k];
+#pragma unroll
+      for (int t = 1; t < SCAN_BT; ++t) s += red[j][t][k];
       p.part_bc[(((int64_t)w.part * p.rows * p.L + flat + t0 + j) * p.G + w.g) * 2 * p.N + c] = s;
     }
   }
@@ -906,7 +917,7 @@ __global__ void __launch_bounds__(64 * SUM_WAVES) scan_params_kernel(const float
 }
 
 // One token per row.  Nearly all of the traffic is the state, read and written once: a lane owns four states of a channel
-// (one 16-byte access each way where N is a multiple of 4), a channel's LPC lanes are neighbours, and the sum over them
+// (one 16-byte access each way where N is a multiple of 4 and all is aligned), a channel's LPC lanes are neighbours, and the sum over them
 // takes two lane exchanges.  What a channel reads besides (inputs, step size) its lanes read and compute alike.  A lane
 // goes through R rows whose loads are in flight together and share its A.
 template <typename T, int LPC, int R, bool VEC>
@@ -924,13 +935,18 @@ __global__ void __launch_bounds__(256) scan_step_kernel(ScanArgs p) {
     const float* s = p.state1 + ((int64_t)row * p.D + d) * p.N + n0;
     const T* B = (const T*)p.B + row * p.B_sb + g * p.B_sg + n0;
     const T* C = (const T*)p.C + row * p.C_sb + g * p.C_sg + n0;
-    if (VEC && n0 < p.N) load_pack<float, 4>(s, h[r]);
+    if (VEC && n0 < p.N) {
+      load_pack<float, 4>(s, h[r]);
+      load_pack<T, 4>(B, Bv[r]);
+      load_pack<T, 4>(C, Cv[r]);
+    } else {
 #pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      const bool there = n0 + n < p.N;
-      if (!VEC || n0 >= p.N) h[r][n] = there ? s[n] : 0.f;
-      Bv[r][n] = there ? to_f32(B[n]) : 0.f;
-      Cv[r][n] = there ? to_f32(C[n]) : 0.f;
+      for (int n = 0; n < 4; ++n) {
+        const bool there = n0 + n < p.N;
+        h[r][n] = there ? s[n] : 0.f;
+        Bv[r][n] = there ? to_f32(B[n]) : 0.f;
+        Cv[r][n] = there ? to_f32(C[n]) : 0.f;
+      }
     }
     uu[r] = to_f32(((const T*)p.u)[row * p.u_sb + d]);
     pre[r] = to_f32(((const T*)p.delta)[row * p.delta_sb + d]);
@@ -979,6 +995,9 @@ static int scan_check(const char* what, int64_t rows, int64_t L, int64_t D, int6
 
 // the kernels step through a block's rows by 32-bit byte offsets
 static bool scan_stride_ok(int64_t st) { return st >= 0 && st < (1ll << 31) / (SCAN_Q * 4); }
+
+// rows of partial sums of dB and dC: one per workgroup of the backward kernel within a group
+static int scan_bc_parts(int tpg) { return (tpg + SCAN_BT - 1) / SCAN_BT; }
 
 static void scan_shape(ScanArgs& p, int64_t rows, int64_t L, int64_t D, int64_t G, int64_t N, int64_t S) {
   p.rows = (int)rows; p.L = (int)L; p.D = (int)D; p.G = (int)G; p.N = (int)N; p.S = (int)S;
@@ -1034,7 +1053,8 @@ template <typename T, int NP, bool PACKED, bool FAST> static void scan_bwd_launc
     DVAE_LAUNCH((scan_bwd_state_kernel<T, NP, PACKED, FAST>), grid, block, 0, s, p);
     scan_join<true>(p, s);
   }
-  DVAE_LAUNCH((scan_bwd_kernel<T, NP, PACKED, FAST>), grid, dim3(256 * (NP / SCAN_NW)), 0, s, p);
+  DVAE_LAUNCH((scan_bwd_kernel<T, NP, PACKED, FAST>), dim3((unsigned)((int64_t)p.rows * p.nch * p.G * scan_bc_parts(p.tpg))),
+              dim3(64 * SCAN_BT * (NP / SCAN_NW)), 0, s, p);
 }
 
 #define SCAN_LAUNCH(K, T, NP, p, s)                                                                   \
@@ -1070,7 +1090,7 @@ extern "C" int64_t dvae_selective_scan_bwd_ws_floats(int64_t rows, int64_t L, in
   ScanArgs p = {};
   if (rows * L <= 0 || D <= 0 || G <= 0) return 0;
   scan_shape(p, rows, L, D, G, N, 1);
-  const int64_t parts = (p.tpg + 3) / 4, chunks = rows * p.nch;
+  const int64_t parts = scan_bc_parts(p.tpg), chunks = rows * p.nch;
   return parts * rows * L * G * 2 * N + chunks * (N + 2) * D + (p.nch == 1 ? 0 : chunks * ((N + 1) * D + 1) + 4);
 }
 
@@ -1124,13 +1144,13 @@ extern "C" int dvae_selective_scan_bwd(const void* u, int64_t u_sb, int64_t u_st
   p.dstate1 = dstate1; p.dstate0 = dstate0; p.ckpt = const_cast<float*>(ckpt);
   p.du = du; p.ddelta = ddelta; p.dz = dz;
   scan_shape(p, rows, L, D, G, N, S);
-  const int parts = (p.tpg + 3) / 4;
+  const int parts = scan_bc_parts(p.tpg);
   float* after = scan_scratch(p, ws);
   if (p.nch == 1) after = ws;
   else { p.leave = after; after += (int64_t)rows * p.nch * N * D; }
   p.part_bc = after;
   p.part_a = after + (int64_t)parts * rows * L * G * 2 * N;
-  DVAE_REQUIRE(rows * p.nch * p.wpg < (1ll << 31), "selective_scan_bwd: too many rows");
+  DVAE_REQUIRE(rows * p.nch * p.G * parts < (1ll << 31), "selective_scan_bwd: too many rows");
   const int e = dtype == DVAE_DT_F32 ? 4 : 2;
   DVAE_WORK(rows * L * (double)e * ((z ? 7 : 5) * D + 4 * G * N), DVAE_UNIT_BYTE);
   SCAN_DISPATCH(scan_bwd_launch, dtype, p, ST(stream));
@@ -1163,7 +1183,9 @@ extern "C" int dvae_selective_scan_step(float* state, const void* u, int64_t u_s
   // four rows per lane where that leaves two workgroups per compute unit: 256 x 2048 x 16, STEP4 against STEP1 us
   const int lpc = N > 8 ? 4 : N > 4 ? 2 : 1;
   const bool many = ceil_div64(rows, 4) * D * lpc >= 512 * 256;
-  const bool vec = N % 4 == 0 && !((uintptr_t)state & 15);
+  const uintptr_t bc = (uintptr_t)B | (uintptr_t)C;
+  const bool vec = N % 4 == 0 && !((uintptr_t)state & 15) && !((B_sb | B_sg | C_sb | C_sg) & 3) &&
+                   !(bc & (dtype == DVAE_DT_F32 ? 15 : 7));
   const int64_t grid = ceil_div64(ceil_div64(rows, many ? 4 : 1) * D * lpc, 256);
   DVAE_REQUIRE(grid < (1ll << 31), "selective_scan_step: too many rows");
   DVAE_WORK(rows * (double)D * N * 8, DVAE_UNIT_BYTE);
