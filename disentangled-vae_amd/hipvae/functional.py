@@ -1000,6 +1000,11 @@ def _wants_grad(*ts: Optional[Tensor]) -> bool:
     return False
 
 
+def _no_second_derivative(what: str):
+    if torch.is_grad_enabled():                     # only so under create_graph=True
+        raise RuntimeError(f"{what}: the gradients cannot be differentiated again (create_graph=True)")
+
+
 class SelectiveScan(torch.autograd.Function):
     """see selective_scan"""
 
@@ -1007,21 +1012,26 @@ class SelectiveScan(torch.autograd.Function):
     def forward(ctx, u, delta, A, B, C, D, z, delta_bias, delta_softplus, state, offsets, want_state):
         a = ops.ScanArgs('selective_scan', u, delta, A, B, C, D, z, delta_bias, delta_softplus, state, offsets)
         out, final, ckpt = ops.selective_scan_fwd(a, want_state, True)
-        ctx.save_for_backward(u, delta, A, B, C, D, z, delta_bias, state, offsets, ckpt)
-        ctx.delta_softplus = delta_softplus
+        ctx.save_for_backward(*a.tensors, ckpt)
+        ctx.args = a.release(), B.shape, C.shape
         ctx.set_materialize_grads(False)
         return out, final
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dout, dfinal):
-        u, delta, A, B, C, D, z, bias, state, offsets, ckpt = ctx.saved_tensors
-        a = ops.ScanArgs('selective_scan', u, delta, A, B, C, D, z, bias, ctx.delta_softplus, state, offsets)
+        _no_second_derivative('selective_scan')
+        *keep, ckpt = ctx.saved_tensors             # (unpacking raises if an input has been changed since)
+        a, b_shape, c_shape = ctx.args
         if dout is None:
-            dout = torch.zeros(u.shape, dtype=u.dtype, device=u.device)
+            dout = torch.zeros(a.shape, dtype=a.act, device=a.device)
         need = ctx.needs_input_grad
         du, dd, dA, dB, dC, dD, dz, db, ds = ops.selective_scan_bwd(a, dout, dfinal, ckpt, need[9])
-        grads = [du, dd, dA, dB.view(B.shape), dC.view(C.shape), dD, dz, db, None, ds]
+        del keep
+        if b_shape != a.bc_shape:
+            dB = dB.view(b_shape)
+        if c_shape != a.bc_shape:
+            dC = dC.view(c_shape)
+        grads = (du, dd, dA, dB, dC, dD, dz, db, None, ds)
         return tuple(g if n else None for g, n in zip(grads, need)) + (None, None)
 
 
@@ -1069,21 +1079,23 @@ class ShortConv(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, silu, state, offsets, want_state):
-        out, final = ops.short_conv_fwd(ops.ConvArgs('short_conv', x, weight, bias, silu, state, offsets), want_state)
-        ctx.save_for_backward(x, weight, bias, state, offsets)
-        ctx.silu = silu
+        a = ops.ConvArgs('short_conv', x, weight, bias, silu, state, offsets)
+        out, final = ops.short_conv_fwd(a, want_state)
+        ctx.save_for_backward(*a.tensors)
+        ctx.args = a.release()
         ctx.set_materialize_grads(False)
         return out, final
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dout, dfinal):
-        x, weight, bias, state, offsets = ctx.saved_tensors
-        a = ops.ConvArgs('short_conv', x, weight, bias, ctx.silu, state, offsets)
+        _no_second_derivative('short_conv')
+        keep = ctx.saved_tensors                    # (unpacking raises if an input has been changed since)
+        a = ctx.args
         if dout is None:
-            dout = torch.zeros(x.shape, dtype=x.dtype, device=x.device)
+            dout = torch.zeros(a.shape, dtype=a.act, device=a.device)
         need = ctx.needs_input_grad
         dx, dw, db, ds = ops.short_conv_bwd(a, dout, dfinal, need[4])
+        del keep
         return tuple(g if n else None for g, n in zip((dx, dw, db, None, ds), need)) + (None, None)
 
 
@@ -1121,8 +1133,8 @@ class AddRMSNorm(torch.autograd.Function):
         return y if residual is None else (y, total)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dsum=None):
+        _no_second_derivative('add_rms_norm')
         total, weight, rstd = ctx.saved_tensors
         if dy is None:
             if dsum is None:

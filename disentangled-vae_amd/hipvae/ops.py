@@ -1072,14 +1072,14 @@ def _act_dtype(what: str, t: Tensor) -> int:
     return code
 
 
-def _act(what: str, name: str, t: Optional[Tensor], shape, like: Tensor) -> Optional[Tensor]:
+def _act(what: str, name: str, t: Optional[Tensor], shape, like: Tensor, dtype=None) -> Optional[Tensor]:
     """checks an activation; a copy where its last dimension is not contiguous"""
     if t is None:
         return None
     if t.shape != shape:
         raise RuntimeError(f"{what}: {name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    if t.dtype != like.dtype or t.device != like.device:
-        raise RuntimeError(f"{what}: {name} is {t.dtype} on {t.device}, expected {like.dtype} on {like.device}")
+    if t.dtype != (dtype or like.dtype) or t.device != like.device:
+        raise RuntimeError(f"{what}: {name} is {t.dtype} on {t.device}, expected {dtype or like.dtype} on {like.device}")
     return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
@@ -1141,61 +1141,65 @@ def _st3(t: Tensor):
 
 
 class ScanArgs:
-    """The checked arguments of a selective scan, as both directions hand them to the library."""
+    """The checked arguments of a selective scan, as both directions hand them to the library.  The backward pass works
+    from what was prepared here: `release` drops the tensors, which the caller has to keep (`tensors`)."""
 
     def __init__(self, what, u, delta, A, B, C, D, z, delta_bias, delta_softplus, state, offsets):
         self.dtype = _act_dtype(what, u)
-        self.lead, self.rows, self.L, ch, self.S = _sequence_form(what, u, offsets)
-        self.D = ch
+        self.lead, rows, L, ch, S = _sequence_form(what, u, offsets)
         if A.dim() != 2:
             raise RuntimeError(f"{what}: A must be [channels, states], got {tuple(A.shape)}")
-        N = self.N = A.shape[1]
-        self.u = _act(what, 'u', u, u.shape, u)
-        self.delta = _act(what, 'delta', delta, u.shape, u)
-        self.z = _act(what, 'z', z, u.shape, u)
-        self.B = _bc_form(what, 'B', B, self.lead, u)
-        G = self.G = self.B.shape[-2]
-        self.C = _bc_form(what, 'C', C, self.lead, u)
-        if self.C.shape != self.B.shape or self.B.shape[-1] != N:
+        N = A.shape[1]
+        self.shape, self.device, self.act = u.shape, u.device, u.dtype
+        u = _act(what, 'u', u, u.shape, u)
+        delta = _act(what, 'delta', delta, u.shape, u)
+        z = _act(what, 'z', z, u.shape, u)
+        B, C = _bc_form(what, 'B', B, self.lead, u), _bc_form(what, 'C', C, self.lead, u)
+        G = B.shape[-2]
+        if C.shape != B.shape or B.shape[-1] != N:
             raise RuntimeError(f"{what}: B {tuple(B.shape)} and C {tuple(C.shape)} must both be [..., groups, {N}]")
         if G < 1 or ch % G:
             raise RuntimeError(f"{what}: {ch} channels do not divide into {G} groups")
-        self.A = _param(what, 'A', A, (ch, N), u)
-        self.Dp = _param(what, 'D', D, (ch,), u)
-        self.bias = _param(what, 'delta_bias', delta_bias, (ch,), u)
-        self.state = _param(what, 'state', state, (self.S, ch, N), u)
-        self.softplus = int(bool(delta_softplus))
-        self.offsets = offsets
+        A = _param(what, 'A', A, (ch, N), u)
+        D = _param(what, 'D', D, (ch,), u)
+        delta_bias = _param(what, 'delta_bias', delta_bias, (ch,), u)
+        self.state_shape, self.bc_shape = (S, ch, N), B.shape
+        state = _param(what, 'state', state, self.state_shape, u)
+        self.tensors = (u, delta, A, B, C, D, z, delta_bias, state, offsets)
+        self.has_D, self.has_z, self.has_bias = D is not None, z is not None, delta_bias is not None
+        self.packed, self.tokens = offsets is not None, rows * L
+        self.sizes = rows, L, ch, G, N
+        self.head = (u.data_ptr(), *_st2(u), delta.data_ptr(), *_st2(delta), A.data_ptr(), B.data_ptr(), *_st3(B),
+                     C.data_ptr(), *_st3(C), _p(D), _p(z), *_st2(z), _p(delta_bias), int(bool(delta_softplus)), _p(state))
+        self.offsets_ptr = _p(offsets)
+        self.tail = rows, L, ch, G, N, S, self.dtype
 
-    def head(self):
-        return (_p(self.u), *_st2(self.u), _p(self.delta), *_st2(self.delta), _p(self.A), _p(self.B), *_st3(self.B),
-                _p(self.C), *_st3(self.C), _p(self.Dp), _p(self.z), *_st2(self.z), _p(self.bias), self.softplus,
-                _p(self.state))
-
-    def shape(self):
-        return self.rows, self.L, self.D, self.G, self.N, self.S, self.dtype
+    def release(self):
+        self.tensors = None
+        return self
 
 
-def _final_like(state: Optional[Tensor], shape, like: Tensor, dtype, offsets, tokens: int) -> Tensor:
+def _final_states(shape, dtype, device, entering: Optional[Tensor], packed: bool, tokens: int) -> Tensor:
     """where final states go.  Sequences without tokens are not written: they keep what they entered with."""
-    if offsets is None and tokens > 0:
-        return torch.empty(shape, dtype=dtype, device=like.device)
-    return torch.zeros(shape, dtype=dtype, device=like.device) if state is None else state.clone()
+    if tokens > 0 and not packed:
+        return torch.empty(shape, dtype=dtype, device=device)
+    return torch.zeros(shape, dtype=dtype, device=device) if entering is None else entering.clone()
 
 
 def selective_scan_fwd(a: ScanArgs, want_state: bool, keep: bool):
     """-> (out, final state or None, what the backward pass starts from or None)"""
-    dev = a.u.device
+    dev = a.device
     if dev.index != _device_now():
         with torch.cuda.device(dev):
             return selective_scan_fwd(a, want_state, keep)
-    out = torch.empty(a.u.shape, dtype=a.u.dtype, device=dev)
-    final = _final_like(a.state, (a.S, a.D, a.N), a.u, torch.float32, a.offsets, a.rows * a.L) if want_state else None
-    ckpt = torch.empty(lib.dvae_selective_scan_ckpt_floats(a.rows, a.L, a.D, a.N), dtype=torch.float32,
+    out = torch.empty(a.shape, dtype=a.act, device=dev)
+    final = _final_states(a.state_shape, torch.float32, dev, a.tensors[8], a.packed, a.tokens) if want_state else None
+    rows, L, ch, G, N = a.sizes
+    ckpt = torch.empty(lib.dvae_selective_scan_ckpt_floats(rows, L, ch, N), dtype=torch.float32,
                        device=dev) if keep else None
-    n = lib.dvae_selective_scan_fwd_ws_floats(a.rows, a.L, a.D, a.G, a.N, int(keep))
+    n = lib.dvae_selective_scan_fwd_ws_floats(rows, L, ch, G, N, int(keep))
     ws = torch.empty(n, dtype=torch.float32, device=dev) if n else None
-    check(lib.dvae_selective_scan_fwd(*a.head(), _p(final), _p(a.offsets), _p(out), _p(ckpt), *a.shape(), _p(ws),
+    check(lib.dvae_selective_scan_fwd(*a.head, _p(final), a.offsets_ptr, out.data_ptr(), _p(ckpt), *a.tail, _p(ws),
                                       _stream_of(dev.index)), 'selective_scan_fwd')
     return out, final, ckpt
 
@@ -1203,28 +1207,30 @@ def selective_scan_fwd(a: ScanArgs, want_state: bool, keep: bool):
 def selective_scan_bwd(a: ScanArgs, dout: Tensor, dfinal: Optional[Tensor], ckpt: Tensor, want_dstate: bool):
     """-> du, ddelta, dA, dB, dC, dD, dz, ddelta_bias, dstate (None where there is no such input)"""
     what = 'selective_scan_bwd'
-    dev = a.u.device
+    dev = a.device
     if dev.index != _device_now():
         with torch.cuda.device(dev):
             return selective_scan_bwd(a, dout, dfinal, ckpt, want_dstate)
-    dout = _act(what, 'dout', dout, a.u.shape, a.u)
-    dfinal = _param(what, 'dstate', dfinal, (a.S, a.D, a.N), a.u)
-    act = dict(dtype=a.u.dtype, device=dev)
-    par = dict(dtype=torch.float32, device=dev)
-    du, dd = torch.empty(a.u.shape, **act), torch.empty(a.u.shape, **act)
-    dz = None if a.z is None else torch.empty(a.u.shape, **act)
-    dB, dC = torch.empty(a.B.shape, **act), torch.empty(a.B.shape, **act)
-    if a.rows * a.L == 0:
-        zero = lambda t: None if t is None else torch.zeros(t.shape, **par)                          # noqa: E731
-        return du, dd, zero(a.A), dB, dC, zero(a.Dp), dz, zero(a.bias), dfinal if want_dstate else None
-    dA = torch.empty(a.A.shape, **par)
-    dD = None if a.Dp is None else torch.empty(a.D, **par)
-    db = None if a.bias is None else torch.empty(a.D, **par)
-    ds = _final_like(dfinal, (a.S, a.D, a.N), a.u, torch.float32, a.offsets, a.rows * a.L) if want_dstate else None
-    ws = torch.empty(lib.dvae_selective_scan_bwd_ws_floats(a.rows, a.L, a.D, a.G, a.N), **par)
-    check(lib.dvae_selective_scan_bwd(*a.head(), _p(a.offsets), _p(dout), *_st2(dout), _p(dfinal), _p(ckpt), _p(du), _p(dd),
-                                      _p(dA), _p(dB), _p(dC), _p(dD), _p(dz), _p(db), _p(ds), *a.shape(), _p(ws),
-                                      _stream_of(dev.index)), what)
+    dout = _act(what, 'dout', dout, a.shape, ckpt, a.act)
+    dfinal = _param(what, 'dstate', dfinal, a.state_shape, ckpt)
+    f32 = torch.float32
+    du = torch.empty(a.shape, dtype=a.act, device=dev)
+    dd = torch.empty(a.shape, dtype=a.act, device=dev)
+    dz = torch.empty(a.shape, dtype=a.act, device=dev) if a.has_z else None
+    dB = torch.empty(a.bc_shape, dtype=a.act, device=dev)
+    dC = torch.empty(a.bc_shape, dtype=a.act, device=dev)
+    rows, L, ch, G, N = a.sizes
+    new = torch.empty if a.tokens else torch.zeros
+    dA = new((ch, N), dtype=f32, device=dev)
+    dD = new(ch, dtype=f32, device=dev) if a.has_D else None
+    db = new(ch, dtype=f32, device=dev) if a.has_bias else None
+    ds = _final_states(a.state_shape, f32, dev, dfinal, a.packed, a.tokens) if want_dstate else None
+    if a.tokens:
+        ws = torch.empty(lib.dvae_selective_scan_bwd_ws_floats(rows, L, ch, G, N), dtype=f32, device=dev)
+        check(lib.dvae_selective_scan_bwd(*a.head, a.offsets_ptr, dout.data_ptr(), *_st2(dout), _p(dfinal),
+                                          ckpt.data_ptr(), du.data_ptr(), dd.data_ptr(), dA.data_ptr(), dB.data_ptr(),
+                                          dC.data_ptr(), _p(dD), _p(dz), _p(db), _p(ds), *a.tail, ws.data_ptr(),
+                                          _stream_of(dev.index)), what)
     return du, dd, dA, dB, dC, dD, dz, db, ds
 
 
@@ -1263,37 +1269,41 @@ def selective_scan_step(state, u, delta, A, B, C, D=None, z=None, delta_bias=Non
 
 
 class ConvArgs:
-    """The checked arguments of a short convolution."""
+    """The checked arguments of a short convolution (see ScanArgs)."""
 
     def __init__(self, what, x, weight, bias, silu, state, offsets):
         self.dtype = _act_dtype(what, x)
-        self.lead, self.rows, self.L, self.D, self.S = _sequence_form(what, x, offsets)
+        self.lead, rows, L, ch, S = _sequence_form(what, x, offsets)
         if weight.dim() != 2 or not 2 <= weight.shape[1] <= 4:
             raise RuntimeError(f"{what}: weight must be [channels, 2 to 4 taps], got {tuple(weight.shape)}")
-        self.W = weight.shape[1]
-        self.x = _act(what, 'x', x, x.shape, x)
-        self.weight = _param(what, 'weight', weight, (self.D, self.W), x)
-        self.bias = _param(what, 'bias', bias, (self.D,), x)
-        self.state = _param(what, 'state', state, (self.S, self.W - 1, self.D), x, x.dtype)
-        self.silu = int(bool(silu))
-        self.offsets = offsets
+        W = weight.shape[1]
+        self.shape, self.device, self.act = x.shape, x.device, x.dtype
+        self.state_shape = (S, W - 1, ch)
+        x = _act(what, 'x', x, x.shape, x)
+        weight = _param(what, 'weight', weight, (ch, W), x)
+        bias = _param(what, 'bias', bias, (ch,), x)
+        state = _param(what, 'state', state, self.state_shape, x, x.dtype)
+        self.tensors = (x, weight, bias, state, offsets)
+        self.has_bias, self.packed, self.tokens = bias is not None, offsets is not None, rows * L
+        self.sizes = rows, L, ch, W
+        self.head = x.data_ptr(), *_st2(x), weight.data_ptr(), _p(bias), int(bool(silu)), _p(state)
+        self.offsets_ptr = _p(offsets)
+        self.tail = rows, L, ch, W, S, self.dtype
 
-    def head(self):
-        return _p(self.x), *_st2(self.x), _p(self.weight), _p(self.bias), self.silu, _p(self.state)
-
-    def shape(self):
-        return self.rows, self.L, self.D, self.W, self.S, self.dtype
+    def release(self):
+        self.tensors = None
+        return self
 
 
 def short_conv_fwd(a: ConvArgs, want_state: bool):
     """-> out, final state or None"""
-    dev = a.x.device
+    dev = a.device
     if dev.index != _device_now():
         with torch.cuda.device(dev):
             return short_conv_fwd(a, want_state)
-    out = torch.empty(a.x.shape, dtype=a.x.dtype, device=dev)
-    final = _final_like(a.state, (a.S, a.W - 1, a.D), a.x, a.x.dtype, a.offsets, a.rows * a.L) if want_state else None
-    check(lib.dvae_short_conv_fwd(*a.head(), _p(final), _p(a.offsets), _p(out), *a.shape(), _stream_of(dev.index)),
+    out = torch.empty(a.shape, dtype=a.act, device=dev)
+    final = _final_states(a.state_shape, a.act, dev, a.tensors[3], a.packed, a.tokens) if want_state else None
+    check(lib.dvae_short_conv_fwd(*a.head, _p(final), a.offsets_ptr, out.data_ptr(), *a.tail, _stream_of(dev.index)),
           'short_conv_fwd')
     return out, final
 
@@ -1301,23 +1311,22 @@ def short_conv_fwd(a: ConvArgs, want_state: bool):
 def short_conv_bwd(a: ConvArgs, dout: Tensor, dfinal: Optional[Tensor], want_dstate: bool):
     """-> dx, dweight, dbias, dstate"""
     what = 'short_conv_bwd'
-    dev = a.x.device
+    dev = a.device
     if dev.index != _device_now():
         with torch.cuda.device(dev):
             return short_conv_bwd(a, dout, dfinal, want_dstate)
-    dout = _act(what, 'dout', dout, a.x.shape, a.x)
-    shape = (a.S, a.W - 1, a.D)
-    dfinal = _param(what, 'dstate', dfinal, shape, a.x, a.x.dtype)
-    dx = torch.empty(a.x.shape, dtype=a.x.dtype, device=dev)
-    if a.rows * a.L == 0:
-        return (dx, torch.zeros(a.D, a.W, device=dev), None if a.bias is None else torch.zeros(a.D, device=dev),
-                dfinal if want_dstate else None)
-    dw = torch.empty(a.D, a.W, dtype=torch.float32, device=dev)
-    db = None if a.bias is None else torch.empty(a.D, dtype=torch.float32, device=dev)
-    ds = _final_like(dfinal, shape, a.x, a.x.dtype, a.offsets, a.rows * a.L) if want_dstate else None
-    ws = torch.empty(lib.dvae_short_conv_bwd_ws_floats(a.rows, a.L, a.D, a.W), dtype=torch.float32, device=dev)
-    check(lib.dvae_short_conv_bwd(*a.head(), _p(a.offsets), _p(dout), *_st2(dout), _p(dfinal), _p(dx), _p(dw), _p(db),
-                                  _p(ds), *a.shape(), _p(ws), _stream_of(dev.index)), what)
+    dout = _act(what, 'dout', dout, a.shape, dout, a.act)
+    dfinal = _param(what, 'dstate', dfinal, a.state_shape, dout, a.act)
+    rows, L, ch, W = a.sizes
+    dx = torch.empty(a.shape, dtype=a.act, device=dev)
+    new = torch.empty if a.tokens else torch.zeros
+    dw = new((ch, W), dtype=torch.float32, device=dev)
+    db = new(ch, dtype=torch.float32, device=dev) if a.has_bias else None
+    ds = _final_states(a.state_shape, a.act, dev, dfinal, a.packed, a.tokens) if want_dstate else None
+    if a.tokens:
+        ws = torch.empty(lib.dvae_short_conv_bwd_ws_floats(rows, L, ch, W), dtype=torch.float32, device=dev)
+        check(lib.dvae_short_conv_bwd(*a.head, a.offsets_ptr, dout.data_ptr(), *_st2(dout), _p(dfinal), dx.data_ptr(),
+                                      dw.data_ptr(), _p(db), _p(ds), *a.tail, ws.data_ptr(), _stream_of(dev.index)), what)
     return dx, dw, db, ds
 
 
