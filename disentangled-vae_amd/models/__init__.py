@@ -1,5 +1,5 @@
 """Model factory with the reference's names (models/__init__.py:38-76)."""
-from .encoders import (CNNEncoder, LightCNNEncoder, VideoEncoder, LSTMEncoder, VAEEncoder, ContentEncoder,
+from .encoders import (CNNEncoder, LightCNNEncoder, VideoEncoder, LSTMEncoder, SSMEncoder, VAEEncoder, ContentEncoder,
                        MotionEncoder, reparameterize)
 from .decoders import CNNDecoder, LSTMDecoder, VideoDecoder, DisentangledDecoder
 from .baseline_vae import BaselineVAE
@@ -23,7 +23,7 @@ def get_loss_fn(model_type: str):
     return _LOSSES[model_type]
 
 
-__all__ = ['CNNEncoder', 'LightCNNEncoder', 'VideoEncoder', 'LSTMEncoder', 'VAEEncoder', 'ContentEncoder',
+__all__ = ['CNNEncoder', 'LightCNNEncoder', 'VideoEncoder', 'LSTMEncoder', 'SSMEncoder', 'VAEEncoder', 'ContentEncoder',
            'MotionEncoder', 'reparameterize', 'CNNDecoder', 'LSTMDecoder', 'VideoDecoder', 'DisentangledDecoder',
            'BaselineVAE', 'LSTMVAE', 'DisentangledVAE', 'DisentangledVAEWrapper', 'baseline_loss', 'lstm_loss',
            'disentangled_loss', 'get_model', 'get_loss_fn']

@@ -4,6 +4,7 @@ The torch.nn modules created here are parameter/buffer containers only (same nam
 RNG draw order as the reference, models/encoders.py); their own forward() is never called.  All
 arithmetic goes through hipvae.functional, which has no CPU path.
 """
+import math
 from typing import List, Optional, Tuple
 
 import torch
@@ -137,6 +138,97 @@ class LSTMEncoder(nn.Module):
         final, output, h_n, c_n = HF.LSTMEncoder.apply(x, self.num_layers, self.bidirectional, True,
                                                        *self._flat_weights())
         return (output if return_sequence else final), (h_n, c_n)
+
+
+class SSMEncoder(nn.Module):
+    """Selective state-space layers over a sequence: what LSTMEncoder is for recurrences that run step by step, for ones
+    that train in parallel over time.  The reference has no counterpart.
+
+    Each layer is residual: root-mean-square norm -> projection to a path and a gate -> short causal convolution ->
+    projection to step sizes, B and C -> selective scan, gated -> projection back.  Like LSTMEncoder it returns the last
+    token's output, or with return_sequence the whole sequence, and the states that the sequences end with; a caller that
+    has no use for those sets `return_states = False`.
+
+    forward() takes [batch, length, input_dim], or packed [tokens, input_dim] with `offsets` (int32, see
+    hipvae.functional.selective_scan; the output of an empty sequence is 0).  step() takes the next token of every
+    sequence, [batch, input_dim], and updates `states` in place (no gradients): a frame's cost does not grow with the
+    frames before it."""
+    return_states = True
+
+    def __init__(self, input_dim: int = 512, hidden_dim: int = 256, num_layers: int = 1, state_dim: int = 16,
+                 conv_width: int = 4, expand: int = 2, groups: int = 1, dt_min: float = 1e-3, dt_max: float = 0.1):
+        super().__init__()
+        self.hidden_dim, self.num_layers, self.state_dim, self.groups = hidden_dim, num_layers, state_dim, groups
+        self.conv_width = conv_width
+        inner = self.inner_dim = expand * hidden_dim
+        self.dt_rank = max(4, inner // 32 // 4 * 4)
+        self.output_dim = hidden_dim
+        self.proj = nn.Linear(input_dim, hidden_dim)
+        self.layers = nn.ModuleList()
+        for _ in range(num_layers):
+            layer = nn.Module()
+            layer.norm = nn.Parameter(torch.ones(hidden_dim))
+            layer.in_proj = nn.Linear(hidden_dim, 2 * inner, bias=False)
+            layer.conv_weight = nn.Parameter(torch.empty(inner, conv_width).uniform_(-1, 1) * conv_width ** -0.5)
+            layer.conv_bias = nn.Parameter(torch.zeros(inner))
+            layer.x_proj = nn.Linear(inner, self.dt_rank + 2 * groups * state_dim, bias=False)
+            layer.dt_proj = nn.Linear(self.dt_rank, inner, bias=False)
+            # step sizes between dt_min and dt_max, evenly in their logarithm; the bias is softplus's inverse of them
+            dt = torch.exp(torch.rand(inner) * (math.log(dt_max) - math.log(dt_min)) + math.log(dt_min))
+            layer.dt_bias = nn.Parameter(dt + torch.log(-torch.expm1(-dt)))
+            layer.A_log = nn.Parameter(torch.log(torch.arange(1, state_dim + 1, dtype=torch.float32)).repeat(inner, 1))
+            layer.D = nn.Parameter(torch.ones(inner))
+            layer.out_proj = nn.Linear(inner, hidden_dim, bias=False)
+            self.layers.append(layer)
+        self.norm = nn.Parameter(torch.ones(hidden_dim))
+
+    def init_states(self, batch: int):
+        """the states that sequences start from, per layer: the convolution's last inputs and the scan's states"""
+        like = self.norm
+        return [(like.new_zeros(batch, self.conv_width - 1, self.inner_dim),
+                 like.new_zeros(batch, self.inner_dim, self.state_dim)) for _ in range(self.num_layers)]
+
+    def _projected(self, layer, x):
+        p = HF.linear(x, layer.x_proj.weight, None)
+        dt, B, C = p.split([self.dt_rank, self.groups * self.state_dim, self.groups * self.state_dim], -1)
+        shape = (*p.shape[:-1], self.groups, self.state_dim)
+        return HF.linear(dt, layer.dt_proj.weight, None), B.view(shape), C.view(shape)
+
+    def forward(self, x: torch.Tensor, return_sequence: bool = False, states=None, offsets: Optional[torch.Tensor] = None):
+        h, residual, ends = HF.linear(x, self.proj.weight, self.proj.bias), None, []
+        for i, layer in enumerate(self.layers):
+            conv_state, scan_state = states[i] if states is not None else (None, None)
+            y, residual = HF.add_rms_norm(h, residual, layer.norm)
+            u, z = HF.linear(y, layer.in_proj.weight, None).chunk(2, -1)
+            u, conv_end = HF.short_conv(u, layer.conv_weight, layer.conv_bias, silu=True, state=conv_state,
+                                        offsets=offsets, return_state=True)
+            delta, B, C = self._projected(layer, u)
+            y, scan_end = HF.selective_scan(u, delta, -torch.exp(layer.A_log), B, C, D=layer.D, z=z,
+                                            delta_bias=layer.dt_bias, delta_softplus=True, state=scan_state,
+                                            offsets=offsets, return_state=True)
+            h = HF.linear(y, layer.out_proj.weight, None)
+            ends.append((conv_end, scan_end))
+        y, _ = HF.add_rms_norm(h, residual, self.norm)
+        if not return_sequence:
+            if offsets is None:
+                y = y[:, -1]
+            else:
+                last = offsets[1:].long() - 1
+                y = y[last.clamp_min(0)].masked_fill((offsets[1:] == offsets[:-1])[:, None], 0.0)
+        return y, (ends if self.return_states else None)
+
+    @torch.no_grad()
+    def step(self, x: torch.Tensor, states) -> torch.Tensor:
+        h, residual = HF.linear(x, self.proj.weight, self.proj.bias), None
+        for layer, (conv_state, scan_state) in zip(self.layers, states):
+            y, residual = HF.add_rms_norm(h, residual, layer.norm)
+            u, z = HF.linear(y, layer.in_proj.weight, None).chunk(2, -1)
+            u = HF.short_conv_step(conv_state, u, layer.conv_weight, layer.conv_bias, silu=True)
+            delta, B, C = self._projected(layer, u)
+            y = HF.selective_scan_step(scan_state, u, delta, -torch.exp(layer.A_log), B, C, D=layer.D, z=z,
+                                       delta_bias=layer.dt_bias, delta_softplus=True)
+            h = HF.linear(y, layer.out_proj.weight, None)
+        return HF.add_rms_norm(h, residual, self.norm)[0]
 
 
 class VAEEncoder(nn.Module):
