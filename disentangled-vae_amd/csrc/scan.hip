@@ -38,6 +38,13 @@ struct ScanArgs {
   int nch, CL, enter_row, enter_step;   // chunks, their tokens; slots of `enter` per row and from chunk to chunk
 };
 
+// A as the kernels use it, in powers of two.  An infinite one becomes the largest finite number: a step size of 0, which
+// stands for tokens that are not there, has to leave the state as it is.
+__device__ __forceinline__ float decay_rate(float a) {
+  a *= LOG2E_F;
+  return fabsf(a) > 3.402823466e38f ? copysignf(3.402823466e38f, a) : a;
+}
+
 // what happens inside a block of n tokens from t0 on: bit j of `start` / `end` / `valid`: token t0 + j is its
 // sequence's first / its sequence's last / in a sequence at all
 struct Marks { uint32_t start, end, valid; };
@@ -255,7 +262,7 @@ __global__ void __launch_bounds__(256) SCAN_WPE scan_fwd_kernel(ScanArgs p) {
   float A2[NP], h[NP];
 #pragma unroll
   for (int n = 0; n < NP; ++n) {
-    A2[n] = n < p.N ? p.A[(int64_t)w.d * p.N + n] * LOG2E_F : 0.f;
+    A2[n] = n < p.N ? decay_rate(p.A[(int64_t)w.d * p.N + n]) : 0.f;
     h[n] = 0.f;
   }
   if (!STATE_ONLY && w.chunk > 0) load_slot<NP, FAST>(enter_slot(p, row, w.chunk), p, w.d, h, p.N);
@@ -320,7 +327,7 @@ __global__ void __launch_bounds__(256) SCAN_WPE scan_fwd_kernel(ScanArgs p) {
         const float pre = to_f32(pb[j]) + bias;
         const float sp = softplus_hw(pre);
         const float dt = j < n ? (plus ? sp : pre) : 0.f;
-        const float x = dt * uu;
+        const float x = j < n ? dt * uu : 0.f;     // (0 also where u is infinite)
         if (STATE_ONLY) {
           total += dt;
 #pragma unroll
@@ -405,7 +412,7 @@ __global__ void __launch_bounds__(64 * WAVES) scan_join_kernel(ScanArgs p) {
   const int64_t ND = (int64_t)p.N * p.D;
   const int64_t i = min((int64_t)blockIdx.x * 64 + lane, ND - 1);      // (lanes past the last do as it does)
   const int row = blockIdx.y, d = (int)(i % p.D), n = (int)(i / p.D);
-  const float A2 = p.A[(int64_t)d * p.N + n] * LOG2E_F;
+  const float A2 = decay_rate(p.A[(int64_t)d * p.N + n]);
   const float* sumdt = p.sumdt + (int64_t)row * p.nch * p.D + d;
   float x = 0.f;                                   // what enters the chunks of this round
   for (int k0 = 0; k0 + 1 < p.nch; k0 += WAVES * JOIN_AHEAD) {
@@ -502,7 +509,7 @@ __global__ void __launch_bounds__(256) SCAN_WPE scan_bwd_state_kernel(ScanArgs p
   float A2[NP], x[NP];
 #pragma unroll
   for (int n = 0; n < NP; ++n) {
-    A2[n] = n < p.N ? p.A[(int64_t)w.d * p.N + n] * LOG2E_F : 0.f;
+    A2[n] = n < p.N ? decay_rate(p.A[(int64_t)w.d * p.N + n]) : 0.f;
     x[n] = 0.f;
   }
   const float bias = p.bias ? p.bias[w.d] : 0.f;
@@ -621,7 +628,7 @@ __global__ void __launch_bounds__(64 * SCAN_BT * (NP / SCAN_NW), 2) scan_bwd_ker
   float A2[SCAN_NW], dh[SCAN_NW], dA[SCAN_NW];
 #pragma unroll
   for (int i = 0; i < SCAN_NW; ++i) {
-    A2[i] = i < Nw ? p.A[(int64_t)w.d * p.N + n0 + i] * LOG2E_F : 0.f;
+    A2[i] = i < Nw ? decay_rate(p.A[(int64_t)w.d * p.N + n0 + i]) : 0.f;
     dh[i] = dA[i] = 0.f;
   }
   const int64_t skip = (int64_t)n0 * p.D;          // this wave's rows of a slot
@@ -691,7 +698,7 @@ __global__ void __launch_bounds__(64 * SCAN_BT * (NP / SCAN_NW), 2) scan_bwd_ker
       z_[jj] = to_f32(zn[jj]);
       g_[jj] = there ? to_f32(gn[jj]) : 0.f;
       in[j0 + jj][0][w.wave][w.lane] = dt_[jj];
-      in[j0 + jj][1][w.wave][w.lane] = dt_[jj] * u_[jj];
+      in[j0 + jj][1][w.wave][w.lane] = there ? dt_[jj] * u_[jj] : 0.f;      // (0 also where u is infinite)
       in[j0 + jj][2][w.wave][w.lane] = gated ? g_[jj] * (z_[jj] * sigmoid_hw(z_[jj])) : g_[jj];
     }
     __syncthreads();                               // and everyone has read the sums of the block behind
@@ -953,7 +960,7 @@ __global__ void __launch_bounds__(256) scan_step_kernel(ScanArgs p) {
     zz[r] = p.z ? to_f32(((const T*)p.z)[row * p.z_sb + d]) : 0.f;
   }
 #pragma unroll
-  for (int n = 0; n < 4; ++n) A2[n] = n0 + n < p.N ? A[n] * LOG2E_F : 0.f;
+  for (int n = 0; n < 4; ++n) A2[n] = n0 + n < p.N ? decay_rate(A[n]) : 0.f;
   const float bias = p.bias ? p.bias[d] : 0.f, Dp = p.Dp ? p.Dp[d] : 0.f;
 #pragma unroll
   for (int r = 0; r < R; ++r) {

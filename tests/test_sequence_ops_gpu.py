@@ -233,6 +233,64 @@ def test_scan_of_nothing(F):
         assert all(not a.any() for k, a in zip(v, g) if k != 'state') and torch.equal(g[-1], torch.ones_like(state))
 
 
+def test_scan_packed_nothing(F):
+    c = ScanCase(16, 4, 1, torch.float32, lengths=[0, 0])
+    out, state = c.call(F, c.gpu)
+    assert out.shape == (0, 16) and torch.equal(state, c.gpu['state'])
+    x, w = torch.empty(0, 16, device='cuda'), torch.randn(16, 4, device='cuda')
+    out, state = F.short_conv(x, w, offsets=c.offsets, return_state=True)
+    assert out.shape == (0, 16) and not state.any() and state.shape == (2, 3, 16)
+
+
+def test_scan_gradients_from_the_state_alone(F):
+    """only the final states are used: the same gradients as with an output gradient of zeros"""
+    c = ScanCase(24, 16, 1, torch.float32, lengths=[9, 0, 40, 3], tail=2, seed=9)
+    names = list(c.gpu)
+    res = []
+    for both in (False, True):
+        v = {k: t.clone().requires_grad_() for k, t in c.gpu.items()}
+        out, state = c.call(F, v)
+        outs, grads = ((out, state), (torch.zeros_like(out), c.dstate.cuda())) if both else ((state,), (c.dstate.cuda(),))
+        res.append(torch.autograd.grad(outs, [v[k] for k in names], grads))
+    for k, a, b in zip(names, *res):
+        assert torch.equal(a, b), k
+    assert torch.equal(res[0][-1][1], c.dstate.cuda()[1])                             # the empty sequence passes it on
+
+
+def test_scan_infinite_inputs_and_rates(F):
+    """lengths that end inside a block of eight: what fills the block up must not turn infinities into NaN.  An infinite
+    rate forgets everything at once: as a rate so large that exp underflows."""
+    for L in (3, 11):
+        c = ScanCase(16, 4, 1, torch.float32, rows=(1, L), seed=12, z=False)
+        v = {k: None if t is None else t.clone() for k, t in c.gpu.items()}
+        v['A'][3] = float('-inf')
+        w = dict(v, A=v['A'].clone())
+        w['A'][3] = -1e30
+        (o1, s1), (o2, s2) = c.call(F, v), c.call(F, w)
+        assert torch.equal(o1, o2) and torch.equal(s1, s2) and torch.isfinite(o1).all()
+        v = {k: None if t is None else t.clone() for k, t in c.gpu.items()}
+        v['u'][L - 1, 5] = float('inf')
+        v['B'] = v['B'].abs() + 0.1
+        _, s = c.call(F, v)
+        assert torch.isposinf(s[0, 5]).all() and torch.isfinite(s[0, :5]).all() and torch.isfinite(s[0, 6:]).all()
+
+
+def test_a_second_backward_and_a_changed_input(F):
+    c = ScanCase(24, 8, 1, torch.float32, rows=(2, 12), seed=10)
+    v = {k: t.clone().requires_grad_() for k, t in c.gpu.items()}
+    out = c.call(F, v, False)
+    d = torch.ones_like(out)
+    a = torch.autograd.grad(out, list(v.values()), d, retain_graph=True)
+    b = torch.autograd.grad(out, list(v.values()), d, retain_graph=True)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    with pytest.raises(RuntimeError, match='differentiated again'):
+        torch.autograd.grad(out, list(v.values()), d, retain_graph=True, create_graph=True)
+    with torch.no_grad():
+        v['delta'].add_(1.0)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        torch.autograd.grad(out, list(v.values()), d)
+
+
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize('rows,D,N,G', [(1, 1, 1, 1), (3, 96, 16, 2), (5, 70, 5, 1), (33, 512, 16, 1), (2, 64, 12, 1)])
 def test_scan_steps_follow_the_scan(F, rows, D, N, G, dtype):
@@ -423,6 +481,18 @@ def test_norm_gradients_of_the_leaves_do_not_share_memory(F):
     torch.testing.assert_close(x.grad, r.grad, rtol=0, atol=0)
 
 
+def test_norm_of_a_tensor_with_itself_as_residual(F):
+    x = torch.randn(5, 64, device='cuda', requires_grad=True)
+    y0 = x.detach().clone().requires_grad_()
+    w = torch.rand(64, device='cuda') + 0.5
+    y, s = F.add_rms_norm(x, x, w)
+    dy, ds = torch.randn_like(y), torch.randn_like(y)
+    (g,) = torch.autograd.grad((y, s), (x,), (dy, ds))
+    a, b = F.add_rms_norm(y0, x.detach(), w)
+    (h,) = torch.autograd.grad((a, b), (y0,), (dy, ds))
+    assert torch.equal(g, h + h)
+
+
 def test_norm_reads_strided_rows_and_any_leading_shape(F):
     g = gen(1)
     big = rnd(g, 6, 5, 200).cuda()
@@ -534,6 +604,40 @@ def test_captured_and_replayed_beside_a_second_graph(F, lengths):
             for i, (a, b) in enumerate(zip(o, e)):
                 assert torch.equal(a, b), i
     del graphs
+
+
+def test_tensors_of_more_than_2_to_the_31_elements(F):
+    """the last tokens of a packed batch whose tensors pass 2^31 elements: as those tokens alone"""
+    D, T, n = 32768, 66000, 40                                                        # 2.16e9 elements, 4.3 GB each
+    off = torch.tensor([0, 7, T - n, T], dtype=torch.int32, device='cuda')
+    x = torch.zeros(T, D, dtype=torch.bfloat16, device='cuda')
+    x[T - n:] = torch.randn(n, D, device='cuda').bfloat16()
+    tail = x[T - n:]
+    w, b = torch.randn(D, 4, device='cuda'), torch.randn(D, device='cuda')
+    out, st = F.short_conv(x, w, b, silu=True, offsets=off, return_state=True)
+    alone, st1 = F.short_conv(tail[None], w, b, silu=True, return_state=True)
+    assert torch.equal(out[T - n:], alone[0]) and torch.equal(st[2], st1[0])
+    del out
+    y, s = F.add_rms_norm(x, x, b)
+    y1, s1 = F.add_rms_norm(tail, tail, b)
+    assert torch.equal(y[T - n:], y1) and torch.equal(s[T - n:], s1)
+    del y, s
+    A = -torch.rand(D, 4, device='cuda') - 0.5
+    B = torch.randn(T, 4, device='cuda').bfloat16()
+    leaf = x.requires_grad_()
+    out, st = F.selective_scan(leaf, leaf, A, B, B, delta_softplus=True, offsets=off, return_state=True)
+    t1 = tail.detach()[None].requires_grad_()
+    alone, st1 = F.selective_scan(t1, t1, A, B[None, T - n:], B[None, T - n:], delta_softplus=True, return_state=True)
+    bound = 2 * HALF[torch.bfloat16]                                                  # two roundings, and fp32's below
+    assert ((out[T - n:] - alone[0]).abs() <= bound * alone[0].abs() + 1e-4).all()
+    assert ((st[2] - st1[0]).abs() <= 1e-4).all()
+    d = torch.zeros_like(out)
+    d[T - n:] = 1
+    (g,) = torch.autograd.grad(out, (leaf,), d)
+    (g1,) = torch.autograd.grad(alone, (t1,), torch.ones_like(alone))
+    # u and delta are one tensor: its gradient is the sum of two rounded ones
+    assert ((g[T - n:] - g1[0]).abs() <= 3 * bound * (g1[0].abs() + g1[0].abs().max() * 0.05) + 1e-3).all()
+    assert not g[:T - n].any()
 
 
 def test_results_repeat_bit_for_bit(F):
