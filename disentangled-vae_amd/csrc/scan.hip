@@ -167,25 +167,49 @@ struct Tile {
   }
 };
 
-// NP states of a channel from the n0-th on, of a state tensor [S][D][N]
-template <int NP>
+// NP states of a channel from the n0-th on, of a state tensor [S][D][N] or of A [D][N].  FULL: all of them exist, and a
+// lane's come as 16-byte accesses (from and to addresses that need 4-byte alignment only).
+template <int NP, bool FULL>
 __device__ __forceinline__ void load_state(const float* s, int64_t seq, const ScanArgs& p, int d, float (&h)[NP], int n0 = 0) {
   const float* q = s + (seq * p.D + d) * p.N + n0;
+  if (FULL) {
 #pragma unroll
-  for (int n = 0; n < NP; ++n) h[n] = n0 + n < p.N ? q[n] : 0.f;
+    for (int n = 0; n < NP; n += 4) {
+      const Pack<float, 4> v = *reinterpret_cast<const Pack<float, 4>*>(q + n);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) h[n + i] = v.v[i];
+    }
+  } else {
+#pragma unroll
+    for (int n = 0; n < NP; ++n) h[n] = n0 + n < p.N ? q[n] : 0.f;
+  }
 }
-template <int NP>
+template <int NP, bool FULL>
 __device__ __forceinline__ void store_state(float* s, int64_t seq, const ScanArgs& p, int d, const float (&h)[NP], int n0 = 0) {
   float* q = s + (seq * p.D + d) * p.N + n0;
+  if (FULL) {
 #pragma unroll
-  for (int n = 0; n < NP; ++n)
-    if (n0 + n < p.N) q[n] = h[n];
+    for (int n = 0; n < NP; n += 4) {
+      const Pack<float, 4> v = {{h[n], h[n + 1], h[n + 2], h[n + 3]}};
+      *reinterpret_cast<Pack<float, 4>*>(q + n) = v;
+    }
+  } else {
+#pragma unroll
+    for (int n = 0; n < NP; ++n)
+      if (n0 + n < p.N) q[n] = h[n];
+  }
+}
+template <int NP, bool FULL>
+__device__ __forceinline__ void load_rates(const ScanArgs& p, int d, float (&a)[NP], int n0 = 0) {
+  load_state<NP, FULL>(p.A, 0, p, d, a, n0);
+#pragma unroll
+  for (int n = 0; n < NP; ++n) a[n] = decay_rate(a[n]);
 }
 
 // the state that a sequence starts with
-template <int NP>
+template <int NP, bool FULL>
 __device__ __forceinline__ void entering_state(const ScanArgs& p, int64_t seq, int d, float (&h)[NP], int n0 = 0) {
-  if (p.state0) load_state<NP>(p.state0, seq, p, d, h, n0);
+  if (p.state0) load_state<NP, FULL>(p.state0, seq, p, d, h, n0);
   else {
 #pragma unroll
     for (int n = 0; n < NP; ++n) h[n] = 0.f;
@@ -259,16 +283,22 @@ __global__ void __launch_bounds__(256) SCAN_WPE scan_fwd_kernel(ScanArgs p) {
   const Tile w(p);
   if (w.idle || (STATE_ONLY && w.chunk + 1 == p.nch)) return;
   const int row = w.row;
-  float A2[NP], h[NP];
-#pragma unroll
-  for (int n = 0; n < NP; ++n) {
-    A2[n] = n < p.N ? decay_rate(p.A[(int64_t)w.d * p.N + n]) : 0.f;
-    h[n] = 0.f;
-  }
-  if (!STATE_ONLY && w.chunk > 0) load_slot<NP, FAST>(enter_slot(p, row, w.chunk), p, w.d, h, p.N);
-  if (!PACKED && w.chunk == 0) entering_state<NP>(p, row, w.d, h);
-  const float Dp = p.Dp ? p.Dp[w.d] : 0.f, bias = p.bias ? p.bias[w.d] : 0.f;
   const bool gated = p.z != nullptr, plus = p.softplus;
+  const uint32_t at = w.d * (uint32_t)sizeof(T);
+  Rows<T> ur(p.u, p.u_sb, p.u_st, row, w.t0), dr(p.delta, p.delta_sb, p.delta_st, row, w.t0);
+  Rows<T> zr(gated ? p.z : p.u, gated ? p.z_sb : p.u_sb, gated ? p.z_st : p.u_st, row, w.t0);
+  T un[SCAN_Q], dn[SCAN_Q], zn[SCAN_Q];            // the block ahead
+  BCAhead<T, NP, FAST> ahead;
+  ur.load(un, w.t1 - w.t0, at);
+  dr.load(dn, w.t1 - w.t0, at);
+  if (!STATE_ONLY) zr.load(zn, w.t1 - w.t0, at);
+  float A2[NP], h[NP];
+  load_rates<NP, FAST>(p, w.d, A2);
+#pragma unroll
+  for (int n = 0; n < NP; ++n) h[n] = 0.f;
+  if (!STATE_ONLY && w.chunk > 0) load_slot<NP, FAST>(enter_slot(p, row, w.chunk), p, w.d, h, p.N);
+  if (!PACKED && w.chunk == 0) entering_state<NP, FAST>(p, row, w.d, h);
+  const float Dp = p.Dp ? p.Dp[w.d] : 0.f, bias = p.bias ? p.bias[w.d] : 0.f;
   const T* u = (const T*)p.u + row * p.u_sb;
   const T* dl = (const T*)p.delta + row * p.delta_sb;
   const T* z = gated ? (const T*)p.z + row * p.z_sb : u;        // (read and not used without z)
@@ -276,19 +306,10 @@ __global__ void __launch_bounds__(256) SCAN_WPE scan_fwd_kernel(ScanArgs p) {
   const T* B = (const T*)p.B + row * p.B_sb + w.g * p.B_sg;
   const T* C = (const T*)p.C + row * p.C_sb + w.g * p.C_sg;
   T* out = (T*)p.out + (int64_t)row * p.L * p.D;
-  const uint32_t at = w.d * (uint32_t)sizeof(T);
   SeqWalk q = {p.offsets, p.S, p.L, p.L, row, 0, p.L};
   if (PACKED) q.seek(w.t0);
   float total = 0.f;
   bool cut = false;
-  Rows<T> ur(p.u, p.u_sb, p.u_st, row, w.t0), dr(p.delta, p.delta_sb, p.delta_st, row, w.t0);
-  Rows<T> zr(gated ? p.z : p.u, gated ? p.z_sb : p.u_sb, z_st, row, w.t0);
-  T un[SCAN_Q], dn[SCAN_Q], zn[SCAN_Q];            // the block ahead
-  BCAhead<T, NP, FAST> ahead;
-  ur.load(un, w.t1 - w.t0, at);
-  dr.load(dn, w.t1 - w.t0, at);
-  if (!STATE_ONLY) zr.load(zn, w.t1 - w.t0, at);
-
   for (int t0 = w.t0; t0 < w.t1; t0 += SCAN_Q) {
     const int n = min(SCAN_Q, w.t1 - t0);
     T ub[SCAN_Q], pb[SCAN_Q], zb[SCAN_Q];
@@ -355,7 +376,7 @@ __global__ void __launch_bounds__(256) SCAN_WPE scan_fwd_kernel(ScanArgs p) {
         continue;
       }
       if (m.start >> j & 1) {
-        entering_state<NP>(p, q.seq(), w.d, h);
+        entering_state<NP, FAST>(p, q.seq(), w.d, h);
         cut = true;
       }
       const float uu = to_f32(lane_load(u + t * p.u_st, at));
@@ -384,7 +405,7 @@ __global__ void __launch_bounds__(256) SCAN_WPE scan_fwd_kernel(ScanArgs p) {
         lane_store(out + t * p.D, at, from_f32<T>(y));
       }
       if (m.end >> j & 1) {
-        if (!STATE_ONLY && p.state1 && w.on) store_state<NP>(p.state1, q.seq(), p, w.d, h);
+        if (!STATE_ONLY && p.state1 && w.on) store_state<NP, FAST>(p.state1, q.seq(), p, w.d, h);
         q.next((int)t + 1);
       }
     }
@@ -396,7 +417,7 @@ __global__ void __launch_bounds__(256) SCAN_WPE scan_fwd_kernel(ScanArgs p) {
     }
     if (w.g == 0 && w.part == 0 && threadIdx.x == 0) p.keep[row * p.nch + w.chunk] = cut ? 0.f : 1.f;
   } else if (!PACKED && p.state1 && w.on && w.chunk + 1 == p.nch) {
-    store_state<NP>(p.state1, row, p, w.d, h);
+    store_state<NP, FAST>(p.state1, row, p, w.d, h);
   }
 }
 
@@ -507,11 +528,9 @@ __global__ void __launch_bounds__(256) SCAN_WPE scan_bwd_state_kernel(ScanArgs p
   if (w.idle || w.chunk == 0) return;
   const int row = w.row;
   float A2[NP], x[NP];
+  load_rates<NP, FAST>(p, w.d, A2);
 #pragma unroll
-  for (int n = 0; n < NP; ++n) {
-    A2[n] = n < p.N ? decay_rate(p.A[(int64_t)w.d * p.N + n]) : 0.f;
-    x[n] = 0.f;
-  }
+  for (int n = 0; n < NP; ++n) x[n] = 0.f;
   const float bias = p.bias ? p.bias[w.d] : 0.f;
   const bool gated = p.z != nullptr, plus = p.softplus;
   const T* dl = (const T*)p.delta + row * p.delta_sb;
@@ -584,7 +603,7 @@ __global__ void __launch_bounds__(256) SCAN_WPE scan_bwd_state_kernel(ScanArgs p
       if (m.end >> j & 1) {
         if (p.dstate1) {
           float e[NP];
-          load_state<NP>(p.dstate1, q.seq(), p, w.d, e);
+          load_state<NP, FAST>(p.dstate1, q.seq(), p, w.d, e);
 #pragma unroll
           for (int i = 0; i < NP; ++i) x[i] = fmaf(exp2_hw(total * A2[i]), e[i], x[i]);
         }
@@ -594,7 +613,7 @@ __global__ void __launch_bounds__(256) SCAN_WPE scan_bwd_state_kernel(ScanArgs p
   }
   if (!PACKED && p.dstate1 && w.chunk + 1 == p.nch) {
     float e[NP];
-    load_state<NP>(p.dstate1, row, p, w.d, e);
+    load_state<NP, FAST>(p.dstate1, row, p, w.d, e);
 #pragma unroll
     for (int i = 0; i < NP; ++i) x[i] = fmaf(exp2_hw(total * A2[i]), e[i], x[i]);
   }
@@ -626,14 +645,12 @@ __global__ void __launch_bounds__(64 * SCAN_BT * (NP / SCAN_NW), 2) scan_bwd_ker
   const bool idle = w.idle;                     // such a wave only takes part in the sums
   const int Nw = min(max(p.N - n0, 0), SCAN_NW);   // states that this wave has
   float A2[SCAN_NW], dh[SCAN_NW], dA[SCAN_NW];
+  load_rates<SCAN_NW, FAST>(p, w.d, A2, n0);
 #pragma unroll
-  for (int i = 0; i < SCAN_NW; ++i) {
-    A2[i] = i < Nw ? decay_rate(p.A[(int64_t)w.d * p.N + n0 + i]) : 0.f;
-    dh[i] = dA[i] = 0.f;
-  }
+  for (int i = 0; i < SCAN_NW; ++i) dh[i] = dA[i] = 0.f;
   const int64_t skip = (int64_t)n0 * p.D;          // this wave's rows of a slot
   if (w.chunk + 1 < p.nch) load_slot<SCAN_NW, FAST>(leave_slot(p, row, w.chunk) + skip, p, w.d, dh, Nw);
-  else if (!PACKED && p.dstate1) load_state<SCAN_NW>(p.dstate1, row, p, w.d, dh, n0);
+  else if (!PACKED && p.dstate1) load_state<SCAN_NW, FAST>(p.dstate1, row, p, w.d, dh, n0);
   float dD = 0.f, dbias = 0.f;
   const float Dp = p.Dp ? p.Dp[w.d] : 0.f, bias = p.bias ? p.bias[w.d] : 0.f;
   const bool gated = p.z != nullptr, plus = p.softplus;
@@ -779,7 +796,7 @@ __global__ void __launch_bounds__(64 * SCAN_BT * (NP / SCAN_NW), 2) scan_bwd_ker
         for (int i = 0; i < SCAN_NW; ++i) hs[j + 1][i] = hs[j][i];
         if (!(m.valid >> j & 1)) continue;
         const int64_t t = t0 + j;
-        if (m.start >> j & 1) entering_state<SCAN_NW>(p, f.seq(), w.d, hs[j + 1], n0);
+        if (m.start >> j & 1) entering_state<SCAN_NW, FAST>(p, f.seq(), w.d, hs[j + 1], n0);
         float Bv[SCAN_NW];
         BCLoad<T, SCAN_NW, FAST>::get(B, t * p.B_st, Nw, Bv);
         const float dt = in[j][0][w.wave][w.lane], x = in[j][1][w.wave][w.lane];
@@ -797,7 +814,7 @@ __global__ void __launch_bounds__(64 * SCAN_BT * (NP / SCAN_NW), 2) scan_bwd_ker
           continue;
         }
         if (m.end >> j & 1) {
-          if (p.dstate1) load_state<SCAN_NW>(p.dstate1, q.seq(), p, w.d, dh, n0);
+          if (p.dstate1) load_state<SCAN_NW, FAST>(p.dstate1, q.seq(), p, w.d, dh, n0);
           else {
 #pragma unroll
             for (int i = 0; i < SCAN_NW; ++i) dh[i] = 0.f;
@@ -810,7 +827,7 @@ __global__ void __launch_bounds__(64 * SCAN_BT * (NP / SCAN_NW), 2) scan_bwd_ker
         float y = 0.f, through = 0.f, ka = 0.f, pv[2 * SCAN_NW], hb[SCAN_NW];
 #pragma unroll
         for (int i = 0; i < SCAN_NW; ++i) hb[i] = hs[j][i];
-        if (m.start >> j & 1) entering_state<SCAN_NW>(p, q.seq(), w.d, hb, n0);
+        if (m.start >> j & 1) entering_state<SCAN_NW, FAST>(p, q.seq(), w.d, hb, n0);
 #pragma unroll
         for (int i = 0; i < SCAN_NW; ++i) {
           y = fmaf(Cv[i], hs[j + 1][i], y);
@@ -830,7 +847,7 @@ __global__ void __launch_bounds__(64 * SCAN_BT * (NP / SCAN_NW), 2) scan_bwd_ker
         const int c = sum_index(w.lane);
         red[j][w.wave][c < SCAN_NW ? n0 + c : NP + n0 + c - SCAN_NW] = sum;    // (four lanes alike)
         if (m.start >> j & 1) {
-          if (p.dstate0 && w.on && !idle) store_state<SCAN_NW>(p.dstate0, q.seq(), p, w.d, dh, n0);
+          if (p.dstate0 && w.on && !idle) store_state<SCAN_NW, FAST>(p.dstate0, q.seq(), p, w.d, dh, n0);
           q.prev((int)t - 1);
         }
       }
@@ -874,7 +891,7 @@ __global__ void __launch_bounds__(64 * SCAN_BT * (NP / SCAN_NW), 2) scan_bwd_ker
       p.part_bc[(((int64_t)w.part * p.rows * p.L + flat + t0 + j) * p.G + w.g) * 2 * p.N + c] = s;
     }
   }
-  if (!PACKED && w.chunk == 0 && p.dstate0 && w.on && !idle) store_state<SCAN_NW>(p.dstate0, row, p, w.d, dh, n0);
+  if (!PACKED && w.chunk == 0 && p.dstate0 && w.on && !idle) store_state<SCAN_NW, FAST>(p.dstate0, row, p, w.d, dh, n0);
   __syncthreads();
   part[0][0][wv][w.lane] = dD;
   part[0][1][wv][w.lane] = dbias;
