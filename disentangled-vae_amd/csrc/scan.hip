@@ -17,9 +17,6 @@
 
 #define SCAN_Q 8       // tokens per block: what is loaded ahead, and how far apart training keeps states
 #define SCAN_MAX_N 16
-#ifndef SCAN_WPE
-#define SCAN_WPE
-#endif
 #define SCAN_WAVES 2048    // two waves for each of the chip's SIMDs
 
 struct ScanArgs {
@@ -34,7 +31,7 @@ struct ScanArgs {
   float *enter, *leave;        // the states that enter the chunks, and the adjoints that enter them from the right
   float *sumdt, *keep;         // [row][chunk][D]: sum of step sizes; [row][chunk]: 1 where no sequence starts
   const int32_t* offsets;
-  int rows, L, D, G, N, S, Dg, tpg, ntiles, wpg, softplus, blocks;
+  int rows, L, D, G, N, S, Dg, tpg, wpg, softplus, blocks;    // tpg: tiles of 64 channels per group
   int nch, CL, enter_row, enter_step;   // chunks, their tokens; slots of `enter` per row and from chunk to chunk
 };
 
@@ -49,16 +46,9 @@ __device__ __forceinline__ float decay_rate(float a) {
 // sequence's first / its sequence's last / in a sequence at all
 struct Marks { uint32_t start, end, valid; };
 
-template <bool PACKED>
-__device__ __forceinline__ Marks block_marks(SeqWalk w, int t0, int n, int L) {
+__device__ __forceinline__ Marks block_marks(SeqWalk w, int t0, int n) {
   Marks m = {0u, 0u, 0u};
   const uint32_t all = (1u << n) - 1u;
-  if (!PACKED) {
-    m.start = t0 == 0 ? 1u : 0u;
-    m.end = t0 + n == L ? 1u << (n - 1) : 0u;
-    m.valid = all;
-    return m;
-  }
   while (w.s < w.S && w.b < t0 + n) {
     if (w.b >= t0) m.start |= 1u << (w.b - t0);
     if (w.e <= t0 + n) m.end |= 1u << (w.e - 1 - t0);
@@ -279,7 +269,7 @@ template <typename T> struct Rows {
 // last one with a step size of 0, which leaves the state as it is and gives the same output again.
 // Other blocks (packed sequences' borders) go token by token.
 template <typename T, int NP, bool PACKED, bool FAST, bool STATE_ONLY>
-__global__ void __launch_bounds__(256) SCAN_WPE scan_fwd_kernel(ScanArgs p) {
+__global__ void __launch_bounds__(256) scan_fwd_kernel(ScanArgs p) {
   const Tile w(p);
   if (w.idle || (STATE_ONLY && w.chunk + 1 == p.nch)) return;
   const int row = w.row;
@@ -323,7 +313,7 @@ __global__ void __launch_bounds__(256) SCAN_WPE scan_fwd_kernel(ScanArgs p) {
     if (!STATE_ONLY && p.ckpt)
       store_slot<NP, FAST>(p.ckpt + ((int64_t)row * p.blocks + t0 / SCAN_Q) * p.N * p.D, p, w.d, h, p.N);
     Marks m = {0u, 0u, 0u};
-    if (PACKED) m = block_marks<PACKED>(q, t0, n, p.L);
+    if (PACKED) m = block_marks(q, t0, n);
     if (!PACKED || !(m.start | m.end | (m.valid ^ ((1u << n) - 1u)))) {
       const T *Bt = B + t0 * p.B_st, *Ct = C + t0 * p.C_st;
       T* ot = out + (int64_t)t0 * p.D;
@@ -349,15 +339,19 @@ __global__ void __launch_bounds__(256) SCAN_WPE scan_fwd_kernel(ScanArgs p) {
         const float sp = softplus_hw(pre);
         const float dt = j < n ? (plus ? sp : pre) : 0.f;
         const float x = j < n ? dt * uu : 0.f;     // (0 also where u is infinite)
+        float a[NP];
+#pragma unroll
+        for (int i = 0; i < NP; ++i) a[i] = exp2_hw(dt * A2[i]);
+        if (STATE_ONLY) __builtin_amdgcn_sched_barrier(0);       // (all of them first: 39 -> 36 us at 1 x 4096 x 2048)
         if (STATE_ONLY) {
           total += dt;
 #pragma unroll
-          for (int i = 0; i < NP; ++i) h[i] = fmaf(exp2_hw(dt * A2[i]), h[i], x * Bv[i]);
+          for (int i = 0; i < NP; ++i) h[i] = fmaf(a[i], h[i], x * Bv[i]);
         } else {
           float y = Dp * uu;
 #pragma unroll
           for (int i = 0; i < NP; ++i) {
-            h[i] = fmaf(exp2_hw(dt * A2[i]), h[i], x * Bv[i]);
+            h[i] = fmaf(a[i], h[i], x * Bv[i]);
             y = fmaf(Cv[i], h[i], y);
           }
           const float zz = to_f32(zb[j]);
@@ -523,7 +517,7 @@ __device__ __forceinline__ float wave_sums16(float (&v)[16], int lane) {
 // The adjoint that leaves a chunk to the left if nothing enters it from the right: the sum of C[n] g of its tokens up to
 // the first start of a sequence, each through the decays from the chunk's first token to its own.
 template <typename T, int NP, bool PACKED, bool FAST>
-__global__ void __launch_bounds__(256) SCAN_WPE scan_bwd_state_kernel(ScanArgs p) {
+__global__ void __launch_bounds__(256) scan_bwd_state_kernel(ScanArgs p) {
   const Tile w(p);
   if (w.idle || w.chunk == 0) return;
   const int row = w.row;
@@ -560,7 +554,7 @@ __global__ void __launch_bounds__(256) SCAN_WPE scan_bwd_state_kernel(ScanArgs p
     zr.load(zn, left, at);
     gr.load(gn, left, at);
     Marks m = {0u, 0u, 0u};
-    if (PACKED) m = block_marks<PACKED>(q, t0, n, p.L);
+    if (PACKED) m = block_marks(q, t0, n);
     if (!PACKED || !(m.start | m.end | (m.valid ^ ((1u << n) - 1u)))) {
       BCAhead<T, NP, FAST> ahead;
       const T* Ct = C + t0 * p.C_st;
@@ -631,9 +625,7 @@ __global__ void __launch_bounds__(256) SCAN_WPE scan_bwd_state_kernel(ScanArgs p
 // block's tokens: it loads their inputs, computes their step sizes and gates for the others, and finishes their gradients
 // from the waves' parts of y, of the sum of dh B and of that of k A, all by way of LDS.
 #define SCAN_NW 8
-#ifndef SCAN_BT
-#define SCAN_BT 2
-#endif
+#define SCAN_BT 2      // tiles per workgroup
 template <typename T, int NP, bool PACKED, bool FAST>
 __global__ void __launch_bounds__(64 * SCAN_BT * (NP / SCAN_NW), 2) scan_bwd_kernel(ScanArgs p) {
   constexpr int SHARE = NP / SCAN_NW, OWN = SCAN_Q / SHARE;      // waves per tile; tokens of a block that a wave finishes
@@ -685,8 +677,8 @@ __global__ void __launch_bounds__(64 * SCAN_BT * (NP / SCAN_NW), 2) scan_bwd_ker
     SeqWalk f = q;                                 // the sequence that the states' second computation is in
     Marks m = {0u, 0u, 0u};
     if (PACKED) {
-      f.seek(t0);
-      m = block_marks<PACKED>(f, t0, n, p.L);
+      if (q.s < 0 || q.b > t0 || q.e <= t0) f.seek(t0);
+      m = block_marks(f, t0, n);
     }
     const bool plain = !PACKED || !(m.start | m.end | (m.valid ^ ((1u << n) - 1u)));
     // Requests the block before this one.  Called when half of this one's tokens are done, whose registers it takes.
@@ -750,7 +742,7 @@ __global__ void __launch_bounds__(64 * SCAN_BT * (NP / SCAN_NW), 2) scan_bwd_ker
           a[j][i] = exp2_hw(dt * A2[i]);
           hs[j + 1][i] = fmaf(a[j][i], hs[j][i], x * Bv[i]);
         }
-        __builtin_amdgcn_sched_barrier(0);         // (mixing tokens spills registers: SB0 against SB2 us)
+        __builtin_amdgcn_sched_barrier(0);         // (mixing tokens spills registers: 808 against 580 us)
       }
 #pragma unroll
       for (int j = SCAN_Q - 1; j >= 0; --j) {
@@ -1030,7 +1022,9 @@ static void scan_shape(ScanArgs& p, int64_t rows, int64_t L, int64_t D, int64_t 
   p.wpg = p.G * ((p.tpg + 3) / 4);
   p.blocks = (int)ceil_div64(L, SCAN_Q);
   // chunks: as many as it takes to reach two waves per SIMD, none shorter than 32 tokens; from there on to four per SIMD,
-  // none shorter than 128.  NOTE_CHUNKS
+  // none shorter than 128.  Two against four, 8 x 2048 x 2048 bf16: outputs 225 and 172 us, chunk states 161 and 124, chunk
+  // adjoints 178 and 140, joins 4 us more; 1 x 4096 x 2048, where four are 32 tokens each: 109 and 117 us in all.  One
+  // against two, 5003 x 1002: 380 and 319 us.
   const int64_t waves = rows * p.tpg * G;
   const int64_t two = waves > 0 ? ceil_div64(SCAN_WAVES, waves) : 1, four = 2 * two;
   const int64_t n2 = two < L / 32 ? two : L / 32, n4 = four < L / 128 ? four : L / 128;
