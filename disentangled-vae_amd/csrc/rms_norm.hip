@@ -5,6 +5,10 @@
 // Bound by memory.  A wave owns a row and holds it in registers between the reduction and the output (up to 64 values
 // per lane: rows of up to 4096 elements whose tensors are 16-byte aligned), so every tensor crosses memory once and no
 // barrier is needed.  Longer or unaligned rows take one workgroup each, which reads its row a second time.
+//
+// 16384 x 2048 bf16: forward 57 us (4.7 TB/s of x, residual, sum and y), backward 65 us (4.1 TB/s of dy, dsum, sum and
+// dresidual) and 4 us for the sums of its partial rows; 4099 x 2560 bf16 into 8 bits: 17.5 us (4.2 TB/s).  A copy of 2 GiB
+// runs at 4.9 TB/s on the same card.
 #include "seq_common.h"
 
 struct NormArgs {
@@ -121,7 +125,7 @@ __device__ __forceinline__ float block_sum4(float v, float* red) {
   return (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-// any row: one workgroup, element by element, the row read again for the output
+// any row: one workgroup, element by element, the row read again for the output (out of the L2)
 template <typename T, typename R, bool Q8>
 __global__ void __launch_bounds__(256) norm_any_kernel(NormArgs p) {
   __shared__ float red[4];
@@ -223,6 +227,7 @@ __global__ void __launch_bounds__(256) norm_bwd_row_kernel(NormArgs p) {
   }
 }
 
+// any row: one workgroup, as in the forward pass; dw comes from a pass of its own, column by column
 template <typename T, typename R>
 __global__ void __launch_bounds__(256) norm_bwd_any_kernel(NormArgs p) {
   __shared__ float red[4];
@@ -262,7 +267,7 @@ __global__ void __launch_bounds__(64 * SUM_WAVES) norm_dw_sum_kernel(const float
 }
 
 // ------------------------------------------------------------------------------------------------ host side
-#define NORM_MAX_GRID 512
+#define NORM_MAX_GRID 512     // workgroups of the backward kernel, and with that partial rows of dw: two per compute unit
 static int64_t norm_row_grid(int64_t rows) { const int64_t g = ceil_div64(rows, 4); return g < NORM_MAX_GRID ? g : NORM_MAX_GRID; }
 
 static int norm_check(const char* what, int64_t rows, int64_t D, int dtype, int rdtype) {

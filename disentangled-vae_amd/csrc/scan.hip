@@ -268,6 +268,11 @@ template <typename T> struct Rows {
 // channel compute that channel too and store the same values to the same places; tokens past the chunk's last repeat the
 // last one with a step size of 0, which leaves the state as it is and gives the same output again.
 // Other blocks (packed sequences' borders) go token by token.
+//
+// Bound by vector arithmetic: a state of a token takes five issue slots in the state pass (two of them the exponential) and
+// six in the output pass, a channel's token about 25 more (softplus, gate, conversions).  8 x 2048 x 2048 bf16, N = 16:
+// states 117 us, of which 80 are issue slots; outputs 172 us, of which 119, while it reads 268 MB and writes as much again
+// of kept states (3.1 TB/s).  1 x 4096 x 2048: 36 and 49 us.  256 x 20 x 1024 fp32 (one chunk): 41 us.
 template <typename T, int NP, bool PACKED, bool FAST, bool STATE_ONLY>
 __global__ void __launch_bounds__(256) scan_fwd_kernel(ScanArgs p) {
   const Tile w(p);
@@ -419,6 +424,7 @@ __global__ void __launch_bounds__(256) scan_fwd_kernel(ScanArgs p) {
 // starts inside a chunk nothing of what enters it gets through.  Bound by the wait for memory, so a workgroup takes 64
 // elements and WAVES * JOIN_AHEAD chunks at a time, all requested at once: a wave runs through its JOIN_AHEAD chunks
 // from zero, the waves' ends are joined through LDS, and each runs through its chunks again from what really enters them.
+// 64 chunks of 2048 channels x 16 states: 7 us; 16 chunks of 8 x 2048 x 16: 13 us (67 MB).
 #define JOIN_AHEAD 16
 template <bool BACK, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES) scan_join_kernel(ScanArgs p) {
@@ -515,7 +521,8 @@ __device__ __forceinline__ float wave_sums16(float (&v)[16], int lane) {
 }
 
 // The adjoint that leaves a chunk to the left if nothing enters it from the right: the sum of C[n] g of its tokens up to
-// the first start of a sequence, each through the decays from the chunk's first token to its own.
+// the first start of a sequence, each through the decays from the chunk's first token to its own: the exponential of the
+// step sizes added up so far, so no token waits for another.  8 x 2048 x 2048 bf16: 137 us, 90 of them issue slots.
 template <typename T, int NP, bool PACKED, bool FAST>
 __global__ void __launch_bounds__(256) scan_bwd_state_kernel(ScanArgs p) {
   const Tile w(p);
@@ -624,6 +631,11 @@ __global__ void __launch_bounds__(256) scan_bwd_state_kernel(ScanArgs p) {
 // 790 against 651 us).  What a channel's token needs besides its states, each wave of a tile does for its share of the
 // block's tokens: it loads their inputs, computes their step sizes and gates for the others, and finishes their gradients
 // from the waves' parts of y, of the sum of dh B and of that of k A, all by way of LDS.
+//
+// Bound by vector arithmetic: 185 instructions per token and wave (8 states of 64 channels), 47 slots of them the sums over
+// the lanes.  8 x 2048 x 2048 bf16: 555 us, of which 355 are issue slots at two waves per SIMD; it moves 0.77 GB.  Without
+// keeping the decays three waves would fit a SIMD but for spilled registers: 927 us.  Two tiles per workgroup, not four:
+// fewer waves wait at a barrier (586 us with four, 566 with one, which doubles the partial rows).
 #define SCAN_NW 8
 #define SCAN_BT 2      // tiles per workgroup
 template <typename T, int NP, bool PACKED, bool FAST>
@@ -905,34 +917,36 @@ __global__ void __launch_bounds__(64 * SCAN_BT * (NP / SCAN_NW), 2) scan_bwd_ker
   }
 }
 
-// dB and dC of every token: the sum of its tiles' partial rows, in the tiles' order
+// The gradients that are sums of partial rows, in one launch.  The first `bc_groups` workgroups add up dB and dC of every
+// token over the backward kernel's workgroups; the others dA [D][N], dD [D] and dbias [D] over rows and chunks.  Always in
+// the same order, so results repeat bit for bit.  8 x 2048 x 2048: 14 us for 53 MB.
 template <typename T>
-__global__ void __launch_bounds__(256) scan_bc_kernel(const float* part, T* dB, T* dC, int64_t rows_g, int N, int tiles) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t total = rows_g * 2 * N;
-  if (i >= total) return;
-  float s = 0.f;
-  for (int k = 0; k < tiles; ++k) s += part[k * total + i];
-  const int64_t r = i / (2 * N);
-  const int c = (int)(i % (2 * N));
-  if (c < N) dB[r * N + c] = from_f32<T>(s);
-  else dC[r * N + c - N] = from_f32<T>(s);
-}
-
-// dA [D][N], dD [D], dbias [D] from the partial rows [parts][N + 2][D]
-__global__ void __launch_bounds__(64 * SUM_WAVES) scan_params_kernel(const float* part, float* dA, float* dD, float* dbias,
-                                                                     int parts, int N, int D) {
-  const int64_t total = (int64_t)(N + 2) * D;
-  const int64_t i = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
-  const float s = column_sum(part, parts, total, i, i < total);
+__global__ void __launch_bounds__(64 * SUM_WAVES) scan_sums_kernel(ScanArgs p, T* dB, T* dC, float* dA, float* dD,
+                                                                   float* dbias, int64_t tokens_g, int parts,
+                                                                   unsigned bc_groups) {
+  if (blockIdx.x < bc_groups) {
+    const int64_t i = (int64_t)blockIdx.x * (64 * SUM_WAVES) + threadIdx.x;
+    const int64_t total = tokens_g * 2 * p.N;
+    if (i >= total) return;
+    float s = 0.f;
+    for (int k = 0; k < parts; ++k) s += p.part_bc[k * total + i];
+    const int64_t r = i / (2 * p.N);
+    const int c = (int)(i % (2 * p.N));
+    if (c < p.N) dB[r * p.N + c] = from_f32<T>(s);
+    else dC[r * p.N + c - p.N] = from_f32<T>(s);
+    return;
+  }
+  const int64_t total = (int64_t)(p.N + 2) * p.D;
+  const int64_t i = (int64_t)(blockIdx.x - bc_groups) * 64 + (threadIdx.x & 63);
+  const float s = column_sum(p.part_a, (int64_t)p.rows * p.nch, total, i, i < total);
   if (threadIdx.x >= 64 || i >= total) return;
-  const int n = (int)(i / D), d = (int)(i % D);
-  if (n < N) { if (dA) dA[(int64_t)d * N + n] = s; }
-  else if (n == N) { if (dD) dD[d] = s; }
+  const int n = (int)(i / p.D), d = (int)(i % p.D);
+  if (n < p.N) { if (dA) dA[(int64_t)d * p.N + n] = s; }
+  else if (n == p.N) { if (dD) dD[d] = s; }
   else if (dbias) dbias[d] = s;
 }
 
-// One token per row.  Nearly all of the traffic is the state, read and written once: a lane owns four states of a channel
+// One token per row.  256 x 2048 x 16 bf16: 19 us for 69 MB (3.6 TB/s); 1 x 512: 4 us.  Nearly all of the traffic is the state, read and written once: a lane owns four states of a channel
 // (one 16-byte access each way where N is a multiple of 4 and all is aligned), a channel's LPC lanes are neighbours, and the sum over them
 // takes two lane exchanges.  What a channel reads besides (inputs, step size) its lanes read and compute alike.  A lane
 // goes through R rows whose loads are in flight together and share its A.
@@ -1173,14 +1187,13 @@ extern "C" int dvae_selective_scan_bwd(const void* u, int64_t u_sb, int64_t u_st
   DVAE_WORK(rows * L * (double)e * ((z ? 7 : 5) * D + 4 * G * N), DVAE_UNIT_BYTE);
   SCAN_DISPATCH(scan_bwd_launch, dtype, p, ST(stream));
   DVAE_LAUNCH_CHECK("selective_scan_bwd");
-  const int64_t bc = rows * L * G;
-  const dim3 gbc((unsigned)ceil_div64(bc * 2 * N, 256));
-  if (dtype == DVAE_DT_F32)
-    DVAE_LAUNCH((scan_bc_kernel<float>), gbc, dim3(256), 0, ST(stream), p.part_bc, (float*)dB, (float*)dC, bc, p.N, parts);
-  else
-    DVAE_LAUNCH((scan_bc_kernel<bf16_t>), gbc, dim3(256), 0, ST(stream), p.part_bc, (bf16_t*)dB, (bf16_t*)dC, bc, p.N, parts);
-  DVAE_LAUNCH(scan_params_kernel, dim3((unsigned)ceil_div64((int64_t)(p.N + 2) * D, 64)), dim3(64 * SUM_WAVES), 0, ST(stream),
-              p.part_a, dA, dD, dbias, p.rows * p.nch, p.N, p.D);
+  const int64_t bc = rows * L * G, bc_groups = ceil_div64(bc * 2 * N, 64 * SUM_WAVES);
+  const int64_t sums = bc_groups + ceil_div64((N + 2) * D, 64);
+  DVAE_REQUIRE(sums < (1ll << 31), "selective_scan_bwd: too many tokens and groups");
+#define SCAN_SUMS(T)                                                                                                  \
+  DVAE_LAUNCH((scan_sums_kernel<T>), dim3((unsigned)sums), dim3(64 * SUM_WAVES), 0, ST(stream), p, (T*)dB, (T*)dC, dA, \
+              dD, dbias, bc, parts, (unsigned)bc_groups)
+  if (dtype == DVAE_DT_F32) SCAN_SUMS(float); else SCAN_SUMS(bf16_t);
   DVAE_LAUNCH_CHECK("selective_scan_bwd: sums");
   return 0;
 }
@@ -1198,7 +1211,7 @@ extern "C" int dvae_selective_scan_step(float* state, const void* u, int64_t u_s
   p.C = C; p.C_sb = C_sb; p.C_sg = C_sg; p.Dp = Dp; p.z = z; p.z_sb = z_sb; p.bias = bias; p.softplus = softplus;
   p.state1 = state; p.out = out;
   scan_shape(p, rows, 1, D, G, N, rows);
-  // four rows per lane where that leaves two workgroups per compute unit: 256 x 2048 x 16, STEP4 against STEP1 us
+  // four rows per lane where that leaves two workgroups per compute unit: 256 x 2048 x 16, 19 against 22 us
   const int lpc = N > 8 ? 4 : N > 4 ? 2 : 1;
   const bool many = ceil_div64(rows, 4) * D * lpc >= 512 * 256;
   const uintptr_t bc = (uintptr_t)B | (uintptr_t)C;
