@@ -263,11 +263,11 @@ template <typename T> struct Rows {
 
 // STATE_ONLY: the chunk's last state from a zero start, into the next chunk's slot; else the outputs.
 //
-// A block of SCAN_Q tokens in which no sequence starts or ends is straight-line code: its inputs were requested a block
-// ahead, and the compiler can request B and C tokens ahead.  Nothing in it is conditional.  Lanes past the group's last
-// channel compute that channel too and store the same values to the same places; tokens past the chunk's last repeat the
-// last one with a step size of 0, which leaves the state as it is and gives the same output again.
-// Other blocks (packed sequences' borders) go token by token.
+// A block's inputs were requested a block ahead, B and C are a token ahead.  Lanes past the group's last channel compute
+// that channel too and store the same values to the same places, so that no store depends on the lane.  Without packed
+// sequences a block is straight-line code: tokens past the chunk's last repeat the last one with a step size of 0, which
+// leaves the state as it is and stores the same output again.  What packed sequences' borders need stands behind
+// wave-uniform branches, and so do their chunks' ends.  (Branches for both: 8 x 2048 x 2048 backward 555 -> 623 us.)
 //
 // Bound by vector arithmetic: a state of a token takes five issue slots in the state pass (two of them the exponential) and
 // six in the output pass, a channel's token about 25 more (softplus, gate, conversions).  8 x 2048 x 2048 bf16, N = 16:
@@ -294,10 +294,6 @@ __global__ void __launch_bounds__(256) scan_fwd_kernel(ScanArgs p) {
   if (!STATE_ONLY && w.chunk > 0) load_slot<NP, FAST>(enter_slot(p, row, w.chunk), p, w.d, h, p.N);
   if (!PACKED && w.chunk == 0) entering_state<NP, FAST>(p, row, w.d, h);
   const float Dp = p.Dp ? p.Dp[w.d] : 0.f, bias = p.bias ? p.bias[w.d] : 0.f;
-  const T* u = (const T*)p.u + row * p.u_sb;
-  const T* dl = (const T*)p.delta + row * p.delta_sb;
-  const T* z = gated ? (const T*)p.z + row * p.z_sb : u;        // (read and not used without z)
-  const int64_t z_st = gated ? p.z_st : p.u_st;
   const T* B = (const T*)p.B + row * p.B_sb + w.g * p.B_sg;
   const T* C = (const T*)p.C + row * p.C_sb + w.g * p.C_sg;
   T* out = (T*)p.out + (int64_t)row * p.L * p.D;
@@ -319,93 +315,64 @@ __global__ void __launch_bounds__(256) scan_fwd_kernel(ScanArgs p) {
       store_slot<NP, FAST>(p.ckpt + ((int64_t)row * p.blocks + t0 / SCAN_Q) * p.N * p.D, p, w.d, h, p.N);
     Marks m = {0u, 0u, 0u};
     if (PACKED) m = block_marks(q, t0, n);
-    if (!PACKED || !(m.start | m.end | (m.valid ^ ((1u << n) - 1u)))) {
-      const T *Bt = B + t0 * p.B_st, *Ct = C + t0 * p.C_st;
-      T* ot = out + (int64_t)t0 * p.D;
-      if (STATE_ONLY) ahead.request_b(Bt, p.N);
-      else ahead.request(Bt, Ct, p.N);
+    const T *Bt = B + t0 * p.B_st, *Ct = C + t0 * p.C_st;
+    T* ot = out + (int64_t)t0 * p.D;
+    if (STATE_ONLY) ahead.request_b(Bt, p.N);
+    else ahead.request(Bt, Ct, p.N);
 #pragma unroll
-      for (int j = 0; j < SCAN_Q; ++j) {
-        BCAhead<T, NP, FAST> now = ahead;
-        float Bv[NP], Cv[NP];
-        Bt += j + 1 < n ? p.B_st : 0;
-        Ct += j + 1 < n ? p.C_st : 0;
-        if (STATE_ONLY) {
-          now.arrived_b(Bt);
-          if (j + 1 < SCAN_Q) ahead.request_b(Bt, p.N);
-          now.get_b(Bv);
-        } else {
-          now.arrived(Bt, Ct);
-          if (j + 1 < SCAN_Q) ahead.request(Bt, Ct, p.N);
-          now.get(Bv, Cv);
-        }
-        const float uu = to_f32(ub[j]);
-        const float pre = to_f32(pb[j]) + bias;
-        const float sp = softplus_hw(pre);
-        const float dt = j < n ? (plus ? sp : pre) : 0.f;
-        const float x = j < n ? dt * uu : 0.f;     // (0 also where u is infinite)
-        float a[NP];
-#pragma unroll
-        for (int i = 0; i < NP; ++i) a[i] = exp2_hw(dt * A2[i]);
-        if (STATE_ONLY) __builtin_amdgcn_sched_barrier(0);       // (all of them first: 39 -> 36 us at 1 x 4096 x 2048)
-        if (STATE_ONLY) {
-          total += dt;
-#pragma unroll
-          for (int i = 0; i < NP; ++i) h[i] = fmaf(a[i], h[i], x * Bv[i]);
-        } else {
-          float y = Dp * uu;
-#pragma unroll
-          for (int i = 0; i < NP; ++i) {
-            h[i] = fmaf(a[i], h[i], x * Bv[i]);
-            y = fmaf(Cv[i], h[i], y);
-          }
-          const float zz = to_f32(zb[j]);
-          const float gate = zz * sigmoid_hw(zz);
-          lane_store(ot, at, from_f32<T>(gated ? y * gate : y));
-          ot += j + 1 < n ? p.D : 0;
-        }
+    for (int j = 0; j < SCAN_Q; ++j) {
+      if (PACKED && j >= n) continue;
+      const bool there = PACKED || j < n;
+      BCAhead<T, NP, FAST> now = ahead;
+      float Bv[NP], Cv[NP];
+      Bt += j + 1 < n ? p.B_st : 0;
+      Ct += j + 1 < n ? p.C_st : 0;
+      if (STATE_ONLY) {
+        now.arrived_b(Bt);
+        if (j + 1 < SCAN_Q) ahead.request_b(Bt, p.N);
+        now.get_b(Bv);
+      } else {
+        now.arrived(Bt, Ct);
+        if (j + 1 < SCAN_Q) ahead.request(Bt, Ct, p.N);
+        now.get(Bv, Cv);
       }
-      continue;
-    }
-#pragma unroll 1
-    for (int j = 0; j < n; ++j) {
-      const int64_t t = t0 + j;
-      if (!(m.valid >> j & 1)) {
-        if (!STATE_ONLY) lane_store(out + t * p.D, at, from_f32<T>(0.f));
+      if (PACKED && !(m.valid >> j & 1)) {
+        if (!STATE_ONLY) lane_store(ot, at, from_f32<T>(0.f));
+        ot += p.D;
         continue;
       }
-      if (m.start >> j & 1) {
+      if (PACKED && (m.start >> j & 1)) {
         entering_state<NP, FAST>(p, q.seq(), w.d, h);
         cut = true;
       }
-      const float uu = to_f32(lane_load(u + t * p.u_st, at));
-      const float pre = to_f32(lane_load(dl + t * p.delta_st, at)) + bias;
-      const float dt = plus ? softplus_hw(pre) : pre;
-      float Bv[NP];
-      BCLoad<T, NP, FAST>::get(B, t * p.B_st, p.N, Bv);
-      const float x = dt * uu;
+      const float uu = to_f32(ub[j]);
+      const float pre = to_f32(pb[j]) + bias;
+      const float sp = softplus_hw(pre);
+      const float dt = there ? (plus ? sp : pre) : 0.f;
+      const float x = there ? dt * uu : 0.f;       // (0 also where u is infinite)
+      float a[NP];
+#pragma unroll
+      for (int i = 0; i < NP; ++i) a[i] = exp2_hw(dt * A2[i]);
       if (STATE_ONLY) {
+        __builtin_amdgcn_sched_barrier(0);         // (all of them first: 39 -> 36 us at 1 x 4096 x 2048)
         total += dt;
 #pragma unroll
-        for (int i = 0; i < NP; ++i) h[i] = fmaf(exp2_hw(dt * A2[i]), h[i], x * Bv[i]);
+        for (int i = 0; i < NP; ++i) h[i] = fmaf(a[i], h[i], x * Bv[i]);
       } else {
-        float Cv[NP];
-        BCLoad<T, NP, FAST>::get(C, t * p.C_st, p.N, Cv);
         float y = Dp * uu;
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
-          h[i] = fmaf(exp2_hw(dt * A2[i]), h[i], x * Bv[i]);
+          h[i] = fmaf(a[i], h[i], x * Bv[i]);
           y = fmaf(Cv[i], h[i], y);
         }
-        if (gated) {
-          const float zz = to_f32(lane_load(z + t * z_st, at));
-          y *= zz * sigmoid_hw(zz);
-        }
-        lane_store(out + t * p.D, at, from_f32<T>(y));
+        const float zz = to_f32(zb[j]);
+        const float gate = zz * sigmoid_hw(zz);
+        lane_store(ot, at, from_f32<T>(gated ? y * gate : y));
+        ot += j + 1 < n ? p.D : 0;
       }
-      if (m.end >> j & 1) {
+      if (PACKED && (m.end >> j & 1)) {
         if (!STATE_ONLY && p.state1 && w.on) store_state<NP, FAST>(p.state1, q.seq(), p, w.d, h);
-        q.next((int)t + 1);
+        q.next(t0 + j + 1);
       }
     }
   }
@@ -534,10 +501,6 @@ __global__ void __launch_bounds__(256) scan_bwd_state_kernel(ScanArgs p) {
   for (int n = 0; n < NP; ++n) x[n] = 0.f;
   const float bias = p.bias ? p.bias[w.d] : 0.f;
   const bool gated = p.z != nullptr, plus = p.softplus;
-  const T* dl = (const T*)p.delta + row * p.delta_sb;
-  const T* go = (const T*)p.dout + row * p.dout_sb;
-  const T* z = gated ? (const T*)p.z + row * p.z_sb : go;
-  const int64_t z_st = gated ? p.z_st : p.dout_st;
   const T* C = (const T*)p.C + row * p.C_sb + w.g * p.C_sg;
   const uint32_t at = w.d * (uint32_t)sizeof(T);
   SeqWalk q = {p.offsets, p.S, p.L, p.L, row, 0, p.L};
@@ -545,7 +508,7 @@ __global__ void __launch_bounds__(256) scan_bwd_state_kernel(ScanArgs p) {
   float total = 0.f;
   bool cut = false;
   Rows<T> dr(p.delta, p.delta_sb, p.delta_st, row, w.t0), gr(p.dout, p.dout_sb, p.dout_st, row, w.t0);
-  Rows<T> zr(gated ? p.z : p.dout, gated ? p.z_sb : p.dout_sb, z_st, row, w.t0);
+  Rows<T> zr(gated ? p.z : p.dout, gated ? p.z_sb : p.dout_sb, gated ? p.z_st : p.dout_st, row, w.t0);
   T dn[SCAN_Q], zn[SCAN_Q], gn[SCAN_Q];            // the block ahead
   dr.load(dn, w.t1 - w.t0, at);
   zr.load(zn, w.t1 - w.t0, at);
@@ -562,53 +525,37 @@ __global__ void __launch_bounds__(256) scan_bwd_state_kernel(ScanArgs p) {
     gr.load(gn, left, at);
     Marks m = {0u, 0u, 0u};
     if (PACKED) m = block_marks(q, t0, n);
-    if (!PACKED || !(m.start | m.end | (m.valid ^ ((1u << n) - 1u)))) {
-      BCAhead<T, NP, FAST> ahead;
-      const T* Ct = C + t0 * p.C_st;
-      ahead.request_b(Ct, p.N);
+    BCAhead<T, NP, FAST> ahead;
+    const T* Ct = C + t0 * p.C_st;
+    ahead.request_b(Ct, p.N);
 #pragma unroll
-      for (int j = 0; j < SCAN_Q; ++j) {
-        BCAhead<T, NP, FAST> now = ahead;
-        float Cv[NP];
-        Ct += j + 1 < n ? p.C_st : 0;
-        now.arrived_b(Ct);
-        if (j + 1 < SCAN_Q) ahead.request_b(Ct, p.N);
-        now.get_b(Cv);
-        const float pre = to_f32(pb[j]) + bias;
-        const float sp = softplus_hw(pre);
-        total += j < n ? (plus ? sp : pre) : 0.f;
-        const float zz = to_f32(zb[j]), gate = zz * sigmoid_hw(zz);
-        float g = to_f32(gb[j]);
-        g = j < n ? (gated ? g * gate : g) : 0.f;
-#pragma unroll
-        for (int i = 0; i < NP; ++i) x[i] = fmaf(exp2_hw(total * A2[i]), Cv[i] * g, x[i]);
-      }
-      continue;
-    }
-#pragma unroll 1
-    for (int j = 0; j < n; ++j) {
-      const int64_t t = t0 + j;
-      if (!(m.valid >> j & 1)) continue;
-      if (m.start >> j & 1) { cut = true; break; }
-      const float pre = to_f32(lane_load(dl + t * p.delta_st, at)) + bias;
-      total += plus ? softplus_hw(pre) : pre;
-      float g = to_f32(lane_load(go + t * p.dout_st, at));
-      if (gated) {
-        const float zz = to_f32(lane_load(z + t * z_st, at));
-        g *= zz * sigmoid_hw(zz);
-      }
+    for (int j = 0; j < SCAN_Q; ++j) {
+      if (PACKED && (j >= n || cut)) continue;
+      const bool there = PACKED || j < n;
+      BCAhead<T, NP, FAST> now = ahead;
       float Cv[NP];
-      BCLoad<T, NP, FAST>::get(C, t * p.C_st, p.N, Cv);
+      Ct += j + 1 < n ? p.C_st : 0;
+      now.arrived_b(Ct);
+      if (j + 1 < SCAN_Q) ahead.request_b(Ct, p.N);
+      now.get_b(Cv);
+      if (PACKED && !(m.valid >> j & 1)) continue;
+      if (PACKED && (m.start >> j & 1)) { cut = true; continue; }
+      const float pre = to_f32(pb[j]) + bias;
+      const float sp = softplus_hw(pre);
+      total += there ? (plus ? sp : pre) : 0.f;
+      const float zz = to_f32(zb[j]), gate = zz * sigmoid_hw(zz);
+      float g = to_f32(gb[j]);
+      g = there ? (gated ? g * gate : g) : 0.f;
 #pragma unroll
       for (int i = 0; i < NP; ++i) x[i] = fmaf(exp2_hw(total * A2[i]), Cv[i] * g, x[i]);
-      if (m.end >> j & 1) {
+      if (PACKED && (m.end >> j & 1)) {
         if (p.dstate1) {
           float e[NP];
           load_state<NP, FAST>(p.dstate1, q.seq(), p, w.d, e);
 #pragma unroll
           for (int i = 0; i < NP; ++i) x[i] = fmaf(exp2_hw(total * A2[i]), e[i], x[i]);
         }
-        q.next((int)t + 1);
+        q.next(t0 + j + 1);
       }
     }
   }
@@ -692,7 +639,6 @@ __global__ void __launch_bounds__(64 * SCAN_BT * (NP / SCAN_NW), 2) scan_bwd_ker
       if (q.s < 0 || q.b > t0 || q.e <= t0) f.seek(t0);
       m = block_marks(f, t0, n);
     }
-    const bool plain = !PACKED || !(m.start | m.end | (m.valid ^ ((1u << n) - 1u)));
     // Requests the block before this one.  Called when half of this one's tokens are done, whose registers it takes.
     auto request = [&]() {
       if (t0 > w.t0) {
@@ -723,138 +669,97 @@ __global__ void __launch_bounds__(64 * SCAN_BT * (NP / SCAN_NW), 2) scan_bwd_ker
       in[j0 + jj][2][w.wave][w.lane] = gated ? g_[jj] * (z_[jj] * sigmoid_hw(z_[jj])) : g_[jj];
     }
     __syncthreads();                               // and everyone has read the sums of the block behind
-    if (plain) {
-      // no sequence starts or ends here: straight-line code, as in the forward pass
-      float a[SCAN_Q][SCAN_NW];
-      BCAhead<T, SCAN_NW, FAST> ahead;
-      const T *Bt = B + t0 * p.B_st, *Ct = C + t0 * p.C_st;
-      // What is read from LDS is read a token ahead too, beside the request for B and C: waiting for LDS alone is not
-      // possible while scalar loads are on the way.
-      float dtn = in[0][0][w.wave][w.lane], xn = in[0][1][w.wave][w.lane], gn_;
-      ahead.request_b(Bt, Nw);
+    float a[SCAN_Q][SCAN_NW];
+    BCAhead<T, SCAN_NW, FAST> ahead;
+    const T *Bt = B + t0 * p.B_st, *Ct = C + t0 * p.C_st;
+    // What is read from LDS is read a token ahead too, beside the request for B and C: waiting for LDS alone is not
+    // possible while scalar loads are on the way.
+    float dtn = in[0][0][w.wave][w.lane], xn = in[0][1][w.wave][w.lane], gn_ = 0.f;
+    ahead.request_b(Bt, Nw);
 #pragma unroll
-      for (int j = 0; j < SCAN_Q; ++j) {
-        BCAhead<T, SCAN_NW, FAST> now = ahead;
-        float Bv[SCAN_NW];
-        Bt += j + 1 < n ? p.B_st : 0;
-        Ct += j + 1 < n ? p.C_st : 0;
-        now.arrived_b(Bt);
-        if (j + 1 < SCAN_Q) ahead.request_b(Bt, Nw);
-        else ahead.request(Bt, Ct, Nw);            // the last token's, where the way back begins
-        now.get_b(Bv);
-        const float dt = dtn, x = xn;
-        if (j + 1 < SCAN_Q) {
-          dtn = in[j + 1][0][w.wave][w.lane];
-          xn = in[j + 1][1][w.wave][w.lane];
-        } else {
-          gn_ = in[j][2][w.wave][w.lane];
-        }
+    for (int j = 0; j < SCAN_Q; ++j) {
 #pragma unroll
-        for (int i = 0; i < SCAN_NW; ++i) {
-          a[j][i] = exp2_hw(dt * A2[i]);
-          hs[j + 1][i] = fmaf(a[j][i], hs[j][i], x * Bv[i]);
-        }
-        __builtin_amdgcn_sched_barrier(0);         // (mixing tokens spills registers: 808 against 580 us)
+      for (int i = 0; i < SCAN_NW; ++i) hs[j + 1][i] = hs[j][i];
+      if (PACKED && j >= n) continue;
+      BCAhead<T, SCAN_NW, FAST> now = ahead;
+      float Bv[SCAN_NW];
+      const bool more = j + 1 < SCAN_Q && (!PACKED || j + 1 < n);
+      Bt += j + 1 < n ? p.B_st : 0;
+      Ct += j + 1 < n ? p.C_st : 0;
+      now.arrived_b(Bt);
+      if (more) ahead.request_b(Bt, Nw);
+      else ahead.request(Bt, Ct, Nw);              // the last token's, where the way back begins
+      now.get_b(Bv);
+      const float dt = dtn, x = xn;
+      const int next = more ? j + 1 : j;
+      dtn = in[next][0][w.wave][w.lane];
+      xn = in[next][1][w.wave][w.lane];
+      gn_ = in[next][2][w.wave][w.lane];
+      if (PACKED && !(m.valid >> j & 1)) continue;
+      if (PACKED && (m.start >> j & 1)) entering_state<SCAN_NW, FAST>(p, f.seq(), w.d, hs[j + 1], n0);
+#pragma unroll
+      for (int i = 0; i < SCAN_NW; ++i) {
+        a[j][i] = exp2_hw(dt * A2[i]);
+        hs[j + 1][i] = fmaf(a[j][i], hs[j + 1][i], x * Bv[i]);
       }
+      if (PACKED && (m.end >> j & 1)) f.next(t0 + j + 1);
+      __builtin_amdgcn_sched_barrier(0);           // (mixing tokens spills registers: 808 against 580 us)
+    }
 #pragma unroll
-      for (int j = SCAN_Q - 1; j >= 0; --j) {
-        if (j == SCAN_Q / 2 - 1) request();
-        BCAhead<T, SCAN_NW, FAST> now = ahead;
-        float Bv[SCAN_NW], Cv[SCAN_NW];
-        Bt -= j > 0 && j < n ? p.B_st : 0;
-        Ct -= j > 0 && j < n ? p.C_st : 0;
-        now.arrived(Bt, Ct);
-        if (j > 0) ahead.request(Bt, Ct, Nw);
-        now.get(Bv, Cv);
-        const float dt = dtn, x = xn, g = gn_;
-        if (j > 0) {
-          dtn = in[j - 1][0][w.wave][w.lane];
-          xn = in[j - 1][1][w.wave][w.lane];
-          gn_ = in[j - 1][2][w.wave][w.lane];
-        }
-        float y = 0.f, through = 0.f, ka = 0.f, pv[2 * SCAN_NW];
-#pragma unroll
-        for (int i = 0; i < SCAN_NW; ++i) {
-          y = fmaf(Cv[i], hs[j + 1][i], y);
-          const float d = fmaf(Cv[i], g, dh[i]);
-          pv[i] = d * x;
-          pv[SCAN_NW + i] = g * hs[j + 1][i];
-          through = fmaf(d, Bv[i], through);
-          dh[i] = d * a[j][i];
-          const float k = dh[i] * hs[j][i];
-          dA[i] = fmaf(k, dt, dA[i]);
-          ka = fmaf(k, A2[i], ka);
-        }
-        part[j][0][wv][w.lane] = y;
-        part[j][1][wv][w.lane] = through;
-        part[j][2][wv][w.lane] = ka;
-        const float sum = wave_sums16(pv, w.lane);
-        const int c = sum_index(w.lane);
-        red[j][w.wave][c < SCAN_NW ? n0 + c : NP + n0 + c - SCAN_NW] = sum;    // (four lanes alike)
-        __builtin_amdgcn_sched_barrier(0);
+    for (int j = SCAN_Q - 1; j >= 0; --j) {
+      if (j == SCAN_Q / 2 - 1) request();
+      if (PACKED && j >= n) continue;
+      BCAhead<T, SCAN_NW, FAST> now = ahead;
+      float Bv[SCAN_NW], Cv[SCAN_NW];
+      Bt -= j > 0 && j < n ? p.B_st : 0;
+      Ct -= j > 0 && j < n ? p.C_st : 0;
+      now.arrived(Bt, Ct);
+      if (j > 0) ahead.request(Bt, Ct, Nw);
+      now.get(Bv, Cv);
+      const float dt = dtn, x = xn, g = gn_;
+      if (j > 0) {
+        dtn = in[j - 1][0][w.wave][w.lane];
+        xn = in[j - 1][1][w.wave][w.lane];
+        gn_ = in[j - 1][2][w.wave][w.lane];
       }
-    } else {
-#pragma unroll
-      for (int j = 0; j < SCAN_Q; ++j) {
-#pragma unroll
-        for (int i = 0; i < SCAN_NW; ++i) hs[j + 1][i] = hs[j][i];
-        if (!(m.valid >> j & 1)) continue;
-        const int64_t t = t0 + j;
-        if (m.start >> j & 1) entering_state<SCAN_NW, FAST>(p, f.seq(), w.d, hs[j + 1], n0);
-        float Bv[SCAN_NW];
-        BCLoad<T, SCAN_NW, FAST>::get(B, t * p.B_st, Nw, Bv);
-        const float dt = in[j][0][w.wave][w.lane], x = in[j][1][w.wave][w.lane];
-#pragma unroll
-        for (int i = 0; i < SCAN_NW; ++i) hs[j + 1][i] = fmaf(exp2_hw(dt * A2[i]), hs[j + 1][i], x * Bv[i]);
-        if (m.end >> j & 1) f.next((int)t + 1);
+      const int c = sum_index(w.lane), cell = c < SCAN_NW ? n0 + c : NP + n0 + c - SCAN_NW;      // (four lanes alike)
+      if (PACKED && !(m.valid >> j & 1)) {
+        red[j][w.wave][cell] = 0.f;
+        continue;
       }
-      request();
+      if (PACKED && (m.end >> j & 1)) {
+        if (p.dstate1) load_state<SCAN_NW, FAST>(p.dstate1, q.seq(), p, w.d, dh, n0);
+        else {
 #pragma unroll
-      for (int j = SCAN_Q - 1; j >= 0; --j) {
-        if (j >= n) continue;
-        const int64_t t = t0 + j;
-        if (!(m.valid >> j & 1)) {
-          if (w.lane < 2 * SCAN_NW) red[j][w.wave][w.lane < SCAN_NW ? n0 + w.lane : NP + n0 + w.lane - SCAN_NW] = 0.f;
-          continue;
-        }
-        if (m.end >> j & 1) {
-          if (p.dstate1) load_state<SCAN_NW, FAST>(p.dstate1, q.seq(), p, w.d, dh, n0);
-          else {
-#pragma unroll
-            for (int i = 0; i < SCAN_NW; ++i) dh[i] = 0.f;
-          }
-        }
-        float Bv[SCAN_NW], Cv[SCAN_NW];
-        BCLoad<T, SCAN_NW, FAST>::get(B, t * p.B_st, Nw, Bv);
-        BCLoad<T, SCAN_NW, FAST>::get(C, t * p.C_st, Nw, Cv);
-        const float dt = in[j][0][w.wave][w.lane], x = in[j][1][w.wave][w.lane], g = in[j][2][w.wave][w.lane];
-        float y = 0.f, through = 0.f, ka = 0.f, pv[2 * SCAN_NW], hb[SCAN_NW];
-#pragma unroll
-        for (int i = 0; i < SCAN_NW; ++i) hb[i] = hs[j][i];
-        if (m.start >> j & 1) entering_state<SCAN_NW, FAST>(p, q.seq(), w.d, hb, n0);
-#pragma unroll
-        for (int i = 0; i < SCAN_NW; ++i) {
-          y = fmaf(Cv[i], hs[j + 1][i], y);
-          const float d = fmaf(Cv[i], g, dh[i]);
-          pv[i] = d * x;
-          pv[SCAN_NW + i] = g * hs[j + 1][i];
-          through = fmaf(d, Bv[i], through);
-          dh[i] = d * exp2_hw(dt * A2[i]);
-          const float k = dh[i] * hb[i];
-          dA[i] = fmaf(k, dt, dA[i]);
-          ka = fmaf(k, A2[i], ka);
-        }
-        part[j][0][wv][w.lane] = y;
-        part[j][1][wv][w.lane] = through;
-        part[j][2][wv][w.lane] = ka;
-        const float sum = wave_sums16(pv, w.lane);
-        const int c = sum_index(w.lane);
-        red[j][w.wave][c < SCAN_NW ? n0 + c : NP + n0 + c - SCAN_NW] = sum;    // (four lanes alike)
-        if (m.start >> j & 1) {
-          if (p.dstate0 && w.on && !idle) store_state<SCAN_NW, FAST>(p.dstate0, q.seq(), p, w.d, dh, n0);
-          q.prev((int)t - 1);
+          for (int i = 0; i < SCAN_NW; ++i) dh[i] = 0.f;
         }
       }
+      float hb[SCAN_NW];                           // the state before the token
+#pragma unroll
+      for (int i = 0; i < SCAN_NW; ++i) hb[i] = hs[j][i];
+      if (PACKED && (m.start >> j & 1)) entering_state<SCAN_NW, FAST>(p, q.seq(), w.d, hb, n0);
+      float y = 0.f, through = 0.f, ka = 0.f, pv[2 * SCAN_NW];
+#pragma unroll
+      for (int i = 0; i < SCAN_NW; ++i) {
+        y = fmaf(Cv[i], hs[j + 1][i], y);
+        const float d = fmaf(Cv[i], g, dh[i]);
+        pv[i] = d * x;
+        pv[SCAN_NW + i] = g * hs[j + 1][i];
+        through = fmaf(d, Bv[i], through);
+        dh[i] = d * a[j][i];
+        const float k = dh[i] * hb[i];
+        dA[i] = fmaf(k, dt, dA[i]);
+        ka = fmaf(k, A2[i], ka);
+      }
+      part[j][0][wv][w.lane] = y;
+      part[j][1][wv][w.lane] = through;
+      part[j][2][wv][w.lane] = ka;
+      red[j][w.wave][cell] = wave_sums16(pv, w.lane);
+      if (PACKED && (m.start >> j & 1)) {
+        if (p.dstate0 && w.on && !idle) store_state<SCAN_NW, FAST>(p.dstate0, q.seq(), p, w.d, dh, n0);
+        q.prev(t0 + j - 1);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
     __syncthreads();
     int64_t o = (flat + t0 + j0) * p.D;
