@@ -1064,40 +1064,41 @@ _stream_of = torch._C._cuda_getCurrentRawStream      # raw handle of a device's 
 
 
 def _act_dtype(what: str, t: Tensor) -> int:
-    if not t.is_cuda:
-        raise RuntimeError(f"{what}: input is on {t.device}; hipvae ops need tensors on the GPU (no CPU path exists)")
     code = _ACT_DTYPES.get(t.dtype)
-    if code is None:
+    if code is None or not t.is_cuda:
+        if not t.is_cuda:
+            raise RuntimeError(f"{what}: input is on {t.device}; hipvae ops need tensors on the GPU (no CPU path exists)")
         raise RuntimeError(f"{what}: activations must be fp32 or bf16, got {t.dtype}")
     return code
 
 
-def _act(what: str, name: str, t: Optional[Tensor], shape, like: Tensor, dtype=None) -> Optional[Tensor]:
+def _refuse(what: str, name: str, t: Tensor, shape, dtype, device: int):
+    raise RuntimeError(f"{what}: {name} is {t.dtype} {tuple(t.shape)} on {t.device}, expected {dtype} {tuple(shape)} on "
+                       f"cuda:{device}")
+
+
+def _act(what: str, name: str, t: Optional[Tensor], shape, dtype, device: int) -> Optional[Tensor]:
     """checks an activation; a copy where its last dimension is not contiguous"""
     if t is None:
         return None
-    if t.shape != shape:
-        raise RuntimeError(f"{what}: {name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    if t.dtype != (dtype or like.dtype) or t.device != like.device:
-        raise RuntimeError(f"{what}: {name} is {t.dtype} on {t.device}, expected {dtype or like.dtype} on {like.device}")
-    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+    if t.shape != shape or t.dtype is not dtype or t.get_device() != device:
+        _refuse(what, name, t, shape, dtype, device)
+    return t if t.is_contiguous() or t.stride(-1) == 1 or shape[-1] <= 1 else t.contiguous()
 
 
-def _param(what: str, name: str, t: Optional[Tensor], shape, like: Tensor, dtype=torch.float32) -> Optional[Tensor]:
+def _param(what: str, name: str, t: Optional[Tensor], shape, device: int, dtype=torch.float32) -> Optional[Tensor]:
     """checks a parameter or state; contiguous"""
     if t is None:
         return None
-    if t.shape != shape:
-        raise RuntimeError(f"{what}: {name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    if t.dtype != dtype or t.device != like.device:
-        raise RuntimeError(f"{what}: {name} is {t.dtype} on {t.device}, expected {dtype} on {like.device}")
+    if t.shape != shape or t.dtype is not dtype or t.get_device() != device:
+        _refuse(what, name, t, shape, dtype, device)
     return t.contiguous()
 
 
-def _in_place(what: str, t: Tensor, shape, like: Tensor, dtype=torch.float32) -> None:
-    if t.shape != shape or t.dtype != dtype or t.device != like.device or not t.is_contiguous():
+def _in_place(what: str, t: Tensor, shape, device: int, dtype=torch.float32) -> None:
+    if t.shape != shape or t.dtype is not dtype or t.get_device() != device or not t.is_contiguous():
         raise RuntimeError(f"{what}: the state is updated in place: it must be a contiguous {dtype} tensor of shape "
-                           f"{tuple(shape)} on {like.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+                           f"{tuple(shape)} on cuda:{device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
 def _sequence_form(what: str, x: Tensor, offsets: Optional[Tensor]):
@@ -1127,13 +1128,18 @@ def _st2(t: Optional[Tensor]):
     return (t.stride(0), t.stride(1)) if t.dim() == 3 else (0, t.stride(0))
 
 
-def _bc_form(what: str, name: str, t: Tensor, lead, like: Tensor) -> Tensor:
-    """B or C as [..., groups, states] with contiguous states"""
-    if t.dim() == len(lead) + 1:
-        t = t.unsqueeze(-2)
-    if t.dim() != len(lead) + 2:
-        raise RuntimeError(f"{what}: {name} has shape {tuple(t.shape)}, expected {tuple(lead)} + (groups, states)")
-    return _act(what, name, t, tuple(lead) + tuple(t.shape[-2:]), like)
+def _bc_form(what: str, B: Tensor, C: Tensor, lead, channels: int, N: int, dtype, device: int):
+    """B and C as [..., groups, states] with contiguous states"""
+    n = len(lead)
+    if B.dim() == n + 1:
+        B = B.unsqueeze(-2)
+    if C.dim() == n + 1:
+        C = C.unsqueeze(-2)
+    shape = B.shape
+    if len(shape) != n + 2 or shape[:n] != lead or shape[-1] != N or shape[-2] < 1 or channels % shape[-2]:
+        raise RuntimeError(f"{what}: B has shape {tuple(B.shape)}, expected {tuple(lead)} + (groups, {N}), groups dividing "
+                           f"{channels} channels")
+    return _act(what, 'B', B, shape, dtype, device), _act(what, 'C', C, shape, dtype, device)
 
 
 def _st3(t: Tensor):
@@ -1150,21 +1156,18 @@ class ScanArgs:
         if A.dim() != 2:
             raise RuntimeError(f"{what}: A must be [channels, states], got {tuple(A.shape)}")
         N = A.shape[1]
-        self.shape, self.device, self.act = u.shape, u.device, u.dtype
-        u = _act(what, 'u', u, u.shape, u)
-        delta = _act(what, 'delta', delta, u.shape, u)
-        z = _act(what, 'z', z, u.shape, u)
-        B, C = _bc_form(what, 'B', B, self.lead, u), _bc_form(what, 'C', C, self.lead, u)
+        shape, dt, dev = self.shape, self.act, self.index = u.shape, u.dtype, u.get_device()
+        self.device = u.device
+        u = _act(what, 'u', u, shape, dt, dev)
+        delta = _act(what, 'delta', delta, shape, dt, dev)
+        z = _act(what, 'z', z, shape, dt, dev)
+        B, C = _bc_form(what, B, C, self.lead, ch, N, dt, dev)
         G = B.shape[-2]
-        if C.shape != B.shape or B.shape[-1] != N:
-            raise RuntimeError(f"{what}: B {tuple(B.shape)} and C {tuple(C.shape)} must both be [..., groups, {N}]")
-        if G < 1 or ch % G:
-            raise RuntimeError(f"{what}: {ch} channels do not divide into {G} groups")
-        A = _param(what, 'A', A, (ch, N), u)
-        D = _param(what, 'D', D, (ch,), u)
-        delta_bias = _param(what, 'delta_bias', delta_bias, (ch,), u)
+        A = _param(what, 'A', A, (ch, N), dev)
+        D = _param(what, 'D', D, (ch,), dev)
+        delta_bias = _param(what, 'delta_bias', delta_bias, (ch,), dev)
         self.state_shape, self.bc_shape = (S, ch, N), B.shape
-        state = _param(what, 'state', state, self.state_shape, u)
+        state = _param(what, 'state', state, self.state_shape, dev)
         self.tensors = (u, delta, A, B, C, D, z, delta_bias, state, offsets)
         self.has_D, self.has_z, self.has_bias = D is not None, z is not None, delta_bias is not None
         self.packed, self.tokens = offsets is not None, rows * L
@@ -1189,7 +1192,7 @@ def _final_states(shape, dtype, device, entering: Optional[Tensor], packed: bool
 def selective_scan_fwd(a: ScanArgs, want_state: bool, keep: bool):
     """-> (out, final state or None, what the backward pass starts from or None)"""
     dev = a.device
-    if dev.index != _device_now():
+    if a.index != _device_now():
         with torch.cuda.device(dev):
             return selective_scan_fwd(a, want_state, keep)
     out = torch.empty(a.shape, dtype=a.act, device=dev)
@@ -1208,11 +1211,11 @@ def selective_scan_bwd(a: ScanArgs, dout: Tensor, dfinal: Optional[Tensor], ckpt
     """-> du, ddelta, dA, dB, dC, dD, dz, ddelta_bias, dstate (None where there is no such input)"""
     what = 'selective_scan_bwd'
     dev = a.device
-    if dev.index != _device_now():
+    if a.index != _device_now():
         with torch.cuda.device(dev):
             return selective_scan_bwd(a, dout, dfinal, ckpt, want_dstate)
-    dout = _act(what, 'dout', dout, a.shape, ckpt, a.act)
-    dfinal = _param(what, 'dstate', dfinal, a.state_shape, ckpt)
+    dout = _act(what, 'dout', dout, a.shape, a.act, a.index)
+    dfinal = _param(what, 'dstate', dfinal, a.state_shape, a.index)
     f32 = torch.float32
     du = torch.empty(a.shape, dtype=a.act, device=dev)
     dd = torch.empty(a.shape, dtype=a.act, device=dev)
@@ -1238,33 +1241,31 @@ def selective_scan_step(state, u, delta, A, B, C, D=None, z=None, delta_bias=Non
     """one token per sequence: u, delta, z [rows, channels], B, C [rows, groups, states]; `state` [rows, channels,
     states] is updated in place -> out [rows, channels]"""
     what = 'selective_scan_step'
-    dtype = _act_dtype(what, u)
-    if u.device.index != _device_now():
-        with torch.cuda.device(u.device):
+    code = _act_dtype(what, u)
+    dev = u.get_device()
+    if dev != _device_now():
+        with torch.cuda.device(dev):
             return selective_scan_step(state, u, delta, A, B, C, D, z, delta_bias, delta_softplus)
-    if u.dim() != 2 or A.dim() != 2:
+    shape, dt = u.shape, u.dtype
+    if len(shape) != 2 or A.dim() != 2:
         raise RuntimeError(f"{what}: expected u [rows, channels] and A [channels, states], got {tuple(u.shape)} and "
                            f"{tuple(A.shape)}")
-    rows, ch = u.shape
+    rows, ch = shape
     N = A.shape[1]
-    _in_place(what, state, (rows, ch, N), u)
-    u = _act(what, 'u', u, u.shape, u)
-    delta = _act(what, 'delta', delta, u.shape, u)
-    z = _act(what, 'z', z, u.shape, u)
-    B, C = _bc_form(what, 'B', B, (rows,), u), _bc_form(what, 'C', C, (rows,), u)
-    G = B.shape[1]
-    if C.shape != B.shape or B.shape[2] != N or G < 1 or ch % G:
-        raise RuntimeError(f"{what}: B {tuple(B.shape)} and C {tuple(C.shape)} must both be [{rows}, groups, {N}], groups "
-                           f"dividing {ch} channels")
-    A = _param(what, 'A', A, (ch, N), u)
-    D = _param(what, 'D', D, (ch,), u)
-    delta_bias = _param(what, 'delta_bias', delta_bias, (ch,), u)
-    out = torch.empty((rows, ch), dtype=u.dtype, device=u.device)
+    _in_place(what, state, (rows, ch, N), dev)
+    u = _act(what, 'u', u, shape, dt, dev)
+    delta = _act(what, 'delta', delta, shape, dt, dev)
+    z = _act(what, 'z', z, shape, dt, dev)
+    B, C = _bc_form(what, B, C, (rows,), ch, N, dt, dev)
+    A = _param(what, 'A', A, (ch, N), dev)
+    D = _param(what, 'D', D, (ch,), dev)
+    delta_bias = _param(what, 'delta_bias', delta_bias, (ch,), dev)
+    out = torch.empty(shape, dtype=dt, device=u.device)
     check(lib.dvae_selective_scan_step(state.data_ptr(), u.data_ptr(), u.stride(0), delta.data_ptr(), delta.stride(0),
                                        A.data_ptr(), B.data_ptr(), B.stride(0), B.stride(1), C.data_ptr(), C.stride(0),
                                        C.stride(1), _p(D), _p(z), 0 if z is None else z.stride(0), _p(delta_bias),
-                                       int(bool(delta_softplus)), out.data_ptr(), rows, ch, G, N, dtype,
-                                       _stream_of(u.device.index)), what)
+                                       1 if delta_softplus else 0, out.data_ptr(), rows, ch, B.shape[1], N, code,
+                                       _stream_of(dev)), what)
     return out
 
 
@@ -1277,12 +1278,13 @@ class ConvArgs:
         if weight.dim() != 2 or not 2 <= weight.shape[1] <= 4:
             raise RuntimeError(f"{what}: weight must be [channels, 2 to 4 taps], got {tuple(weight.shape)}")
         W = weight.shape[1]
-        self.shape, self.device, self.act = x.shape, x.device, x.dtype
+        shape, dt, dev = self.shape, self.act, self.index = x.shape, x.dtype, x.get_device()
+        self.device = x.device
         self.state_shape = (S, W - 1, ch)
-        x = _act(what, 'x', x, x.shape, x)
-        weight = _param(what, 'weight', weight, (ch, W), x)
-        bias = _param(what, 'bias', bias, (ch,), x)
-        state = _param(what, 'state', state, self.state_shape, x, x.dtype)
+        x = _act(what, 'x', x, shape, dt, dev)
+        weight = _param(what, 'weight', weight, (ch, W), dev)
+        bias = _param(what, 'bias', bias, (ch,), dev)
+        state = _param(what, 'state', state, self.state_shape, dev, dt)
         self.tensors = (x, weight, bias, state, offsets)
         self.has_bias, self.packed, self.tokens = bias is not None, offsets is not None, rows * L
         self.sizes = rows, L, ch, W
@@ -1298,7 +1300,7 @@ class ConvArgs:
 def short_conv_fwd(a: ConvArgs, want_state: bool):
     """-> out, final state or None"""
     dev = a.device
-    if dev.index != _device_now():
+    if a.index != _device_now():
         with torch.cuda.device(dev):
             return short_conv_fwd(a, want_state)
     out = torch.empty(a.shape, dtype=a.act, device=dev)
@@ -1312,11 +1314,11 @@ def short_conv_bwd(a: ConvArgs, dout: Tensor, dfinal: Optional[Tensor], want_dst
     """-> dx, dweight, dbias, dstate"""
     what = 'short_conv_bwd'
     dev = a.device
-    if dev.index != _device_now():
+    if a.index != _device_now():
         with torch.cuda.device(dev):
             return short_conv_bwd(a, dout, dfinal, want_dstate)
-    dout = _act(what, 'dout', dout, a.shape, dout, a.act)
-    dfinal = _param(what, 'dstate', dfinal, a.state_shape, dout, a.act)
+    dout = _act(what, 'dout', dout, a.shape, a.act, a.index)
+    dfinal = _param(what, 'dstate', dfinal, a.state_shape, a.index, a.act)
     rows, L, ch, W = a.sizes
     dx = torch.empty(a.shape, dtype=a.act, device=dev)
     new = torch.empty if a.tokens else torch.zeros
@@ -1334,37 +1336,31 @@ def short_conv_step(state, x, weight, bias=None, silu=False) -> Tensor:
     """one token per sequence: x [rows, channels]; `state` [rows, taps - 1, channels], the inputs before it in x's type,
     is updated in place -> out [rows, channels]"""
     what = 'short_conv_step'
-    dtype = _act_dtype(what, x)
-    if x.device.index != _device_now():
-        with torch.cuda.device(x.device):
+    code = _act_dtype(what, x)
+    dev = x.get_device()
+    if dev != _device_now():
+        with torch.cuda.device(dev):
             return short_conv_step(state, x, weight, bias, silu)
-    if x.dim() != 2 or weight.dim() != 2 or not 2 <= weight.shape[1] <= 4:
+    shape, dt = x.shape, x.dtype
+    if len(shape) != 2 or weight.dim() != 2 or not 2 <= weight.shape[1] <= 4:
         raise RuntimeError(f"{what}: expected x [rows, channels] and weight [channels, 2 to 4 taps], got "
                            f"{tuple(x.shape)} and {tuple(weight.shape)}")
-    rows, ch = x.shape
+    rows, ch = shape
     W = weight.shape[1]
-    _in_place(what, state, (rows, W - 1, ch), x, x.dtype)
-    x = _act(what, 'x', x, x.shape, x)
-    weight = _param(what, 'weight', weight, (ch, W), x)
-    bias = _param(what, 'bias', bias, (ch,), x)
-    out = torch.empty((rows, ch), dtype=x.dtype, device=x.device)
+    _in_place(what, state, (rows, W - 1, ch), dev, dt)
+    x = _act(what, 'x', x, shape, dt, dev)
+    weight = _param(what, 'weight', weight, (ch, W), dev)
+    bias = _param(what, 'bias', bias, (ch,), dev)
+    out = torch.empty(shape, dtype=dt, device=x.device)
     check(lib.dvae_short_conv_step(state.data_ptr(), x.data_ptr(), x.stride(0), weight.data_ptr(), _p(bias),
-                                   int(bool(silu)), out.data_ptr(), rows, ch, W, dtype, _stream_of(x.device.index)), what)
+                                   1 if silu else 0, out.data_ptr(), rows, ch, W, code, _stream_of(dev)), what)
     return out
 
 
-def _norm_rows(what: str, name: str, t: Optional[Tensor], shape, like: Tensor, *dtypes) -> Optional[Tensor]:
+def _norm_rows(what: str, name: str, t: Optional[Tensor], shape, dtype, device: int) -> Optional[Tensor]:
     """an activation [..., channels] as rows of equal stride"""
-    if t is None:
-        return None
-    if t.shape != shape:
-        raise RuntimeError(f"{what}: {name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    if t.dtype not in dtypes or t.device != like.device:
-        raise RuntimeError(f"{what}: {name} is {t.dtype} on {t.device}, expected {' or '.join(map(str, dtypes))} on "
-                           f"{like.device}")
-    if len(shape) != 2:
-        t = t.reshape(-1, shape[-1])
-    return t if t.stride(1) == 1 or shape[-1] == 1 else t.contiguous()
+    t = _act(what, name, t, shape, dtype, device)
+    return t if t is None or len(shape) == 2 else t.reshape(-1, shape[-1])
 
 
 class NormArgs:
@@ -1372,16 +1368,19 @@ class NormArgs:
 
     def __init__(self, what, x, residual, weight):
         self.dtype = _act_dtype(what, x)
-        shape = self.shape = x.shape
+        shape, dt, dev = self.shape, self.act, self.index = x.shape, x.dtype, x.get_device()
+        self.device = x.device
         if len(shape) < 1 or shape[-1] < 1:
             raise RuntimeError(f"{what}: expected [..., channels], got {tuple(shape)}")
         self.D = shape[-1]
-        self.x = _norm_rows(what, 'x', x, shape, x, x.dtype)
+        self.x = _norm_rows(what, 'x', x, shape, dt, dev)
         self.rows = self.x.shape[0]
-        self.residual = _norm_rows(what, 'residual', residual, shape, x, x.dtype, torch.float32)
-        self.weight = _param(what, 'weight', weight, (self.D,), x)
-        self.sum_dtype = x.dtype if residual is None else residual.dtype
-        self.rdtype = _ACT_DTYPES[self.sum_dtype]
+        self.sum_dtype, self.rdtype, self.residual = dt, self.dtype, None
+        if residual is not None:
+            if residual.dtype is torch.float32:         # x's type, or fp32
+                self.sum_dtype, self.rdtype = torch.float32, 0
+            self.residual = _norm_rows(what, 'residual', residual, shape, self.sum_dtype, dev)
+        self.weight = _param(what, 'weight', weight, (self.D,), dev)
 
     def head(self, eps):
         r = self.residual
@@ -1391,15 +1390,15 @@ class NormArgs:
 
 def add_rms_norm_fwd(a: NormArgs, eps: float, keep: bool):
     """-> y, sum [..., channels] (None without a residual: it is x), rstd [rows] or None"""
-    dev = a.x.device
-    if dev.index != _device_now():
+    dev = a.device
+    if a.index != _device_now():
         with torch.cuda.device(dev):
             return add_rms_norm_fwd(a, eps, keep)
-    y = torch.empty(a.shape, dtype=a.x.dtype, device=dev)
+    y = torch.empty(a.shape, dtype=a.act, device=dev)
     total = None if a.residual is None else torch.empty(a.shape, dtype=a.sum_dtype, device=dev)
     rstd = torch.empty(a.rows, dtype=torch.float32, device=dev) if keep else None
     check(lib.dvae_add_rms_norm_fwd(*a.head(eps), y.data_ptr(), _p(total), _p(rstd), a.rows, a.D, a.dtype, a.rdtype,
-                                    _stream_of(dev.index)), 'add_rms_norm_fwd')
+                                    _stream_of(a.index)), 'add_rms_norm_fwd')
     return y, total, rstd
 
 
@@ -1407,8 +1406,8 @@ def add_rms_norm_q8(x: Tensor, residual: Optional[Tensor], weight: Tensor, eps: 
     """add_rms_norm with the output in 8 bits -> (q of type float8_e4m3fn, scale [...] fp32, sum): the normalised row
     is q * scale, scale = max|y| / 448 of the row (1 for a row of zeros)"""
     a = NormArgs('add_rms_norm_q8', x, residual, weight)
-    dev = a.x.device
-    if dev.index != _device_now():
+    dev = a.device
+    if a.index != _device_now():
         with torch.cuda.device(dev):
             return add_rms_norm_q8(x, residual, weight, eps)
     q = torch.empty(a.shape, dtype=torch.float8_e4m3fn, device=dev)
@@ -1429,9 +1428,9 @@ def add_rms_norm_bwd(dy: Tensor, dsum: Optional[Tensor], total: Tensor, weight: 
             return add_rms_norm_bwd(dy, dsum, total, weight, rstd, dx_dtype)
     shape = dy.shape
     D = shape[-1]
-    dy2 = _norm_rows(what, 'dy', dy, shape, dy, dx_dtype)
-    ds2 = _norm_rows(what, 'dsum', dsum, shape, dy, total.dtype)
-    s2 = _norm_rows(what, 'sum', total, shape, dy, total.dtype)
+    dy2 = _norm_rows(what, 'dy', dy, shape, dx_dtype, dev.index)
+    ds2 = _norm_rows(what, 'dsum', dsum, shape, total.dtype, dev.index)
+    s2 = _norm_rows(what, 'sum', total, shape, total.dtype, dev.index)
     rows = dy2.shape[0]
     dres = torch.empty(shape, dtype=total.dtype, device=dev)
     dx = dres if total.dtype == dx_dtype else torch.empty(shape, dtype=dx_dtype, device=dev)
