@@ -268,7 +268,10 @@ __global__ void __launch_bounds__(64 * SUM_WAVES) norm_dw_sum_kernel(const float
 
 // ------------------------------------------------------------------------------------------------ host side
 #define NORM_MAX_GRID 512     // workgroups of the backward kernel, and with that partial rows of dw: two per compute unit
-static int64_t norm_row_grid(int64_t rows) { const int64_t g = ceil_div64(rows, 4); return g < NORM_MAX_GRID ? g : NORM_MAX_GRID; }
+static int64_t norm_row_grid(int64_t rows) {
+  const int64_t g = ceil_div64(rows, 4);
+  return g < NORM_MAX_GRID ? g : NORM_MAX_GRID;
+}
 
 static int norm_check(const char* what, int64_t rows, int64_t D, int dtype, int rdtype) {
   DVAE_REQUIRE(dtype == DVAE_DT_F32 || dtype == DVAE_DT_BF16, "%s: dtype must be fp32 (0) or bf16 (1)", what);

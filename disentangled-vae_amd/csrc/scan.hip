@@ -160,7 +160,8 @@ struct Tile {
 // NP states of a channel from the n0-th on, of a state tensor [S][D][N] or of A [D][N].  FULL: all of them exist, and a
 // lane's come as 16-byte accesses (from and to addresses that need 4-byte alignment only).
 template <int NP, bool FULL>
-__device__ __forceinline__ void load_state(const float* s, int64_t seq, const ScanArgs& p, int d, float (&h)[NP], int n0 = 0) {
+__device__ __forceinline__ void load_state(const float* s, int64_t seq, const ScanArgs& p, int d, float (&h)[NP],
+                                           int n0 = 0) {
   const float* q = s + (seq * p.D + d) * p.N + n0;
   if (FULL) {
 #pragma unroll
@@ -175,7 +176,8 @@ __device__ __forceinline__ void load_state(const float* s, int64_t seq, const Sc
   }
 }
 template <int NP, bool FULL>
-__device__ __forceinline__ void store_state(float* s, int64_t seq, const ScanArgs& p, int d, const float (&h)[NP], int n0 = 0) {
+__device__ __forceinline__ void store_state(float* s, int64_t seq, const ScanArgs& p, int d, const float (&h)[NP],
+                                            int n0 = 0) {
   float* q = s + (seq * p.D + d) * p.N + n0;
   if (FULL) {
 #pragma unroll
@@ -618,7 +620,8 @@ __global__ void __launch_bounds__(64 * SCAN_BT * (NP / SCAN_NW), 2) scan_bwd_ker
   const float* ck = p.ckpt + ((int64_t)row * p.blocks + first / SCAN_Q) * p.N * p.D + skip;
   Rows<T> ur(p.u, p.u_sb, p.u_st, row, first), dr(p.delta, p.delta_sb, p.delta_st, row, first);
   Rows<T> gr(p.dout, p.dout_sb, p.dout_st, row, first);
-  Rows<T> zr(gated ? p.z : p.dout, gated ? p.z_sb : p.dout_sb, gated ? p.z_st : p.dout_st, row, first);  // (not used without z)
+  // (without z, dout is read in its place and not used)
+  Rows<T> zr(gated ? p.z : p.dout, gated ? p.z_sb : p.dout_sb, gated ? p.z_st : p.dout_st, row, first);
   T un[OWN], dn[OWN], zn[OWN], gn[OWN];               // this wave's tokens of the block ahead,
   float hn[SCAN_NW];                                  // and the state that enters it
   ur.load(un, w.t1 - first, at, j0);
@@ -851,10 +854,11 @@ __global__ void __launch_bounds__(64 * SUM_WAVES) scan_sums_kernel(ScanArgs p, T
   else if (dbias) dbias[d] = s;
 }
 
-// One token per row.  256 x 2048 x 16 bf16: 19 us for 69 MB (3.6 TB/s); 1 x 512: 4 us.  Nearly all of the traffic is the state, read and written once: a lane owns four states of a channel
-// (one 16-byte access each way where N is a multiple of 4 and all is aligned), a channel's LPC lanes are neighbours, and the sum over them
-// takes two lane exchanges.  What a channel reads besides (inputs, step size) its lanes read and compute alike.  A lane
-// goes through R rows whose loads are in flight together and share its A.
+// One token per row.  Nearly all of the traffic is the state, read and written once: a lane owns four states of a channel
+// (one 16-byte access each way where N is a multiple of 4 and all is aligned), a channel's LPC lanes are neighbours, and the
+// sum over them takes two lane exchanges.  What a channel reads besides (inputs, step size) its lanes read and compute
+// alike.  A lane goes through R rows whose loads are in flight together and share its A.  256 x 2048 x 16 bf16: 19 us for
+// 72 MB (3.8 TB/s); 1 x 512: 4 us.
 template <typename T, int LPC, int R, bool VEC>
 __global__ void __launch_bounds__(256) scan_step_kernel(ScanArgs p) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -990,8 +994,8 @@ template <typename T, int NP, bool PACKED, bool FAST> static void scan_bwd_launc
     DVAE_LAUNCH((scan_bwd_state_kernel<T, NP, PACKED, FAST>), grid, block, 0, s, p);
     scan_join<true>(p, s);
   }
-  DVAE_LAUNCH((scan_bwd_kernel<T, NP, PACKED, FAST>), dim3((unsigned)((int64_t)p.rows * p.nch * p.G * scan_bc_parts(p.tpg))),
-              dim3(64 * SCAN_BT * (NP / SCAN_NW)), 0, s, p);
+  const int64_t groups = (int64_t)p.rows * p.nch * p.G * scan_bc_parts(p.tpg);
+  DVAE_LAUNCH((scan_bwd_kernel<T, NP, PACKED, FAST>), dim3((unsigned)groups), dim3(64 * SCAN_BT * (NP / SCAN_NW)), 0, s, p);
 }
 
 #define SCAN_LAUNCH(K, T, NP, p, s)                                                                   \

@@ -2,11 +2,12 @@
 // where tokens before a sequence's first are the carried state, or zero.  Bound by memory: every element of x is read
 // once (and a block's first W - 1 rows twice, out of the L2) and kept in registers for the W outputs that use it.
 //
-// A lane owns one 32-bit word of a row (V = 2 bf16 channels where the tensors' alignment allows it, else one): with 16 bytes
-// per lane the window, the taps and what is in flight take so many registers that too few waves run (backward, 8 x 2048 x
-// 2048 bf16, four taps: 125 us with 16 bytes, 72 with 8, 57 with 4).  A wave takes p.tb consecutive tokens.  CONV_AHEAD tokens are in flight at any time: a token's registers receive the one CONV_AHEAD further
-// on as soon as it has been used.  A batch is walked as one line of tokens, sequence after sequence, so short clips fill the
-// chip like long sequences do.
+// A lane owns one 32-bit word of a row (V = 2 bf16 channels where the tensors' alignment allows it, else one): with 16
+// bytes per lane the window, the taps and what is in flight take so many registers that too few waves run (backward, 8 x
+// 2048 x 2048 bf16, four taps: 125 us with 16 bytes, 72 with 8, 57 with 4).  A wave takes p.tb consecutive tokens.
+// CONV_AHEAD tokens are in flight at any time: a token's registers receive the one CONV_AHEAD further on as soon as it has
+// been used.  A batch is walked as one line of tokens, sequence after sequence, so short clips fill the chip like long
+// sequences do.
 //
 // 8 x 2048 x 2048 bf16, four taps: forward 33 us (4.1 TB/s of x and out), backward 57 us (3.5 TB/s of x, dout and dx) and
 // 4 us for the sums of its partial rows; 32 x 1024 fp32, one token: 2.7 us.

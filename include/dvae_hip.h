@@ -586,9 +586,11 @@ int dvae_adam_advance_f32(float* dyn, double beta1, double beta2, dvae_stream_t 
  * out = (sum_n C[n] h[n] + Dp u) silu(z).  u, delta, z, out [rows,L,D]; A [D,N], N <= 16; B, C [rows,L,G,N], G divides D;
  * Dp, bias [D]; state0 (entering) and state1 (final) [S,D,N].  NULL: Dp, z, bias, state0, state1, offsets, ckpt.
  * Final states of sequences without tokens are not written.  ckpt (dvae_selective_scan_ckpt_floats): the states that
- * the backward pass starts from, kept if not NULL. */
+ * the backward pass starts from, kept if not NULL.  ws: dvae_selective_scan_fwd_ws_floats floats (0 where the time axis is
+ * not split; NULL then).  Token strides of u, delta, z and dout must be below 2^26 elements. */
 int64_t dvae_selective_scan_ckpt_floats(int64_t rows, int64_t L, int64_t D, int64_t N);
-int64_t dvae_selective_scan_fwd_ws_floats(int64_t rows, int64_t L, int64_t D, int64_t G, int64_t N, int keep /* ckpt given */);
+int64_t dvae_selective_scan_fwd_ws_floats(int64_t rows, int64_t L, int64_t D, int64_t G, int64_t N,
+                                          int keep /* whether ckpt is given */);
 int dvae_selective_scan_fwd(const void* u, int64_t u_sb, int64_t u_st, const void* delta, int64_t delta_sb,
                             int64_t delta_st, const float* A, const void* B, int64_t B_sb, int64_t B_st, int64_t B_sg,
                             const void* C, int64_t C_sb, int64_t C_st, int64_t C_sg, const float* Dp, const void* z,
@@ -596,7 +598,8 @@ int dvae_selective_scan_fwd(const void* u, int64_t u_sb, int64_t u_st, const voi
                             float* state1, const int32_t* offsets, void* out, float* ckpt, int64_t rows, int64_t L,
                             int64_t D, int64_t G, int64_t N, int64_t S, int dtype, float* ws, dvae_stream_t stream);
 /* Gradients from dout and (NULL: zero) dstate1, the gradient of the final states.  dA, dD, dbias, dstate0 may be NULL;
- * dstate0 of sequences without tokens is not written.  ckpt as the forward pass filled it. */
+ * dstate0 of sequences without tokens is not written.  ckpt as the forward pass filled it (it is read only); ws:
+ * dvae_selective_scan_bwd_ws_floats floats. */
 int64_t dvae_selective_scan_bwd_ws_floats(int64_t rows, int64_t L, int64_t D, int64_t G, int64_t N);
 int dvae_selective_scan_bwd(const void* u, int64_t u_sb, int64_t u_st, const void* delta, int64_t delta_sb,
                             int64_t delta_st, const float* A, const void* B, int64_t B_sb, int64_t B_st, int64_t B_sg,
@@ -619,7 +622,8 @@ int dvae_selective_scan_step(float* state, const void* u, int64_t u_sb, const vo
 int dvae_short_conv_fwd(const void* x, int64_t x_sb, int64_t x_st, const float* w, const float* bias, int silu,
                         const void* state0, void* state1, const int32_t* offsets, void* out, int64_t rows, int64_t L,
                         int64_t D, int64_t W, int64_t S, int dtype, dvae_stream_t stream);
-/* dx, dw [D,W], dbias [D] (NULL: not wanted) and dstate0 (NULL likewise) from dout and dstate1 (NULL: zero). */
+/* dx, dw [D,W], dbias [D] (NULL: not wanted) and dstate0 (NULL likewise) from dout and dstate1 (NULL: zero).
+ * ws: dvae_short_conv_bwd_ws_floats floats. */
 int64_t dvae_short_conv_bwd_ws_floats(int64_t rows, int64_t L, int64_t D, int64_t W);
 int dvae_short_conv_bwd(const void* x, int64_t x_sb, int64_t x_st, const float* w, const float* bias, int silu,
                         const void* state0, const int32_t* offsets, const void* dout, int64_t dout_sb, int64_t dout_st,
@@ -641,7 +645,8 @@ int dvae_add_rms_norm_q8(const void* x, int64_t x_st, const void* residual, int6
                          void* q, float* scale, void* sum, int64_t rows, int64_t D, int dtype, int rdtype,
                          dvae_stream_t stream);
 /* dsum_out = rstd (w dy - hat mean(w dy hat)) + dsum, the gradient of the sum, written as dres (type `rdtype`) and, if
- * the types differ and dx is not NULL, as dx (type `dtype`); dw [D].  `sum` (strides s_st) as stored; dsum NULL: zero. */
+ * the types differ and dx is not NULL, as dx (type `dtype`); dw [D].  `sum` (strides s_st) as stored; dsum NULL: zero.
+ * ws: dvae_add_rms_norm_bwd_ws_floats floats. */
 int64_t dvae_add_rms_norm_bwd_ws_floats(int64_t rows, int64_t D);
 int dvae_add_rms_norm_bwd(const void* dy, int64_t dy_st, const void* dsum, int64_t ds_st, const void* sum, int64_t s_st,
                           const float* w, const float* rstd, void* dres, void* dx, float* dw, int64_t rows, int64_t D,
