@@ -1022,6 +1022,7 @@ class SelectiveScan(torch.autograd.Function):
         _no_second_derivative('selective_scan')
         *keep, ckpt = ctx.saved_tensors             # (unpacking raises if an input has been changed since)
         a, b_shape, c_shape = ctx.args
+        a = a.of(keep)
         if dout is None:
             dout = torch.zeros(a.shape, dtype=a.act, device=a.device)
         need = ctx.needs_input_grad
@@ -1090,7 +1091,7 @@ class ShortConv(torch.autograd.Function):
     def backward(ctx, dout, dfinal):
         _no_second_derivative('short_conv')
         keep = ctx.saved_tensors                    # (unpacking raises if an input has been changed since)
-        a = ctx.args
+        a = ctx.args.of(keep)
         if dout is None:
             dout = torch.zeros(a.shape, dtype=a.act, device=a.device)
         need = ctx.needs_input_grad

@@ -1146,9 +1146,25 @@ def _st3(t: Tensor):
     return (t.stride(0), t.stride(1), t.stride(2)) if t.dim() == 4 else (0, t.stride(0), t.stride(1))
 
 
-class ScanArgs:
-    """The checked arguments of a selective scan, as both directions hand them to the library.  The backward pass works
-    from what was prepared here: `release` drops the tensors, which the caller has to keep (`tensors`)."""
+def _places(tensors):
+    return [None if t is None else t.data_ptr() if t.is_contiguous() else (t.data_ptr(), t.stride()) for t in tensors]
+
+
+class _KeptArgs:
+    """Checked arguments that serve both directions.  `release` drops the tensors, which autograd keeps in between;
+    `of` takes them back: saved-tensor hooks (offloading, checkpointing) may have put others in their place, and those are
+    then prepared anew."""
+
+    def release(self):
+        self.places, self.tensors = _places(self.tensors), None
+        return self
+
+    def of(self, tensors):
+        return self if _places(tensors) == self.places else self.again(*tensors)
+
+
+class ScanArgs(_KeptArgs):
+    """The checked arguments of a selective scan, as both directions hand them to the library."""
 
     def __init__(self, what, u, delta, A, B, C, D, z, delta_bias, delta_softplus, state, offsets):
         self.dtype = _act_dtype(what, u)
@@ -1169,6 +1185,7 @@ class ScanArgs:
         self.state_shape, self.bc_shape = (S, ch, N), B.shape
         state = _param(what, 'state', state, self.state_shape, dev)
         self.tensors = (u, delta, A, B, C, D, z, delta_bias, state, offsets)
+        self.softplus = delta_softplus
         self.has_D, self.has_z, self.has_bias = D is not None, z is not None, delta_bias is not None
         self.packed, self.tokens = offsets is not None, rows * L
         self.sizes = rows, L, ch, G, N
@@ -1177,9 +1194,8 @@ class ScanArgs:
         self.offsets_ptr = _p(offsets)
         self.tail = rows, L, ch, G, N, S, self.dtype
 
-    def release(self):
-        self.tensors = None
-        return self
+    def again(self, u, delta, A, B, C, D, z, delta_bias, state, offsets):
+        return ScanArgs('selective_scan_bwd', u, delta, A, B, C, D, z, delta_bias, self.softplus, state, offsets)
 
 
 def _final_states(shape, dtype, device, entering: Optional[Tensor], packed: bool, tokens: int) -> Tensor:
@@ -1269,8 +1285,8 @@ def selective_scan_step(state, u, delta, A, B, C, D=None, z=None, delta_bias=Non
     return out
 
 
-class ConvArgs:
-    """The checked arguments of a short convolution (see ScanArgs)."""
+class ConvArgs(_KeptArgs):
+    """The checked arguments of a short convolution."""
 
     def __init__(self, what, x, weight, bias, silu, state, offsets):
         self.dtype = _act_dtype(what, x)
@@ -1286,15 +1302,15 @@ class ConvArgs:
         bias = _param(what, 'bias', bias, (ch,), dev)
         state = _param(what, 'state', state, self.state_shape, dev, dt)
         self.tensors = (x, weight, bias, state, offsets)
+        self.silu = silu
         self.has_bias, self.packed, self.tokens = bias is not None, offsets is not None, rows * L
         self.sizes = rows, L, ch, W
         self.head = x.data_ptr(), *_st2(x), weight.data_ptr(), _p(bias), int(bool(silu)), _p(state)
         self.offsets_ptr = _p(offsets)
         self.tail = rows, L, ch, W, S, self.dtype
 
-    def release(self):
-        self.tensors = None
-        return self
+    def again(self, x, weight, bias, state, offsets):
+        return ConvArgs('short_conv_bwd', x, weight, bias, self.silu, state, offsets)
 
 
 def short_conv_fwd(a: ConvArgs, want_state: bool):

@@ -640,6 +640,42 @@ def test_tensors_of_more_than_2_to_the_31_elements(F):
     assert not g[:T - n].any()
 
 
+@pytest.mark.parametrize('how', ['offloaded', 'recomputed', 'turned'])
+def test_backward_from_tensors_that_hooks_put_in_place_of_the_kept_ones(F, how):
+    """saved-tensor hooks hand back other memory, or other strides, than the forward pass read: same gradients, also with
+    what the forward pass read overwritten by then"""
+    from torch.utils.checkpoint import checkpoint
+    c = ScanCase(48, 16, 1, torch.float32, lengths=[70, 0, 230], tail=4, seed=41, state=False)
+    w = {'conv': torch.randn(48, 4, device='cuda'), 'norm': torch.rand(48, device='cuda') + 0.5}
+
+    def run(hooked):
+        leaf = {k: t.clone().requires_grad_() for k, t in c.gpu.items() if t is not None}
+        ww = {k: t.clone().requires_grad_() for k, t in w.items()}
+        body = lambda: _block(F, {k: t * 1.0 for k, t in leaf.items()}, c, ww)           # noqa: E731
+
+        def turned(t):                                                                  # the same values, column by column
+            return t.t().contiguous().t() if t.dim() == 2 else t.clone()
+
+        if not hooked:
+            y, s = body()
+        elif how == 'offloaded':
+            with torch.autograd.graph.save_on_cpu():
+                y, s = body()
+        elif how == 'turned':
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t, turned):
+                y, s = body()
+        else:
+            y, s = checkpoint(body, use_reentrant=False)
+        junk = [torch.full((c.gpu['u'].numel(),), float('nan'), device='cuda') for _ in range(64)]   # (in what is free by now)
+        ins = [*leaf.values(), *ww.values()]
+        got = torch.autograd.grad((y, s), ins, (torch.ones_like(y), torch.ones_like(s)))
+        del junk
+        return got
+
+    for a, b in zip(run(False), run(True)):
+        assert torch.equal(a, b)
+
+
 def test_results_repeat_bit_for_bit(F):
     c = ScanCase(200, 16, 2, torch.bfloat16, rows=(3, 150), seed=31, state=False)
     runs = []
