@@ -1061,6 +1061,7 @@ _ACT_DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 
 _device_now = torch._C._cuda_getDevice
 _stream_of = torch._C._cuda_getCurrentRawStream      # raw handle of a device's current stream
+_written = torch._C._increment_version               # tells autograd that tensors have been changed in place
 
 
 def _act_dtype(what: str, t: Tensor) -> int:
@@ -1282,6 +1283,7 @@ def selective_scan_step(state, u, delta, A, B, C, D=None, z=None, delta_bias=Non
                                        C.stride(1), _p(D), _p(z), 0 if z is None else z.stride(0), _p(delta_bias),
                                        1 if delta_softplus else 0, out.data_ptr(), rows, ch, B.shape[1], N, code,
                                        _stream_of(dev)), what)
+    _written((state,))
     return out
 
 
@@ -1370,6 +1372,7 @@ def short_conv_step(state, x, weight, bias=None, silu=False) -> Tensor:
     out = torch.empty(shape, dtype=dt, device=x.device)
     check(lib.dvae_short_conv_step(state.data_ptr(), x.data_ptr(), x.stride(0), weight.data_ptr(), _p(bias),
                                    1 if silu else 0, out.data_ptr(), rows, ch, W, code, _stream_of(dev)), what)
+    _written((state,))
     return out
 
 

@@ -676,6 +676,24 @@ def test_backward_from_tensors_that_hooks_put_in_place_of_the_kept_ones(F, how):
         assert torch.equal(a, b)
 
 
+def test_a_state_that_a_step_has_changed_is_refused_by_the_backward_pass(F):
+    c = ScanCase(16, 4, 1, torch.float32, rows=(2, 6), seed=43)
+    v = dict(c.gpu, u=c.gpu['u'].clone().requires_grad_())
+    x, w = v['u'], torch.randn(16, 4, device='cuda')
+    state, last = v['state'].clone(), torch.randn(2, 3, 16, device='cuda')
+    out = c.call(F, dict(v, state=state), False)
+    conv = F.short_conv(c.lead(x), w, state=last)
+    with torch.no_grad():
+        F.selective_scan_step(state, x[:2], v['delta'][:2], v['A'], v['B'][:2], v['C'][:2])
+        F.short_conv_step(last, x[:2], w)
+    for y in (out, conv):
+        with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+            torch.autograd.grad(y, (x,), torch.ones_like(y))
+    with torch.inference_mode():
+        i = state.clone()
+        F.selective_scan_step(i, x[:2], v['delta'][:2], v['A'], v['B'][:2], v['C'][:2])
+
+
 def test_results_repeat_bit_for_bit(F):
     c = ScanCase(200, 16, 2, torch.bfloat16, rows=(3, 150), seed=31, state=False)
     runs = []
