@@ -400,8 +400,9 @@ __global__ void __launch_bounds__(64 * WAVES) scan_join_kernel(ScanArgs p) {
   __shared__ float end[WAVES][3][64];         // [wave][own, decay, 1 if nothing gets through][lane]
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int64_t ND = (int64_t)p.N * p.D;
-  const int64_t i = min((int64_t)blockIdx.x * 64 + lane, ND - 1);      // (lanes past the last do as it does)
-  const int row = blockIdx.y, d = (int)(i % p.D), n = (int)(i / p.D);
+  const int per = (int)((ND + 63) / 64), row = blockIdx.x / per;
+  const int64_t i = min((int64_t)(blockIdx.x % per) * 64 + lane, ND - 1);      // (lanes past the last do as it does)
+  const int d = (int)(i % p.D), n = (int)(i / p.D);
   const float A2 = decay_rate(p.A[(int64_t)d * p.N + n]);
   const float* sumdt = p.sumdt + (int64_t)row * p.nch * p.D + d;
   float x = 0.f;                                   // what enters the chunks of this round
@@ -927,7 +928,8 @@ static int scan_check(const char* what, int64_t rows, int64_t L, int64_t D, int6
   DVAE_REQUIRE(dtype == DVAE_DT_F32 || dtype == DVAE_DT_BF16, "%s: dtype must be fp32 (0) or bf16 (1)", what);
   DVAE_REQUIRE(rows >= 0 && L >= 0 && D > 0 && G > 0 && D % G == 0, "%s: D must be a multiple of G", what);
   DVAE_REQUIRE(N > 0 && N <= SCAN_MAX_N, "%s: 1 to %d states per channel, got %ld", what, SCAN_MAX_N, (long)N);
-  DVAE_REQUIRE(rows * L < (1ll << 31) && D < (1ll << 24) && rows < (1ll << 31), "%s: too large", what);
+  DVAE_REQUIRE(rows < (1ll << 31) && L < (1ll << 31) && rows * L < SEQ_MAX_TOKENS && D < (1ll << 24), "%s: too large",
+               what);
   DVAE_REQUIRE(!offsets || (rows == 1 && S >= 1 && S < (1ll << 30)), "%s: offsets go with one row and S >= 1", what);
   return 0;
 }
@@ -965,6 +967,13 @@ static float* scan_scratch(ScanArgs& p, float* ws) {
   return ws + (((int64_t)p.rows * p.nch + 3) & ~3ll);
 }
 
+// whether every launch is one that the device takes
+static bool scan_fits(const ScanArgs& p) {
+  const int64_t chunks = (int64_t)p.rows * p.nch;
+  return launch_fits(chunks * p.wpg, 256) && launch_fits(chunks * p.G * scan_bc_parts(p.tpg), 256) &&
+         (p.nch == 1 || launch_fits(ceil_div64((int64_t)p.N * p.D, 64) * p.rows, p.nch > 2 * JOIN_AHEAD + 1 ? 512 : 64));
+}
+
 // whether B and C of every token and group can be read as whole aligned words
 static bool scan_words(const ScanArgs& p, int dtype, int NP) {
   if (p.N != NP) return false;
@@ -976,7 +985,7 @@ static bool scan_words(const ScanArgs& p, int dtype, int NP) {
 // eight waves per workgroup where one would go round more than twice: 126 chunks of 1002 channels 18 -> 9 us, but 16
 // chunks of 8 x 2048 channels 10 -> 27 us
 template <bool BACK> static void scan_join(const ScanArgs& p, hipStream_t s) {
-  const dim3 grid((unsigned)ceil_div64((int64_t)p.N * p.D, 64), p.rows);
+  const dim3 grid((unsigned)(ceil_div64((int64_t)p.N * p.D, 64) * p.rows));
   if (p.nch > 2 * JOIN_AHEAD + 1) DVAE_LAUNCH((scan_join_kernel<BACK, 8>), grid, dim3(64 * 8), 0, s, p);
   else DVAE_LAUNCH((scan_join_kernel<BACK, 1>), grid, dim3(64), 0, s, p);
 }
@@ -1045,6 +1054,7 @@ extern "C" int dvae_selective_scan_fwd(const void* u, int64_t u_sb, int64_t u_st
   const int rc = scan_check("selective_scan_fwd", rows, L, D, G, N, S, offsets, dtype);
   if (rc) return rc;
   if (rows * L == 0) return 0;
+  if (L == 1) u_st = delta_st = z_st = 0;          // (no token to step to)
   DVAE_REQUIRE(scan_stride_ok(u_st) && scan_stride_ok(delta_st) && scan_stride_ok(z_st),
                "selective_scan_fwd: token strides must be below 2^26 elements");
   ScanArgs p = {};
@@ -1054,7 +1064,7 @@ extern "C" int dvae_selective_scan_fwd(const void* u, int64_t u_sb, int64_t u_st
   p.state0 = state0; p.state1 = state1; p.offsets = offsets; p.out = out; p.ckpt = ckpt;
   scan_shape(p, rows, L, D, G, N, S);
   scan_scratch(p, ws);
-  DVAE_REQUIRE(rows * p.nch * p.wpg < (1ll << 31), "selective_scan_fwd: too many rows");
+  DVAE_REQUIRE(scan_fits(p), "selective_scan_fwd: too many rows for one launch");
   const int e = dtype == DVAE_DT_F32 ? 4 : 2;
   DVAE_WORK(rows * L * (double)e * ((z ? 4 : 3) * D + 2 * G * N), DVAE_UNIT_BYTE);
   SCAN_DISPATCH(scan_fwd_launch, dtype, p, ST(stream));
@@ -1074,6 +1084,7 @@ extern "C" int dvae_selective_scan_bwd(const void* u, int64_t u_sb, int64_t u_st
   const int rc = scan_check("selective_scan_bwd", rows, L, D, G, N, S, offsets, dtype);
   if (rc) return rc;
   DVAE_REQUIRE(rows * L > 0, "selective_scan_bwd: no tokens");
+  if (L == 1) u_st = delta_st = z_st = dout_st = 0;
   DVAE_REQUIRE(!z || dz, "selective_scan_bwd: dz is needed with z");
   DVAE_REQUIRE(scan_stride_ok(u_st) && scan_stride_ok(delta_st) && scan_stride_ok(z_st) && scan_stride_ok(dout_st),
                "selective_scan_bwd: token strides must be below 2^26 elements");
@@ -1091,14 +1102,14 @@ extern "C" int dvae_selective_scan_bwd(const void* u, int64_t u_sb, int64_t u_st
   else { p.leave = after; after += (int64_t)rows * p.nch * N * D; }
   p.part_bc = after;
   p.part_a = after + (int64_t)parts * rows * L * G * 2 * N;
-  DVAE_REQUIRE(rows * p.nch * p.G * parts < (1ll << 31), "selective_scan_bwd: too many rows");
+  const int64_t bc = rows * L * G, bc_groups = ceil_div64(bc * 2 * N, 64 * SUM_WAVES);
+  const int64_t sums = bc_groups + ceil_div64((N + 2) * D, 64);
+  DVAE_REQUIRE(scan_fits(p), "selective_scan_bwd: too many rows for one launch");
+  DVAE_REQUIRE(launch_fits(sums, 64 * SUM_WAVES), "selective_scan_bwd: too many tokens and groups for one launch");
   const int e = dtype == DVAE_DT_F32 ? 4 : 2;
   DVAE_WORK(rows * L * (double)e * ((z ? 7 : 5) * D + 4 * G * N), DVAE_UNIT_BYTE);
   SCAN_DISPATCH(scan_bwd_launch, dtype, p, ST(stream));
   DVAE_LAUNCH_CHECK("selective_scan_bwd");
-  const int64_t bc = rows * L * G, bc_groups = ceil_div64(bc * 2 * N, 64 * SUM_WAVES);
-  const int64_t sums = bc_groups + ceil_div64((N + 2) * D, 64);
-  DVAE_REQUIRE(sums < (1ll << 31), "selective_scan_bwd: too many tokens and groups");
 #define SCAN_SUMS(T)                                                                                                  \
   DVAE_LAUNCH((scan_sums_kernel<T>), dim3((unsigned)sums), dim3(64 * SUM_WAVES), 0, ST(stream), p, (T*)dB, (T*)dC, dA, \
               dD, dbias, bc, parts, (unsigned)bc_groups)
@@ -1127,7 +1138,7 @@ extern "C" int dvae_selective_scan_step(float* state, const void* u, int64_t u_s
   const bool vec = N % 4 == 0 && !((uintptr_t)state & 15) && !((B_sb | B_sg | C_sb | C_sg) & 3) &&
                    !(bc & (dtype == DVAE_DT_F32 ? 15 : 7));
   const int64_t grid = ceil_div64(ceil_div64(rows, many ? 4 : 1) * D * lpc, 256);
-  DVAE_REQUIRE(grid < (1ll << 31), "selective_scan_step: too many rows");
+  DVAE_REQUIRE(launch_fits(grid, 256), "selective_scan_step: too many rows for one launch");
   DVAE_WORK(rows * (double)D * N * 8, DVAE_UNIT_BYTE);
 #define SCAN_STEP(T, LPC, R)                                                                               \
   do {                                                                                                     \

@@ -6,6 +6,11 @@
 
 #define ST(s) ((hipStream_t)(s))
 
+// A launch holds fewer than 2^32 threads.
+static inline bool launch_fits(int64_t groups, int threads) { return groups * threads < (1ll << 32); }
+// Most tokens: positions are int, and those of the last workgroups run past the end by less than this margin.
+#define SEQ_MAX_TOKENS ((1ll << 31) - (1ll << 16))
+
 enum bf16_t : uint16_t {};
 
 __device__ __forceinline__ float to_f32(float v) { return v; }

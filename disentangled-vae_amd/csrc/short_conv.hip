@@ -325,7 +325,7 @@ static int conv_check(const char* what, int64_t rows, int64_t L, int64_t D, int6
   DVAE_REQUIRE(dtype == DVAE_DT_F32 || dtype == DVAE_DT_BF16, "%s: dtype must be fp32 (0) or bf16 (1)", what);
   DVAE_REQUIRE(W >= 2 && W <= 4, "%s: 2 to 4 taps, got %ld", what, (long)W);
   DVAE_REQUIRE(rows >= 0 && L >= 0 && D > 0 && D < (1ll << 24), "%s: bad shape", what);
-  DVAE_REQUIRE(rows < (1ll << 31) && L < (1ll << 31) && rows * L < (1ll << 31) - 64, "%s: too many tokens", what);
+  DVAE_REQUIRE(rows < (1ll << 31) && L < (1ll << 31) && rows * L < SEQ_MAX_TOKENS, "%s: too many tokens", what);
   DVAE_REQUIRE(!offsets || (rows == 1 && S >= 1 && S < (1ll << 30)), "%s: offsets go with one row and S >= 1", what);
   return 0;
 }
@@ -379,7 +379,7 @@ extern "C" int dvae_short_conv_fwd(const void* x, int64_t x_sb, int64_t x_st, co
   p.tiles = (int)ceil_div64(D, 64 * (pairs ? 2 : 1));
   p.tb = conv_tb(p.tokens, p.tiles, 0, 8);
   const int64_t grid = p.tiles * ceil_div64(p.tokens, 4 * p.tb);
-  DVAE_REQUIRE(grid < (1ll << 31), "short_conv_fwd: too large");
+  DVAE_REQUIRE(launch_fits(grid, 256), "short_conv_fwd: too large for one launch");
   const int e = dtype == DVAE_DT_F32 ? 4 : 2;
   DVAE_WORK(2.0 * p.tokens * D * e, DVAE_UNIT_BYTE);
   CONV_DISPATCH(conv_fwd_kernel, dtype, pairs, W, dim3((unsigned)grid), p, ST(stream));
@@ -409,7 +409,8 @@ extern "C" int dvae_short_conv_bwd(const void* x, int64_t x_sb, int64_t x_st, co
   p.tiles = (int)ceil_div64(D, 64 * (pairs ? 2 : 1));
   p.tb = conv_tb(p.tokens, p.tiles, (int)W - 1, 16);
   const int64_t parts = conv_parts(p.tokens, D, pairs ? 2 : 1, (int)W);
-  DVAE_REQUIRE(p.tiles * parts < (1ll << 31), "short_conv_bwd: too large");
+  DVAE_REQUIRE(launch_fits(p.tiles * parts, 256) && (!dstate0 || launch_fits(ceil_div64(D, 256) * p.S, 256)),
+               "short_conv_bwd: too large for one launch");
   const int e = dtype == DVAE_DT_F32 ? 4 : 2;
   DVAE_WORK(3.0 * p.tokens * D * e, DVAE_UNIT_BYTE);
   CONV_DISPATCH(conv_bwd_kernel, dtype, pairs, W, dim3((unsigned)(p.tiles * parts)), p, ST(stream));
@@ -418,7 +419,6 @@ extern "C" int dvae_short_conv_bwd(const void* x, int64_t x_sb, int64_t x_st, co
               dbias, (int)parts, (int)W, (int)D);
   if (dstate0) {
     p.tiles = (int)ceil_div64(D, 256);
-    DVAE_REQUIRE((int64_t)p.tiles * p.S < (1ll << 31), "short_conv_bwd: too many sequences");
     const dim3 grid((unsigned)(p.tiles * p.S));
 #define CONV_DSTATE(T)                                                                     \
   do {                                                                                     \
@@ -442,7 +442,7 @@ extern "C" int dvae_short_conv_step(void* state, const void* x, int64_t x_sb, co
   p.tokens = (int)rows;
   const bool pairs = conv_pairs(D, dtype, x, x_sb, 0, nullptr, 0, 0, state, out, nullptr);
   const int64_t grid = ceil_div64(rows * (D / (pairs ? 2 : 1)), 256);
-  DVAE_REQUIRE(grid < (1ll << 31), "short_conv_step: too large");
+  DVAE_REQUIRE(launch_fits(grid, 256), "short_conv_step: too large for one launch");
   DVAE_WORK((2.0 * W) * rows * D * (dtype == DVAE_DT_F32 ? 4 : 2), DVAE_UNIT_BYTE);
   CONV_DISPATCH(conv_step_kernel, dtype, pairs, W, dim3((unsigned)grid), p, ST(stream));
   DVAE_LAUNCH_CHECK("short_conv_step");

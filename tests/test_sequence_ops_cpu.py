@@ -90,6 +90,26 @@ def test_scan_refuses_before_any_launch(bad, text):
     assert text in _lib().dvae_last_error()
 
 
+@pytest.mark.parametrize('rows,L,D,text', [
+    (1, (1 << 31) - (1 << 16), 1, b'too large'), (1 << 30, 2, 1, b'too large'),            # positions are 32 bits
+    (1 << 24, 1, 64, b'one launch'), (1 << 23, 1, 300, b'one launch'),                     # 2^32 threads are too many
+])
+def test_scan_sizes_that_no_launch_takes(rows, L, D, text):
+    assert _scan_fwd(rows=rows, L=L, D=D, S=rows) != 0
+    assert text in _lib().dvae_last_error()
+
+
+def test_conv_sizes_that_no_launch_takes():
+    lib, n = _lib(), None
+    for rows, L in ((1, (1 << 31) - (1 << 16)), (1 << 30, 2)):
+        assert lib.dvae_short_conv_fwd(n, 0, 0, n, n, 0, n, n, n, n, rows, L, 16, 4, rows, 0, n) != 0
+        assert b'too many tokens' in lib.dvae_last_error()
+    assert lib.dvae_short_conv_step(n, n, 0, n, n, 0, n, 1 << 24, 256, 4, 0, n) != 0
+    assert b'one launch' in lib.dvae_last_error()
+    assert lib.dvae_selective_scan_step(n, n, 0, n, 0, n, n, 0, 0, n, 0, 0, n, n, 0, n, 1, n, 1 << 24, 256, 1, 16, 0, n) != 0
+    assert b'one launch' in lib.dvae_last_error()
+
+
 def test_calls_without_tokens_launch_nothing():
     assert _scan_fwd(rows=0) == 0 and _scan_fwd(L=0) == 0
     lib, n = _lib(), None

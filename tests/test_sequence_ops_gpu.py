@@ -694,6 +694,37 @@ def test_a_state_that_a_step_has_changed_is_refused_by_the_backward_pass(F):
         F.selective_scan_step(i, x[:2], v['delta'][:2], v['A'], v['B'][:2], v['C'][:2])
 
 
+def test_scan_of_more_sequences_than_a_grid_has_rows(F):
+    """70000 sequences of two chunks each, the ones at the ends and on both sides of 65536 against the reference"""
+    n, L, D, N = 70000, 256, 8, 2
+    v = dict(u=torch.randn(n, L, D, device='cuda'), delta=torch.randn(n, L, D, device='cuda') - 1,
+             B=torch.randn(n, L, 1, N, device='cuda'), C=torch.randn(n, L, 1, N, device='cuda'))
+    v = {k: t.requires_grad_() for k, t in v.items()}
+    A = -torch.rand(D, N, device='cuda') - 0.1
+    out, state = F.selective_scan(v['u'], v['delta'], A, v['B'], v['C'], delta_softplus=True, return_state=True)
+    got = dict(zip(v, torch.autograd.grad((out, state), list(v.values()), (torch.ones_like(out), torch.ones_like(state)))))
+    for i in (0, 1, 65535, 65536, n - 1):
+        one = np.ones
+        r, m = (R.scan(f64(v['u'][i]), f64(v['delta'][i]), f64(A), f64(v['B'][i]), f64(v['C'][i]), [0, L], None, None, None,
+                       True, None, one((L, D)), one((1, D, N)), size) for size in (False, True))
+        count = 12 * L + L + D + 64
+        close('out', out[i], r['out'], m['out'], count, U32)
+        close('state', state[i:i + 1], r['state'], m['state'], count, U32)
+        for k, t in got.items():
+            close('d' + k, t[i], r[k], m[k], count, U32)
+
+
+def test_scan_of_one_token_takes_any_token_stride(F):
+    c = ScanCase(16, 4, 1, torch.float32, rows=(3, 1), seed=44)
+    want = c.call(F, c.gpu)
+    odd = lambda t: t.as_strided((3, 1, 16), (16, 1 << 27, 1))                            # noqa: E731
+    v = c.gpu
+    out, state = F.selective_scan(odd(v['u']), odd(v['delta']), v['A'], c.lead(v['B']), c.lead(v['C']), D=v['D'],
+                                  z=odd(v['z']), delta_bias=v['bias'], delta_softplus=True, state=v['state'],
+                                  return_state=True)
+    assert torch.equal(out, want[0]) and torch.equal(state, want[1])
+
+
 def test_results_repeat_bit_for_bit(F):
     c = ScanCase(200, 16, 2, torch.bfloat16, rows=(3, 150), seed=31, state=False)
     runs = []
