@@ -53,6 +53,13 @@ __device__ __forceinline__ float max_abs(float m, float v) {
   return v > m || v != v ? v : m;
 }
 
+// The scale of a row whose largest value is `most`, not below the smallest normal number: a scale of fewer bits would be
+// rounded by so much that the largest value comes out behind the type's end.
+__device__ __forceinline__ float row_scale(float most) {
+  const float s = most / FP8_MAX;
+  return most == 0.f ? 1.f : s < __FLT_MIN__ ? __FLT_MIN__ : s;
+}
+
 template <typename T, typename R>
 __device__ __forceinline__ float rounded_sum(float x, float r) { return to_f32(from_f32<R>(x + r)); }
 
@@ -103,7 +110,7 @@ __global__ void __launch_bounds__(256) norm_row_kernel(NormArgs p) {
     return;
   }
   most = wave_max(most);
-  const float scale = most > 0.f || most != most ? most / FP8_MAX : 1.f;
+  const float scale = row_scale(most);
   if (lane == 0) p.scale[row] = scale;
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
@@ -154,7 +161,7 @@ __global__ void __launch_bounds__(256) norm_any_kernel(NormArgs p) {
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = most;
   __syncthreads();
   most = max_abs(max_abs(max_abs(red[0], red[1]), red[2]), red[3]);
-  const float scale = most > 0.f || most != most ? most / FP8_MAX : 1.f;
+  const float scale = row_scale(most);
   if (threadIdx.x == 0) p.scale[row] = scale;
   for (int d = threadIdx.x; d < p.D; d += 256) {
     const float v = r ? rounded_sum<T, R>(to_f32(x[d]), to_f32(r[d])) : to_f32(x[d]);

@@ -1160,7 +1160,7 @@ def add_rms_norm(x: Tensor, residual: Optional[Tensor], weight: Tensor, eps: flo
 
 def add_rms_norm_q8(x: Tensor, residual: Optional[Tensor], weight: Tensor, eps: float = 1e-6):
     """add_rms_norm with y in 8 bits: -> (q, scale, sum), y = q * scale[..., None] with q of type float8_e4m3fn and
-    scale = max|y| / 448 of its row, so that the row's largest value is the type's largest (a row of zeros: 1).  For
-    inference: no gradients."""
+    scale = max|y| / 448 of its row, so that the row's largest value is the type's largest (a row of zeros: 1; not below
+    2^-126).  For inference: no gradients."""
     _no_grad_form('add_rms_norm_q8', x, residual, weight)
     return ops.add_rms_norm_q8(x, residual, weight, eps)

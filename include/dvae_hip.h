@@ -640,7 +640,8 @@ int dvae_short_conv_step(void* state, const void* x, int64_t x_sb, const float* 
 int dvae_add_rms_norm_fwd(const void* x, int64_t x_st, const void* residual, int64_t r_st, const float* w, float eps,
                           void* y, void* sum, float* rstd, int64_t rows, int64_t D, int dtype, int rdtype,
                           dvae_stream_t stream);
-/* The same with y in 8 bits (e4m3, no infinities): scale[row] = max|y| / 448, or 1 for a row of zeros, q = y / scale. */
+/* The same with y in 8 bits (e4m3, no infinities): scale[row] = max|y| / 448 (2^-126 where that is less), or 1 for a
+ * row of zeros, q = y / scale. */
 int dvae_add_rms_norm_q8(const void* x, int64_t x_st, const void* residual, int64_t r_st, const float* w, float eps,
                          void* q, float* scale, void* sum, int64_t rows, int64_t D, int dtype, int rdtype,
                          dvae_stream_t stream);

@@ -530,6 +530,21 @@ def test_norm_in_8_bits(F, rows, D, dtype, rtype):
         assert not q[1].float().any() and scale[1] == 1
 
 
+@pytest.mark.parametrize('D', [64, 13])
+def test_norm_in_8_bits_of_the_smallest_numbers(F, D):
+    """rows whose largest value, over 448, is below the smallest normal number"""
+    g = gen(D)
+    sizes = 2.0 ** -torch.arange(110, 149).float()
+    x, w = torch.rand(39, D, generator=g) + 0.5, torch.ones(D)
+    for i, s in enumerate(sizes):
+        q, scale, _ = F.add_rms_norm_q8(x[i:i + 1].cuda(), None, (w * s).cuda(), 1e-5)
+        y = R.norm(f64(x[i:i + 1]), f64(w * s), 1e-5)['y']
+        got = f64(q.float()) * f64(scale)[:, None]
+        # half a step of e4m3, relative or of its smallest numbers (2^-10 of the scale); y itself has a step of 2^-149
+        bound = 2.0 ** -4 * np.abs(y) * (1 + 1e-3) + 2.0 ** -10 * f64(scale)[:, None] + 2.0 ** -149
+        assert np.all(np.abs(got - y) <= bound) and scale.item() >= 2.0 ** -126, float(s)
+
+
 def test_norm_rows_with_what_is_not_a_number(F):
     g = gen(9)
     x, w = rnd(g, 4, 256).cuda(), torch.ones(256, device='cuda')
