@@ -293,6 +293,21 @@ static int norm_v(int64_t D, int dtype, int64_t strides, uintptr_t ptrs) {
   return (ptrs & 15) || ((D | strides) & (V - 1)) || D > 4096 ? 0 : V;
 }
 
+// A launch holds fewer than 2^32 threads, so a call of very many rows takes several, of this many rows each.
+static int64_t norm_span(int V) { return V ? 1ll << 25 : 1ll << 23; }
+// the arguments of `n` rows from row r0 on; e, re, ye: bytes per element of x, residual and y
+static NormArgs norm_rows(const NormArgs& p, int64_t r0, int64_t n, int e, int re, int ye) {
+  NormArgs q = p;
+  auto in = [&](const void* a, int64_t st, int size) { return a ? (const char*)a + r0 * st * size : nullptr; };
+  auto out = [&](void* a, int64_t st, int size) { return a ? (char*)a + r0 * st * size : nullptr; };
+  q.x = in(p.x, p.x_st, e); q.res = in(p.res, p.r_st, re); q.dy = in(p.dy, p.dy_st, e); q.dsum = in(p.dsum, p.ds_st, re);
+  q.sum_in = in(p.sum_in, p.s_st, re); q.rstd_in = (const float*)in(p.rstd_in, 1, 4);
+  q.y = out(p.y, p.D, ye); q.sum = out(p.sum, p.D, re); q.dres = out(p.dres, p.D, re); q.dx = out(p.dx, p.D, e);
+  q.rstd = (float*)out(p.rstd, 1, 4); q.scale = (float*)out(p.scale, 1, 4);
+  q.rows = n;
+  return q;
+}
+
 #define NORM_NV(K, T, R, V, nv, ...)                                              \
   do {                                                                            \
     if (nv <= 1) K(T, R, V, 1, __VA_ARGS__);                                      \
@@ -308,13 +323,17 @@ static int norm_v(int64_t D, int dtype, int64_t strides, uintptr_t ptrs) {
     else DO(bf16_t, float, 8);                                                    \
   } while (0)
 
-static int norm_fwd(const char* what, bool q8, NormArgs& p, int dtype, int rdtype, hipStream_t s) {
-  if (p.rows == 0) return 0;
-  const int V = norm_v(p.D, dtype, p.x_st | (p.res ? p.r_st : 0),
-                       (uintptr_t)p.x | (uintptr_t)p.res | (uintptr_t)p.w | (uintptr_t)p.y | (uintptr_t)p.sum);
-  const dim3 grid((unsigned)(V ? ceil_div64(p.rows, 4) : p.rows));
-  const int nv = V ? (int)ceil_div64(p.D, 64 * V) : 0;
-  DVAE_WORK((double)p.rows * p.D * (dtype == DVAE_DT_F32 ? 4 : 2) * (p.res ? 4 : 2), DVAE_UNIT_BYTE);
+static int norm_fwd(const char* what, bool q8, const NormArgs& all, int dtype, int rdtype, hipStream_t s) {
+  if (all.rows == 0) return 0;
+  const int V = norm_v(all.D, dtype, all.x_st | (all.res ? all.r_st : 0),
+                       (uintptr_t)all.x | (uintptr_t)all.res | (uintptr_t)all.w | (uintptr_t)all.y | (uintptr_t)all.sum);
+  const int nv = V ? (int)ceil_div64(all.D, 64 * V) : 0;
+  const int e = dtype == DVAE_DT_F32 ? 4 : 2, re = rdtype == DVAE_DT_F32 ? 4 : 2;
+  const int64_t span = norm_span(V);
+  for (int64_t r0 = 0; r0 < all.rows; r0 += span) {
+    const NormArgs p = norm_rows(all, r0, all.rows - r0 < span ? all.rows - r0 : span, e, re, q8 ? 1 : e);
+    const dim3 grid((unsigned)(V ? ceil_div64(p.rows, 4) : p.rows));
+    DVAE_WORK((double)p.rows * p.D * e * (p.res ? 4 : 2), DVAE_UNIT_BYTE);
 #define NORM_ROW(T, R, V, NV, q) DVAE_LAUNCH((norm_row_kernel<T, R, V, NV, q>), grid, dim3(256), 0, s, p)
 #define NORM_FWD(T, R, VV)                                                              \
   do {                                                                                  \
@@ -323,7 +342,8 @@ static int norm_fwd(const char* what, bool q8, NormArgs& p, int dtype, int rdtyp
     else if (q8) DVAE_LAUNCH((norm_any_kernel<T, R, true>), grid, dim3(256), 0, s, p);  \
     else DVAE_LAUNCH((norm_any_kernel<T, R, false>), grid, dim3(256), 0, s, p);         \
   } while (0)
-  NORM_TYPES(NORM_FWD);
+    NORM_TYPES(NORM_FWD);
+  }
   DVAE_LAUNCH_CHECK(what);
   return 0;
 }
@@ -380,13 +400,18 @@ extern "C" int dvae_add_rms_norm_bwd(const void* dy, int64_t dy_st, const void* 
   } else {
     const int tiles = (int)ceil_div64(D, 256);
     parts = ceil_div64(rows, NORM_DW_ROWS);
-    DVAE_REQUIRE(parts * tiles < (1ll << 31), "add_rms_norm_bwd: too large");
-#define NORM_BWD_ANY(T, R, VV)                                                                             \
-  do {                                                                                                     \
-    DVAE_LAUNCH((norm_bwd_any_kernel<T, R>), dim3((unsigned)rows), dim3(256), 0, s, p);                    \
-    DVAE_LAUNCH((norm_dw_any_kernel<T, R>), dim3((unsigned)(parts * tiles)), dim3(256), 0, s, p, tiles);   \
-  } while (0)
-    NORM_TYPES(NORM_BWD_ANY);
+    DVAE_REQUIRE(launch_fits(parts * tiles, 256), "add_rms_norm_bwd: too large for one launch");
+#define NORM_BWD_ANY(T, R, VV) \
+  DVAE_LAUNCH((norm_bwd_any_kernel<T, R>), dim3((unsigned)q.rows), dim3(256), 0, s, q)
+#define NORM_DW_ANY(T, R, VV) \
+  DVAE_LAUNCH((norm_dw_any_kernel<T, R>), dim3((unsigned)(parts * tiles)), dim3(256), 0, s, p, tiles)
+    const int e = dtype == DVAE_DT_F32 ? 4 : 2, re = rdtype == DVAE_DT_F32 ? 4 : 2;
+    const int64_t span = norm_span(0);
+    for (int64_t r0 = 0; r0 < rows; r0 += span) {
+      const NormArgs q = norm_rows(p, r0, rows - r0 < span ? rows - r0 : span, e, re, e);
+      NORM_TYPES(NORM_BWD_ANY);
+    }
+    NORM_TYPES(NORM_DW_ANY);
   }
   DVAE_LAUNCH(norm_dw_sum_kernel, dim3((unsigned)ceil_div64(D, 64)), dim3(64 * SUM_WAVES), 0, s, ws, dw, parts, (int)D);
   DVAE_LAUNCH_CHECK("add_rms_norm_bwd");

@@ -530,6 +530,31 @@ def test_norm_in_8_bits(F, rows, D, dtype, rtype):
         assert not q[1].float().any() and scale[1] == 1
 
 
+@pytest.mark.parametrize('rows,D', [((1 << 23) + 5, 3), ((1 << 25) + 6, 4)])
+def test_norm_of_more_rows_than_one_launch_takes(F, rows, D):
+    """the last rows, and those on both sides of the border between launches, as they are alone; dw against 64 bits"""
+    x, w = torch.randn(rows, D, device='cuda').requires_grad_(), (torch.rand(D, device='cuda') + 0.5).requires_grad_()
+    r = torch.randn(rows, D, device='cuda')
+    border = 1 << rows.bit_length() - 1
+    pick = torch.cat([torch.arange(9), torch.arange(border - 4, rows)]).cuda()
+    y, s = F.add_rms_norm(x, r, w)
+    dy = torch.randn(rows, D, device='cuda')
+    dx, dw = torch.autograd.grad((y, s), (x, w), (dy, dy))
+    x1 = x.detach()[pick].requires_grad_()
+    y1, s1 = F.add_rms_norm(x1, r[pick], w)
+    (dx1,) = torch.autograd.grad((y1, s1), (x1,), (dy[pick], dy[pick]))
+    assert torch.equal(y[pick], y1) and torch.equal(s[pick], s1) and torch.equal(dx[pick], dx1)
+    v = s.detach().double()
+    terms = dy.double() * v * torch.rsqrt((v * v).mean(1, keepdim=True) + 1e-6)
+    # D + 16 roundings per term; a term is then added at most rows / 2048 times within a wave (or 64 times, and to less than
+    # rows / 8192 partial sums before its own), and the partial sums of that less than a thousand times more
+    count = D + 16 + rows // 2048 + 4096
+    assert ((dw.double() - terms.sum(0)).abs() <= count * U32 * terms.abs().sum(0)).all()
+    q, scale, _ = F.add_rms_norm_q8(x.detach(), r, w.detach())
+    q1, scale1, _ = F.add_rms_norm_q8(x1.detach(), r[pick], w.detach())
+    assert torch.equal(q[pick].view(torch.uint8), q1.view(torch.uint8)) and torch.equal(scale[pick], scale1)
+
+
 @pytest.mark.parametrize('D', [64, 13])
 def test_norm_in_8_bits_of_the_smallest_numbers(F, D):
     """rows whose largest value, over 448, is below the smallest normal number"""
