@@ -1026,8 +1026,7 @@ class SelectiveScan(torch.autograd.Function):
         if dout is None:
             dout = torch.zeros(a.shape, dtype=a.act, device=a.device)
         need = ctx.needs_input_grad
-        du, dd, dA, dB, dC, dD, dz, db, ds = ops.selective_scan_bwd(a, dout, dfinal, ckpt, need[9])
-        del keep
+        du, dd, dA, dB, dC, dD, dz, db, ds = ops.selective_scan_bwd(a, keep, dout, dfinal, ckpt, need[9])
         if b_shape != a.bc_shape:
             dB = dB.view(b_shape)
         if c_shape != a.bc_shape:
@@ -1095,8 +1094,7 @@ class ShortConv(torch.autograd.Function):
         if dout is None:
             dout = torch.zeros(a.shape, dtype=a.act, device=a.device)
         need = ctx.needs_input_grad
-        dx, dw, db, ds = ops.short_conv_bwd(a, dout, dfinal, need[4])
-        del keep
+        dx, dw, db, ds = ops.short_conv_bwd(a, keep, dout, dfinal, need[4])
         return tuple(g if n else None for g, n in zip((dx, dw, db, None, ds), need)) + (None, None)
 
 

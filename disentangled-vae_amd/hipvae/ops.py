@@ -1064,6 +1064,11 @@ _stream_of = torch._C._cuda_getCurrentRawStream      # raw handle of a device's 
 _written = torch._C._increment_version               # tells autograd that tensors have been changed in place
 
 
+def _new_like(t: Tensor) -> Tensor:
+    """contiguous, uninitialised (half the time of torch.empty with a shape, a type and a device: 1.1 against 2.1 us)"""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _act_dtype(what: str, t: Tensor) -> int:
     code = _ACT_DTYPES.get(t.dtype)
     if code is None or not t.is_cuda:
@@ -1202,7 +1207,7 @@ class ScanArgs(_KeptArgs):
 def _final_states(shape, dtype, device, entering: Optional[Tensor], packed: bool, tokens: int) -> Tensor:
     """where final states go.  Sequences without tokens are not written: they keep what they entered with."""
     if tokens > 0 and not packed:
-        return torch.empty(shape, dtype=dtype, device=device)
+        return torch.empty(shape, dtype=dtype, device=device) if entering is None else _new_like(entering)
     return torch.zeros(shape, dtype=dtype, device=device) if entering is None else entering.clone()
 
 
@@ -1212,7 +1217,7 @@ def selective_scan_fwd(a: ScanArgs, want_state: bool, keep: bool):
     if a.index != _device_now():
         with torch.cuda.device(dev):
             return selective_scan_fwd(a, want_state, keep)
-    out = torch.empty(a.shape, dtype=a.act, device=dev)
+    out = _new_like(a.tensors[0])
     final = _final_states(a.state_shape, torch.float32, dev, a.tensors[8], a.packed, a.tokens) if want_state else None
     rows, L, ch, G, N = a.sizes
     ckpt = torch.empty(lib.dvae_selective_scan_ckpt_floats(rows, L, ch, N), dtype=torch.float32,
@@ -1224,26 +1229,22 @@ def selective_scan_fwd(a: ScanArgs, want_state: bool, keep: bool):
     return out, final, ckpt
 
 
-def selective_scan_bwd(a: ScanArgs, dout: Tensor, dfinal: Optional[Tensor], ckpt: Tensor, want_dstate: bool):
-    """-> du, ddelta, dA, dB, dC, dD, dz, ddelta_bias, dstate (None where there is no such input)"""
+def selective_scan_bwd(a: ScanArgs, tensors, dout: Tensor, dfinal: Optional[Tensor], ckpt: Tensor, want_dstate: bool):
+    """`tensors`: those of a -> du, ddelta, dA, dB, dC, dD, dz, ddelta_bias, dstate (None where there is no such input)"""
     what = 'selective_scan_bwd'
     dev = a.device
     if a.index != _device_now():
         with torch.cuda.device(dev):
-            return selective_scan_bwd(a, dout, dfinal, ckpt, want_dstate)
+            return selective_scan_bwd(a, tensors, dout, dfinal, ckpt, want_dstate)
     dout = _act(what, 'dout', dout, a.shape, a.act, a.index)
     dfinal = _param(what, 'dstate', dfinal, a.state_shape, a.index)
     f32 = torch.float32
-    du = torch.empty(a.shape, dtype=a.act, device=dev)
-    dd = torch.empty(a.shape, dtype=a.act, device=dev)
-    dz = torch.empty(a.shape, dtype=a.act, device=dev) if a.has_z else None
-    dB = torch.empty(a.bc_shape, dtype=a.act, device=dev)
-    dC = torch.empty(a.bc_shape, dtype=a.act, device=dev)
+    _, _, A, B, C, D, _, bias, *_ = tensors
+    du, dd, dz = _new_like(dout), _new_like(dout), _new_like(dout) if a.has_z else None
+    dB, dC = _new_like(B), _new_like(C)
     rows, L, ch, G, N = a.sizes
-    new = torch.empty if a.tokens else torch.zeros
-    dA = new((ch, N), dtype=f32, device=dev)
-    dD = new(ch, dtype=f32, device=dev) if a.has_D else None
-    db = new(ch, dtype=f32, device=dev) if a.has_bias else None
+    new = _new_like if a.tokens else torch.zeros_like
+    dA, dD, db = new(A), new(D) if a.has_D else None, new(bias) if a.has_bias else None
     ds = _final_states(a.state_shape, f32, dev, dfinal, a.packed, a.tokens) if want_dstate else None
     if a.tokens:
         ws = torch.empty(lib.dvae_selective_scan_bwd_ws_floats(rows, L, ch, G, N), dtype=f32, device=dev)
@@ -1277,7 +1278,7 @@ def selective_scan_step(state, u, delta, A, B, C, D=None, z=None, delta_bias=Non
     A = _param(what, 'A', A, (ch, N), dev)
     D = _param(what, 'D', D, (ch,), dev)
     delta_bias = _param(what, 'delta_bias', delta_bias, (ch,), dev)
-    out = torch.empty(shape, dtype=dt, device=u.device)
+    out = _new_like(u)
     check(lib.dvae_selective_scan_step(state.data_ptr(), u.data_ptr(), u.stride(0), delta.data_ptr(), delta.stride(0),
                                        A.data_ptr(), B.data_ptr(), B.stride(0), B.stride(1), C.data_ptr(), C.stride(0),
                                        C.stride(1), _p(D), _p(z), 0 if z is None else z.stride(0), _p(delta_bias),
@@ -1321,27 +1322,25 @@ def short_conv_fwd(a: ConvArgs, want_state: bool):
     if a.index != _device_now():
         with torch.cuda.device(dev):
             return short_conv_fwd(a, want_state)
-    out = torch.empty(a.shape, dtype=a.act, device=dev)
+    out = _new_like(a.tensors[0])
     final = _final_states(a.state_shape, a.act, dev, a.tensors[3], a.packed, a.tokens) if want_state else None
     check(lib.dvae_short_conv_fwd(*a.head, _p(final), a.offsets_ptr, out.data_ptr(), *a.tail, _stream_of(dev.index)),
           'short_conv_fwd')
     return out, final
 
 
-def short_conv_bwd(a: ConvArgs, dout: Tensor, dfinal: Optional[Tensor], want_dstate: bool):
-    """-> dx, dweight, dbias, dstate"""
+def short_conv_bwd(a: ConvArgs, tensors, dout: Tensor, dfinal: Optional[Tensor], want_dstate: bool):
+    """`tensors`: those of a -> dx, dweight, dbias, dstate"""
     what = 'short_conv_bwd'
     dev = a.device
     if a.index != _device_now():
         with torch.cuda.device(dev):
-            return short_conv_bwd(a, dout, dfinal, want_dstate)
+            return short_conv_bwd(a, tensors, dout, dfinal, want_dstate)
     dout = _act(what, 'dout', dout, a.shape, a.act, a.index)
     dfinal = _param(what, 'dstate', dfinal, a.state_shape, a.index, a.act)
     rows, L, ch, W = a.sizes
-    dx = torch.empty(a.shape, dtype=a.act, device=dev)
-    new = torch.empty if a.tokens else torch.zeros
-    dw = new((ch, W), dtype=torch.float32, device=dev)
-    db = new(ch, dtype=torch.float32, device=dev) if a.has_bias else None
+    new = _new_like if a.tokens else torch.zeros_like
+    dx, dw, db = _new_like(dout), new(tensors[1]), new(tensors[2]) if a.has_bias else None
     ds = _final_states(a.state_shape, a.act, dev, dfinal, a.packed, a.tokens) if want_dstate else None
     if a.tokens:
         ws = torch.empty(lib.dvae_short_conv_bwd_ws_floats(rows, L, ch, W), dtype=torch.float32, device=dev)
@@ -1369,7 +1368,7 @@ def short_conv_step(state, x, weight, bias=None, silu=False) -> Tensor:
     x = _act(what, 'x', x, shape, dt, dev)
     weight = _param(what, 'weight', weight, (ch, W), dev)
     bias = _param(what, 'bias', bias, (ch,), dev)
-    out = torch.empty(shape, dtype=dt, device=x.device)
+    out = _new_like(x)
     check(lib.dvae_short_conv_step(state.data_ptr(), x.data_ptr(), x.stride(0), weight.data_ptr(), _p(bias),
                                    1 if silu else 0, out.data_ptr(), rows, ch, W, code, _stream_of(dev)), what)
     _written((state,))
@@ -1392,12 +1391,14 @@ class NormArgs:
         if len(shape) < 1 or shape[-1] < 1:
             raise RuntimeError(f"{what}: expected [..., channels], got {tuple(shape)}")
         self.D = shape[-1]
+        self.like = x
         self.x = _norm_rows(what, 'x', x, shape, dt, dev)
         self.rows = self.x.shape[0]
         self.sum_dtype, self.rdtype, self.residual = dt, self.dtype, None
         if residual is not None:
             if residual.dtype is torch.float32:         # x's type, or fp32
                 self.sum_dtype, self.rdtype = torch.float32, 0
+            self.sum_like = residual
             self.residual = _norm_rows(what, 'residual', residual, shape, self.sum_dtype, dev)
         self.weight = _param(what, 'weight', weight, (self.D,), dev)
 
@@ -1413,8 +1414,8 @@ def add_rms_norm_fwd(a: NormArgs, eps: float, keep: bool):
     if a.index != _device_now():
         with torch.cuda.device(dev):
             return add_rms_norm_fwd(a, eps, keep)
-    y = torch.empty(a.shape, dtype=a.act, device=dev)
-    total = None if a.residual is None else torch.empty(a.shape, dtype=a.sum_dtype, device=dev)
+    y = _new_like(a.like)
+    total = None if a.residual is None else _new_like(a.sum_like)
     rstd = torch.empty(a.rows, dtype=torch.float32, device=dev) if keep else None
     check(lib.dvae_add_rms_norm_fwd(*a.head(eps), y.data_ptr(), _p(total), _p(rstd), a.rows, a.D, a.dtype, a.rdtype,
                                     _stream_of(a.index)), 'add_rms_norm_fwd')
@@ -1431,7 +1432,7 @@ def add_rms_norm_q8(x: Tensor, residual: Optional[Tensor], weight: Tensor, eps: 
             return add_rms_norm_q8(x, residual, weight, eps)
     q = torch.empty(a.shape, dtype=torch.float8_e4m3fn, device=dev)
     scale = torch.empty(a.shape[:-1], dtype=torch.float32, device=dev)
-    total = None if a.residual is None else torch.empty(a.shape, dtype=a.sum_dtype, device=dev)
+    total = None if a.residual is None else _new_like(a.sum_like)
     check(lib.dvae_add_rms_norm_q8(*a.head(eps), q.data_ptr(), scale.data_ptr(), _p(total), a.rows, a.D, a.dtype, a.rdtype,
                                    _stream_of(dev.index)), 'add_rms_norm_q8')
     return q, scale, x if total is None else total
@@ -1451,11 +1452,11 @@ def add_rms_norm_bwd(dy: Tensor, dsum: Optional[Tensor], total: Tensor, weight: 
     ds2 = _norm_rows(what, 'dsum', dsum, shape, total.dtype, dev.index)
     s2 = _norm_rows(what, 'sum', total, shape, total.dtype, dev.index)
     rows = dy2.shape[0]
-    dres = torch.empty(shape, dtype=total.dtype, device=dev)
-    dx = dres if total.dtype == dx_dtype else torch.empty(shape, dtype=dx_dtype, device=dev)
+    dres = _new_like(total)
+    dx = dres if total.dtype == dx_dtype else _new_like(dy)
     if rows == 0:
-        return dx, dres, torch.zeros(D, dtype=torch.float32, device=dev)
-    dw = torch.empty(D, dtype=torch.float32, device=dev)
+        return dx, dres, torch.zeros_like(weight)
+    dw = _new_like(weight)
     ws = torch.empty(lib.dvae_add_rms_norm_bwd_ws_floats(rows, D), dtype=torch.float32, device=dev)
     check(lib.dvae_add_rms_norm_bwd(_p(dy2), dy2.stride(0), _p(ds2), 0 if ds2 is None else ds2.stride(0), _p(s2),
                                     s2.stride(0), _p(weight), _p(rstd), _p(dres), _p(dx), _p(dw), rows, D,
