@@ -132,6 +132,16 @@ template <typename T, int NP> struct BCAhead<T, NP, false> {
   }
 };
 
+// Asks for one element of each end of B's and C's rows of a block of n tokens (four lanes alike), so that the lines are in
+// the L2 when the scalar unit asks for them a token ahead: from there that is time enough, from memory it is not.
+template <typename T>
+__device__ __forceinline__ T touch_rows(const T* B, int64_t b_st, const T* C, int64_t c_st, int n, int N, int lane) {
+  const int j = min(lane & 7, n - 1);
+  return (lane & 8 ? C + j * c_st : B + j * b_st)[lane & 16 ? N - 1 : 0];
+}
+__device__ __forceinline__ void touched(float v) { asm volatile("" :: "v"(v)); }
+__device__ __forceinline__ void touched(bf16_t v) { asm volatile("" :: "v"((uint32_t)v)); }
+
 // 64 channels of one group, one chunk of one row.  A workgroup's tiles are neighbours in a group; a tile is the work of
 // one wave, or of `share` waves that have a part of the states each.
 struct Tile {
@@ -222,17 +232,22 @@ template <typename T> __device__ __forceinline__ void lane_store(T* row, uint32_
   *(DVAE_GLOBAL T*)((DVAE_GLOBAL char*)r + at) = v;
 }
 
-// FULL: all NP states exist, else the first N
+// The states of a slot, FULL: all NP of them, else the first N.  One scalar address and running offsets, computed anew at
+// every call: addresses of their own are kept from block to block, in registers that the states need.
 template <int NP, bool FULL>
 __device__ __forceinline__ void load_slot(const float* slot, const ScanArgs& p, int d, float (&h)[NP], int N) {
+  uint32_t at = d * 4u;
+  asm volatile("" : "+v"(at));
 #pragma unroll
-  for (int n = 0; n < NP; ++n) h[n] = FULL || n < N ? lane_load(slot + (int64_t)n * p.D, d * 4u) : 0.f;
+  for (int n = 0; n < NP; ++n, at += p.D * 4u) h[n] = FULL || n < N ? lane_load(slot, at) : 0.f;
 }
 template <int NP, bool FULL>
 __device__ __forceinline__ void store_slot(float* slot, const ScanArgs& p, int d, const float (&h)[NP], int N) {
+  uint32_t at = d * 4u;
+  asm volatile("" : "+v"(at));
 #pragma unroll
-  for (int n = 0; n < NP; ++n)
-    if (FULL || n < N) lane_store(slot + (int64_t)n * p.D, d * 4u, h[n]);
+  for (int n = 0; n < NP; ++n, at += p.D * 4u)
+    if (FULL || n < N) lane_store(slot, at, h[n]);
 }
 __device__ __forceinline__ float* enter_slot(const ScanArgs& p, int row, int chunk) {
   return p.enter + ((int64_t)row * p.enter_row + (int64_t)chunk * p.enter_step) * p.N * p.D;
@@ -246,10 +261,11 @@ __device__ __forceinline__ float* leave_slot(const ScanArgs& p, int row, int chu
 // address each, requested together, spilled a hundred scalar registers).
 template <typename T> struct Rows {
   const T* base;       // row of the block's first token
-  int64_t block;       // elements from block to block
   uint32_t step;       // bytes from token to token (the host checked that a block's rows span less than 2 GiB)
   __device__ __forceinline__ Rows(const void* p, int64_t sb, int64_t st, int row, int t0)
-      : base((const T*)p + row * sb + t0 * st), block(st * SCAN_Q), step((uint32_t)st * (uint32_t)sizeof(T)) {}
+      : base((const T*)p + row * sb + t0 * st), step((uint32_t)st * (uint32_t)sizeof(T)) {}
+  __device__ __forceinline__ void next() { base = (const T*)((const char*)base + step * SCAN_Q); }
+  __device__ __forceinline__ void prev() { base = (const T*)((const char*)base - step * SCAN_Q); }
   // K tokens of the block from the j0-th on; those past the n-th are the n-th again
   template <int K> __device__ __forceinline__ void load(T (&v)[K], int n, uint32_t at, int j0 = 0) const {
     uint64_t r = (uint64_t)base;
@@ -303,16 +319,22 @@ __global__ void __launch_bounds__(256) scan_fwd_kernel(ScanArgs p) {
   if (PACKED) q.seek(w.t0);
   float total = 0.f;
   bool cut = false;
+  T bc = {};
   for (int t0 = w.t0; t0 < w.t1; t0 += SCAN_Q) {
     const int n = min(SCAN_Q, w.t1 - t0);
+    if (!STATE_ONLY) touched(bc);
     T ub[SCAN_Q], pb[SCAN_Q], zb[SCAN_Q];
 #pragma unroll
     for (int j = 0; j < SCAN_Q; ++j) { ub[j] = un[j]; pb[j] = dn[j]; if (!STATE_ONLY) zb[j] = zn[j]; }
     const int left = w.t1 - t0 - SCAN_Q;
-    if (left > 0) { ur.base += ur.block; dr.base += dr.block; zr.base += zr.block; }
+    if (left > 0) { ur.next(); dr.next(); zr.next(); }
     ur.load(un, left, at);                         // (the same block again where it was the last)
     dr.load(dn, left, at);
     if (!STATE_ONLY) zr.load(zn, left, at);
+    if (!STATE_ONLY && left > 0) {
+      const int64_t t = t0 + SCAN_Q;
+      bc = touch_rows(B + t * p.B_st, p.B_st, C + t * p.C_st, p.C_st, left, p.N, w.lane);
+    }
     if (!STATE_ONLY && p.ckpt)
       store_slot<NP, FAST>(p.ckpt + ((int64_t)row * p.blocks + t0 / SCAN_Q) * p.N * p.D, p, w.d, h, p.N);
     Marks m = {0u, 0u, 0u};
@@ -522,7 +544,7 @@ __global__ void __launch_bounds__(256) scan_bwd_state_kernel(ScanArgs p) {
 #pragma unroll
     for (int j = 0; j < SCAN_Q; ++j) { pb[j] = dn[j]; zb[j] = zn[j]; gb[j] = gn[j]; }
     const int left = w.t1 - t0 - SCAN_Q;
-    if (left > 0) { dr.base += dr.block; zr.base += zr.block; gr.base += gr.block; }
+    if (left > 0) { dr.next(); zr.next(); gr.next(); }
     dr.load(dn, left, at);
     zr.load(zn, left, at);
     gr.load(gn, left, at);
@@ -623,7 +645,7 @@ __global__ void __launch_bounds__(64 * SCAN_BT * (NP / SCAN_NW), 2) scan_bwd_ker
   Rows<T> gr(p.dout, p.dout_sb, p.dout_st, row, first);
   // (without z, dout is read in its place and not used)
   Rows<T> zr(gated ? p.z : p.dout, gated ? p.z_sb : p.dout_sb, gated ? p.z_st : p.dout_st, row, first);
-  T un[OWN], dn[OWN], zn[OWN], gn[OWN];               // this wave's tokens of the block ahead,
+  T un[OWN], dn[OWN], zn[OWN], gn[OWN], bc = {};      // this wave's tokens of the block ahead,
   float hn[SCAN_NW];                                  // and the state that enters it
   ur.load(un, w.t1 - first, at, j0);
   dr.load(dn, w.t1 - first, at, j0);
@@ -633,6 +655,7 @@ __global__ void __launch_bounds__(64 * SCAN_BT * (NP / SCAN_NW), 2) scan_bwd_ker
 
   for (int t0 = first; t0 >= w.t0; t0 -= SCAN_Q) {
     const int n = min(SCAN_Q, w.t1 - t0);
+    touched(bc);
     float hs[SCAN_Q + 1][SCAN_NW];
     float dt_[OWN], slope[OWN], u_[OWN], z_[OWN], g_[OWN];      // of this wave's tokens
 #pragma unroll
@@ -647,9 +670,11 @@ __global__ void __launch_bounds__(64 * SCAN_BT * (NP / SCAN_NW), 2) scan_bwd_ker
     auto request = [&]() {
       if (t0 > w.t0) {
         ck -= (int64_t)p.N * p.D;
-        ur.base -= ur.block; dr.base -= dr.block; zr.base -= zr.block; gr.base -= gr.block;
+        ur.prev(); dr.prev(); zr.prev(); gr.prev();
       }
       const int left = t0 > w.t0 ? SCAN_Q : n;
+      const int64_t t = t0 > w.t0 ? t0 - SCAN_Q : t0;
+      bc = touch_rows(B + t * p.B_st, p.B_st, C + t * p.C_st, p.C_st, left, Nw, w.lane);
       ur.load(un, left, at, j0);
       dr.load(dn, left, at, j0);
       zr.load(zn, left, at, j0);
@@ -766,7 +791,9 @@ __global__ void __launch_bounds__(64 * SCAN_BT * (NP / SCAN_NW), 2) scan_bwd_ker
       __builtin_amdgcn_sched_barrier(0);
     }
     __syncthreads();
-    int64_t o = (flat + t0 + j0) * p.D;
+    const int64_t o = (flat + t0 + j0) * p.D;
+    uint32_t to = at;
+    asm volatile("" : "+v"(to));
 #pragma unroll
     for (int jj = 0; jj < OWN; ++jj) {
       const int j = j0 + jj;
@@ -789,19 +816,20 @@ __global__ void __launch_bounds__(64 * SCAN_BT * (NP / SCAN_NW), 2) scan_bwd_ker
           dbias += dd;
         }
         if (w.on && !idle) {
-          if (gated) lane_store((T*)p.dz + o, at, from_f32<T>(dz));
-          lane_store((T*)p.du + o, at, from_f32<T>(du));
-          lane_store((T*)p.ddelta + o, at, from_f32<T>(dd));
+          if (gated) lane_store((T*)p.dz + o, to, from_f32<T>(dz));
+          lane_store((T*)p.du + o, to, from_f32<T>(du));
+          lane_store((T*)p.ddelta + o, to, from_f32<T>(dd));
         }
       }
-      o += p.D;
+      to += (uint32_t)p.D * (uint32_t)sizeof(T);
     }
-    for (int i = threadIdx.x; i < n * 2 * p.N; i += 64 * SCAN_BT * SHARE) {
-      const int j = i / (2 * p.N), c = i % (2 * p.N), k = c < p.N ? c : c - p.N + NP;
+    const int N = FAST ? NP : p.N;
+    for (int i = threadIdx.x; i < n * 2 * N; i += 64 * SCAN_BT * SHARE) {
+      const int j = i / (2 * N), c = i % (2 * N), k = c < N ? c : c - N + NP;
       float s = red[j][0][k];
 #pragma unroll
       for (int t = 1; t < SCAN_BT; ++t) s += red[j][t][k];
-      p.part_bc[(((int64_t)w.part * p.rows * p.L + flat + t0 + j) * p.G + w.g) * 2 * p.N + c] = s;
+      p.part_bc[(((int64_t)w.part * p.rows * p.L + flat + t0 + j) * p.G + w.g) * 2 * N + c] = s;
     }
   }
   if (!PACKED && w.chunk == 0 && p.dstate0 && w.on && !idle) store_state<SCAN_NW, FAST>(p.dstate0, row, p, w.d, dh, n0);

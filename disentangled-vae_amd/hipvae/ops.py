@@ -1131,7 +1131,8 @@ def _st2(t: Optional[Tensor]):
     """(sequence, token) strides of an activation in either form"""
     if t is None:
         return 0, 0
-    return (t.stride(0), t.stride(1)) if t.dim() == 3 else (0, t.stride(0))
+    s = t.stride()
+    return s[:2] if len(s) == 3 else (0, s[0])
 
 
 def _bc_form(what: str, B: Tensor, C: Tensor, lead, channels: int, N: int, dtype, device: int):
@@ -1149,7 +1150,8 @@ def _bc_form(what: str, B: Tensor, C: Tensor, lead, channels: int, N: int, dtype
 
 
 def _st3(t: Tensor):
-    return (t.stride(0), t.stride(1), t.stride(2)) if t.dim() == 4 else (0, t.stride(0), t.stride(1))
+    s = t.stride()
+    return s[:3] if len(s) == 4 else (0, s[0], s[1])
 
 
 def _places(tensors):
