@@ -314,6 +314,12 @@ __global__ void __launch_bounds__(256) scan_fwd_kernel(ScanArgs p) {
   const float Dp = p.Dp ? p.Dp[w.d] : 0.f, bias = p.bias ? p.bias[w.d] : 0.f;
   const T* B = (const T*)p.B + row * p.B_sb + w.g * p.B_sg;
   const T* C = (const T*)p.C + row * p.C_sb + w.g * p.C_sg;
+  const T *Bt = B + w.t0 * p.B_st, *Ct = C + w.t0 * p.C_st;      // the token ahead
+  // A block's first token is requested by the block before it, but not where B and C of two tokens are 64 scalar registers
+  // (8 x 2048 x 2048 fp32, outputs: 199 us with it, 184 without; bf16, 1 x 4096: 43 and 45 us).
+  constexpr bool CARRY = STATE_ONLY || sizeof(T) * NP < 64;
+  if (STATE_ONLY) ahead.request_b(Bt, p.N);
+  else if (CARRY) ahead.request(Bt, Ct, p.N);
   T* out = (T*)p.out + (int64_t)row * p.L * p.D;
   SeqWalk q = {p.offsets, p.S, p.L, p.L, row, 0, p.L};
   if (PACKED) q.seek(w.t0);
@@ -339,25 +345,23 @@ __global__ void __launch_bounds__(256) scan_fwd_kernel(ScanArgs p) {
       store_slot<NP, FAST>(p.ckpt + ((int64_t)row * p.blocks + t0 / SCAN_Q) * p.N * p.D, p, w.d, h, p.N);
     Marks m = {0u, 0u, 0u};
     if (PACKED) m = block_marks(q, t0, n);
-    const T *Bt = B + t0 * p.B_st, *Ct = C + t0 * p.C_st;
     T* ot = out + (int64_t)t0 * p.D;
-    if (STATE_ONLY) ahead.request_b(Bt, p.N);
-    else ahead.request(Bt, Ct, p.N);
+    if (!CARRY) ahead.request(Bt, Ct, p.N);
 #pragma unroll
     for (int j = 0; j < SCAN_Q; ++j) {
       if (PACKED && j >= n) continue;
       const bool there = PACKED || j < n;
       BCAhead<T, NP, FAST> now = ahead;
       float Bv[NP], Cv[NP];
-      Bt += j + 1 < n ? p.B_st : 0;
-      Ct += j + 1 < n ? p.C_st : 0;
+      Bt += t0 + j + 1 < w.t1 ? p.B_st : 0;        // (the chunk's last token is requested again)
+      Ct += t0 + j + 1 < w.t1 ? p.C_st : 0;
       if (STATE_ONLY) {
         now.arrived_b(Bt);
-        if (j + 1 < SCAN_Q) ahead.request_b(Bt, p.N);
+        ahead.request_b(Bt, p.N);
         now.get_b(Bv);
       } else {
         now.arrived(Bt, Ct);
-        if (j + 1 < SCAN_Q) ahead.request(Bt, Ct, p.N);
+        if (CARRY || j + 1 < SCAN_Q) ahead.request(Bt, Ct, p.N);
         now.get(Bv, Cv);
       }
       if (PACKED && !(m.valid >> j & 1)) {
@@ -535,6 +539,9 @@ __global__ void __launch_bounds__(256) scan_bwd_state_kernel(ScanArgs p) {
   Rows<T> dr(p.delta, p.delta_sb, p.delta_st, row, w.t0), gr(p.dout, p.dout_sb, p.dout_st, row, w.t0);
   Rows<T> zr(gated ? p.z : p.dout, gated ? p.z_sb : p.dout_sb, gated ? p.z_st : p.dout_st, row, w.t0);
   T dn[SCAN_Q], zn[SCAN_Q], gn[SCAN_Q];            // the block ahead
+  BCAhead<T, NP, FAST> ahead;
+  const T* Ct = C + w.t0 * p.C_st;                 // the token ahead
+  ahead.request_b(Ct, p.N);
   dr.load(dn, w.t1 - w.t0, at);
   zr.load(zn, w.t1 - w.t0, at);
   gr.load(gn, w.t1 - w.t0, at);
@@ -550,18 +557,15 @@ __global__ void __launch_bounds__(256) scan_bwd_state_kernel(ScanArgs p) {
     gr.load(gn, left, at);
     Marks m = {0u, 0u, 0u};
     if (PACKED) m = block_marks(q, t0, n);
-    BCAhead<T, NP, FAST> ahead;
-    const T* Ct = C + t0 * p.C_st;
-    ahead.request_b(Ct, p.N);
 #pragma unroll
     for (int j = 0; j < SCAN_Q; ++j) {
       if (PACKED && (j >= n || cut)) continue;
       const bool there = PACKED || j < n;
       BCAhead<T, NP, FAST> now = ahead;
       float Cv[NP];
-      Ct += j + 1 < n ? p.C_st : 0;
+      Ct += t0 + j + 1 < w.t1 ? p.C_st : 0;
       now.arrived_b(Ct);
-      if (j + 1 < SCAN_Q) ahead.request_b(Ct, p.N);
+      ahead.request_b(Ct, p.N);
       now.get_b(Cv);
       if (PACKED && !(m.valid >> j & 1)) continue;
       if (PACKED && (m.start >> j & 1)) { cut = true; continue; }
@@ -660,6 +664,9 @@ __global__ void __launch_bounds__(64 * SCAN_BT * (NP / SCAN_NW), 2) scan_bwd_ker
     float dt_[OWN], slope[OWN], u_[OWN], z_[OWN], g_[OWN];      // of this wave's tokens
 #pragma unroll
     for (int i = 0; i < SCAN_NW; ++i) hs[0][i] = hn[i];
+    BCAhead<T, SCAN_NW, FAST> ahead;
+    const T *Bt = B + t0 * p.B_st, *Ct = C + t0 * p.C_st;
+    ahead.request_b(Bt, Nw);
     SeqWalk f = q;                                 // the sequence that the states' second computation is in
     Marks m = {0u, 0u, 0u};
     if (PACKED) {
@@ -699,12 +706,9 @@ __global__ void __launch_bounds__(64 * SCAN_BT * (NP / SCAN_NW), 2) scan_bwd_ker
     }
     __syncthreads();                               // and everyone has read the sums of the block behind
     float a[SCAN_Q][SCAN_NW];
-    BCAhead<T, SCAN_NW, FAST> ahead;
-    const T *Bt = B + t0 * p.B_st, *Ct = C + t0 * p.C_st;
     // What is read from LDS is read a token ahead too, beside the request for B and C: waiting for LDS alone is not
     // possible while scalar loads are on the way.
     float dtn = in[0][0][w.wave][w.lane], xn = in[0][1][w.wave][w.lane], gn_ = 0.f;
-    ahead.request_b(Bt, Nw);
 #pragma unroll
     for (int j = 0; j < SCAN_Q; ++j) {
 #pragma unroll
