@@ -346,6 +346,7 @@ __global__ void __launch_bounds__(256) scan_fwd_kernel(ScanArgs p) {
     Marks m = {0u, 0u, 0u};
     if (PACKED) m = block_marks(q, t0, n);
     T* ot = out + (int64_t)t0 * p.D;
+    uint32_t to = at;
     if (!CARRY) ahead.request(Bt, Ct, p.N);
 #pragma unroll
     for (int j = 0; j < SCAN_Q; ++j) {
@@ -365,8 +366,8 @@ __global__ void __launch_bounds__(256) scan_fwd_kernel(ScanArgs p) {
         now.get(Bv, Cv);
       }
       if (PACKED && !(m.valid >> j & 1)) {
-        if (!STATE_ONLY) lane_store(ot, at, from_f32<T>(0.f));
-        ot += p.D;
+        if (!STATE_ONLY) lane_store(ot, to, from_f32<T>(0.f));
+        to += p.D * (uint32_t)sizeof(T);
         continue;
       }
       if (PACKED && (m.start >> j & 1)) {
@@ -395,8 +396,8 @@ __global__ void __launch_bounds__(256) scan_fwd_kernel(ScanArgs p) {
         }
         const float zz = to_f32(zb[j]);
         const float gate = zz * sigmoid_hw(zz);
-        lane_store(ot, at, from_f32<T>(gated ? y * gate : y));
-        ot += j + 1 < n ? p.D : 0;
+        lane_store(ot, to, from_f32<T>(gated ? y * gate : y));
+        to += j + 1 < n ? p.D * (uint32_t)sizeof(T) : 0u;
       }
       if (PACKED && (m.end >> j & 1)) {
         if (!STATE_ONLY && p.state1 && w.on) store_state<NP, FAST>(p.state1, q.seq(), p, w.d, h);
