@@ -133,7 +133,9 @@ template <typename T, int NP> struct BCAhead<T, NP, false> {
 };
 
 // Asks for one element of each end of B's and C's rows of a block of n tokens (four lanes alike), so that the lines are in
-// the L2 when the scalar unit asks for them a token ahead: from there that is time enough, from memory it is not.
+// the L2 when the scalar unit asks for them a token ahead: from there that is time enough, from memory it is not.  Measured
+// with and without: 8 x 2048 x 2048 backward fp32 610 and 640 us, bf16 565 and 574; outputs of 1 x 4096 45 and 48 us.  The
+// chunk passes read one of the two only and lose by it: 8 x 2048 x 2048 fp32, adjoints 153 and 140 us.
 template <typename T>
 __device__ __forceinline__ T touch_rows(const T* B, int64_t b_st, const T* C, int64_t c_st, int n, int N, int lane) {
   const int j = min(lane & 7, n - 1);
@@ -233,7 +235,8 @@ template <typename T> __device__ __forceinline__ void lane_store(T* row, uint32_
 }
 
 // The states of a slot, FULL: all NP of them, else the first N.  One scalar address and running offsets, computed anew at
-// every call: addresses of their own are kept from block to block, in registers that the states need.
+// every call: addresses of their own are kept from block to block, in scalar registers that spill (backward 534 us, with
+// this 497), and offsets that are not made anew in vector registers (outputs 162 -> 175 us: a wave less per SIMD).
 template <int NP, bool FULL>
 __device__ __forceinline__ void load_slot(const float* slot, const ScanArgs& p, int d, float (&h)[NP], int N) {
   uint32_t at = d * 4u;
@@ -285,12 +288,12 @@ template <typename T> struct Rows {
 // that channel too and store the same values to the same places, so that no store depends on the lane.  Without packed
 // sequences a block is straight-line code: tokens past the chunk's last repeat the last one with a step size of 0, which
 // leaves the state as it is and stores the same output again.  What packed sequences' borders need stands behind
-// wave-uniform branches, and so do their chunks' ends.  (Branches for both: 8 x 2048 x 2048 backward 555 -> 623 us.)
+// wave-uniform branches, and so do their chunks' ends.  (Branches for both: 8 x 2048 x 2048 backward 12 % slower.)
 //
 // Bound by vector arithmetic: a state of a token takes five issue slots in the state pass (two of them the exponential) and
 // six in the output pass, a channel's token about 25 more (softplus, gate, conversions).  8 x 2048 x 2048 bf16, N = 16:
-// states 117 us, of which 80 are issue slots; outputs 172 us, of which 119, while it reads 268 MB and writes as much again
-// of kept states (3.1 TB/s).  1 x 4096 x 2048: 36 and 49 us.  256 x 20 x 1024 fp32 (one chunk): 41 us.
+// states 114 us, of which 80 are issue slots; outputs 160 us, of which 119, while it reads 268 MB and writes as much again
+// of kept states (3.4 TB/s).  1 x 4096 x 2048: 33 and 42 us.  256 x 20 x 1024 fp32 (one chunk): 41 us.
 template <typename T, int NP, bool PACKED, bool FAST, bool STATE_ONLY>
 __global__ void __launch_bounds__(256) scan_fwd_kernel(ScanArgs p) {
   const Tile w(p);
@@ -609,10 +612,10 @@ __global__ void __launch_bounds__(256) scan_bwd_state_kernel(ScanArgs p) {
 // block's tokens: it loads their inputs, computes their step sizes and gates for the others, and finishes their gradients
 // from the waves' parts of y, of the sum of dh B and of that of k A, all by way of LDS.
 //
-// Bound by vector arithmetic: 185 instructions per token and wave (8 states of 64 channels), 47 slots of them the sums over
-// the lanes.  8 x 2048 x 2048 bf16: 555 us, of which 355 are issue slots at two waves per SIMD; it moves 0.77 GB.  Without
-// keeping the decays three waves would fit a SIMD but for spilled registers: 927 us.  Two tiles per workgroup, not four:
-// fewer waves wait at a barrier (586 us with four, 566 with one, which doubles the partial rows).
+// Bound by vector arithmetic: 177 instructions per token and wave (8 states of 64 channels), 47 slots of them the sums over
+// the lanes.  8 x 2048 x 2048 bf16: 505 us, of which 355 are issue slots at two waves per SIMD; it moves 0.77 GB.  256 x 20
+// x 1024 fp32: 98 us.  Without keeping the decays three waves would fit a SIMD but for spilled registers: 927 us.  Two
+// tiles per workgroup, not four: fewer waves wait at a barrier (four: 6 % slower; one: 2 %, and twice the partial rows).
 #define SCAN_NW 8
 #define SCAN_BT 2      // tiles per workgroup
 template <typename T, int NP, bool PACKED, bool FAST>
