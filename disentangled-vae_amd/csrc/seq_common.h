@@ -139,17 +139,23 @@ struct SeqWalk {
   }
   // the current sequence as an index that exists, also where wrong offsets have led the walk past the last one
   __device__ __forceinline__ int64_t seq() const { return min(max(s, 0), S - 1); }
-  // first sequence that ends behind token t (empty ones are skipped by that)
+  // first sequence that ends behind token t (empty ones are skipped by that).  The wave's 64 lanes, all of which have to be
+  // there, probe 64 ends at once, so that up to 64 sequences take one wait for memory and 4096 two.
   __device__ __forceinline__ void seek(int t) {
     if (!off) {
       s = t / L;
     } else {
-      int lo = 0, hi = S;
+      int lo = 0, hi = S;                     // the answer is one of lo ... hi
       while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (at(mid + 1) > t) hi = mid; else lo = mid + 1;
+        const int step = (hi - lo + 63) >> 6;
+        const int64_t probe = lo + ((int64_t)(threadIdx.x & 63) + 1) * step - 1;
+        const bool past = probe < hi && min(max(off[probe < hi ? probe + 1 : hi], 0), tokens) <= t;
+        const int n = __popcll(__ballot(past));
+        lo = uniform(lo + n * step);
+        hi = uniform(min(hi, lo + step - 1));
       }
       s = lo;
+      while (s < S && at(s + 1) <= t) ++s;    // (wrong offsets only: what follows relies on an end behind t)
     }
     load();
   }

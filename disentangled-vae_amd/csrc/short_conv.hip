@@ -92,12 +92,13 @@ template <typename T, int V, int W>
 __global__ void __launch_bounds__(256) conv_fwd_kernel(ConvArgs p) {
   const int d = ((int)(blockIdx.x % p.tiles) * 64 + (threadIdx.x & 63)) * V;
   const int t0 = ((int)(blockIdx.x / p.tiles) * 4 + uniform(threadIdx.x >> 6)) * p.tb;
-  if (t0 >= p.tokens || d >= p.D) return;
+  if (t0 >= p.tokens) return;
   const int t1 = min(t0 + p.tb, p.tokens);
   float w[W][V], bias[V], win[W][V];
-  load_weights<V, W>(p, d, w, bias);
+  load_weights<V, W>(p, d < p.D ? d : 0, w, bias);
   SeqWalk q = {p.offsets, p.S, p.L, p.tokens, 0, 0, 0};
   q.seek(t0);
+  if (d >= p.D) return;
   if (q.s < q.S && q.b < t0) {
 #pragma unroll
     for (int k = 1; k < W; ++k) load_input<T, V, W>(p, q, t0 - W + k, d, win[k]);

@@ -765,6 +765,24 @@ def test_scan_of_one_token_takes_any_token_stride(F):
     assert torch.equal(out, want[0]) and torch.equal(state, want[1])
 
 
+@pytest.mark.parametrize('S', [63, 64, 65, 200, 4096, 4097, 9000])
+def test_many_packed_sequences(F, S):
+    """searches over one, two and three rounds of 64 ends, with empty sequences between"""
+    lens = torch.randint(0, 4, (S,), generator=gen(S)).tolist()
+    c = ScanCase(5, 3, 1, torch.float32, lengths=lens, tail=3, seed=S)
+    c.check(F, grads=False)
+    x, w, st = rnd(gen(S + 1), c.T, 5), rnd(gen(S + 2), 5, 3), rnd(gen(S + 3), S, 2, 5)
+    out, last = F.short_conv(x.cuda(), w.cuda(), state=st.cuda(), offsets=c.offsets, return_state=True)
+    want, ends, off = torch.zeros(c.T, 5, dtype=torch.float64), st.double(), c.off
+    for s in range(S):
+        h = torch.cat([st[s], x[off[s]:off[s + 1]]]).double()
+        ends[s] = h[len(h) - 2:]
+        for t in range(off[s], off[s + 1]):
+            want[t] = (h[t - off[s]:t - off[s] + 3] * w.t().double()).sum(0)
+    assert torch.equal(last.cpu().double(), ends)
+    assert ((out.cpu().double() - want).abs() <= 8 * U32 * 3 * x.abs().max() * w.abs().max()).all()
+
+
 def test_results_repeat_bit_for_bit(F):
     c = ScanCase(200, 16, 2, torch.bfloat16, rows=(3, 150), seed=31, state=False)
     runs = []
