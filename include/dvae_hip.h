@@ -578,7 +578,8 @@ int dvae_adam_advance_f32(float* dyn, double beta1, double beta2, dvae_stream_t 
  *      A batch is `rows` sequences of L tokens.  With `offsets` (S + 1 ascending int32 positions on the device, the
  *      first 0) there is one row of L tokens that holds S sequences one after the other, some possibly empty; tokens
  *      behind the last one belong to none: outputs and gradients are 0 there.  Offsets are not checked: wrong ones give
- *      wrong results, never an access outside the tensors.  S is the number of sequences in either form. */
+ *      wrong results, never an access outside the tensors.  S is the number of sequences in either form.
+ *      Sizes: fewer than 2^31 - 2^16 tokens and 2^24 channels, and launches of fewer than 2^32 threads (-EINVAL beyond). */
 #define DVAE_DT_F32 0
 #define DVAE_DT_BF16 1
 
@@ -587,7 +588,7 @@ int dvae_adam_advance_f32(float* dyn, double beta1, double beta2, dvae_stream_t 
  * Dp, bias [D]; state0 (entering) and state1 (final) [S,D,N].  NULL: Dp, z, bias, state0, state1, offsets, ckpt.
  * Final states of sequences without tokens are not written.  ckpt (dvae_selective_scan_ckpt_floats): the states that
  * the backward pass starts from, kept if not NULL.  ws: dvae_selective_scan_fwd_ws_floats floats (0 where the time axis is
- * not split; NULL then).  Token strides of u, delta, z and dout must be below 2^26 elements. */
+ * not split; NULL then).  Token strides of u, delta, z and dout must be below 2^26 elements where L > 1. */
 int64_t dvae_selective_scan_ckpt_floats(int64_t rows, int64_t L, int64_t D, int64_t N);
 int64_t dvae_selective_scan_fwd_ws_floats(int64_t rows, int64_t L, int64_t D, int64_t G, int64_t N,
                                           int keep /* whether ckpt is given */);
