@@ -416,6 +416,11 @@ __global__ void __launch_bounds__(256) scan_fwd_kernel(ScanArgs p) {
     if (w.g == 0 && w.part == 0 && threadIdx.x == 0) p.keep[row * p.nch + w.chunk] = cut ? 0.f : 1.f;
   } else if (!PACKED && p.state1 && w.on && w.chunk + 1 == p.nch) {
     store_state<NP, FAST>(p.state1, row, p, w.d, h);
+  } else if (PACKED && p.state1) {              // sequences without tokens end with what they entered with
+    q.for_empty(w.chunk, p.nch, [&](int s) {
+      entering_state<NP, FAST>(p, s, w.d, h);
+      if (w.on) store_state<NP, FAST>(p.state1, s, p, w.d, h);
+    });
   }
 }
 

@@ -149,7 +149,7 @@ struct SeqWalk {
       while (lo < hi) {
         const int step = (hi - lo + 63) >> 6;
         const int64_t probe = lo + ((int64_t)(threadIdx.x & 63) + 1) * step - 1;
-        const bool past = probe < hi && min(max(off[probe < hi ? probe + 1 : hi], 0), tokens) <= t;
+        const bool past = probe < hi && lane_at(probe < hi ? probe + 1 : hi) <= t;
         const int n = __popcll(__ballot(past));
         lo = uniform(lo + n * step);
         hi = uniform(min(hi, lo + step - 1));
@@ -159,6 +159,18 @@ struct SeqWalk {
     }
     load();
   }
+  // f(s) for the sequences s without tokens: every of-th 64 of all from the part-th 64 on, looked at by 64 lanes at once
+  template <typename F> __device__ __forceinline__ void for_empty(int part, int of, F f) const {
+    for (int64_t s0 = (int64_t)part * 64; s0 < S; s0 += (int64_t)of * 64) {
+      const int64_t i = s0 + (threadIdx.x & 63);
+      uint64_t left = __ballot(i < S && lane_at(i < S ? i + 1 : S) <= lane_at(i < S ? i : S));
+      while (left) {
+        f(uniform((int)s0 + __builtin_ctzll(left)));
+        left &= left - 1;
+      }
+    }
+  }
+  __device__ __forceinline__ int lane_at(int64_t i) const { return min(max(off[i], 0), tokens); }
   // forward: the next sequence with tokens from t on
   __device__ __forceinline__ void next(int t) {
     do { ++s; } while (s < S && at(s + 1) <= t);

@@ -98,6 +98,18 @@ __global__ void __launch_bounds__(256) conv_fwd_kernel(ConvArgs p) {
   load_weights<V, W>(p, d < p.D ? d : 0, w, bias);
   SeqWalk q = {p.offsets, p.S, p.L, p.tokens, 0, 0, 0};
   q.seek(t0);
+  if (p.state1 && p.offsets) {                 // sequences without tokens end with what they entered with
+    q.for_empty(t0 / p.tb, (p.tokens + p.tb - 1) / p.tb, [&](int s) {
+      if (d >= p.D) return;
+#pragma unroll
+      for (int k = 0; k + 1 < W; ++k) {
+        float v[V] = {};
+        const int64_t i = ((int64_t)s * (W - 1) + k) * p.D + d;
+        if (p.state0) load_pack<T, V>((const T*)p.state0 + i, v);
+        store_pack<T, V>((T*)p.state1 + i, v);
+      }
+    });
+  }
   if (d >= p.D) return;
   if (q.s < q.S && q.b < t0) {
 #pragma unroll
@@ -268,13 +280,13 @@ __global__ void __launch_bounds__(64 * SUM_WAVES) conv_params_kernel(const float
 }
 
 // the gradient of the carried inputs: row j of a sequence's state reaches the tokens p <= j with tap j - p, and the
-// final state where the sequence is shorter than the window
+// final state where the sequence is shorter than the window, or has no tokens
 template <typename T, int W>
 __global__ void __launch_bounds__(256) conv_dstate_kernel(ConvArgs p) {
   const int d = (int)(blockIdx.x % p.tiles) * 256 + threadIdx.x;
   SeqWalk q = {p.offsets, p.S, p.L, p.tokens, (int)(blockIdx.x / p.tiles), 0, 0};
   q.load();
-  if (d >= p.D || q.e <= q.b) return;
+  if (d >= p.D) return;
   float w[W][1], bias[1], ds[W] = {};
   load_weights<1, W>(p, d, w, bias);
 #pragma unroll
@@ -290,7 +302,7 @@ __global__ void __launch_bounds__(256) conv_dstate_kernel(ConvArgs p) {
   }
 #pragma unroll
   for (int r = 0; r < W - 1; ++r) {
-    const int from = r - (q.e - q.b);
+    const int from = r - max(q.e - q.b, 0);
     if (p.dstate1 && from >= 0) ds[r] += to_f32(((const T*)p.dstate1)[((int64_t)q.s * (W - 1) + from) * p.D + d]);
     ((T*)p.dstate0)[((int64_t)q.s * (W - 1) + r) * p.D + d] = from_f32<T>(ds[r]);
   }

@@ -1206,9 +1206,9 @@ class ScanArgs(_KeptArgs):
         return ScanArgs('selective_scan_bwd', u, delta, A, B, C, D, z, delta_bias, self.softplus, state, offsets)
 
 
-def _final_states(shape, dtype, device, entering: Optional[Tensor], packed: bool, tokens: int) -> Tensor:
-    """where final states go.  Sequences without tokens are not written: they keep what they entered with."""
-    if tokens > 0 and not packed:
+def _final_states(shape, dtype, device, entering: Optional[Tensor], tokens: int) -> Tensor:
+    """where final states go: without any tokens, those that were entered with"""
+    if tokens > 0:
         return torch.empty(shape, dtype=dtype, device=device) if entering is None else _new_like(entering)
     return torch.zeros(shape, dtype=dtype, device=device) if entering is None else entering.clone()
 
@@ -1220,7 +1220,7 @@ def selective_scan_fwd(a: ScanArgs, want_state: bool, keep: bool):
         with torch.cuda.device(dev):
             return selective_scan_fwd(a, want_state, keep)
     out = _new_like(a.tensors[0])
-    final = _final_states(a.state_shape, torch.float32, dev, a.tensors[8], a.packed, a.tokens) if want_state else None
+    final = _final_states(a.state_shape, torch.float32, dev, a.tensors[8], a.tokens) if want_state else None
     rows, L, ch, G, N = a.sizes
     ckpt = torch.empty(lib.dvae_selective_scan_ckpt_floats(rows, L, ch, N), dtype=torch.float32,
                        device=dev) if keep else None
@@ -1247,7 +1247,8 @@ def selective_scan_bwd(a: ScanArgs, tensors, dout: Tensor, dfinal: Optional[Tens
     rows, L, ch, G, N = a.sizes
     new = _new_like if a.tokens else torch.zeros_like
     dA, dD, db = new(A), new(D) if a.has_D else None, new(bias) if a.has_bias else None
-    ds = _final_states(a.state_shape, f32, dev, dfinal, a.packed, a.tokens) if want_dstate else None
+    # (sequences without tokens are not written: they keep dfinal)
+    ds = _final_states(a.state_shape, f32, dev, dfinal, 0 if a.packed else a.tokens) if want_dstate else None
     if a.tokens:
         ws = torch.empty(lib.dvae_selective_scan_bwd_ws_floats(rows, L, ch, G, N), dtype=f32, device=dev)
         check(lib.dvae_selective_scan_bwd(*a.head, a.offsets_ptr, dout.data_ptr(), *_st2(dout), _p(dfinal),
@@ -1308,7 +1309,7 @@ class ConvArgs(_KeptArgs):
         state = _param(what, 'state', state, self.state_shape, dev, dt)
         self.tensors = (x, weight, bias, state, offsets)
         self.silu = silu
-        self.has_bias, self.packed, self.tokens = bias is not None, offsets is not None, rows * L
+        self.has_bias, self.tokens = bias is not None, rows * L
         self.sizes = rows, L, ch, W
         self.head = x.data_ptr(), *_st2(x), weight.data_ptr(), _p(bias), int(bool(silu)), _p(state)
         self.offsets_ptr = _p(offsets)
@@ -1325,7 +1326,7 @@ def short_conv_fwd(a: ConvArgs, want_state: bool):
         with torch.cuda.device(dev):
             return short_conv_fwd(a, want_state)
     out = _new_like(a.tensors[0])
-    final = _final_states(a.state_shape, a.act, dev, a.tensors[3], a.packed, a.tokens) if want_state else None
+    final = _final_states(a.state_shape, a.act, dev, a.tensors[3], a.tokens) if want_state else None
     check(lib.dvae_short_conv_fwd(*a.head, _p(final), a.offsets_ptr, out.data_ptr(), *a.tail, _stream_of(dev.index)),
           'short_conv_fwd')
     return out, final
@@ -1343,7 +1344,7 @@ def short_conv_bwd(a: ConvArgs, tensors, dout: Tensor, dfinal: Optional[Tensor],
     rows, L, ch, W = a.sizes
     new = _new_like if a.tokens else torch.zeros_like
     dx, dw, db = _new_like(dout), new(tensors[1]), new(tensors[2]) if a.has_bias else None
-    ds = _final_states(a.state_shape, a.act, dev, dfinal, a.packed, a.tokens) if want_dstate else None
+    ds = _final_states(a.state_shape, a.act, dev, dfinal, a.tokens) if want_dstate else None
     if a.tokens:
         ws = torch.empty(lib.dvae_short_conv_bwd_ws_floats(rows, L, ch, W), dtype=torch.float32, device=dev)
         check(lib.dvae_short_conv_bwd(*a.head, a.offsets_ptr, dout.data_ptr(), *_st2(dout), _p(dfinal), dx.data_ptr(),

@@ -586,7 +586,7 @@ int dvae_adam_advance_f32(float* dyn, double beta1, double beta2, dvae_stream_t 
 /* dt = softplus(delta + bias) (softplus != 0; else delta + bias), h[n] = exp(dt A[d,n]) h[n] + dt u B[n],
  * out = (sum_n C[n] h[n] + Dp u) silu(z).  u, delta, z, out [rows,L,D]; A [D,N], N <= 16; B, C [rows,L,G,N], G divides D;
  * Dp, bias [D]; state0 (entering) and state1 (final) [S,D,N].  NULL: Dp, z, bias, state0, state1, offsets, ckpt.
- * Final states of sequences without tokens are not written.  ckpt (dvae_selective_scan_ckpt_floats): the states that
+ * Final states of sequences without tokens are those they enter with (nothing is written if there is no token at all).  ckpt (dvae_selective_scan_ckpt_floats): the states that
  * the backward pass starts from, kept if not NULL.  ws: dvae_selective_scan_fwd_ws_floats floats (0 where the time axis is
  * not split; NULL then).  Token strides of u, delta, z and dout must be below 2^26 elements where L > 1. */
 int64_t dvae_selective_scan_ckpt_floats(int64_t rows, int64_t L, int64_t D, int64_t N);
@@ -599,7 +599,7 @@ int dvae_selective_scan_fwd(const void* u, int64_t u_sb, int64_t u_st, const voi
                             float* state1, const int32_t* offsets, void* out, float* ckpt, int64_t rows, int64_t L,
                             int64_t D, int64_t G, int64_t N, int64_t S, int dtype, float* ws, dvae_stream_t stream);
 /* Gradients from dout and (NULL: zero) dstate1, the gradient of the final states.  dA, dD, dbias, dstate0 may be NULL;
- * dstate0 of sequences without tokens is not written.  ckpt as the forward pass filled it (it is read only); ws:
+ * dstate0 of sequences without tokens is not written (it is dstate1 there).  ckpt as the forward pass filled it (it is read only); ws:
  * dvae_selective_scan_bwd_ws_floats floats. */
 int64_t dvae_selective_scan_bwd_ws_floats(int64_t rows, int64_t L, int64_t D, int64_t G, int64_t N);
 int dvae_selective_scan_bwd(const void* u, int64_t u_sb, int64_t u_st, const void* delta, int64_t delta_sb,
@@ -619,7 +619,7 @@ int dvae_selective_scan_step(float* state, const void* u, int64_t u_sb, const vo
 /* Depthwise convolution over the last W tokens (2 <= W <= 4) of the same sequence:
  * out[t] = act(bias + sum_k w[d,k] x[t - (W-1) + k]), act = silu if `silu` != 0.  x, out [rows,L,D]; w [D,W]; bias [D] or
  * NULL.  What lies before a sequence's first token is state0 [S,W-1,D] (type `dtype`; NULL: zeros); state1, if not NULL,
- * receives the last W - 1 inputs of every sequence that has tokens. */
+ * receives the last W - 1 inputs of every sequence (nothing is written if there is no token at all). */
 int dvae_short_conv_fwd(const void* x, int64_t x_sb, int64_t x_st, const float* w, const float* bias, int silu,
                         const void* state0, void* state1, const int32_t* offsets, void* out, int64_t rows, int64_t L,
                         int64_t D, int64_t W, int64_t S, int dtype, dvae_stream_t stream);
