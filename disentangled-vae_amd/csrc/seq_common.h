@@ -122,8 +122,10 @@ template <typename V> __device__ __forceinline__ V uniform_load(const V* p, int6
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // The sequence that a walk over tokens is in.  With `off`, sequence s is [off[s], off[s + 1]) of S ascending int32
-// positions; without, all S sequences have L tokens.  Positions are clamped to the tokens there are, so wrong offsets
-// give wrong results but never an access out of range, and every loop here ends: the index only moves one way.
+// positions; without, all S sequences have L tokens.  Wrong offsets give wrong results but never an access out of range:
+// positions are clamped to the tokens there are, a sequence whose end does not lie behind its begin has no tokens, and the
+// sequence that the walk is in always has some, the last of them at or behind the token it was looked for (what the rows of
+// carried states are computed from).  Every loop here ends: the index only moves one way.
 struct SeqWalk {
   const int32_t* off;
   int S, L;     // number of sequences; tokens of each (off == nullptr)
@@ -139,7 +141,7 @@ struct SeqWalk {
   }
   // the current sequence as an index that exists, also where wrong offsets have led the walk past the last one
   __device__ __forceinline__ int64_t seq() const { return min(max(s, 0), S - 1); }
-  // first sequence that ends behind token t (empty ones are skipped by that).  The wave's 64 lanes, all of which have to be
+  // first sequence that ends behind token t (empty ones are skipped).  The wave's 64 lanes, all of which have to be
   // there, probe 64 ends at once, so that up to 64 sequences take one wait for memory and 4096 two.
   __device__ __forceinline__ void seek(int t) {
     if (!off) {
@@ -155,9 +157,9 @@ struct SeqWalk {
         hi = uniform(min(hi, lo + step - 1));
       }
       s = lo;
-      while (s < S && at(s + 1) <= t) ++s;    // (wrong offsets only: what follows relies on an end behind t)
     }
     load();
+    settle(t);
   }
   // f(s) for the sequences s without tokens: every of-th 64 of all from the part-th 64 on, looked at by 64 lanes at once
   template <typename F> __device__ __forceinline__ void for_empty(int part, int of, F f) const {
@@ -173,8 +175,16 @@ struct SeqWalk {
   __device__ __forceinline__ int lane_at(int64_t i) const { return min(max(off[i], 0), tokens); }
   // forward: the next sequence with tokens from t on
   __device__ __forceinline__ void next(int t) {
-    do { ++s; } while (s < S && at(s + 1) <= t);
-    load();
+    step();
+    settle(t);
+  }
+  __device__ __forceinline__ void step() {
+    ++s;
+    b = e;
+    if (s < S) e = at(s + 1); else b = e = tokens;
+  }
+  __device__ __forceinline__ void settle(int t) {
+    while (s < S && (e <= t || e <= b)) step();
   }
   // backward: the last sequence that starts at or before token t and has tokens
   __device__ __forceinline__ void prev(int t) {

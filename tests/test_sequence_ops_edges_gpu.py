@@ -1,0 +1,54 @@
+"""The sequence operators at their edges: offsets in the wrong order, infinities where a block is filled up, forward-mode
+derivatives.  Cases, references and tolerances are those of test_sequence_ops_gpu."""
+import numpy as np
+import pytest
+import torch
+
+import seq_reference as R
+from test_sequence_ops_gpu import F, ConvCase, ScanCase, U32, HALF, close, f64, gen, rnd      # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def inside_nan(t):
+    """the same values in memory that is NaN before and behind them"""
+    if t is None:
+        return None
+    pad = 4096
+    big = torch.full((t.numel() + 2 * pad,), float('nan'), dtype=t.dtype, device='cuda')
+    view = big[pad:pad + t.numel()].view(t.shape)
+    view.copy_(t)
+    return view
+
+
+WRONG = [[15, 10], [2, 2], [2, 2, 40], [0, 100], [-5, 3, 2, 60], [40, 30, 20, 10, 0], [7, 0, 40], [39, 1, 39, 2, 39], [90, 80],
+         [-9, -8], [0, 20, 10, 30], [13, 12, 14, 13, 15], [0, 40, 0, 40]]
+
+
+@pytest.mark.parametrize('scale', [1, 7])
+@pytest.mark.parametrize('off', WRONG)
+def test_offsets_in_the_wrong_order_reach_nothing_outside(F, off, scale):
+    """What is in a sequence then is not defined, but every value read lies in the tensors: NaN around all of them reaches
+    neither the outputs nor a gradient."""
+    T, S = 40 * scale, len(off) - 1
+    offsets = torch.tensor(off, dtype=torch.int32, device='cuda') * scale
+    for D, W, N, dtype in ((64, 4, 16, torch.bfloat16), (5, 2, 3, torch.float32), (130, 3, 8, torch.float32)):
+        c = ConvCase(D, W, dtype, lengths=[T], seed=D)
+        v = {k: inside_nan(t) for k, t in c.gpu.items()}
+        v['state'] = inside_nan(rnd(gen(1), S, W - 1, D).to(dtype))
+        v = {k: t.requires_grad_() for k, t in v.items()}
+        out, state = F.short_conv(v['x'], v['weight'], v['bias'], silu=True, state=v['state'], offsets=offsets,
+                                  return_state=True)
+        got = torch.autograd.grad((out, state), list(v.values()),
+                                  (inside_nan(c.dout), inside_nan(rnd(gen(2), S, W - 1, D).to(dtype))))
+        for k, t in zip(('out', *v), (out, *got)):
+            assert torch.isfinite(t).all(), ('conv', k, D, W)
+        c = ScanCase(D, N, 1, dtype, lengths=[T], seed=D)
+        v = {k: inside_nan(t) for k, t in c.gpu.items()}
+        v['state'] = inside_nan(rnd(gen(3), S, D, N))
+        v = {k: t.requires_grad_() for k, t in v.items()}
+        out, state = F.selective_scan(v['u'], v['delta'], v['A'], v['B'], v['C'], D=v['D'], z=v['z'], delta_bias=v['bias'],
+                                      delta_softplus=True, state=v['state'], offsets=offsets, return_state=True)
+        got = torch.autograd.grad((out, state), list(v.values()), (inside_nan(c.dout), inside_nan(rnd(gen(4), S, D, N))))
+        for k, t in zip(('out', *v), (out, *got)):
+            assert torch.isfinite(t).all(), ('scan', k, D, N)
