@@ -213,8 +213,8 @@ class SSMEncoder(nn.Module):
             if offsets is None:
                 y = y[:, -1]
             else:
-                last = offsets[1:].long() - 1
-                y = y[last.clamp_min(0)].masked_fill((offsets[1:] == offsets[:-1])[:, None], 0.0)
+                last = (offsets[1:].long() - 1).clamp(0, y.shape[0] - 1)         # (an index, whatever the offsets are)
+                y = y[last].masked_fill((offsets[1:] <= offsets[:-1])[:, None], 0.0)
         return y, (ends if self.return_states else None)
 
     @torch.no_grad()

@@ -52,3 +52,22 @@ def test_offsets_in_the_wrong_order_reach_nothing_outside(F, off, scale):
         got = torch.autograd.grad((out, state), list(v.values()), (inside_nan(c.dout), inside_nan(rnd(gen(4), S, D, N))))
         for k, t in zip(('out', *v), (out, *got)):
             assert torch.isfinite(t).all(), ('scan', k, D, N)
+
+
+# ------------------------------------------------------------------------------------------------ models.SSMEncoder
+def ssm(**more):
+    import models
+    torch.manual_seed(5)
+    return models.SSMEncoder(**{**dict(input_dim=24, hidden_dim=32, num_layers=2, state_dim=8), **more}).cuda()
+
+
+@pytest.mark.parametrize('off', [[0, 9, 60], [0, 90, 95], [20, 3, 3, 0], [-4, -2, 7]])
+def test_encoder_takes_no_output_from_outside(off):
+    """offsets behind the last token, before the first, in the wrong order: an output of some token, or 0"""
+    m = ssm()
+    x = torch.randn(40, 24, device='cuda', requires_grad=True)
+    y, _ = m(x, offsets=torch.tensor(off, dtype=torch.int32, device='cuda'))
+    (g,) = torch.autograd.grad(y.square().sum(), (x,))
+    assert y.shape == (len(off) - 1, 32) and torch.isfinite(y).all() and torch.isfinite(g).all()
+    for s in range(len(off) - 1):
+        assert off[s + 1] > off[s] or not y[s].any()
