@@ -150,7 +150,8 @@ class SSMEncoder(nn.Module):
     has no use for those sets `return_states = False`.
 
     forward() takes [batch, length, input_dim], or packed [tokens, input_dim] with `offsets` (int32, see
-    hipvae.functional.selective_scan; the output of an empty sequence is 0).  step() takes the next token of every
+    hipvae.functional.selective_scan; the output of an empty sequence is 0, and where there are no tokens at all nothing
+    depends on the parameters).  step() takes the next token of every
     sequence, [batch, input_dim], and updates `states` in place (no gradients): a frame's cost does not grow with the
     frames before it."""
     return_states = True
@@ -194,7 +195,16 @@ class SSMEncoder(nn.Module):
         shape = (*p.shape[:-1], self.groups, self.state_dim)
         return HF.linear(dt, layer.dt_proj.weight, None), B.view(shape), C.view(shape)
 
+    def _without_tokens(self, x, return_sequence, states, offsets):
+        """no sequence has a token: outputs of 0, and the states that were entered with"""
+        n = x.shape[0] if offsets is None else offsets.numel() - 1
+        shape = x.shape[:-1] if return_sequence else (n,)
+        ends = self.init_states(n) if states is None else [(a.clone(), b.clone()) for a, b in states]
+        return x.new_zeros(*shape, self.hidden_dim), (ends if self.return_states else None)
+
     def forward(self, x: torch.Tensor, return_sequence: bool = False, states=None, offsets: Optional[torch.Tensor] = None):
+        if x.numel() == 0:
+            return self._without_tokens(x, return_sequence, states, offsets)
         h, residual, ends = HF.linear(x, self.proj.weight, self.proj.bias), None, []
         for i, layer in enumerate(self.layers):
             conv_state, scan_state = states[i] if states is not None else (None, None)

@@ -61,6 +61,25 @@ def ssm(**more):
     return models.SSMEncoder(**{**dict(input_dim=24, hidden_dim=32, num_layers=2, state_dim=8), **more}).cuda()
 
 
+@pytest.mark.parametrize('shape,off', [((0, 24), [0, 0, 0]), ((3, 0, 24), None), ((0, 5, 24), None)])
+def test_encoder_without_tokens(shape, off):
+    """outputs of 0 and the states as they were, as the operators have it"""
+    m = ssm()
+    off = None if off is None else torch.tensor(off, dtype=torch.int32, device='cuda')
+    n = shape[0] if off is None else len(off) - 1
+    x = torch.empty(shape, device='cuda')
+    y, states = m(x, offsets=off)
+    assert y.shape == (n, 32) and not y.any() and len(states) == 2
+    assert all(a.shape == (n, 3, 64) and b.shape == (n, 64, 8) and not a.any() and not b.any() for a, b in states)
+    y, _ = m(x, return_sequence=True, offsets=off)
+    assert y.shape == (*shape[:-1], 32)
+    given = [(torch.randn_like(a), torch.randn_like(b)) for a, b in states]
+    _, ends = m(x, states=given, offsets=off)
+    for one, two in zip(given, ends):
+        for a, b in zip(one, two):
+            assert torch.equal(a, b) and (a is not b)
+
+
 @pytest.mark.parametrize('off', [[0, 9, 60], [0, 90, 95], [20, 3, 3, 0], [-4, -2, 7]])
 def test_encoder_takes_no_output_from_outside(off):
     """offsets behind the last token, before the first, in the wrong order: an output of some token, or 0"""
