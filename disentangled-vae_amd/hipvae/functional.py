@@ -992,7 +992,14 @@ class LSTMDecoder(torch.autograd.Function):
 
 
 # ------------------------------------------------------------------------------------------------ sequence operators
-def _wants_grad(*ts: Optional[Tensor]) -> bool:
+_forward_ad = torch.autograd.forward_ad
+
+
+def _wants_grad(what: str, *ts: Optional[Tensor]) -> bool:
+    if _forward_ad._current_level >= 0:             # inside a dual level: a tangent must not be dropped without a word
+        for t in ts:
+            if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{what}: forward-mode derivatives are not computed")
     if torch.is_grad_enabled():
         for t in ts:
             if t is not None and t.requires_grad:
@@ -1051,8 +1058,9 @@ def selective_scan(u: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: Tensor, D:
     other into [tokens, channels]; sequence s is tokens offsets[s] to offsets[s + 1].  Tokens behind the last sequence
     get 0, and gradients of 0.  The offsets are read on the device only and not checked.
     `state` [sequences, channels, states]: what the sequences start from (default zeros); it is not modified.
-    `return_state`: also returns the final states.  Gradients flow to every tensor argument and through both states."""
-    if _wants_grad(u, delta, A, B, C, D, z, delta_bias, state):
+    `return_state`: also returns the final states.  Gradients flow to every tensor argument and through both states;
+    second derivatives and forward mode are refused."""
+    if _wants_grad('selective_scan', u, delta, A, B, C, D, z, delta_bias, state):
         out, final = SelectiveScan.apply(u, delta, A, B, C, D, z, delta_bias, delta_softplus, state, offsets, return_state)
     else:
         a = ops.ScanArgs('selective_scan', u, delta, A, B, C, D, z, delta_bias, delta_softplus, state, offsets)
@@ -1070,7 +1078,7 @@ def selective_scan_step(state: Tensor, u: Tensor, delta: Tensor, A: Tensor, B: T
 
 
 def _no_grad_form(what: str, *ts):
-    if _wants_grad(*ts):
+    if _wants_grad(what, *ts):
         raise RuntimeError(f"{what} computes no gradients: call it under torch.no_grad()")
 
 
@@ -1105,7 +1113,7 @@ def short_conv(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, silu: b
     bias [channels], both fp32.  `state` [sequences, taps - 1, channels] of x's type holds the inputs before a sequence's
     first token (default zeros); `return_state` also returns the last taps - 1 inputs of every sequence.  `offsets` as in
     selective_scan.  Gradients flow to every tensor argument and through both states."""
-    if _wants_grad(x, weight, bias, state):
+    if _wants_grad('short_conv', x, weight, bias, state):
         out, final = ShortConv.apply(x, weight, bias, silu, state, offsets, return_state)
     else:
         out, final = ops.short_conv_fwd(ops.ConvArgs('short_conv', x, weight, bias, silu, state, offsets), return_state)
@@ -1149,7 +1157,7 @@ def add_rms_norm(x: Tensor, residual: Optional[Tensor], weight: Tensor, eps: flo
     channels] fp32 or bf16, y of its type; residual of the same type or fp32 (a residual stream kept in fp32 beside bf16
     activations), sum of the residual's; weight [channels] fp32.  The norm is that of the sum as stored.  Without a
     residual the sum is x itself."""
-    if _wants_grad(x, residual, weight):
+    if _wants_grad('add_rms_norm', x, residual, weight):
         got = AddRMSNorm.apply(x, residual, weight, eps)
         return (got, x) if residual is None else got
     y, total, _ = ops.add_rms_norm_fwd(ops.NormArgs('add_rms_norm', x, residual, weight), eps, False)
