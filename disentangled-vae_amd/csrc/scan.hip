@@ -282,6 +282,8 @@ template <typename T> struct Rows {
   }
 };
 
+static __device__ const float no_input[SCAN_MAX_N] = {};     // B where there is no token
+
 // STATE_ONLY: the chunk's last state from a zero start, into the next chunk's slot; else the outputs.
 //
 // A block's inputs were requested a block ahead, B and C are a token ahead.  Lanes past the group's last channel compute
@@ -321,6 +323,7 @@ __global__ void __launch_bounds__(256) scan_fwd_kernel(ScanArgs p) {
   // A block's first token is requested by the block before it, but not where B and C of two tokens are 64 scalar registers
   // (8 x 2048 x 2048 fp32, outputs: 199 us with it, 184 without; bf16, 1 x 4096: 43 and 45 us).
   constexpr bool CARRY = STATE_ONLY || sizeof(T) * NP < 64;
+  constexpr bool FILLS = !PACKED && !STATE_ONLY;   // (the state pass leaves the last chunk out, and the others are whole blocks)
   if (STATE_ONLY) ahead.request_b(Bt, p.N);
   else if (CARRY) ahead.request(Bt, Ct, p.N);
   T* out = (T*)p.out + (int64_t)row * p.L * p.D;
@@ -357,7 +360,9 @@ __global__ void __launch_bounds__(256) scan_fwd_kernel(ScanArgs p) {
       const bool there = PACKED || j < n;
       BCAhead<T, NP, FAST> now = ahead;
       float Bv[NP], Cv[NP];
-      Bt += t0 + j + 1 < w.t1 ? p.B_st : 0;        // (the chunk's last token is requested again)
+      // behind the chunk's last token: its C again, and a B of zeros, so that B's infinities stay out of the state
+      if (FILLS && FAST) Bt = t0 + j + 1 < w.t1 ? Bt + p.B_st : (const T*)no_input;
+      else Bt += t0 + j + 1 < w.t1 ? p.B_st : 0;
       Ct += t0 + j + 1 < w.t1 ? p.C_st : 0;
       if (STATE_ONLY) {
         now.arrived_b(Bt);
@@ -367,6 +372,10 @@ __global__ void __launch_bounds__(256) scan_fwd_kernel(ScanArgs p) {
         now.arrived(Bt, Ct);
         if (CARRY || j + 1 < SCAN_Q) ahead.request(Bt, Ct, p.N);
         now.get(Bv, Cv);
+      }
+      if (FILLS && !FAST) {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) Bv[i] = there ? Bv[i] : 0.f;
       }
       if (PACKED && !(m.valid >> j & 1)) {
         if (!STATE_ONLY) lane_store(ot, to, from_f32<T>(0.f));
@@ -751,6 +760,13 @@ __global__ void __launch_bounds__(64 * SCAN_BT * (NP / SCAN_NW), 2) scan_bwd_ker
     for (int j = SCAN_Q - 1; j >= 0; --j) {
       if (j == SCAN_Q / 2 - 1) request();
       if (PACKED && j >= n) continue;
+      if (!PACKED && j + 1 < SCAN_Q && j + 1 == n) {
+        // What the tokens that fill the row's last block up have added: 0, or NaN where the last state is infinite.  (The
+        // block is the first one here.  8 x 2048 x 2048 826 us in all without this, 837 with it; leaving those tokens out by
+        // a branch 893, which more live scalars cost as well.)
+#pragma unroll
+        for (int i = 0; i < SCAN_NW; ++i) dA[i] = 0.f;
+      }
       BCAhead<T, SCAN_NW, FAST> now = ahead;
       float Bv[SCAN_NW], Cv[SCAN_NW];
       Bt -= j > 0 && j < n ? p.B_st : 0;

@@ -90,3 +90,37 @@ def test_encoder_takes_no_output_from_outside(off):
     assert y.shape == (len(off) - 1, 32) and torch.isfinite(y).all() and torch.isfinite(g).all()
     for s in range(len(off) - 1):
         assert off[s + 1] > off[s] or not y[s].any()
+
+
+# ------------------------------------------------------------------------------------------------ infinities
+def same_where_finite(name, got, ref, size, count, u_out):
+    """not a finite number in the same places, and close elsewhere"""
+    got = f64(got)
+    assert np.array_equal(np.isfinite(got), np.isfinite(ref)), (name, np.argwhere(np.isfinite(got) != np.isfinite(ref))[:4])
+    ok = np.isfinite(ref)
+    close(name, torch.from_numpy(got[ok]), ref[ok], size[ok], count, u_out)
+
+
+@pytest.mark.parametrize('what', ['u', 'B', 'C', 'dout'])
+@pytest.mark.parametrize('L,D,N', [(3, 16, 4), (8, 16, 16), (11, 70, 16), (13, 64, 8), (700, 10, 16), (515, 16, 5)])
+def test_an_infinity_at_the_last_token_stays_where_the_formulas_put_it(F, L, D, N, what):
+    """in the state that is kept, in that token's values; not in what has to do with the tokens before it only, such as dA"""
+    for packed in (False, True):
+        c = ScanCase(D, N, 1, torch.float32, rows=None if packed else (1, L), lengths=[L] if packed else None, seed=17)
+        at = {'u': (L - 1, 5), 'B': (L - 1, 0, 2), 'C': (L - 1, 0, 1), 'dout': (L - 1, 5)}[what]
+        for t in (c.dout,) if what == 'dout' else (c.cpu[what], c.gpu[what]):
+            t[at] = float('inf')
+        with np.errstate(all='ignore'):
+            r, m = c.ref(), c.ref(True)
+        v = {k: t.clone().requires_grad_() for k, t in c.gpu.items()}
+        out, state = c.call(F, v)
+        count = 12 * L + N + 64
+        flat = lambda t: t if packed else t.flatten(0, 1)                              # noqa: E731
+        same_where_finite('out', flat(out), r['out'], m['out'], count, U32)
+        same_where_finite('state', state, r['state'], m['state'], count, U32)
+        if what in ('u', 'B'):
+            assert np.array_equal(np.isinf(f64(state)), np.isinf(r['state']))
+        got = torch.autograd.grad((flat(out), state), list(v.values()), (c.dout.cuda(), c.dstate.cuda()))
+        for k, t in zip(v, got):
+            key = 'state_in' if k == 'state' else k
+            same_where_finite('d' + k, t, r[key], m[key], count + L + D, U32)
