@@ -40,3 +40,16 @@ def test_forward_mode_transforms_are_refused():
     for f in (torch.func.jvp, lambda f, a, b: torch.func.jacfwd(f)(*a)):
         with pytest.raises(RuntimeError, match='forward-mode'):
             f(lambda t: F.add_rms_norm(t, None, n)[0], (x,), (x,))
+
+
+@pytest.mark.parametrize('rows,L,D,G,split', [
+    (1, 4096, 2048, 1, True), (8, 2048, 2048, 1, True), (16, 1024, 2048, 1, True), (1, 31, 64, 1, False), (1, 1, 64, 1, False),
+    # a wave for most SIMDs, and many for each: the passes that chunks need cost more than they gain
+    (24, 512, 2048, 1, False), (32, 1024, 2048, 1, False), (96, 512, 2048, 1, False), (256, 512, 2048, 1, False),
+    (4096, 4096, 64, 1, False), (512, 512, 256, 4, False),
+])
+def test_the_scan_splits_the_time_axis_where_there_are_few_rows(rows, L, D, G, split):
+    """scratch is what tells from outside: without chunks the forward pass needs none"""
+    from hipvae._lib import lib
+    for keep in (0, 1):
+        assert (lib.dvae_selective_scan_fwd_ws_floats(rows, L, D, G, 16, keep) > 0) == split
