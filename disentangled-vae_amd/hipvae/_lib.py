@@ -1,4 +1,4 @@
-"""ctypes binding of libdvae_hip.so (the C ABI declared in include/dvae_hip.h).
+"""ctypes binding of libdvae_hip.so (the C ABI declared in include/dvae_hip.h), and what of the binding is in C++.
 
 There is no fallback: if the library has not been built, importing this module raises.
 """
@@ -165,3 +165,13 @@ def check(rc: int, what: str = ''):
     if rc != 0:
         msg = lib.dvae_last_error()
         raise DvaeError(f"{what} failed with code {rc}: {msg.decode() if msg else ''}")
+
+
+try:
+    from . import _norm as norm     # add_rms_norm, add_rms_norm_q8: the part of the binding that is in C++
+except ImportError as e:
+    raise ImportError(f"hipvae/_norm.so is missing or was built for another torch ({e}): build it with "
+                      f"`make -C {os.path.join(os.path.dirname(_HERE), 'csrc')}` or __graft_entry__.build()") from e
+norm.init(*(ctypes.cast(getattr(lib, n), c_void_p).value for n in (
+    'dvae_add_rms_norm_fwd', 'dvae_add_rms_norm_q8', 'dvae_add_rms_norm_bwd', 'dvae_add_rms_norm_bwd_ws_floats',
+    'dvae_last_error')))

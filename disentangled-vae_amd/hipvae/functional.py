@@ -23,6 +23,7 @@ from typing import List, Optional, Tuple
 import torch
 
 from . import ops
+from ._lib import norm
 
 Tensor = torch.Tensor
 BN_EPS = 1e-5
@@ -995,11 +996,15 @@ class LSTMDecoder(torch.autograd.Function):
 _forward_ad = torch.autograd.forward_ad
 
 
-def _wants_grad(what: str, *ts: Optional[Tensor]) -> bool:
+def _no_tangents(what: str, *ts: Optional[Tensor]):
     if _forward_ad._current_level >= 0:             # inside a dual level: a tangent must not be dropped without a word
         for t in ts:
             if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
                 raise RuntimeError(f"{what}: forward-mode derivatives are not computed")
+
+
+def _wants_grad(what: str, *ts: Optional[Tensor]) -> bool:
+    _no_tangents(what, *ts)
     if torch.is_grad_enabled():
         for t in ts:
             if t is not None and t.requires_grad:
@@ -1127,41 +1132,14 @@ def short_conv_step(state: Tensor, x: Tensor, weight: Tensor, bias: Optional[Ten
     return ops.short_conv_step(state, x, weight, bias, silu)
 
 
-class AddRMSNorm(torch.autograd.Function):
-    """see add_rms_norm"""
-
-    @staticmethod
-    def forward(ctx, x, residual, weight, eps):
-        a = ops.NormArgs('add_rms_norm', x, residual, weight)
-        y, total, rstd = ops.add_rms_norm_fwd(a, eps, True)
-        ctx.save_for_backward(x if residual is None else total, a.weight, rstd)
-        ctx.x_dtype = x.dtype
-        ctx.set_materialize_grads(False)
-        return y if residual is None else (y, total)
-
-    @staticmethod
-    def backward(ctx, dy, dsum=None):
-        _no_second_derivative('add_rms_norm')
-        total, weight, rstd = ctx.saved_tensors
-        if dy is None:
-            if dsum is None:
-                return None, None, None, None
-            dy = torch.zeros(dsum.shape, dtype=ctx.x_dtype, device=dsum.device)
-        dx, dres, dw = ops.add_rms_norm_bwd(dy, dsum, total, weight, rstd, ctx.x_dtype)
-        need = ctx.needs_input_grad
-        return dx if need[0] else None, dres if need[1] else None, dw if need[2] else None, None
-
-
 def add_rms_norm(x: Tensor, residual: Optional[Tensor], weight: Tensor, eps: float = 1e-6):
     """-> (y, sum): sum = x + residual, y = sum / sqrt(mean(sum^2) + eps) * weight over the last dimension.  x [...,
     channels] fp32 or bf16, y of its type; residual of the same type or fp32 (a residual stream kept in fp32 beside bf16
     activations), sum of the residual's; weight [channels] fp32.  The norm is that of the sum as stored.  Without a
     residual the sum is x itself."""
-    if _wants_grad('add_rms_norm', x, residual, weight):
-        got = AddRMSNorm.apply(x, residual, weight, eps)
-        return (got, x) if residual is None else got
-    y, total, _ = ops.add_rms_norm_fwd(ops.NormArgs('add_rms_norm', x, residual, weight), eps, False)
-    return y, x if residual is None else total
+    _no_tangents('add_rms_norm', x, residual, weight)
+    y, total = norm.add_rms_norm(x, residual, weight, eps)
+    return y, x if total is None else total
 
 
 def add_rms_norm_q8(x: Tensor, residual: Optional[Tensor], weight: Tensor, eps: float = 1e-6):
@@ -1169,4 +1147,5 @@ def add_rms_norm_q8(x: Tensor, residual: Optional[Tensor], weight: Tensor, eps: 
     scale = max|y| / 448 of its row, so that the row's largest value is the type's largest (a row of zeros: 1; not below
     2^-126).  For inference: no gradients."""
     _no_grad_form('add_rms_norm_q8', x, residual, weight)
-    return ops.add_rms_norm_q8(x, residual, weight, eps)
+    q, scale, total = norm.add_rms_norm_q8(x, residual, weight, eps)
+    return q, scale, x if total is None else total

@@ -1378,95 +1378,6 @@ def short_conv_step(state, x, weight, bias=None, silu=False) -> Tensor:
     return out
 
 
-def _norm_rows(what: str, name: str, t: Optional[Tensor], shape, dtype, device: int) -> Optional[Tensor]:
-    """an activation [..., channels] as rows of equal stride"""
-    t = _act(what, name, t, shape, dtype, device)
-    return t if t is None or len(shape) == 2 else t.reshape(-1, shape[-1])
-
-
-class NormArgs:
-    """The checked arguments of a norm."""
-
-    def __init__(self, what, x, residual, weight):
-        self.dtype = _act_dtype(what, x)
-        shape, dt, dev = self.shape, self.act, self.index = x.shape, x.dtype, x.get_device()
-        self.device = x.device
-        if len(shape) < 1 or shape[-1] < 1:
-            raise RuntimeError(f"{what}: expected [..., channels], got {tuple(shape)}")
-        self.D = shape[-1]
-        self.like = x
-        self.x = _norm_rows(what, 'x', x, shape, dt, dev)
-        self.rows = self.x.shape[0]
-        self.sum_dtype, self.rdtype, self.residual = dt, self.dtype, None
-        if residual is not None:
-            if residual.dtype is torch.float32:         # x's type, or fp32
-                self.sum_dtype, self.rdtype = torch.float32, 0
-            self.sum_like = residual
-            self.residual = _norm_rows(what, 'residual', residual, shape, self.sum_dtype, dev)
-        self.weight = _param(what, 'weight', weight, (self.D,), dev)
-
-    def head(self, eps):
-        r = self.residual
-        return (self.x.data_ptr(), self.x.stride(0), None if r is None else r.data_ptr(), 0 if r is None else r.stride(0),
-                self.weight.data_ptr(), eps)
-
-
-def add_rms_norm_fwd(a: NormArgs, eps: float, keep: bool):
-    """-> y, sum [..., channels] (None without a residual: it is x), rstd [rows] or None"""
-    dev = a.device
-    if a.index != _device_now():
-        with torch.cuda.device(dev):
-            return add_rms_norm_fwd(a, eps, keep)
-    y = _new_like(a.like)
-    total = None if a.residual is None else _new_like(a.sum_like)
-    rstd = torch.empty(a.rows, dtype=torch.float32, device=dev) if keep else None
-    check(lib.dvae_add_rms_norm_fwd(*a.head(eps), y.data_ptr(), _p(total), _p(rstd), a.rows, a.D, a.dtype, a.rdtype,
-                                    _stream_of(a.index)), 'add_rms_norm_fwd')
-    return y, total, rstd
-
-
-def add_rms_norm_q8(x: Tensor, residual: Optional[Tensor], weight: Tensor, eps: float = 1e-6):
-    """add_rms_norm with the output in 8 bits -> (q of type float8_e4m3fn, scale [...] fp32, sum): the normalised row
-    is q * scale, scale = max|y| / 448 of the row (1 for a row of zeros)"""
-    a = NormArgs('add_rms_norm_q8', x, residual, weight)
-    dev = a.device
-    if a.index != _device_now():
-        with torch.cuda.device(dev):
-            return add_rms_norm_q8(x, residual, weight, eps)
-    q = torch.empty(a.shape, dtype=torch.float8_e4m3fn, device=dev)
-    scale = torch.empty(a.shape[:-1], dtype=torch.float32, device=dev)
-    total = None if a.residual is None else _new_like(a.sum_like)
-    check(lib.dvae_add_rms_norm_q8(*a.head(eps), q.data_ptr(), scale.data_ptr(), _p(total), a.rows, a.D, a.dtype, a.rdtype,
-                                   _stream_of(dev.index)), 'add_rms_norm_q8')
-    return q, scale, x if total is None else total
-
-
-def add_rms_norm_bwd(dy: Tensor, dsum: Optional[Tensor], total: Tensor, weight: Tensor, rstd: Tensor, dx_dtype):
-    """dy [..., channels] of x's type, dsum and total of the sum's -> dx, dresidual (the same tensor where the types are
-    the same: autograd then copies before it keeps either), dweight"""
-    what = 'add_rms_norm_bwd'
-    dev = dy.device
-    if dev.index != _device_now():
-        with torch.cuda.device(dev):
-            return add_rms_norm_bwd(dy, dsum, total, weight, rstd, dx_dtype)
-    shape = dy.shape
-    D = shape[-1]
-    dy2 = _norm_rows(what, 'dy', dy, shape, dx_dtype, dev.index)
-    ds2 = _norm_rows(what, 'dsum', dsum, shape, total.dtype, dev.index)
-    s2 = _norm_rows(what, 'sum', total, shape, total.dtype, dev.index)
-    rows = dy2.shape[0]
-    dres = _new_like(total)
-    dx = dres if total.dtype == dx_dtype else _new_like(dy)
-    if rows == 0:
-        return dx, dres, torch.zeros_like(weight)
-    dw = _new_like(weight)
-    ws = torch.empty(lib.dvae_add_rms_norm_bwd_ws_floats(rows, D), dtype=torch.float32, device=dev)
-    check(lib.dvae_add_rms_norm_bwd(_p(dy2), dy2.stride(0), _p(ds2), 0 if ds2 is None else ds2.stride(0), _p(s2),
-                                    s2.stride(0), _p(weight), _p(rstd), _p(dres), _p(dx), _p(dw), rows, D,
-                                    _ACT_DTYPES[dx_dtype], _ACT_DTYPES[total.dtype], _p(ws), _stream_of(dev.index)), what)
-    return dx, dres, dw
-
-
 # ---------------------------------------------------------------------------- launch trace (benchmarks)
 def trace_begin(max_launches: int = 1 << 16):
     """From here to trace_collect() every kernel launch of the library is timed with two events on its

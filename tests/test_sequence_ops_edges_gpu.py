@@ -124,3 +124,103 @@ def test_an_infinity_at_the_last_token_stays_where_the_formulas_put_it(F, L, D, 
         for k, t in zip(v, got):
             key = 'state_in' if k == 'state' else k
             same_where_finite('d' + k, t, r[key], m[key], count + L + D, U32)
+
+
+# ------------------------------------------------------------------------------------------------ the norm's node
+def norm_leaves(shape, dtype=torch.float32, rtype=torch.float32, seed=0):
+    g = gen(seed)
+    return (rnd(g, *shape).to(dtype).cuda().requires_grad_(), rnd(g, *shape).to(rtype).cuda().requires_grad_(),
+            (1 + rnd(g, shape[-1], scale=0.3)).cuda().requires_grad_())
+
+
+@pytest.mark.parametrize('dtype,rtype', [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16),
+                                         (torch.bfloat16, torch.float32)])
+@pytest.mark.parametrize('shape', [(96,), (1, 96), (6, 96), (2, 3, 96), (2, 3, 1), (5, 13)])
+def test_norm_gradients_in_any_layout(F, shape, dtype, rtype):
+    """incoming gradients that are transposed, cut out of something wider, or one row for all: as their contiguous copies"""
+    x, r, w = norm_leaves(shape, dtype, rtype)
+    y, s = F.add_rms_norm(x, r, w)
+    g = gen(3)
+    dy, ds = rnd(g, *shape).to(dtype).cuda(), rnd(g, *shape).to(rtype).cuda()
+    grads = lambda a, b: torch.autograd.grad((y, s), (x, r, w), (a, b), retain_graph=True)                # noqa: E731
+    turned = lambda t: t.transpose(0, -1).contiguous().transpose(0, -1) if t.dim() > 1 else t.repeat_interleave(2)[::2]  # noqa: E731
+    cut = lambda t: torch.nn.functional.pad(t, (3, 5), value=9.0)[..., 3:-5]                              # noqa: E731
+    want = grads(dy, ds)
+    for f in (turned, cut):
+        assert torch.equal(f(dy), dy)
+        # (the cut rows are no longer on 16 bytes and take the other kernel: its sums are in another order)
+        for a, b in zip(want, grads(f(dy), f(ds))):
+            torch.testing.assert_close(a, b, rtol=2 * HALF[a.dtype] if a.dtype != torch.float32 else 1e-5, atol=1e-5)
+    row = dy.reshape(-1, shape[-1])[:1].reshape((1,) * (len(shape) - 1) + (-1,)).expand(shape)
+    for a, b in zip(grads(row, ds), grads(row.contiguous(), ds)):
+        torch.testing.assert_close(a, b, rtol=2 * HALF[a.dtype] if a.dtype != torch.float32 else 1e-5, atol=1e-5)
+
+
+def test_norm_with_one_of_its_outputs_used(F):
+    x, r, w = norm_leaves((7, 64), torch.bfloat16, torch.float32)
+    y, s = F.add_rms_norm(x, r, w)
+    d = torch.randn_like(s)
+    dx, dr, dw = torch.autograd.grad(s, (x, r, w), d, retain_graph=True)
+    assert torch.equal(dr, d) and torch.equal(dx, d.bfloat16()) and not dw.any()
+    one = torch.autograd.grad(y, (x, r, w), torch.ones_like(y), retain_graph=True)
+    two = torch.autograd.grad((y, s), (x, r, w), (torch.ones_like(y), torch.zeros_like(s)))
+    assert all(torch.equal(a, b) for a, b in zip(one, two))
+
+
+@pytest.mark.parametrize('which', [0, 1, 2])
+def test_norm_with_one_leaf(F, which):
+    leaves = norm_leaves((9, 64))
+    y, s = F.add_rms_norm(*leaves)
+    want = torch.autograd.grad((y, s), leaves, (torch.ones_like(y), torch.ones_like(s)))
+    some = [t.detach() for t in leaves]
+    some[which].requires_grad_()
+    y, s = F.add_rms_norm(*some)
+    (got,) = torch.autograd.grad((y, s), (some[which],), (torch.ones_like(y), torch.ones_like(s)))
+    assert torch.equal(got, want[which])
+    with torch.no_grad():
+        assert not F.add_rms_norm(*leaves)[0].requires_grad
+    assert not F.add_rms_norm(*(t.detach() for t in leaves))[0].requires_grad
+
+
+def test_norm_of_no_rows_has_gradients(F):
+    for shape in ((0, 64), (2, 0, 64)):
+        x, r, w = norm_leaves(shape, torch.bfloat16, torch.float32)
+        y, s = F.add_rms_norm(x, r, w)
+        dx, dr, dw = torch.autograd.grad((y, s), (x, r, w), (torch.ones_like(y), torch.ones_like(s)))
+        assert dx.shape == x.shape and dr.shape == r.shape and dw.shape == w.shape and not dw.any()
+        q, scale, total = F.add_rms_norm_q8(x.detach(), r.detach(), w.detach())
+        assert q.shape == shape and scale.shape == shape[:-1] and total.dtype == torch.float32
+
+
+def test_norm_backward_twice_again_and_after_a_change(F):
+    leaves = norm_leaves((5, 64))
+    y, s = F.add_rms_norm(*leaves)
+    d = torch.ones_like(y)
+    a = torch.autograd.grad(y, leaves, d, retain_graph=True)
+    b = torch.autograd.grad(y, leaves, d, retain_graph=True)
+    assert all(torch.equal(u, v) for u, v in zip(a, b))
+    with pytest.raises(RuntimeError, match='differentiated again'):
+        torch.autograd.grad(y, leaves, d, retain_graph=True, create_graph=True)
+    with torch.no_grad():
+        s.add_(1.0)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        torch.autograd.grad(y, leaves, d)
+    y, _ = F.add_rms_norm(leaves[0], None, leaves[2])
+    with torch.no_grad():
+        leaves[0].add_(1.0)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        torch.autograd.grad(y, leaves[0], d)
+
+
+def test_norm_gradients_on_another_stream(F):
+    leaves = norm_leaves((3000, 256))
+    y, s = F.add_rms_norm(*leaves)
+    want = torch.autograd.grad((y, s), leaves, (torch.ones_like(y), torch.ones_like(s)))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        mine = [(t.detach() * 1.0).requires_grad_() for t in leaves]
+        y, s = F.add_rms_norm(*mine)
+        got = torch.autograd.grad((y, s), mine, (torch.ones_like(y), torch.ones_like(s)))
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
