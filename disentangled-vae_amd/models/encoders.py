@@ -147,13 +147,13 @@ class SSMEncoder(nn.Module):
     Each layer is residual: root-mean-square norm -> projection to a path and a gate -> short causal convolution ->
     projection to step sizes, B and C -> selective scan, gated -> projection back.  Like LSTMEncoder it returns the last
     token's output, or with return_sequence the whole sequence, and the states that the sequences end with; a caller that
-    has no use for those sets `return_states = False`.
+    has no use for those sets `return_states = False`, and none are made.
 
     forward() takes [batch, length, input_dim], or packed [tokens, input_dim] with `offsets` (int32, see
     hipvae.functional.selective_scan; the output of an empty sequence is 0, and where there are no tokens at all nothing
-    depends on the parameters).  step() takes the next token of every
-    sequence, [batch, input_dim], and updates `states` in place (no gradients): a frame's cost does not grow with the
-    frames before it."""
+    depends on the parameters).  step() takes the next token of every sequence, [batch, input_dim], and updates `states` in
+    place (no gradients): a frame's cost does not grow with the frames before it.  fp32, as the matrix products of this
+    package; training needs input_dim, hidden_dim and 2 * groups * state_dim to be multiples of 4."""
     return_states = True
 
     def __init__(self, input_dim: int = 512, hidden_dim: int = 256, num_layers: int = 1, state_dim: int = 16,
@@ -210,12 +210,13 @@ class SSMEncoder(nn.Module):
             conv_state, scan_state = states[i] if states is not None else (None, None)
             y, residual = HF.add_rms_norm(h, residual, layer.norm)
             u, z = HF.linear(y, layer.in_proj.weight, None).chunk(2, -1)
-            u, conv_end = HF.short_conv(u, layer.conv_weight, layer.conv_bias, silu=True, state=conv_state,
-                                        offsets=offsets, return_state=True)
+            u = HF.short_conv(u, layer.conv_weight, layer.conv_bias, silu=True, state=conv_state, offsets=offsets,
+                              return_state=self.return_states)
+            u, conv_end = u if self.return_states else (u, None)
             delta, B, C = self._projected(layer, u)
-            y, scan_end = HF.selective_scan(u, delta, -torch.exp(layer.A_log), B, C, D=layer.D, z=z,
-                                            delta_bias=layer.dt_bias, delta_softplus=True, state=scan_state,
-                                            offsets=offsets, return_state=True)
+            y = HF.selective_scan(u, delta, -torch.exp(layer.A_log), B, C, D=layer.D, z=z, delta_bias=layer.dt_bias,
+                                  delta_softplus=True, state=scan_state, offsets=offsets, return_state=self.return_states)
+            y, scan_end = y if self.return_states else (y, None)
             h = HF.linear(y, layer.out_proj.weight, None)
             ends.append((conv_end, scan_end))
         y, _ = HF.add_rms_norm(h, residual, self.norm)

@@ -224,3 +224,18 @@ def test_norm_gradients_on_another_stream(F):
         got = torch.autograd.grad((y, s), mine, (torch.ones_like(y), torch.ones_like(s)))
     torch.cuda.current_stream().wait_stream(side)
     assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.parametrize('packed', [False, True])
+def test_encoder_that_returns_no_states_makes_none(F, monkeypatch, packed):
+    m = ssm()
+    x = torch.randn(*((23,) if packed else (3, 9)), 24, device='cuda')
+    off = torch.tensor([0, 5, 5, 23], dtype=torch.int32, device='cuda') if packed else None
+    want, states = m(x, return_sequence=True, offsets=off)
+    asked = []
+    for name in ('short_conv', 'selective_scan'):
+        real = getattr(F, name)
+        monkeypatch.setattr(F, name, lambda *a, real=real, **k: asked.append(k.get('return_state', False)) or real(*a, **k))
+    m.return_states = False
+    y, none = m(x, return_sequence=True, offsets=off)
+    assert none is None and asked == [False] * 4 and torch.equal(y, want)
