@@ -61,35 +61,15 @@ __device__ __forceinline__ Marks block_marks(SeqWalk w, int t0, int n) {
   return m;
 }
 
-// the N values of B or C at one token.  FAST: N == NP and 4-byte aligned, read as whole words
-template <typename T, int NP, bool FAST> struct BCLoad;
-template <int NP> struct BCLoad<float, NP, true> {
-  static __device__ __forceinline__ void get(const float* p, int64_t off, int, float (&v)[NP]) {
+// the N values of B or C at one token, element by element
+template <typename T, int NP> __device__ __forceinline__ void load_each(const T* p, int N, float (&v)[NP]) {
 #pragma unroll
-    for (int n = 0; n < NP; ++n) v[n] = uniform_load(p + off, n);
-  }
-};
-template <int NP> struct BCLoad<bf16_t, NP, true> {
-  static __device__ __forceinline__ void get(const bf16_t* p, int64_t off, int, float (&v)[NP]) {
-    const uint32_t* q = (const uint32_t*)(p + off);
-#pragma unroll
-    for (int n = 0; n < NP / 2; ++n) {
-      const uint32_t w = uniform_load(q, n);
-      v[2 * n] = __uint_as_float(w << 16);
-      v[2 * n + 1] = __uint_as_float(w & 0xffff0000u);
-    }
-  }
-};
-template <typename T, int NP> struct BCLoad<T, NP, false> {
-  static __device__ __forceinline__ void get(const T* p, int64_t off, int N, float (&v)[NP]) {
-#pragma unroll
-    for (int n = 0; n < NP; ++n) v[n] = n < N ? to_f32(p[off + n]) : 0.f;
-  }
-};
+  for (int n = 0; n < NP; ++n) v[n] = n < N ? to_f32(p[n]) : 0.f;
+}
 
-// The same, requested ahead.  Scalar loads return in any order, so waiting for one means waiting for all: `arrived`
-// makes the words of this token a dependence of the address of the next one's, which puts the wait before the next
-// request and a token's arithmetic between a request and its wait.
+// B and C, requested a token ahead.  FAST: N == NP and 4-byte aligned, read as whole words.  Scalar loads return in any
+// order, so waiting for one means waiting for all: `arrived` makes the words of this token a dependence of the address of
+// the next one's, which puts the wait before the next request and a token's arithmetic between a request and its wait.
 template <int K> struct Words { typedef uint32_t vec __attribute__((ext_vector_type(K), aligned(4))); };
 template <typename T, int NP, bool FAST> struct BCAhead {
   typename Words<NP * sizeof(T) / 4>::vec b, c;
@@ -116,10 +96,10 @@ template <typename T, int NP, bool FAST> struct BCAhead {
 template <typename T, int NP> struct BCAhead<T, NP, false> {
   float b[NP], c[NP];
   __device__ __forceinline__ void request(const T* B, const T* C, int N) {
-    BCLoad<T, NP, false>::get(B, 0, N, b);
-    BCLoad<T, NP, false>::get(C, 0, N, c);
+    load_each(B, N, b);
+    load_each(C, N, c);
   }
-  __device__ __forceinline__ void request_b(const T* B, int N) { BCLoad<T, NP, false>::get(B, 0, N, b); }
+  __device__ __forceinline__ void request_b(const T* B, int N) { load_each(B, N, b); }
   __device__ __forceinline__ void arrived(const T*&, const T*&) {}
   __device__ __forceinline__ void arrived_b(const T*&) {}
   __device__ __forceinline__ void get(float (&bv)[NP], float (&cv)[NP]) const {
