@@ -239,3 +239,62 @@ def test_encoder_that_returns_no_states_makes_none(F, monkeypatch, packed):
     m.return_states = False
     y, none = m(x, return_sequence=True, offsets=off)
     assert none is None and asked == [False] * 4 and torch.equal(y, want)
+
+
+# ------------------------------------------------------------------------------------------------ roundings, quantity by quantity
+def check_each(F, c):
+    """Every output and gradient with the roundings of its own sums: 12 per token of the longest sequence for the decays that a
+    term passes, one per summed state, 64 for step sizes and gates; where a sum runs over channels (dB, dC) or tokens (dA, dD,
+    ddelta_bias), one for each of those."""
+    D, N = c.cpu['A'].shape
+    base = 12 * c.longest + N + 64
+    more = {'B': D, 'C': D, 'A': c.T, 'D': c.T, 'bias': c.T}
+    r, m = c.ref(), c.ref(True)
+    flat = lambda t: t.flatten(0, 1) if c.rows else t                                  # noqa: E731
+    v = {k: None if t is None else t.clone().requires_grad_() for k, t in c.gpu.items()}
+    out, state = c.call(F, v)
+    close('out', flat(out), r['out'], m['out'], base, HALF[c.dtype])
+    close('state', state, r['state'], m['state'], base, U32)
+    names = [k for k in v if v[k] is not None]
+    got = torch.autograd.grad((flat(out), state), [v[k] for k in names], (c.dout.cuda(), c.dstate.cuda()))
+    for k, t in zip(names, got):
+        key = 'state_in' if k == 'state' else k
+        close('d' + k, t, r[key], m[key], base + more.get(k, 0), HALF[t.dtype])
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('D,N,G', [(20, 16, 1), (70, 8, 2), (33, 5, 1), (24, 13, 2), (8, 1, 1)])
+@pytest.mark.parametrize('lengths,tail', [([3] * 300, 0), ([64, 64, 500, 0, 1, 700, 63], 5), ([0, 900, 0], 200)])
+def test_packed_gradients_over_several_chunks(F, lengths, tail, D, N, G, dtype):
+    check_each(F, ScanCase(D, N, G, dtype, lengths=lengths, tail=tail, seed=N))
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('rows,D,N,G', [((2, 17), 96, 8, 3), ((3, 33), 256, 16, 1), ((2, 130), 24, 13, 1), ((1, 700), 64, 16, 1),
+                                        ((2, 515), 10, 16, 1), ((1, 1025), 130, 8, 2), ((800, 70), 40, 16, 1)])
+def test_roundings_of_each_quantity(F, rows, D, N, G, dtype):
+    check_each(F, ScanCase(D, N, G, dtype, rows=rows, seed=3))
+
+
+def test_gradients_past_2_to_the_31_elements(F):
+    """the last tokens' gradient of u, in the first and the last channels, against the formulas"""
+    D, T, n, N = 32768, 66000, 40, 4
+    off = torch.tensor([0, 7, T - n, T], dtype=torch.int32, device='cuda')
+    x = torch.zeros(T, D, dtype=torch.bfloat16, device='cuda')
+    x[T - n:] = torch.randn(n, D, device='cuda').bfloat16()
+    delta = x.detach()
+    A = -torch.rand(D, N, device='cuda') - 0.5
+    B = torch.randn(T, N, device='cuda').bfloat16()
+    x = x.requires_grad_()
+    out = F.selective_scan(x, delta, A, B, B, delta_softplus=True, offsets=off)
+    d = torch.zeros_like(out)
+    d[T - n:] = torch.randn(n, D, device='cuda').bfloat16()
+    (g,) = torch.autograd.grad(out, (x,), d)
+    assert not g[:T - n].any()
+    for c in (slice(0, 64), slice(D - 64, D)):
+        tail = lambda t: f64(t[T - n:])                                                # noqa: E731
+        args = (tail(x[:, c]), tail(delta[:, c]), f64(A[c]), tail(B)[:, None], tail(B)[:, None], [0, n])
+        r, m = (R.scan(*args, dout=tail(d[:, c]), size=s) for s in (False, True))
+        count = 12 * n + N + 64
+        close('out', out[T - n:, c], r['out'], m['out'], count, HALF[torch.bfloat16])
+        close('du', g[T - n:, c], r['u'], m['u'], count, HALF[torch.bfloat16])
