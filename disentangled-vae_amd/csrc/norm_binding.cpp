@@ -2,8 +2,8 @@
 //
 // In C++ because the norm's smallest training calls are shorter than what a node written in Python costs: the autograd
 // engine runs it in a thread of its own, which has to take the interpreter's lock and hand it back, and where idle cores
-// sleep each of those turns wakes one up.  255 x 64 fp32, forward and backward: 66 us with a Python node, 45 with this; where
-// idle cores sleep 126 and 79.  The same in elementary torch operations, without the engine: 90.
+// sleep each of those turns wakes one up.  255 x 64 fp32, forward and backward: 66 us with a Python node, 47 with this; where
+// idle cores sleep 126 and 78.  The same in elementary torch operations, without the engine: 91.
 #include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>

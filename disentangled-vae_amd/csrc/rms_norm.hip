@@ -4,11 +4,13 @@
 //
 // Bound by memory.  A wave owns a row and holds it in registers between the reduction and the output (up to 64 values
 // per lane: rows of up to 4096 elements whose tensors are 16-byte aligned), so every tensor crosses memory once and no
-// barrier is needed.  Longer or unaligned rows take one workgroup each, which reads its row a second time.
+// barrier is needed.  Longer or unaligned rows take one workgroup each, which goes element by element and reads its row a
+// second time, and dw is a pass of its own.
 //
 // 16384 x 2048 bf16: forward 57 us (4.7 TB/s of x, residual, sum and y), backward 65 us (4.1 TB/s of dy, dsum, sum and
-// dresidual) and 4 us for the sums of its partial rows; 4099 x 2560 bf16 into 8 bits: 17.5 us (4.2 TB/s).  A copy of 2 GiB
-// runs at 4.9 TB/s on the same card.
+// dresidual) and 4 us for the sums of its partial rows; with an fp32 residual 85 us (4.7 TB/s) and 112 us (4.8 TB/s); 4099 x
+// 2560 bf16 into 8 bits: 18 us (4.1 TB/s).  A copy of 2 GiB runs at 4.9 TB/s on the same card.  Rows of the second kind:
+// 4096 x 8192 bf16 forward 101 us (2.7 TB/s), backward 109 and 28 for dw; 16384 x 2047 bf16 113, 109 and 30 us.
 #include "seq_common.h"
 
 struct NormArgs {

@@ -61,7 +61,9 @@ __device__ __forceinline__ Marks block_marks(SeqWalk w, int t0, int n) {
   return m;
 }
 
-// the N values of B or C at one token, element by element
+// The N values of B or C at one token, element by element: other numbers of states than 8 and 16, and bf16 rows off 4 bytes.
+// No scalar loads of 16 bits exist, so in bf16 these come through the vector unit, the same for all lanes: 8 x 2048 x 2048
+// with 12 states 541 us for the outputs and 1388 for the way back, with 16 states 156 and 496.
 template <typename T, int NP> __device__ __forceinline__ void load_each(const T* p, int N, float (&v)[NP]) {
 #pragma unroll
   for (int n = 0; n < NP; ++n) v[n] = n < N ? to_f32(p[n]) : 0.f;
@@ -124,8 +126,9 @@ __device__ __forceinline__ T touch_rows(const T* B, int64_t b_st, const T* C, in
 __device__ __forceinline__ void touched(float v) { asm volatile("" :: "v"(v)); }
 __device__ __forceinline__ void touched(bf16_t v) { asm volatile("" :: "v"((uint32_t)v)); }
 
-// 64 channels of one group, one chunk of one row.  A workgroup's tiles are neighbours in a group; a tile is the work of
-// one wave, or of `share` waves that have a part of the states each.
+// 64 channels of one group, one chunk of one row (of narrower groups the lanes left over repeat the last channel: 8 x 2048 x
+// 2048 bf16 in 64 groups of 32, outputs 366 us and way back 1666, in one group 156 and 496).  A workgroup's tiles are
+// neighbours in a group; a tile is the work of one wave, or of `share` waves that have a part of the states each.
 struct Tile {
   int g, d, lane, wave, part, chunk, row, t0, t1;
   bool on, idle;
@@ -268,14 +271,14 @@ static __device__ const float no_input[SCAN_MAX_N] = {};     // B where there is
 //
 // A block's inputs were requested a block ahead, B and C are a token ahead.  Lanes past the group's last channel compute
 // that channel too and store the same values to the same places, so that no store depends on the lane.  Without packed
-// sequences a block is straight-line code: tokens past the chunk's last repeat the last one with a step size of 0, which
-// leaves the state as it is and stores the same output again.  What packed sequences' borders need stands behind
-// wave-uniform branches, and so do their chunks' ends.  (Branches for both: 8 x 2048 x 2048 backward 12 % slower.)
+// sequences a block is straight-line code: tokens past the chunk's last repeat the last one with a step size of 0 and a B of
+// zeros, which leaves the state as it is and stores the same output again.  What packed sequences' borders need stands
+// behind wave-uniform branches, and so do their chunks' ends.  (Branches for both: 8 x 2048 x 2048 training 8 % slower.)
 //
 // Bound by vector arithmetic: a state of a token takes five issue slots in the state pass (two of them the exponential) and
 // six in the output pass, a channel's token about 25 more (softplus, gate, conversions).  8 x 2048 x 2048 bf16, N = 16:
-// states 114 us, of which 80 are issue slots; outputs 160 us, of which 119, while it reads 268 MB and writes as much again
-// of kept states (3.4 TB/s).  1 x 4096 x 2048: 33 and 42 us.  256 x 20 x 1024 fp32 (one chunk): 41 us.
+// states 110 us, of which 80 are issue slots; outputs 156 us, of which 119, while it reads 201 MB and writes 335, 268 of them
+// kept states (3.4 TB/s).  1 x 4096 x 2048: 33 and 42 us.  256 x 20 x 1024 fp32 (one chunk): 42 us.
 template <typename T, int NP, bool PACKED, bool FAST, bool STATE_ONLY>
 __global__ void __launch_bounds__(256) scan_fwd_kernel(ScanArgs p) {
   const Tile w(p);
@@ -516,7 +519,7 @@ __device__ __forceinline__ float wave_sums16(float (&v)[16], int lane) {
 
 // The adjoint that leaves a chunk to the left if nothing enters it from the right: the sum of C[n] g of its tokens up to
 // the first start of a sequence, each through the decays from the chunk's first token to its own: the exponential of the
-// step sizes added up so far, so no token waits for another.  8 x 2048 x 2048 bf16: 137 us, 90 of them issue slots.
+// step sizes added up so far, so no token waits for another.  8 x 2048 x 2048 bf16: 134 us, 90 of them issue slots.
 template <typename T, int NP, bool PACKED, bool FAST>
 __global__ void __launch_bounds__(256) scan_bwd_state_kernel(ScanArgs p) {
   const Tile w(p);
@@ -607,8 +610,8 @@ __global__ void __launch_bounds__(256) scan_bwd_state_kernel(ScanArgs p) {
 // from the waves' parts of y, of the sum of dh B and of that of k A, all by way of LDS.
 //
 // Bound by vector arithmetic: 177 instructions per token and wave (8 states of 64 channels), 47 slots of them the sums over
-// the lanes.  8 x 2048 x 2048 bf16: 505 us, of which 355 are issue slots at two waves per SIMD; it moves 0.77 GB.  256 x 20
-// x 1024 fp32: 98 us.  Without keeping the decays three waves would fit a SIMD but for spilled registers: 927 us.  Two
+// the lanes.  8 x 2048 x 2048 bf16: 496 us, of which 355 are issue slots at two waves per SIMD; it moves 0.77 GB.  256 x 20
+// x 1024 fp32: 103 us.  Without keeping the decays three waves would fit a SIMD but for spilled registers: 927 us.  Two
 // tiles per workgroup, not four: fewer waves wait at a barrier (four: 6 % slower; one: 2 %, and twice the partial rows).
 #define SCAN_NW 8
 #define SCAN_BT 2      // tiles per workgroup

@@ -1057,7 +1057,9 @@ def selective_scan(u: Tensor, delta: Tensor, A: Tensor, B: Tensor, C: Tensor, D:
 
     u, delta, z [batch, length, channels] fp32 or bf16; A [channels, states], at most 16 states; B, C [batch, length,
     groups, states] (or without the group dimension), groups dividing the channels; D, delta_bias [channels]; parameters
-    and states fp32.  Any strides: only the last dimension of an activation is copied if it is not contiguous.
+    and states fp32.  Any strides (from token to token below 2^26 elements): only the last dimension of an activation is
+    copied if it is not contiguous.  For the backward pass the states are kept every eight tokens, in fp32: half a byte per
+    token, channel and state.
 
     `offsets` (int32, ascending, first 0): sequences of different lengths, some possibly empty, packed one after the
     other into [tokens, channels]; sequence s is tokens offsets[s] to offsets[s + 1].  Tokens behind the last sequence

@@ -586,9 +586,9 @@ int dvae_adam_advance_f32(float* dyn, double beta1, double beta2, dvae_stream_t 
 /* dt = softplus(delta + bias) (softplus != 0; else delta + bias), h[n] = exp(dt A[d,n]) h[n] + dt u B[n],
  * out = (sum_n C[n] h[n] + Dp u) silu(z).  u, delta, z, out [rows,L,D]; A [D,N], N <= 16; B, C [rows,L,G,N], G divides D;
  * Dp, bias [D]; state0 (entering) and state1 (final) [S,D,N].  NULL: Dp, z, bias, state0, state1, offsets, ckpt.
- * Final states of sequences without tokens are those they enter with (nothing is written if there is no token at all).  ckpt (dvae_selective_scan_ckpt_floats): the states that
- * the backward pass starts from, kept if not NULL.  ws: dvae_selective_scan_fwd_ws_floats floats (0 where the time axis is
- * not split; NULL then).  Token strides of u, delta, z and dout must be below 2^26 elements where L > 1. */
+ * Final states of sequences without tokens are those they enter with (nothing is written if there is no token at all).
+ * ckpt (dvae_selective_scan_ckpt_floats): the states that the backward pass starts from, kept if not NULL.
+ * ws: dvae_selective_scan_fwd_ws_floats floats (0 where the time axis is not split; NULL then).  Token strides of u, delta, z and dout must be below 2^26 elements where L > 1. */
 int64_t dvae_selective_scan_ckpt_floats(int64_t rows, int64_t L, int64_t D, int64_t N);
 int64_t dvae_selective_scan_fwd_ws_floats(int64_t rows, int64_t L, int64_t D, int64_t G, int64_t N,
                                           int keep /* whether ckpt is given */);
@@ -599,8 +599,8 @@ int dvae_selective_scan_fwd(const void* u, int64_t u_sb, int64_t u_st, const voi
                             float* state1, const int32_t* offsets, void* out, float* ckpt, int64_t rows, int64_t L,
                             int64_t D, int64_t G, int64_t N, int64_t S, int dtype, float* ws, dvae_stream_t stream);
 /* Gradients from dout and (NULL: zero) dstate1, the gradient of the final states.  dA, dD, dbias, dstate0 may be NULL;
- * dstate0 of sequences without tokens is not written (it is dstate1 there).  ckpt as the forward pass filled it (it is read only); ws:
- * dvae_selective_scan_bwd_ws_floats floats. */
+ * dstate0 of sequences without tokens is not written (it is dstate1 there).  ckpt as the forward pass filled it (it is read
+ * only); ws: dvae_selective_scan_bwd_ws_floats floats. */
 int64_t dvae_selective_scan_bwd_ws_floats(int64_t rows, int64_t L, int64_t D, int64_t G, int64_t N);
 int dvae_selective_scan_bwd(const void* u, int64_t u_sb, int64_t u_st, const void* delta, int64_t delta_sb,
                             int64_t delta_st, const float* A, const void* B, int64_t B_sb, int64_t B_st, int64_t B_sg,

@@ -12,7 +12,8 @@ def _calls(dual):
     return {
         'selective_scan': [lambda: F.selective_scan(dual(x), x, w, bc, bc), lambda: F.selective_scan(x, x, w, bc, bc, D=dual(n)),
                            lambda: F.selective_scan(x, x, w, bc, bc, state=dual(torch.randn(2, 8, 4)))],
-        'selective_scan_step': [lambda: F.selective_scan_step(torch.zeros(2, 8, 4), x[:, 0], dual(x[:, 0]), w, bc[:, 0], bc[:, 0])],
+        'selective_scan_step': [lambda: F.selective_scan_step(torch.zeros(2, 8, 4), x[:, 0], dual(x[:, 0]), w, bc[:, 0],
+                                                              bc[:, 0])],
         'short_conv': [lambda: F.short_conv(x, dual(w))],
         'short_conv_step': [lambda: F.short_conv_step(dual(torch.zeros(2, 3, 8)), x[:, 0], w)],
         'add_rms_norm': [lambda: F.add_rms_norm(dual(x), x, n), lambda: F.add_rms_norm(x, None, dual(n))],
