@@ -298,3 +298,43 @@ def test_gradients_past_2_to_the_31_elements(F):
         count = 12 * n + N + 64
         close('out', out[T - n:, c], r['out'], m['out'], count, HALF[torch.bfloat16])
         close('du', g[T - n:, c], r['u'], m['u'], count, HALF[torch.bfloat16])
+
+
+@pytest.mark.parametrize('form', ['clips', 'packed', 'long'])
+def test_encoder_in_captured_steps(form):
+    """training steps and forward passes from captured graphs, with eager work between the replays, as the eager ones"""
+    from hipvae.graph import GraphedForward, GraphedTrainStep
+    from hipvae.optim import FusedAdam
+    off = torch.tensor([0, 9, 9, 40, 41], dtype=torch.int32, device='cuda') if form == 'packed' else None
+    shape = {'clips': (5, 11, 24), 'packed': (43, 24), 'long': (1, 333, 24)}[form]
+    data = [rnd(gen(k), *shape).cuda() for k in range(4)]
+    loss_of = lambda m, x: {'total_loss': (m(x, offsets=off)[0] - 0.3).square().mean()}      # noqa: E731
+    models_, losses = [ssm(), ssm()], []
+    for m, captured in zip(models_, (False, True)):
+        m.return_states = False
+        opt = FusedAdam(m.parameters(), lr=1e-2)
+        if captured:
+            step = GraphedTrainStep(m, opt, loss_of, data[0])
+            losses.append([])
+            for x in data:
+                losses[-1].append(float(step(x)['total_loss'].detach()))
+                loss_of(models_[0], x)
+        else:
+            losses.append([])
+            for x in data:
+                opt.zero_grad(set_to_none=True)
+                loss = loss_of(m, x)['total_loss']
+                loss.backward()
+                opt.step()
+                losses[-1].append(float(loss.detach()))
+                del loss
+    assert losses[0] == pytest.approx(losses[1], rel=1e-6) and len(set(losses[0])) == 4
+    for (k, a), b in zip(models_[0].state_dict().items(), models_[1].state_dict().values()):
+        # (the captured optimizer takes its step count from device memory: its bias corrections differ in the last bits)
+        assert float((a - b).abs().max()) <= 1e-6 + 1e-5 * float(a.abs().max()), k
+    m = models_[0].eval()
+    run = GraphedForward(m, data[0], fn=lambda m, x: m(x, return_sequence=True, offsets=off)[0])
+    for x in data[::-1] + data:
+        y = run(x).clone()
+        with torch.no_grad():
+            assert torch.equal(y, m(x, return_sequence=True, offsets=off)[0])
