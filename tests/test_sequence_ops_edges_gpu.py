@@ -338,3 +338,19 @@ def test_encoder_in_captured_steps(form):
         y = run(x).clone()
         with torch.no_grad():
             assert torch.equal(y, m(x, return_sequence=True, offsets=off)[0])
+
+
+def test_function_transforms_are_refused(F):
+    """transforms that wrap tensors: an error, never a call that ignores the wrapping"""
+    x, w, a, bc = (torch.randn(*s, device='cuda') for s in ((2, 5, 8), (8, 4), (8,), (2, 5, 4)))
+    calls = [lambda t: F.add_rms_norm(t, None, a)[0], lambda t: F.add_rms_norm(t, t, a)[1], lambda t: F.add_rms_norm_q8(t, None, a)[1],
+             lambda t: F.short_conv(t, w), lambda t: F.selective_scan(t, t, -w.abs(), bc, bc)]
+    for i, f in enumerate(calls):
+        with pytest.raises(RuntimeError):
+            torch.func.grad(lambda t: f(t).sum())(x)
+            pytest.fail(f'grad {i}')
+        with pytest.raises(RuntimeError, match='forward-mode'):
+            torch.func.jvp(f, (x,), (x,))
+        with pytest.raises(RuntimeError):
+            torch.vmap(f)(x[None])
+            pytest.fail(f'vmap {i}')
