@@ -986,16 +986,20 @@ static void scan_shape(ScanArgs& p, int64_t rows, int64_t L, int64_t D, int64_t 
   p.tpg = (p.Dg + 63) / 64;
   p.wpg = p.G * ((p.tpg + 3) / 4);
   p.blocks = (int)ceil_div64(L, SCAN_Q);
-  // Chunks: none where there are three waves for every four SIMDs without them, since the passes that chunks need cost more
-  // than idle SIMDs (split against whole, bf16, outputs: 24 x 512 x 2048 197 and 201 us, 32 x 1024 x 2048 452 and 395, 256 x
-  // 512 x 2048 1695 and 872; 16 x 1024 x 2048, two waves for four SIMDs: 236 and 392).  Else as many as it takes to reach two
-  // waves per SIMD, none shorter than 32 tokens; from there on to four per SIMD, none shorter than 64.  Two against four: 8 x
-  // 2048 x 2048 training 914 and 834 us, outputs of 1 x 8192 x 2048 139 and 127 us; 1 x 131072 x 64, where four are 32 tokens
-  // each: 160 and 218 us.
-  const int64_t waves = rows * p.tpg * G;
+  // Chunks: none where the rows give every SIMD two waves without them, since the passes that chunks need cost more than a
+  // third and a fourth wave gain (split against whole, bf16, outputs of 256 x 512 x 2048: 1695 and 872 us).  With 16 states
+  // and several rows that is so from three waves for every four SIMDs on (outputs of 24 x 512 x 2048 197 and 201 us, 32 x
+  // 1024 x 2048 452 and 395, training of 28 x 4096 x 2048 fp32 6001 and 5136; but 16 x 1024 x 2048, two waves for four SIMDs:
+  // outputs 236 and 392).  Fewer states have one wave per tile on the way back, and packed sequences' borders are waits that
+  // other waves fill: training of 28 x 2048 x 2048 with 8 states 2143 and 2854 us, of 40 sequences packed into 8192 x 49152
+  // fp32 11310 and 14928.
+  // Else as many as it takes to reach two waves per SIMD, none shorter than 32 tokens; from there on to four per SIMD, none
+  // shorter than 64.  Two against four: 8 x 2048 x 2048 training 914 and 834 us, outputs of 1 x 8192 x 2048 139 and 127 us;
+  // 1 x 131072 x 64, where four are 32 tokens each: 160 and 218 us.
+  const int64_t waves = rows * p.tpg * G, enough = N == 16 && rows > 1 ? SCAN_WAVES / 8 * 3 : SCAN_WAVES;
   const int64_t two = waves > 0 ? ceil_div64(SCAN_WAVES, waves) : 1, four = 2 * two;
   const int64_t n2 = two < L / 32 ? two : L / 32, n4 = four < L / 64 ? four : L / 64;
-  const int64_t n = 8 * waves >= 3 * SCAN_WAVES ? 1 : n2 > n4 ? n2 : n4;
+  const int64_t n = waves >= enough ? 1 : n2 > n4 ? n2 : n4;
   p.CL = (int)(n > 1 ? ceil_div64(ceil_div64(L, n), SCAN_Q) * SCAN_Q : p.blocks * SCAN_Q);
   p.nch = (int)(L > 0 ? ceil_div64(L, p.CL) : 1);
 }

@@ -43,14 +43,16 @@ def test_forward_mode_transforms_are_refused():
             f(lambda t: F.add_rms_norm(t, None, n)[0], (x,), (x,))
 
 
-@pytest.mark.parametrize('rows,L,D,G,split', [
-    (1, 4096, 2048, 1, True), (8, 2048, 2048, 1, True), (16, 1024, 2048, 1, True), (1, 31, 64, 1, False), (1, 1, 64, 1, False),
+@pytest.mark.parametrize('rows,L,D,G,N,split', [
+    (1, 4096, 2048, 1, 16, True), (8, 2048, 2048, 1, 16, True), (16, 1024, 2048, 1, 16, True), (1, 31, 64, 1, 16, False),
+    (1, 1, 64, 1, 16, False), (28, 2048, 2048, 1, 8, True), (32, 512, 2048, 1, 5, True), (1, 8192, 49152, 1, 16, True),
     # a wave for most SIMDs, and many for each: the passes that chunks need cost more than they gain
-    (24, 512, 2048, 1, False), (32, 1024, 2048, 1, False), (96, 512, 2048, 1, False), (256, 512, 2048, 1, False),
-    (4096, 4096, 64, 1, False), (512, 512, 256, 4, False),
+    (24, 512, 2048, 1, 16, False), (32, 1024, 2048, 1, 16, False), (96, 512, 2048, 1, 16, False),
+    (256, 512, 2048, 1, 16, False), (4096, 4096, 64, 1, 16, False), (512, 512, 256, 4, 16, False),
+    (64, 512, 2048, 1, 8, False), (64, 4096, 2048, 1, 5, False), (1, 1024, 131072, 1, 16, False),
 ])
-def test_the_scan_splits_the_time_axis_where_there_are_few_rows(rows, L, D, G, split):
+def test_the_scan_splits_the_time_axis_where_there_are_few_rows(rows, L, D, G, N, split):
     """scratch is what tells from outside: without chunks the forward pass needs none"""
     from hipvae._lib import lib
     for keep in (0, 1):
-        assert (lib.dvae_selective_scan_fwd_ws_floats(rows, L, D, G, 16, keep) > 0) == split
+        assert (lib.dvae_selective_scan_fwd_ws_floats(rows, L, D, G, N, keep) > 0) == split
